@@ -291,6 +291,79 @@ int grouped_gemm_offsets_scatter_launch(const void* a, const void* b, const int3
                                         const mgb_tile_config* config, void* scratch, size_t scratch_bytes,
                                         void* stream, mgb_launch_info* info);
 
+/* The gated feed-forward block of every expert over expert-sorted rows, with
+ * what a training step needs.  The reference stops at the expert GEMMs
+ * (SiLU(gate) * up and every gradient stay outside its timed path,
+ * README.md:55-60), so none of these replaces one of its launches.
+ *
+ * Rows of segment e are [offs[e-1], offs[e]) (int32 cumulative row ends on the
+ * device, one per expert; offs = null is one segment of every row, experts =
+ * 1).  Rows past the last end are neither read nor written.  An end below its
+ * predecessor or past `rows` is clamped and reported (error bit 6).
+ * dtype MGB_FP16 or MGB_BF16; bases 16-byte aligned; columns contiguous; row
+ * pitches and expert strides in elements, multiples of 8; hidden and ffn
+ * multiples of 8; otherwise MGB_ERR_INVALID.  fp32 accumulation, one rounding
+ * per stored value.  Inputs and outputs must not overlap.
+ * scratch: ffn_scratch_bytes(experts, jobs) bytes, 128-byte aligned, not
+ * shared by launches that overlap. */
+typedef struct mgb_ffn_args {
+  int32_t dtype;
+  int32_t experts;
+  int64_t rows;   /* T */
+  int64_t hidden; /* H */
+  int64_t ffn;    /* F */
+  const int32_t* offs;
+  const void* x; /* [T, H] */
+  int64_t x_pitch;
+  const void* w13; /* [E, H, 2F] packed [gate | up] */
+  int64_t w13_pitch, w13_stride;
+  const void* w2; /* [E, F, H] */
+  int64_t w2_pitch, w2_stride;
+  void* gate_up; /* [T, 2F] x W13: written forward, read backward */
+  int64_t gate_up_pitch;
+  void* h; /* [T, F] silu(gate) * up: written forward, read backward */
+  int64_t h_pitch;
+  void* y; /* [T, H] forward output h W2; backward its gradient (read) */
+  int64_t y_pitch;
+  void* dgate_up; /* backward: [T, 2F] gradient of gate_up (written) */
+  int64_t dgate_up_pitch;
+  void* dx; /* backward: [T, H] */
+  int64_t dx_pitch;
+  void* dw13; /* backward: [E, H, 2F]; zeros for an expert without rows */
+  int64_t dw13_pitch, dw13_stride;
+  void* dw2; /* backward: [E, F, H] */
+  int64_t dw2_pitch, dw2_stride;
+  void* scratch;
+  size_t scratch_bytes;
+  void* stream;
+} mgb_ffn_args;
+
+/* Scratch of a call with `jobs` products: forward 2 (1 without w2), backward
+ * 4, the gradients below 1. */
+size_t ffn_scratch_bytes(int32_t experts, int32_t jobs);
+
+/* gate_up = x W13, h = silu(gate) * up (both from one kernel) and, unless w2
+ * is null, y = h W2. */
+int gated_ffn_forward_launch(const mgb_ffn_args* args);
+
+/* From y (the output's gradient), x, h, gate_up, W13, W2: dgate_up, dx, dW13, dW2. */
+int gated_ffn_backward_launch(const mgb_ffn_args* args);
+
+/* Gradient of grouped_gemm_offsets_launch's C = A B_e with respect to A:
+ * out[rows of e] = dC[rows of e] B_e^T, dC [rows, n], B [E, k, n], out
+ * [rows, k].  With gate_up [rows, 2k] non-null the product is the gradient of
+ * h = silu(gate) * up and out [rows, 2k] receives the gradient of gate_up. */
+int grouped_gemm_dgrad_launch(const void* dc, int64_t dc_pitch, const void* b, int64_t b_pitch, int64_t b_stride,
+                              const int32_t* offs, int32_t experts, int64_t rows, int64_t n, int64_t k,
+                              const void* gate_up, int64_t gate_up_pitch, void* out, int64_t out_pitch, int32_t dtype,
+                              void* scratch, size_t scratch_bytes, void* stream);
+
+/* ... and with respect to B: dB_e = A[rows of e]^T dC[rows of e], dB [E, k, n]
+ * (zeros for an expert without rows). */
+int grouped_gemm_wgrad_launch(const void* a, int64_t a_pitch, const void* dc, int64_t dc_pitch, const int32_t* offs,
+                              int32_t experts, int64_t rows, int64_t n, int64_t k, void* db, int64_t db_pitch,
+                              int64_t db_stride, int32_t dtype, void* scratch, size_t scratch_bytes, void* stream);
+
 /* Masked single GEMM C[m, n] = A[m, k] @ B[k, n] with arbitrary element strides.
  * Replaces the Triton launch of launch_matmul (kernels/matmul.py:332-392,
  * kernel _matmul_kernel_impl :223-273).  Operands that satisfy the TMA rules

@@ -546,6 +546,20 @@ int grouped_launch_impl(const int64_t* a_ptrs, const int64_t* b_ptrs, const int6
 }  // namespace
 
 namespace mgb {
+bool current_launch_limits(int* sm_count, long long* wait_budget) {
+  DeviceState ds;
+  if (device_state(&ds) != MGB_OK) return false;
+  *sm_count = ds.sm_count;
+  *wait_budget = g_wait_budget;
+  return true;
+}
+
+bool encode_map_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch,
+                   uint32_t box_inner, uint32_t box_outer) {
+  return g_encode != nullptr &&
+         encode_2d(map, dtype, base, inner, outer, pitch, box_inner, box_outer, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 uint32_t* current_error_word() {
   DeviceState ds;
   return device_state(&ds) == MGB_OK ? ds.error_word : nullptr;

@@ -1,0 +1,667 @@
+// Grouped products of the gated feed-forward block and its backward pass,
+// fp16 / bf16, tokens sorted by expert.
+//
+// A launch runs up to kFfnMaxJobs jobs of one epilogue kind over the same
+// expert segments.  Segment e holds the rows [offs[e-1], offs[e]) of every
+// token tensor.  A job is, per expert e,
+//   rows  C[rows of e, N] = A[rows of e, K] op(B_e)     M = rows of e
+//   wgrad C_e[M, N] = A[rows of e, M]^T B[rows of e, N]  contraction over rows of e
+// with either operand K-major (contraction contiguous) or MN-major, chosen at
+// run time: TMA loads it in the box its layout needs (K-major: 64 contraction
+// x 128 outer; MN-major: 64 outer x 64 contraction, two boxes) and the MMA
+// descriptors name the layout, so no operand is ever transposed in memory:
+//   x W13, h W2          A K-major,  B MN-major
+//   dy W2^T, dgu W13^T   A K-major,  B K-major
+//   x^T dgu, h^T dy      A MN-major, B MN-major
+// Every expert has its own tensor maps, whose row extent ends with the
+// segment: the tail of a segment's last contraction block reads zeros, never
+// the next expert's rows (a zero times their NaN would be NaN), and stores
+// past a segment are clipped.
+//
+// Epilogues (fp32 accumulators, one rounding per stored value):
+//   plain            C
+//   swiglu           gate | up tiles side by side in one accumulator; stores
+//                    h = silu(g) u, g and u (the backward pass reads g, u)
+//   swiglu backward  accumulator = dh; g, u arrive by TMA while the MMAs run;
+//                    stores dg = dh u s (1 + g (1 - s)), du = dh g s, s = sigmoid(g)
+//
+// One CTA per SM, roles by warp: 0 TMA producer, 1 MMA issuer, 2-5 epilogue.
+// G = 2: CTA pairs, 256 x 256 tiles (tcgen05 cta_group::2, M = 256, N = 256);
+// G = 1: one CTA, 128 x 128 tiles, four times as many, for launches whose
+// 256 x 256 tiles would leave most SMs idle.  Both load 128 rows of A and
+// 128 columns of B per CTA and 64-deep contraction block (32 KB a stage).
+// Every wait is bounded; loads carry no multicast.
+#pragma once
+
+#include "mgb_tc_kernel.cuh"
+
+namespace mgb {
+
+constexpr int kFfnMaxJobs = 3;
+constexpr int kFfnMaps = 6;  // per job and expert: A, B, then the epilogue's
+enum FfnEpilogue : int { kFfnPlain = 0, kFfnSwiglu = 1, kFfnSwigluBwd = 2 };
+
+// One tensor of a job: rows follow the segments (token tensors) or the
+// expert (weights, `expert_stride` elements apart).
+struct FfnTensor {
+  char* data;
+  int64_t pitch;          // elements between rows
+  int64_t expert_stride;  // weights: elements between experts
+  int32_t token;          // 1: rows are token rows
+};
+
+struct FfnJob {
+  FfnTensor t[kFfnMaps];
+  int32_t maps;   // tensors used
+  int32_t wgrad;  // contraction over the segment's rows
+  int32_t a_mn, b_mn;
+  int64_t m;      // wgrad: output rows
+  int64_t n;      // output columns
+  int64_t k;      // rows: contraction depth
+  int64_t up;     // swiglu: column of B where the up half starts
+};
+
+struct FfnParams {
+  FfnJob job[kFfnMaxJobs];
+  int32_t jobs;
+  int32_t experts;
+  const int32_t* offs;  // [experts] row ends; nullptr: one segment of `rows`
+  int64_t rows;
+  uint8_t* maps;        // [jobs][experts][kFfnMaps] tensor maps
+  int64_t* tile_start;  // [jobs * experts + 1] first tile of every (job, expert)
+  int32_t tile_rows, tile_cols;  // output tile (the walk's)
+  long long wait_budget;
+  uint32_t* error_word;
+};
+
+struct FfnTemplates {
+  CUtensorMap map[kFfnMaxJobs][kFfnMaps];
+};
+
+// Rows [start, start + len) of expert e, clamped into the tensor whatever offs holds.
+__device__ __forceinline__ int64_t ffn_segment(const FfnParams& p, int e, int64_t& start, bool* bad = nullptr) {
+  if (p.offs == nullptr) {
+    start = 0;
+    return p.rows;
+  }
+  const int64_t lo = e > 0 ? p.offs[e - 1] : 0, hi = p.offs[e];
+  if (bad != nullptr) *bad = lo < 0 || hi < lo || hi > p.rows;
+  start = lo < 0 ? 0 : lo > p.rows ? p.rows : lo;
+  const int64_t end = hi < start ? start : hi > p.rows ? p.rows : hi;
+  return end - start;
+}
+
+// Tensor maps of every (job, expert), one warp each, and the tiles' prefix
+// sums (last block).
+__global__ void __launch_bounds__(32)
+    ffn_plan_kernel(const __grid_constant__ FfnTemplates tmpl, const __grid_constant__ FfnParams p) {
+  __shared__ alignas(128) CUtensorMap staging[kFfnMaps];
+  const int lane = threadIdx.x;
+  const int pairs = p.jobs * p.experts;
+  grid_launch_dependents();
+  if (blockIdx.x == pairs) {
+    const int per = (pairs + 31) / 32;
+    const int lo = lane * per, hi = lo + per < pairs ? lo + per : pairs;
+    auto tiles_of = [&](int i) -> int64_t {
+      const FfnJob& j = p.job[i / p.experts];
+      int64_t start;
+      const int64_t rows = j.wgrad ? j.m : ffn_segment(p, i % p.experts, start);
+      return ceil_div64(rows, p.tile_rows) * ceil_div64(j.n, p.tile_cols);
+    };
+    int64_t sum = 0;
+    for (int i = lo; i < hi; ++i) sum += tiles_of(i);
+    int64_t incl = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += v;
+    }
+    int64_t run = incl - sum;
+    for (int i = lo; i < hi; ++i) {
+      p.tile_start[i] = run;
+      run += tiles_of(i);
+    }
+    if (lane == 31) p.tile_start[pairs] = incl;
+    return;
+  }
+  const int job = blockIdx.x / p.experts, e = blockIdx.x % p.experts;
+  const FfnJob& j = p.job[job];
+  bool bad = false;
+  int64_t start = 0;
+  const int64_t len = ffn_segment(p, e, start, &bad);
+  if (bad && lane == 0) atomicOr(p.error_word, kErrBadDims);
+  // One lane per map: copy the template, move its base, end its rows with the segment.
+  if (lane < j.maps) {
+    const uint4* src = reinterpret_cast<const uint4*>(&tmpl.map[job][lane]);
+    uint4* dst = reinterpret_cast<uint4*>(&staging[lane]);
+    for (int i = 0; i < 8; ++i) dst[i] = src[i];
+    const FfnTensor& t = j.t[lane];
+    if (t.token) {
+      if (len > 0) {  // an empty segment's maps are never used
+        tmap_replace_address(&staging[lane], t.data + start * t.pitch * 2);
+        tmap_replace_dim(&staging[lane], 1, static_cast<uint32_t>(len));
+      }
+    } else {
+      tmap_replace_address(&staging[lane], t.data + e * t.expert_stride * 2);
+    }
+  }
+  __syncwarp();
+  CUtensorMap* g = reinterpret_cast<CUtensorMap*>(p.maps) + static_cast<int64_t>(blockIdx.x) * kFfnMaps;
+  for (int i = 0; i < j.maps; ++i) tmap_publish(&g[i], &staging[i]);
+}
+
+// A role's position in the tile list.
+struct FfnWalk {
+  int pair = -1;  // job * experts + e
+  int64_t first = 0, end = 0;
+  int64_t len = 0;     // rows of the expert's segment
+  int64_t rows = 0;    // output rows
+  int64_t m_blocks = 1, n_blocks = 1;
+  int64_t kblocks = 0;
+  const FfnJob* job = nullptr;
+
+  __device__ __forceinline__ bool seek(const FfnParams& p, int64_t t) {
+    const int64_t* ts = p.tile_start;
+    const int pairs = p.jobs * p.experts;
+    if (t >= end || pair < 0) {
+      if (t >= ts[pairs]) return false;
+      int lo = pair < 0 ? 0 : pair, hi = pairs - 1;
+      while (lo < hi) {  // the last pair whose first tile is <= t owns it (empty pairs share their successor's)
+        const int mid = (lo + hi + 1) >> 1;
+        if (ts[mid] <= t) {
+          lo = mid;
+        } else {
+          hi = mid - 1;
+        }
+      }
+      pair = lo;
+      first = ts[lo];
+      end = ts[lo + 1];
+      job = &p.job[lo / p.experts];
+      int64_t start;
+      len = ffn_segment(p, lo % p.experts, start);
+      rows = job->wgrad ? job->m : len;
+      m_blocks = ceil_div64(rows, p.tile_rows);
+      n_blocks = ceil_div64(job->n, p.tile_cols);
+      kblocks = ceil_div64(job->wgrad ? len : job->k, 64);
+    }
+    return true;
+  }
+  // Bands of 8 row blocks, row block fastest inside a band (as TileWalk).
+  __device__ __forceinline__ void blocks(int64_t t, int64_t& mb, int64_t& nb) const {
+    const int64_t local = t - first;
+    const int64_t band_tiles = 8 * n_blocks;
+    const int64_t band = local / band_tiles;
+    const int64_t in = local - band * band_tiles;
+    const int64_t rows_in = m_blocks - band * 8 < 8 ? m_blocks - band * 8 : 8;
+    mb = band * 8 + in % rows_in;
+    nb = in / rows_in;
+  }
+};
+
+template <typename T, int EPI, int G>
+struct FfnCfg {
+  static_assert(sizeof(T) == 2 && (G == 1 || G == 2), "16-bit types, one CTA or a pair");
+  static constexpr int kBK = 64;
+  static constexpr int kOperand = 128 * 128;  // 128 rows (or columns) x 64 contraction
+  static constexpr int kStageBytes = 2 * kOperand;
+  static constexpr int kTileM = 128 * G;
+  static constexpr int kAccCols = 128 * G;
+  static constexpr int kTileOut = EPI == kFfnSwiglu ? kAccCols / 2 : kAccCols;  // output columns per tile
+  static constexpr int kTmemCols = 2 * kAccCols;                                // two accumulators
+  // Staging blocks (32 rows x 128 bytes) per epilogue warp: plain two, in
+  // turn; swiglu h, g and u of one chunk; backward two pairs (g, u), each
+  // overwritten in place by (dg, du).
+  static constexpr int kEpiBlocks = EPI == kFfnPlain ? 2 : EPI == kFfnSwiglu ? 3 : 4;
+  static constexpr int kEpiBytes = 4 * kEpiBlocks * kEpiWarpBytes;
+  static constexpr int kStages = (kTcSmemBudget - kEpiBytes) / kStageBytes;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + 2048 + 1024;
+  static constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  static_assert(kStages >= 4 && kSmemBytes <= 232448, "shared memory");
+};
+
+// Swiglu epilogue of one warp: gate columns [0, TO), up columns [TO, 2 TO) of
+// the accumulator; h from the fp32 values, g and u rounded once as stored.
+template <typename T, int TO>
+__device__ __forceinline__ void ffn_store_swiglu(const CUtensorMap* maps, uint32_t taddr, int64_t rows, int64_t cols,
+                                                 int32_t row0, int32_t o0, uint8_t* blocks, int lane) {
+  if (row0 >= rows || o0 >= cols) return;
+  const int64_t left = cols - o0;
+  const int chunks = left >= TO ? TO / 64 : static_cast<int>((left + 63) / 64);
+#pragma unroll 1
+  for (int c = 0; c < chunks; ++c) {
+    if (lane == 0) bulk_wait_group_read<0>();  // the previous chunk's stores have read the blocks
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      uint32_t gate[32], up[32];
+      tmem_ld32(taddr + c * 64 + u * 32, gate);
+      tmem_ld32(taddr + TO + c * 64 + u * 32, up);
+      tmem_ld_wait();
+      write_unit_smem<T>(gate, blocks + kEpiWarpBytes, lane, u);
+      write_unit_smem<T>(up, blocks + 2 * kEpiWarpBytes, lane, u);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        gate[i] = __float_as_uint(silu_mul(__uint_as_float(gate[i]), __uint_as_float(up[i])));
+      }
+      write_unit_smem<T>(gate, blocks, lane, u);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      const uint64_t pol = policy_evict_normal();
+#pragma unroll
+      for (int i = 0; i < 3; ++i) tma_store_2d(&maps[2 + i], blocks + i * kEpiWarpBytes, o0 + c * 64, row0, pol);
+      bulk_commit_group();
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t v) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+  } else {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  }
+}
+
+// Gradients of h = silu(g) u: s = sigmoid(g) with the fast exponential and
+// divide (a few ulp in fp32, far below the 16-bit rounding of what is stored).
+__device__ __forceinline__ void swiglu_grad(float dh, float g, float u, float& dg, float& du) {
+  const float s = __fdividef(1.0f, 1.0f + __expf(-g));
+  du = dh * g * s;
+  dg = dh * u * s * (1.0f + g * (1.0f - s));
+}
+
+// One warp's state of the swiglu backward epilogue: two pairs of blocks, each
+// with an mbarrier its loads land on.
+struct FfnGateLoads {
+  uint8_t* blocks;
+  uint64_t* bars;  // two
+  uint32_t issued = 0, used = 0;
+
+  // Lane 0: loads the (g, u) chunk at (x, y) into the next pair, once the
+  // stores issued from it have read it.
+  __device__ __forceinline__ void issue(const CUtensorMap* maps, int32_t x, int32_t y) {
+    const int set = issued & 1;
+    bulk_wait_group_read<0>();
+    mbar_arrive_expect_tx(&bars[set], 2 * kEpiWarpBytes);
+    const uint64_t pol = policy_evict_first();
+    tma_load_2d(&maps[4], &bars[set], blocks + set * 2 * kEpiWarpBytes, x, y, pol);
+    tma_load_2d(&maps[5], &bars[set], blocks + set * 2 * kEpiWarpBytes + kEpiWarpBytes, x, y, pol);
+  }
+};
+
+template <typename T, int EPI, int G>
+__global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constant__ FfnParams p) {
+  using Cfg = FfnCfg<T, EPI, G>;
+  constexpr int S = Cfg::kStages;
+  constexpr int BK = Cfg::kBK;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem;
+  uint8_t* epi_stage = smem + S * Cfg::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(epi_stage + Cfg::kEpiBytes);
+  uint64_t* empty = full + S;
+  uint64_t* acc_full = empty + S;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drain_bar = acc_empty + 2;
+  uint64_t* gate_bars = drain_bar + 1;  // two per epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gate_bars + 8);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* never = abort + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = G == 2 ? cluster_ctarank() : 0u;
+  const bool leader = rank == 0;
+  const int64_t first_item = blockIdx.x / G;
+  const int64_t items_step = gridDim.x / G;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4 * G);
+    }
+    mbar_init(drain_bar, 1);
+    for (int i = 0; i < 8; ++i) mbar_init(&gate_bars[i], 1);
+    *abort = 0;
+    *never = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if constexpr (G == 2) {
+      tmem_alloc_pair(tmem_slot, Cfg::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, Cfg::kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (G == 2) cluster_sync();  // the peer's barriers exist before anything lands on them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const long long budget = p.wait_budget;
+  grid_dependency_wait();  // global memory is read only from here on
+  const CUtensorMap* all_maps = reinterpret_cast<const CUtensorMap*>(p.maps);
+
+  auto fail = [&](uint32_t bits) {
+    atomicOr(p.error_word, bits);
+    *abort = 1;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    const uint64_t pol_keep = policy_evict_last();
+    const uint64_t pol_shared = policy_evict_normal();
+    const uint64_t pol_stream = policy_evict_first();
+    FfnWalk walk;
+    uint32_t it = 0;
+    int built = -1;
+    bool ok = true;
+    for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+      const FfnJob& j = *walk.job;
+      int64_t mb, nb;
+      walk.blocks(t, mb, nb);
+      const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.pair) * kFfnMaps;
+      if (walk.pair != built) {
+        if (lane == 0) {
+          tmap_acquire(&g[0]);
+          tmap_acquire(&g[1]);
+        }
+        __syncwarp();
+        built = walk.pair;
+      }
+      const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128);
+      // First B column of this CTA's two 64-column boxes (swiglu: gate and up
+      // columns of the same outputs; a pair's CTA 0 holds gate, CTA 1 up).
+      int32_t b0, b1;
+      if constexpr (EPI == kFfnSwiglu) {
+        const int32_t o = static_cast<int32_t>(nb * Cfg::kTileOut);
+        if constexpr (G == 2) {
+          b0 = o + (rank ? static_cast<int32_t>(j.up) : 0);
+          b1 = b0 + 64;
+        } else {
+          b0 = o;
+          b1 = o + static_cast<int32_t>(j.up);
+        }
+      } else {
+        b0 = static_cast<int32_t>(nb * Cfg::kAccCols + rank * 128);
+        b1 = b0 + 64;
+      }
+      // Weights that one row block reads are streamed; shared operands keep
+      // normal priority; activations of a rows job are kept for the other
+      // column blocks.
+      const uint64_t pol_a = j.wgrad ? pol_shared : pol_keep;
+      const uint64_t pol_b = !j.wgrad && walk.m_blocks == 1 ? pol_stream : pol_shared;
+      for (int64_t kb = 0; kb < walk.kblocks; ++kb) {
+        const int s = static_cast<int>(it % S);
+        if (!mbar_wait_warp(&empty[s], ((it / S) & 1u) ^ 1u, budget, abort)) {
+          if (lane == 0) fail(kErrWaitEmpty);
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          uint8_t* st_a = ring + s * Cfg::kStageBytes;
+          uint8_t* st_b = st_a + Cfg::kOperand;
+          const int32_t kx = static_cast<int32_t>(kb * BK);
+          auto load = [&](const CUtensorMap* map, uint8_t* dst, int32_t x, int32_t y, uint64_t pol) {
+            if constexpr (G == 2) {
+              tma_load_2d_pair(map, mapa_shared(smem_u32(&full[s]), 0), dst, x, y, pol);
+            } else {
+              tma_load_2d(map, &full[s], dst, x, y, pol);
+            }
+          };
+          if (leader) mbar_arrive_expect_tx(&full[s], G * Cfg::kStageBytes);
+          if (j.a_mn) {
+            load(&g[0], st_a, m0, kx, pol_a);
+            load(&g[0], st_a + Cfg::kOperand / 2, m0 + 64, kx, pol_a);
+          } else {
+            load(&g[0], st_a, kx, m0, pol_a);
+          }
+          if (j.b_mn) {
+            load(&g[1], st_b, b0, kx, pol_b);
+            load(&g[1], st_b + Cfg::kOperand / 2, b1, kx, pol_b);
+          } else {
+            load(&g[1], st_b, kx, b0, pol_b);
+          }
+        }
+        __syncwarp();
+        ++it;
+      }
+    }
+    if (*abort && leader && lane == 0) {  // loads in flight land before the CTA's memory goes away
+      for (uint32_t i = it > static_cast<uint32_t>(S) ? it - S : 0u; i < it; ++i) {
+        if (!mbar_wait(&full[i % S], (i / S) & 1u, budget, never)) {
+          atomicOr(p.error_word, kErrWaitTeardown);
+          break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ MMA issuer (leader only)
+    if (lane == 0 && leader) {
+      FfnWalk walk;
+      uint32_t it = 0, acc_it = 0;
+      bool ok = true;
+      for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+        if (walk.kblocks <= 0) continue;
+        const FfnJob& j = *walk.job;
+        // K-major: a k-step of 16 is 32 bytes along the swizzled row.
+        // MN-major: 16 contraction rows of 128 bytes; the second 64 columns
+        // one box (8 KB) on.
+        const uint64_t a_desc = smem_desc(smem_u32(ring), j.a_mn ? Cfg::kOperand / 2 : 16, 1024, kLayoutSw128);
+        const uint64_t b_desc =
+            smem_desc(smem_u32(ring) + Cfg::kOperand, j.b_mn ? Cfg::kOperand / 2 : 16, 1024, kLayoutSw128);
+        const uint32_t a_step = j.a_mn ? 16 * 128 / 16 : 32 / 16;
+        const uint32_t b_step = j.b_mn ? 16 * 128 / 16 : 32 / 16;
+        const uint32_t idesc = instr_desc(Cfg::kFmt, j.a_mn, j.b_mn, Cfg::kTileM, Cfg::kAccCols);
+        const int buf = static_cast<int>(acc_it & 1);
+        if (!mbar_wait(&acc_empty[buf], ((acc_it >> 1) & 1u) ^ 1u, budget, abort)) {
+          fail(kErrWaitAccEmpty);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem_base + buf * Cfg::kAccCols;
+        for (int64_t kb = 0; kb < walk.kblocks; ++kb) {
+          const int s = static_cast<int>(it % S);
+          if (!mbar_wait(&full[s], (it / S) & 1u, budget, abort)) {
+            fail(kErrWaitFull);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t stage = static_cast<uint64_t>(s * (Cfg::kStageBytes >> 4));
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            const uint64_t ad = a_desc + stage + ks * a_step, bd = b_desc + stage + ks * b_step;
+            const uint32_t acc = (kb > 0 || ks > 0) ? 1u : 0u;
+            if constexpr (G == 2) {
+              mma_f16_pair(d, ad, bd, idesc, acc);
+            } else {
+              mma_f16(d, ad, bd, idesc, acc);
+            }
+          }
+          if constexpr (G == 2) {
+            mma_commit_pair(&empty[s], 0x3);
+          } else {
+            mma_commit(&empty[s]);
+          }
+          ++it;
+        }
+        if (!ok) break;
+        if constexpr (G == 2) {
+          mma_commit_pair(&acc_full[buf], 0x3);
+        } else {
+          mma_commit(&acc_full[buf]);
+        }
+        ++acc_it;
+      }
+      if (*abort) {
+        if constexpr (G == 2) {
+          mma_commit_pair(drain_bar, 0x1);
+        } else {
+          mma_commit(drain_bar);
+        }
+        if (!mbar_wait(drain_bar, 0, budget, never)) atomicOr(p.error_word, kErrWaitTeardown);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int quarter = warp & 3;
+    uint8_t* blocks = epi_stage + quarter * Cfg::kEpiBlocks * kEpiWarpBytes;
+    const uint64_t pol_out = policy_evict_normal();
+    FfnGateLoads gates{blocks, gate_bars + 2 * quarter};
+    FfnWalk walk;
+    uint32_t acc_it = 0, chunk_seq = 0;
+    int built = -1;
+    for (int64_t t = first_item; walk.seek(p, t); t += items_step) {
+      const FfnJob& j = *walk.job;
+      int64_t mb, nb;
+      walk.blocks(t, mb, nb);
+      const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.pair) * kFfnMaps;
+      if (walk.pair != built) {
+        if (lane == 0) {
+          for (int i = 2; i < j.maps; ++i) tmap_acquire(&g[i]);
+        }
+        __syncwarp();
+        built = walk.pair;
+      }
+      const int32_t row0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128 + quarter * 32);
+      const int32_t n0 = static_cast<int32_t>(nb * Cfg::kTileOut);
+      if (walk.kblocks <= 0) {
+        // An expert without rows: its weight gradient is zero.
+        const FfnTensor& c = j.t[2];
+        T* out = reinterpret_cast<T*>(c.data) + (walk.pair % p.experts) * c.expert_stride;
+        for (int r = 0; r < 32 && row0 + r < walk.rows; ++r) {
+          for (int64_t col = n0 + lane * 8; col < j.n && col < n0 + Cfg::kTileOut; col += 256) {
+            T* dst = out + (row0 + r) * c.pitch + col;  // n is a multiple of 8: whole 16-byte pieces
+            *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        continue;
+      }
+      int chunks = 0;
+      if constexpr (EPI == kFfnSwigluBwd) {
+        if (row0 < walk.rows) {
+          const int64_t left = j.n - n0;
+          chunks = left >= Cfg::kTileOut ? Cfg::kTileOut / 64 : static_cast<int>((left + 63) / 64);
+          if (lane == 0) gates.issue(g, n0, row0);  // the first chunk arrives while the MMAs run
+          ++gates.issued;
+        }
+      }
+      const int buf = static_cast<int>(acc_it & 1);
+      if (!mbar_wait_warp(&acc_full[buf], (acc_it >> 1) & 1u, budget, abort)) {
+        if (lane == 0) fail(kErrWaitAccFull);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * Cfg::kAccCols;
+      if constexpr (EPI == kFfnPlain) {
+        Problem q;
+        q.m = walk.rows;
+        q.n = j.n;
+        store_rows_tma<T, Cfg::kTileOut, Cfg::kEpiBlocks>(q, &g[2], taddr, row0, n0, blocks, lane, chunk_seq, pol_out,
+                                                          p.error_word);
+      } else if constexpr (EPI == kFfnSwiglu) {
+        ffn_store_swiglu<T, Cfg::kTileOut>(g, taddr, walk.rows, j.n, row0, n0, blocks, lane);
+      } else {
+        bool lost = false;
+#pragma unroll 1
+        for (int c = 0; c < chunks; ++c) {
+          const int set = gates.used & 1;
+          if (c + 1 < chunks) {
+            if (lane == 0) gates.issue(g, n0 + (c + 1) * 64, row0);
+            ++gates.issued;
+          }
+          if (!mbar_wait_warp(&gates.bars[set], (gates.used >> 1) & 1u, budget, abort)) {
+            lost = true;
+            break;
+          }
+          ++gates.used;
+          uint8_t* gb = blocks + set * 2 * kEpiWarpBytes + lane * 128;
+          uint8_t* ub = gb + kEpiWarpBytes;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t dh[32];
+            tmem_ld32(taddr + c * 64 + u * 32, dh);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int at = ((4 * u + i) ^ (lane & 7)) << 4;
+              uint4 gv = *reinterpret_cast<const uint4*>(gb + at), uv = *reinterpret_cast<const uint4*>(ub + at);
+              uint32_t* gw = &gv.x;
+              uint32_t* uw = &uv.x;
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const float2 gf = unpack_pair<T>(gw[w]), uf = unpack_pair<T>(uw[w]);
+                float dg0, dg1, du0, du1;
+                swiglu_grad(__uint_as_float(dh[8 * i + 2 * w]), gf.x, uf.x, dg0, du0);
+                swiglu_grad(__uint_as_float(dh[8 * i + 2 * w + 1]), gf.y, uf.y, dg1, du1);
+                gw[w] = pack_pair<T>(__float_as_uint(dg0), __float_as_uint(dg1));
+                uw[w] = pack_pair<T>(__float_as_uint(du0), __float_as_uint(du1));
+              }
+              *reinterpret_cast<uint4*>(gb + at) = gv;
+              *reinterpret_cast<uint4*>(ub + at) = uv;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            uint8_t* from = blocks + set * 2 * kEpiWarpBytes;
+            tma_store_2d(&g[2], from, n0 + c * 64, row0, pol_out);
+            tma_store_2d(&g[3], from + kEpiWarpBytes, n0 + c * 64, row0, pol_out);
+            bulk_commit_group();
+          }
+        }
+        if (lost) {
+          if (lane == 0) fail(kErrWaitAccFull);
+          break;
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (G == 2) {
+          mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&acc_empty[buf]), 0));
+        } else {
+          mbar_arrive_relaxed(&acc_empty[buf]);
+        }
+      }
+      ++acc_it;
+    }
+    if (EPI == kFfnSwigluBwd && *abort) {  // (g, u) loads in flight land first
+      for (; gates.used != gates.issued; ++gates.used) {
+        if (!mbar_wait_warp(&gates.bars[gates.used & 1], (gates.used >> 1) & 1u, budget, never)) {
+          if (lane == 0) atomicOr(p.error_word, kErrWaitTeardown);
+          break;
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_group_all();  // tensor stores done before the CTA's shared memory goes away
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (G == 2) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (G == 2) {
+      tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    } else {
+      tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    }
+  }
+}
+
+}  // namespace mgb

@@ -26,6 +26,12 @@ from .fp8 import (
     quantize_activations,
     quantize_weight,
 )
+from .gated_ffn import (
+    gated_ffn_backward,
+    gated_ffn_forward,
+    launch_grouped_mm_dgrad,
+    launch_grouped_mm_wgrad,
+)
 from .matmul import (
     KernelConfig,
     last_matmul_config,
@@ -36,6 +42,10 @@ from .matmul import (
 )
 
 __all__ = [
+    "gated_ffn_backward",
+    "gated_ffn_forward",
+    "launch_grouped_mm_dgrad",
+    "launch_grouped_mm_wgrad",
     "Fp8GroupedWorkspace",
     "GroupedWorkspace",
     "build_fp8_workspace",

@@ -49,6 +49,11 @@ EXPORTED_SYMBOLS = (
     "moe_ep_combine",
     "grouped_gemm_fp8_launch",
     "grouped_gemm_launch_noalloc",
+    "ffn_scratch_bytes",
+    "gated_ffn_forward_launch",
+    "gated_ffn_backward_launch",
+    "grouped_gemm_dgrad_launch",
+    "grouped_gemm_wgrad_launch",
     "matmul_launch",
     "matrix_repack",
     "matrix_split_tf32x3",
@@ -143,6 +148,46 @@ class EpRegion(ctypes.Structure):
     ]
 
 
+class FfnArgs(ctypes.Structure):
+    """mgb_ffn_args: the gated feed-forward block's tensors and sizes."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("experts", ctypes.c_int32),
+        ("rows", ctypes.c_int64),
+        ("hidden", ctypes.c_int64),
+        ("ffn", ctypes.c_int64),
+        ("offs", ctypes.c_void_p),
+        ("x", ctypes.c_void_p),
+        ("x_pitch", ctypes.c_int64),
+        ("w13", ctypes.c_void_p),
+        ("w13_pitch", ctypes.c_int64),
+        ("w13_stride", ctypes.c_int64),
+        ("w2", ctypes.c_void_p),
+        ("w2_pitch", ctypes.c_int64),
+        ("w2_stride", ctypes.c_int64),
+        ("gate_up", ctypes.c_void_p),
+        ("gate_up_pitch", ctypes.c_int64),
+        ("h", ctypes.c_void_p),
+        ("h_pitch", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_pitch", ctypes.c_int64),
+        ("dgate_up", ctypes.c_void_p),
+        ("dgate_up_pitch", ctypes.c_int64),
+        ("dx", ctypes.c_void_p),
+        ("dx_pitch", ctypes.c_int64),
+        ("dw13", ctypes.c_void_p),
+        ("dw13_pitch", ctypes.c_int64),
+        ("dw13_stride", ctypes.c_int64),
+        ("dw2", ctypes.c_void_p),
+        ("dw2_pitch", ctypes.c_int64),
+        ("dw2_stride", ctypes.c_int64),
+        ("scratch", ctypes.c_void_p),
+        ("scratch_bytes", ctypes.c_size_t),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
 class NativeLaunchError(RuntimeError):
     """A native launch returned a non-OK status."""
 
@@ -232,6 +277,18 @@ def _declare(lib) -> None:
         ctypes.c_void_p, ctypes.POINTER(LaunchInfo),
     ]
     lib.grouped_gemm_fp8_launch.restype = ctypes.c_int
+    i32, i64, ptr, size = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
+    lib.ffn_scratch_bytes.argtypes = [i32, i32]
+    lib.ffn_scratch_bytes.restype = size
+    for entry in (lib.gated_ffn_forward_launch, lib.gated_ffn_backward_launch):
+        entry.argtypes = [ctypes.POINTER(FfnArgs)]
+        entry.restype = ctypes.c_int
+    lib.grouped_gemm_dgrad_launch.argtypes = [ptr, i64, ptr, i64, i64, ptr, i32, i64, i64, i64, ptr, i64, ptr, i64,
+                                              i32, ptr, size, ptr]
+    lib.grouped_gemm_dgrad_launch.restype = ctypes.c_int
+    lib.grouped_gemm_wgrad_launch.argtypes = [ptr, i64, ptr, i64, ptr, i32, i64, i64, i64, ptr, i64, i64, i32, ptr,
+                                              size, ptr]
+    lib.grouped_gemm_wgrad_launch.restype = ctypes.c_int
     lib.matmul_launch.argtypes = [
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
@@ -451,6 +508,38 @@ def fp8_launch(
     )
     _check(status, "grouped_gemm_fp8_launch")
     return info
+
+
+def ffn_scratch_bytes(experts: int, jobs: int) -> int:
+    return int(load().ffn_scratch_bytes(int(experts), int(jobs)))
+
+
+def gated_ffn_forward(args: FfnArgs, scratch: int, scratch_nbytes: int, stream: int) -> None:
+    args.scratch, args.scratch_bytes, args.stream = scratch, scratch_nbytes, stream
+    _check(load().gated_ffn_forward_launch(ctypes.byref(args)), "gated_ffn_forward_launch")
+
+
+def gated_ffn_backward(args: FfnArgs, scratch: int, scratch_nbytes: int, stream: int) -> None:
+    args.scratch, args.scratch_bytes, args.stream = scratch, scratch_nbytes, stream
+    _check(load().gated_ffn_backward_launch(ctypes.byref(args)), "gated_ffn_backward_launch")
+
+
+def grouped_dgrad(dc: int, dc_pitch: int, b: int, b_pitch: int, b_stride: int, offs: int, experts: int, rows: int,
+                  n: int, k: int, gate_up: int, gate_up_pitch: int, out: int, out_pitch: int, dtype: int,
+                  scratch: int, scratch_nbytes: int, stream: int) -> None:
+    """grouped_gemm_dgrad_launch (`dtype` an enum value)."""
+    _check(load().grouped_gemm_dgrad_launch(dc, dc_pitch, b, b_pitch, b_stride, offs, experts, rows, n, k, gate_up,
+                                            gate_up_pitch, out, out_pitch, dtype, scratch, scratch_nbytes, stream),
+           "grouped_gemm_dgrad_launch")
+
+
+def grouped_wgrad(a: int, a_pitch: int, dc: int, dc_pitch: int, offs: int, experts: int, rows: int, n: int, k: int,
+                  db: int, db_pitch: int, db_stride: int, dtype: int, scratch: int, scratch_nbytes: int,
+                  stream: int) -> None:
+    """grouped_gemm_wgrad_launch (`dtype` an enum value)."""
+    _check(load().grouped_gemm_wgrad_launch(a, a_pitch, dc, dc_pitch, offs, experts, rows, n, k, db, db_pitch,
+                                            db_stride, dtype, scratch, scratch_nbytes, stream),
+           "grouped_gemm_wgrad_launch")
 
 
 # Size of the library's fixed scratch array (MGB_NOALLOC_SCRATCH_BYTES in the header).
