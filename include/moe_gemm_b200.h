@@ -364,6 +364,43 @@ int grouped_gemm_wgrad_launch(const void* a, int64_t a_pitch, const void* dc, in
                               int32_t experts, int64_t rows, int64_t n, int64_t k, void* db, int64_t db_pitch,
                               int64_t db_stride, int32_t dtype, void* scratch, size_t scratch_bytes, void* stream);
 
+/* e4m3 with power-of-two (e8m0) scales: block-scaled products whose scales the
+ * tensor core applies, and the quantisation to them.  No counterpart in the
+ * reference, which does not emulate the model's FP8 quantization
+ * (README.md:298); grouped_gemm_fp8_launch serves fp32 scales.
+ *
+ * quantize_rows_launch: for every row and 128-column block the smallest power
+ * of two s with max |x| <= 448 s over the block's finite values (1 for a block
+ * of zeros), q = x / s rounded to nearest even (infinities and NaNs become
+ * NaN).  x [rows, cols] fp16 / bf16 / fp32 with contiguous columns, q e4m3
+ * [rows, cols], scale e8m0 [rows, ceil(cols / 128)] contiguous. */
+int quantize_rows_launch(const void* x, int64_t rows, int64_t cols, int64_t pitch, int32_t dtype, void* q,
+                         int64_t q_pitch, void* scale, void* stream);
+
+/* The same with one scale per 128 x 128 block of each of `matrices` matrices,
+ * `stride` elements apart: q [matrices, rows, cols] and scale [matrices,
+ * ceil(rows / 128), ceil(cols / 128)], both contiguous. */
+int quantize_blocks_launch(const void* x, int64_t matrices, int64_t rows, int64_t cols, int64_t pitch, int64_t stride,
+                           int32_t dtype, void* q, void* scale, void* stream);
+
+size_t block_scaled_mm_scratch_bytes(int32_t experts);
+
+/* c[rows of e, :] = sum over 128-deep K blocks kb of
+ *   2^(sa[row, kb] - 127) 2^(sb[e, col / 128, kb] - 127) a[row, kb] b[e, col, kb]
+ * a e4m3 [rows, k], sa e8m0 [rows, ceil(k / 128)], b e4m3 [experts, n, k] (a
+ * linear weight as checkpoints store it), sb e8m0 [experts, ceil(n / 128),
+ * ceil(k / 128)], c bf16 [rows, n]; fp32 accumulation.  Segments as in
+ * gated_ffn_forward_launch (offs null: one segment of every row, experts 1).
+ * k a multiple of 16, n of 8; a, b and c 16-byte aligned with row pitches of
+ * whole 16 bytes; scales contiguous.  info->path 2: CTA pairs, 0: one CTA,
+ * 3: the kernel for few tokens per expert.  Scratch
+ * block_scaled_mm_scratch_bytes(experts), 128-byte aligned, not shared by
+ * launches that overlap. */
+int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const void* b, int64_t b_pitch,
+                           int64_t b_stride, const void* sb, void* c, int64_t c_pitch, const int32_t* offs,
+                           int32_t experts, int64_t rows, int64_t n, int64_t k, void* scratch, size_t scratch_bytes,
+                           void* stream, mgb_launch_info* info);
+
 /* Masked single GEMM C[m, n] = A[m, k] @ B[k, n] with arbitrary element strides.
  * Replaces the Triton launch of launch_matmul (kernels/matmul.py:332-392,
  * kernel _matmul_kernel_impl :223-273).  Operands that satisfy the TMA rules

@@ -555,9 +555,10 @@ bool current_launch_limits(int* sm_count, long long* wait_budget) {
 }
 
 bool encode_map_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch,
-                   uint32_t box_inner, uint32_t box_outer) {
+                   uint32_t box_inner, uint32_t box_outer, int swizzle_bytes) {
   return g_encode != nullptr &&
-         encode_2d(map, dtype, base, inner, outer, pitch, box_inner, box_outer, CU_TENSOR_MAP_SWIZZLE_128B);
+         encode_2d(map, dtype, base, inner, outer, pitch, box_inner, box_outer,
+                   swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 uint32_t* current_error_word() {

@@ -64,13 +64,13 @@ uint32_t* current_error_word();
 // (mgb_set_debug); false when the CUDA runtime cannot resolve them.
 bool current_launch_limits(int* sm_count, long long* wait_budget);
 
-// 2-D row-major tensor map with the 128-byte swizzle: `inner` contiguous
+// 2-D row-major tensor map with the 128- or 64-byte swizzle: `inner` contiguous
 // elements per row, `outer` rows, `pitch` bytes between rows, boxes of
 // box_inner x box_outer.  `dtype` is an mgb_dtype, or kMapBytes8 for bytes.
 // current_launch_limits must have succeeded before.
 constexpr int kMapBytes8 = 100;
 bool encode_map_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch,
-                   uint32_t box_inner, uint32_t box_outer);
+                   uint32_t box_inner, uint32_t box_outer, int swizzle_bytes = 128);
 
 // Launches simt_grouped_kernel<T>; returns a cudaError_t value.
 template <typename T>

@@ -1,0 +1,245 @@
+// Host side of the e8m0 block-scaled products and quantisation
+// (mgb_mx_kernel.cuh): argument checks, the choice of kernel, launches.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/moe_gemm_b200.h"
+#include "mgb_dispatch.cuh"
+#include "mgb_mx_kernel.cuh"
+
+namespace {
+
+using namespace mgb;
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+template <int G>
+int launch_mx(const MxParams& p, int64_t tiles, int sm_count, cudaStream_t stream) {
+  using Cfg = MxCfg<G>;
+  static bool configured[128] = {};
+  static int clusters[128] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return MGB_ERR_CUDA;
+  cudaLaunchAttribute attr[2] = {};
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kMxThreads, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = G;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(mx_kernel<G>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) !=
+        cudaSuccess) {
+      return MGB_ERR_CUDA;
+    }
+    clusters[dev] = sm_count / G;
+    if (G == 2) {
+      cfg.gridDim = dim3(static_cast<unsigned>(sm_count & ~1), 1, 1);
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, mx_kernel<G>, &cfg) == cudaSuccess && n > 0) {
+        clusters[dev] = n;
+      } else {
+        cudaGetLastError();
+      }
+    }
+    configured[dev] = true;
+  }
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(tiles, clusters[dev]));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid * G), 1, 1);
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, mx_kernel<G>, p) == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
+}
+
+template <typename T>
+int rows_typed(const void* x, int64_t rows, int64_t cols, int64_t pitch, void* q, int64_t q_pitch, void* scale, int sms,
+               cudaStream_t s) {
+  const int64_t blocks = rows * cdiv(cols, 128);
+  const int grid = static_cast<int>(std::min<int64_t>(cdiv(blocks, 16), 8ll * sms));
+  const bool vec = aligned(x, 16) && pitch % (16 / static_cast<int>(sizeof(T))) == 0 && cols % 8 == 0 && aligned(q, 8) &&
+                   q_pitch % 8 == 0;
+  const T* in = static_cast<const T*>(x);
+  uint8_t* out = static_cast<uint8_t*>(q);
+  uint8_t* sc = static_cast<uint8_t*>(scale);
+  if (vec) {
+    quantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(in, rows, cols, pitch, out, q_pitch, sc);
+  } else {
+    quantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(in, rows, cols, pitch, out, q_pitch, sc);
+  }
+  return cudaGetLastError() == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
+}
+
+template <typename T>
+int blocks_typed(const void* x, int64_t matrices, int64_t rows, int64_t cols, int64_t pitch, int64_t stride, void* q,
+                 void* scale, cudaStream_t s) {
+  const int64_t kb = cdiv(cols, 128), per = cdiv(rows, 128) * kb;
+  if (matrices * per >= (1ll << 31)) return MGB_ERR_INVALID;
+  const int e = 16 / static_cast<int>(sizeof(T));
+  const bool vec = aligned(x, 16) && pitch % e == 0 && stride % e == 0 && cols % 8 == 0 && aligned(q, 8);
+  const unsigned grid = static_cast<unsigned>(matrices * per);
+  const T* in = static_cast<const T*>(x);
+  uint8_t* out = static_cast<uint8_t*>(q);
+  uint8_t* sc = static_cast<uint8_t*>(scale);
+  if (vec) {
+    quantize_blocks_kernel<T, true><<<grid, 256, 0, s>>>(in, rows, cols, pitch, stride, out, cols, rows * cols, sc, kb, per);
+  } else {
+    quantize_blocks_kernel<T, false><<<grid, 256, 0, s>>>(in, rows, cols, pitch, stride, out, cols, rows * cols, sc, kb, per);
+  }
+  return cudaGetLastError() == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
+}
+
+// Average rows of an expert up to which the weight-streaming kernel runs
+// (dense: the rows), and the tokens it takes per pass over its weight rows.
+constexpr int64_t kFewRows = 32;
+
+}  // namespace
+
+extern "C" {
+
+size_t block_scaled_mm_scratch_bytes(int32_t experts) {
+  if (experts <= 0) return 0;
+  return static_cast<size_t>(experts) * 3 * sizeof(CUtensorMap) +
+         (static_cast<size_t>(experts) + 1 + 15) / 16 * 16 * sizeof(int64_t);
+}
+
+int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const void* b, int64_t b_pitch,
+                           int64_t b_stride, const void* sb, void* c, int64_t c_pitch, const int32_t* offs,
+                           int32_t experts, int64_t rows, int64_t n, int64_t k, void* scratch, size_t scratch_bytes,
+                           void* stream, mgb_launch_info* info) {
+  if (experts <= 0 || experts > (1 << 20) || rows < 0 || rows >= (1ll << 31) || n <= 0 || n >= (1ll << 31) || k <= 0 ||
+      k >= (1ll << 31) || k % 16 != 0 || n % 8 != 0 || (offs == nullptr && experts != 1)) {
+    return MGB_ERR_INVALID;
+  }
+  if ((rows > 0 && (a == nullptr || sa == nullptr || c == nullptr)) || b == nullptr || sb == nullptr ||
+      !aligned(a, 16) || !aligned(b, 16) || !aligned(c, 16) || a_pitch < k || a_pitch % 16 != 0 || b_pitch < k ||
+      b_pitch % 16 != 0 || b_stride % 16 != 0 || (experts > 1 && b_stride < (n - 1) * b_pitch + k) || c_pitch < n ||
+      c_pitch % 8 != 0) {
+    return MGB_ERR_INVALID;
+  }
+  if (scratch == nullptr || !aligned(scratch, 128) || scratch_bytes < block_scaled_mm_scratch_bytes(experts)) {
+    return MGB_ERR_SCRATCH;
+  }
+  int sms = 0;
+  MxParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.error_word = current_error_word();
+  if (p.error_word == nullptr || !current_launch_limits(&sms, &p.wait_budget)) return MGB_ERR_CUDA;
+  if (info != nullptr) std::memset(info, 0, sizeof(*info));
+  if (rows == 0) return MGB_OK;
+  p.a = static_cast<const uint8_t*>(a);
+  p.sa = static_cast<const uint8_t*>(sa);
+  p.b = static_cast<const uint8_t*>(b);
+  p.sb = static_cast<const uint8_t*>(sb);
+  p.c = static_cast<__nv_bfloat16*>(c);
+  p.a_pitch = a_pitch;
+  p.b_pitch = b_pitch;
+  p.b_stride = b_stride;
+  p.c_pitch = c_pitch;
+  p.offs = offs;
+  p.experts = experts;
+  p.rows = rows;
+  p.n = n;
+  p.k = k;
+  p.kb = cdiv(k, 128);
+  p.nb = cdiv(n, 128);
+  p.scale_words = p.kb % 4 == 0 && aligned(sa, 4) && aligned(sb, 4);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t each = cdiv(rows, experts);
+  const int64_t groups = cdiv(n, 16) * experts;
+  if (each <= kFewRows && groups < (1ll << 31)) {
+    const unsigned grid = static_cast<unsigned>(groups);
+    const int nt = each <= 8 ? 1 : each <= 16 ? 2 : 4;
+    if (nt == 1) {
+      mx_few_kernel<1><<<grid, kFewWarps * 32, 0, s>>>(p);
+    } else if (nt == 2) {
+      mx_few_kernel<2><<<grid, kFewWarps * 32, 0, s>>>(p);
+    } else {
+      mx_few_kernel<4><<<grid, kFewWarps * 32, 0, s>>>(p);
+    }
+    if (info != nullptr) {
+      info->path = 3;
+      info->swap_ab = 1;
+      info->tile_m = 8 * nt;
+      info->tile_n = 16;
+      info->tile_k = 128;
+      info->grid = static_cast<int32_t>(grid);
+    }
+    return cudaGetLastError() == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
+  }
+  // Pairs' 256 x 224 tiles where experts fill 256 rows and the tiles the
+  // device; else one CTA's 128 x 128 tiles.
+  const int64_t pair_tiles = (cdiv(rows, 256) + experts - 1) * cdiv(n, MxCfg<2>::kTileN);
+  const bool pair = each > 192 && pair_tiles >= sms / 2;
+  p.tile_rows = pair ? MxCfg<2>::kTileM : MxCfg<1>::kTileM;
+  p.tile_cols = pair ? MxCfg<2>::kTileN : MxCfg<1>::kTileN;
+  p.maps = static_cast<uint8_t*>(scratch);
+  p.tile_start = reinterpret_cast<int64_t*>(p.maps + static_cast<size_t>(experts) * 3 * sizeof(CUtensorMap));
+  MxTemplates tmpl;
+  if (!encode_map_2d(&tmpl.map[0], kMapBytes8, a, k, rows, a_pitch, 128, 128) ||
+      !encode_map_2d(&tmpl.map[1], kMapBytes8, b, k, n, b_pitch, 128, pair ? MxCfg<2>::kColsCta : MxCfg<1>::kColsCta) ||
+      !encode_map_2d(&tmpl.map[2], MGB_BF16, c, n, rows, c_pitch * 2, 32, 32, 64)) {
+    return MGB_ERR_CUDA;
+  }
+  mx_plan_kernel<<<static_cast<unsigned>(experts) + 1, 32, 0, s>>>(tmpl, p);
+  if (cudaGetLastError() != cudaSuccess) return MGB_ERR_CUDA;
+  const int64_t tiles = (cdiv(rows, p.tile_rows) + experts - 1) * cdiv(n, p.tile_cols);
+  if (info != nullptr) {
+    info->path = pair ? 2 : 0;
+    info->tile_m = p.tile_rows;
+    info->tile_n = p.tile_cols;
+    info->tile_k = 128;
+    info->stages = pair ? MxCfg<2>::kStages : MxCfg<1>::kStages;
+    info->grid = static_cast<int32_t>(std::min<int64_t>(tiles, sms));
+  }
+  return pair ? launch_mx<2>(p, tiles, sms, s) : launch_mx<1>(p, tiles, sms, s);
+}
+
+int quantize_rows_launch(const void* x, int64_t rows, int64_t cols, int64_t pitch, int32_t dtype, void* q,
+                         int64_t q_pitch, void* scale, void* stream) {
+  if (rows < 0 || cols <= 0 || pitch < cols || q_pitch < cols || (rows > 0 && (x == nullptr || q == nullptr || scale == nullptr))) {
+    return MGB_ERR_INVALID;
+  }
+  if (dtype != MGB_FP16 && dtype != MGB_BF16 && dtype != MGB_FP32) return MGB_ERR_INVALID;
+  if (!aligned(x, dtype == MGB_FP32 ? 4 : 2)) return MGB_ERR_INVALID;
+  int sms = 0;
+  long long budget = 0;
+  if (!current_launch_limits(&sms, &budget)) return MGB_ERR_CUDA;
+  if (rows == 0) return MGB_OK;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case MGB_FP16: return rows_typed<__half>(x, rows, cols, pitch, q, q_pitch, scale, sms, s);
+    case MGB_BF16: return rows_typed<__nv_bfloat16>(x, rows, cols, pitch, q, q_pitch, scale, sms, s);
+    default: return rows_typed<float>(x, rows, cols, pitch, q, q_pitch, scale, sms, s);
+  }
+}
+
+int quantize_blocks_launch(const void* x, int64_t matrices, int64_t rows, int64_t cols, int64_t pitch, int64_t stride,
+                           int32_t dtype, void* q, void* scale, void* stream) {
+  if (matrices < 0 || rows <= 0 || cols <= 0 || pitch < cols || (matrices > 0 && (x == nullptr || q == nullptr || scale == nullptr))) {
+    return MGB_ERR_INVALID;
+  }
+  if (dtype != MGB_FP16 && dtype != MGB_BF16 && dtype != MGB_FP32) return MGB_ERR_INVALID;
+  if (!aligned(x, dtype == MGB_FP32 ? 4 : 2)) return MGB_ERR_INVALID;
+  if (matrices == 0) return MGB_OK;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case MGB_FP16: return blocks_typed<__half>(x, matrices, rows, cols, pitch, stride, q, scale, s);
+    case MGB_BF16: return blocks_typed<__nv_bfloat16>(x, matrices, rows, cols, pitch, stride, q, scale, s);
+    default: return blocks_typed<float>(x, matrices, rows, cols, pitch, stride, q, scale, s);
+  }
+}
+
+}  // extern "C"

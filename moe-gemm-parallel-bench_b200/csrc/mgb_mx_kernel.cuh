@@ -1,0 +1,859 @@
+// e4m3 products with power-of-two block scales, and the quantisation to them.
+//
+//   C[m, n] = sum_kb 2^(sa[m, kb] - 127) 2^(sb[n / 128, kb] - 127) sum_{k in kb} A[m, k] B[n, k]
+//
+// over 128-deep K blocks kb; scales are e8m0 bytes (byte 255 is NaN).  The
+// sm_100 block-scaled MMA (tcgen05.mma kind::mxf8f6f4.block_scale) applies one
+// such byte per row and 32 K inside the tensor core, so a 128-deep block is
+// four MMAs that name the same byte and the accumulator stays in TMEM for all
+// of K: no partial is read back and scaled in registers, which is what bounds
+// the fp32-scaled path (mgb_fp8_kernel.cuh).
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "mgb_tc_kernel.cuh"
+
+namespace mgb {
+
+// ------------------------------------------------------------ quantisation
+// Exponent byte of the smallest power of two s with amax <= 448 s (clamped to
+// the format; 1 for a block of zeros).  amax = 1.f 2^(E - 127): 448 = 1.75 2^8,
+// so s = 2^(E - 127 - 8), doubled when 1.f > 1.75.
+__device__ __forceinline__ int scale_byte(uint32_t amax_bits) {
+  if (amax_bits == 0) return 127;
+  const int e = static_cast<int>(amax_bits >> 23) - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return e < 0 ? 0 : e > 254 ? 254 : e;
+}
+
+// 2^(127 - byte): what an element is multiplied by (exact: a power of two).
+__device__ __forceinline__ float inverse_scale(int byte) {
+  const int b = 254 - byte;
+  return __uint_as_float(b > 0 ? static_cast<uint32_t>(b) << 23 : 0x00400000u);
+}
+
+// 2^(byte - 127); byte 255 is NaN.
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
+}
+
+// |v| as bits, 0 for infinities and NaNs: the scale goes by the finite values.
+__device__ __forceinline__ uint32_t finite_abs(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+  return b >= 0x7F800000u ? 0u : b;
+}
+
+// Two e4m3 values, round to nearest even; infinities and NaNs become NaN.
+__device__ __forceinline__ uint32_t e4m3_pair(float a, float b, float inv) {
+  const float nan = __uint_as_float(0x7FC00000u);
+  a = isinf(a) ? nan : a * inv;
+  b = isinf(b) ? nan : b * inv;
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+  if constexpr (std::is_same<T, float>::value) {
+    return v;
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return __bfloat162float(v);
+  } else {
+    return __half2float(v);
+  }
+}
+
+// Eight consecutive elements from column `col`; columns past `cols` are 0.
+// VEC: the address is 16-byte aligned and the eight lie inside the row.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int64_t col, int64_t cols, float (&v)[8]) {
+  if constexpr (VEC) {
+    alignas(16) T raw[8];
+    if (col < cols) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+        reinterpret_cast<uint4*>(raw)[i] = __ldcs(reinterpret_cast<const uint4*>(row + col) + i);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = to_float(raw[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? to_float(row[col + i]) : 0.0f;
+  }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store8(uint8_t* row, int64_t col, int64_t cols, const float (&v)[8], float inv) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = e4m3_pair(v[2 * i], v[2 * i + 1], inv);
+  if constexpr (VEC) {
+    if (col < cols) {
+      *reinterpret_cast<uint2*>(row + col) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (col + i < cols) row[col + i] = static_cast<uint8_t>(w[i / 2] >> (8 * (i % 2)));
+    }
+  }
+}
+
+// Rows: 16 lanes hold one 1 x 128 block (8 elements each), so a warp's loads
+// are whole 256-byte pieces; kRowsUnroll blocks per half warp are in flight.
+constexpr int kRowsUnroll = 4;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
+                                                            int64_t pitch, uint8_t* __restrict__ q, int64_t q_pitch,
+                                                            uint8_t* __restrict__ scale) {
+  const int64_t kb = (cols + 127) / 128;
+  const int64_t blocks = rows * kb;
+  const int l = threadIdx.x & 15;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 16;
+  for (int64_t b0 = blockIdx.x * 16ll + (threadIdx.x >> 4); b0 < blocks; b0 += stride * kRowsUnroll) {
+    float v[kRowsUnroll][8];
+    int64_t row[kRowsUnroll], col[kRowsUnroll];
+#pragma unroll
+    for (int u = 0; u < kRowsUnroll; ++u) {
+      const int64_t b = b0 + u * stride;
+      row[u] = b < blocks ? b / kb : -1;
+      col[u] = b < blocks ? (b - row[u] * kb) * 128 + l * 8 : 0;
+      if (row[u] >= 0) {
+        load8<T, VEC>(x + row[u] * pitch, col[u], cols, v[u]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRowsUnroll; ++u) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, finite_abs(v[u][i]));
+      // The 16 lanes of a block take every branch together; the other half
+      // warp may be past the end, so the shuffle names its own half only.
+      const uint32_t half = 0xFFFFu << (threadIdx.x & 16);
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(half, top, d));
+      if (row[u] >= 0) {
+        const int byte = scale_byte(top);
+        store8<VEC>(q + row[u] * q_pitch, col[u], cols, v[u], inverse_scale(byte));
+        if (l == 0) scale[row[u] * kb + col[u] / 128] = static_cast<uint8_t>(byte);
+      }
+    }
+  }
+}
+
+// Blocks: one CTA per 128 x 128 block, its 16384 elements in registers (16
+// threads by 8 elements across, 16 rows per step), one pass over memory.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
+                                                              int64_t pitch, int64_t matrix, uint8_t* __restrict__ q,
+                                                              int64_t q_pitch, int64_t q_matrix,
+                                                              uint8_t* __restrict__ scale, int64_t kb, int64_t per) {
+  __shared__ uint32_t tops[8];
+  const int64_t e = blockIdx.x / per, in = blockIdx.x - e * per;
+  const int64_t r0 = in / kb * 128, c = (in - in / kb * kb) * 128 + (threadIdx.x & 15) * 8;
+  const T* base = x + e * matrix;
+  float v[8][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = r0 + i * 16 + (threadIdx.x >> 4);
+    if (r < rows) {
+      load8<T, VEC>(base + r * pitch, c, cols, v[i]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = max(top, finite_abs(v[i][k]));
+  }
+  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
+  const int byte = scale_byte(top);
+  const float inv = inverse_scale(byte);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = r0 + i * 16 + (threadIdx.x >> 4);
+    if (r < rows) store8<VEC>(q + e * q_matrix + r * q_pitch, c, cols, v[i], inv);
+  }
+  if (threadIdx.x == 0) scale[blockIdx.x] = static_cast<uint8_t>(byte);
+}
+
+// ------------------------------------------------------------------ product
+struct MxParams {
+  const uint8_t* a;   // [rows, k]
+  const uint8_t* sa;  // [rows, kb]
+  const uint8_t* b;   // [experts, n, k]
+  const uint8_t* sb;  // [experts, nb, kb]
+  __nv_bfloat16* c;   // [rows, n]
+  int64_t a_pitch, b_pitch, b_stride, c_pitch;  // elements
+  const int32_t* offs;
+  int32_t experts;
+  int64_t rows, n, k;
+  int64_t kb, nb;       // scale columns and rows: ceil(k / 128), ceil(n / 128)
+  int32_t scale_words;  // scale rows are whole, aligned 32-bit words
+  uint8_t* maps;        // [experts][3] tensor maps: A, B, C
+  int64_t* tile_start;  // [experts + 1]
+  int32_t tile_rows, tile_cols;
+  long long wait_budget;
+  uint32_t* error_word;
+};
+
+__device__ __forceinline__ int64_t mx_segment(const MxParams& p, int e, int64_t& start, bool* bad = nullptr) {
+  if (p.offs == nullptr) {
+    start = 0;
+    return p.rows;
+  }
+  const int64_t lo = e > 0 ? p.offs[e - 1] : 0, hi = p.offs[e];
+  if (bad != nullptr) *bad = lo < 0 || hi < lo || hi > p.rows;
+  start = lo < 0 ? 0 : lo > p.rows ? p.rows : lo;
+  const int64_t end = hi < start ? start : hi > p.rows ? p.rows : hi;
+  return end - start;
+}
+
+struct MxTemplates {
+  CUtensorMap map[3];
+};
+
+// Tensor maps of every expert, one warp each, and the tiles' prefix sums (last block).
+__global__ void __launch_bounds__(32)
+    mx_plan_kernel(const __grid_constant__ MxTemplates tmpl, const __grid_constant__ MxParams p) {
+  __shared__ alignas(128) CUtensorMap staging[3];
+  const int lane = threadIdx.x;
+  grid_launch_dependents();
+  if (blockIdx.x == p.experts) {
+    const int per = (p.experts + 31) / 32;
+    const int lo = lane * per, hi = lo + per < p.experts ? lo + per : p.experts;
+    const int64_t n_blocks = ceil_div64(p.n, p.tile_cols);
+    auto tiles_of = [&](int e) -> int64_t {
+      int64_t start;
+      return ceil_div64(mx_segment(p, e, start), p.tile_rows) * n_blocks;
+    };
+    int64_t sum = 0;
+    for (int e = lo; e < hi; ++e) sum += tiles_of(e);
+    int64_t incl = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += v;
+    }
+    int64_t run = incl - sum;
+    for (int e = lo; e < hi; ++e) {
+      p.tile_start[e] = run;
+      run += tiles_of(e);
+    }
+    if (lane == 31) p.tile_start[p.experts] = incl;
+    return;
+  }
+  const int e = blockIdx.x;
+  bool bad = false;
+  int64_t start = 0;
+  const int64_t len = mx_segment(p, e, start, &bad);
+  if (bad && lane == 0) atomicOr(p.error_word, kErrBadDims);
+  if (lane < 3) {
+    const uint4* src = reinterpret_cast<const uint4*>(&tmpl.map[lane]);
+    uint4* dst = reinterpret_cast<uint4*>(&staging[lane]);
+    for (int i = 0; i < 8; ++i) dst[i] = src[i];
+    if (lane == 1) {
+      tmap_replace_address(&staging[1], p.b + e * p.b_stride);
+    } else if (len > 0) {  // an empty segment's maps are never used
+      tmap_replace_address(&staging[lane], lane == 0 ? static_cast<const void*>(p.a + start * p.a_pitch)
+                                                     : static_cast<const void*>(p.c + start * p.c_pitch));
+      tmap_replace_dim(&staging[lane], 1, static_cast<uint32_t>(len));
+    }
+  }
+  __syncwarp();
+  CUtensorMap* g = reinterpret_cast<CUtensorMap*>(p.maps) + static_cast<int64_t>(e) * 3;
+  for (int i = 0; i < 3; ++i) tmap_publish(&g[i], &staging[i]);
+}
+
+struct MxWalk {
+  int e = -1;
+  int64_t first = 0, end = 0, len = 0, start = 0, m_blocks = 1;
+
+  __device__ __forceinline__ bool seek(const MxParams& p, int64_t t) {
+    const int64_t* ts = p.tile_start;
+    if (t >= end || e < 0) {
+      if (t >= ts[p.experts]) return false;
+      int lo = e < 0 ? 0 : e, hi = p.experts - 1;
+      while (lo < hi) {  // empty experts share their successor's first tile
+        const int mid = (lo + hi + 1) >> 1;
+        if (ts[mid] <= t) {
+          lo = mid;
+        } else {
+          hi = mid - 1;
+        }
+      }
+      e = lo;
+      first = ts[lo];
+      end = ts[lo + 1];
+      len = mx_segment(p, lo, start);
+      m_blocks = ceil_div64(len, p.tile_rows);
+    }
+    return true;
+  }
+  __device__ __forceinline__ void blocks(int64_t t, int64_t& mb, int64_t& nb) const {
+    const int64_t local = t - first;
+    const int64_t band_tiles = 8 * ((end - first) / m_blocks);
+    const int64_t band = local / band_tiles;
+    const int64_t in = local - band * band_tiles;
+    const int64_t rows_in = m_blocks - band * 8 < 8 ? m_blocks - band * 8 : 8;
+    mb = band * 8 + in % rows_in;
+    nb = in / rows_in;
+  }
+};
+
+// D[tmem] (+)= (A 2^sa) (B 2^sb), e4m3 operands, one e8m0 scale per row and 32 K.
+template <int G>
+__device__ __forceinline__ void mma_mx(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                       uint32_t sfb, uint32_t accumulate) {
+  if constexpr (G == 2) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// 32 rows x 16 bytes of shared memory into 4 TMEM columns, repeated for the
+// four lane quarters (the layout in which the MMA reads scales).
+template <int G>
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+  if constexpr (G == 2) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  } else {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  }
+}
+
+// Instruction descriptor of the block-scaled MMA: e4m3 operands (format 0),
+// both K-major, e8m0 scales (bit 23); `byte` names the scale byte of a
+// 32-bit TMEM word for both operands.
+__host__ __device__ constexpr uint32_t instr_desc_mx(uint32_t m, uint32_t n, uint32_t byte) {
+  return (byte << 4) | ((n >> 3) << 17) | (1u << 23) | ((m >> 7) << 27) | (byte << 29);
+}
+
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, long long budget,
+                                                  volatile int* abort) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const long long start = clock64();
+  while (true) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    if (*abort || clock64() - start > budget) return false;
+  }
+}
+
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// Tile: 256 x 224 for a pair, 128 x 128 for one CTA.  Two accumulators and the
+// scale words share the 512 TMEM columns: 2 x 224 + 2 x 12 for a pair (N = 256
+// would leave none for the scales), 2 x 128 + 2 x 8 for one CTA.
+template <int G>
+struct MxCfg {
+  static constexpr int kBK = 128;
+  static constexpr int kColsCta = G == 2 ? 112 : 128;  // weight rows a CTA loads
+  static constexpr int kTileM = 128 * G, kTileN = kColsCta * G;
+  static constexpr int kABytes = 128 * 128, kBBytes = kColsCta * 128;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kScaleAtoms = 1 + G;           // 128 rows x 4 bytes each: A, then B's 128-row groups
+  static constexpr int kScaleBytes = kScaleAtoms * 512;  // one slot: four K blocks
+  static constexpr int kScaleCols = 4 * kScaleAtoms;
+  static constexpr int kTmemCols = 512;
+  static constexpr int kScaleTmem = 2 * kTileN;  // first scale column
+  static constexpr int kEpiBlocks = 2;
+  static constexpr int kEpiBytes = 4 * kEpiBlocks * kEpiWarpBytes;
+  static constexpr int kStages = (kTcSmemBudget - kEpiBytes - 2 * kScaleBytes) / kStageBytes;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + 2 * kScaleBytes + 2048 + 1024;
+  static_assert(kStageBytes % 1024 == 0 && kABytes % 1024 == 0, "swizzle atoms");
+  static_assert(kScaleTmem + 2 * kScaleCols <= kTmemCols, "TMEM columns");
+  static_assert(kSmemBytes <= 232448 && kStages >= 4, "shared memory");
+};
+
+constexpr int kMxThreads = 256;
+
+// Warps: 0 TMA producer, 1 MMA issuer, 2 scales, 3 idle, 4-7 epilogue.
+// Scales: warp 2 gathers the bytes of four K blocks (one 32-bit word per row)
+// into the slot's 512-byte atoms, row j 32 + l at byte 16 l + 4 j; the issuer
+// copies them to TMEM and names byte kb % 4 in the MMAs of K block kb.  A
+// slot (its shared memory and its TMEM columns) is free again when the MMAs
+// of its four K blocks are done.
+template <int G>
+__global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant__ MxParams p) {
+  using Cfg = MxCfg<G>;
+  constexpr int S = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem;
+  uint8_t* epi_stage = smem + S * Cfg::kStageBytes;
+  uint8_t* scales = epi_stage + Cfg::kEpiBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + 2 * Cfg::kScaleBytes);
+  uint64_t* empty = full + S;
+  uint64_t* sf_full = empty + S;
+  uint64_t* sf_empty = sf_full + 2;
+  uint64_t* acc_full = sf_empty + 2;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drain_bar = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* never = abort + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = G == 2 ? cluster_ctarank() : 0u;
+  const bool leader = rank == 0;
+  const int64_t first_item = blockIdx.x / G;
+  const int64_t items_step = gridDim.x / G;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sf_full[b], G);
+      mbar_init(&sf_empty[b], 1);
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4 * G);
+    }
+    mbar_init(drain_bar, 1);
+    *abort = 0;
+    *never = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if constexpr (G == 2) {
+      tmem_alloc_pair(tmem_slot, Cfg::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, Cfg::kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (G == 2) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const long long budget = p.wait_budget;
+  grid_dependency_wait();
+  const CUtensorMap* all_maps = reinterpret_cast<const CUtensorMap*>(p.maps);
+  const int64_t kblocks = p.kb;
+
+  auto fail = [&](uint32_t bits) {
+    atomicOr(p.error_word, bits);
+    *abort = 1;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    const uint64_t pol_keep = policy_evict_last(), pol_shared = policy_evict_normal(), pol_stream = policy_evict_first();
+    MxWalk walk;
+    uint32_t it = 0;
+    int built = -1;
+    bool ok = true;
+    for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+      int64_t mb, nb;
+      walk.blocks(t, mb, nb);
+      const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.e) * 3;
+      if (walk.e != built) {
+        if (lane == 0) {
+          tmap_acquire(&g[0]);
+          tmap_acquire(&g[1]);
+        }
+        __syncwarp();
+        built = walk.e;
+      }
+      const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128);
+      const int32_t n0 = static_cast<int32_t>(nb * Cfg::kTileN + rank * Cfg::kColsCta);
+      const uint64_t pol_b = walk.m_blocks == 1 ? pol_stream : pol_shared;
+      for (int64_t kb = 0; kb < kblocks; ++kb) {
+        const int s = static_cast<int>(it % S);
+        if (!mbar_wait_warp(&empty[s], ((it / S) & 1u) ^ 1u, budget, abort)) {
+          if (lane == 0) fail(kErrWaitEmpty);
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          uint8_t* st = ring + s * Cfg::kStageBytes;
+          const int32_t kx = static_cast<int32_t>(kb * Cfg::kBK);
+          if (leader) mbar_arrive_expect_tx(&full[s], G * Cfg::kStageBytes);
+          if constexpr (G == 2) {
+            const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+            tma_load_2d_pair(&g[0], bar, st, kx, m0, pol_keep);
+            tma_load_2d_pair(&g[1], bar, st + Cfg::kABytes, kx, n0, pol_b);
+          } else {
+            tma_load_2d(&g[0], &full[s], st, kx, m0, pol_keep);
+            tma_load_2d(&g[1], &full[s], st + Cfg::kABytes, kx, n0, pol_b);
+          }
+        }
+        __syncwarp();
+        ++it;
+      }
+    }
+    if (*abort && leader && lane == 0) {
+      for (uint32_t i = it > static_cast<uint32_t>(S) ? it - S : 0u; i < it; ++i) {
+        if (!mbar_wait(&full[i % S], (i / S) & 1u, budget, never)) {
+          atomicOr(p.error_word, kErrWaitTeardown);
+          break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ MMA issuer (leader only)
+    if (lane == 0 && leader) {
+      MxWalk walk;
+      uint32_t it = 0, acc_it = 0, sf_it = 0;
+      bool ok = true;
+      const uint64_t a_desc = smem_desc(smem_u32(ring), 16, 1024, kLayoutSw128);
+      const uint64_t b_desc = smem_desc(smem_u32(ring) + Cfg::kABytes, 16, 1024, kLayoutSw128);
+      // Scale atoms: no swizzle, 8-row groups of 16-byte rows 128 bytes apart.
+      const uint64_t s_desc = smem_desc(smem_u32(scales), 0, 128, 0);
+      for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+        const int buf = static_cast<int>(acc_it & 1);
+        if (!mbar_wait(&acc_empty[buf], ((acc_it >> 1) & 1u) ^ 1u, budget, abort)) {
+          fail(kErrWaitAccEmpty);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem_base + buf * Cfg::kTileN;
+        for (int64_t kb = 0; kb < kblocks; ++kb) {
+          const int slot = static_cast<int>(sf_it & 1);
+          const uint32_t sf = tmem_base + Cfg::kScaleTmem + slot * Cfg::kScaleCols;
+          if ((kb & 3) == 0) {
+            if (!mbar_wait_cluster(&sf_full[slot], (sf_it >> 1) & 1u, budget, abort)) {
+              fail(kErrWaitFull);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int i = 0; i < Cfg::kScaleAtoms; ++i) {
+              tmem_copy_scales<G>(sf + 4 * i, s_desc + ((slot * Cfg::kScaleBytes + i * 512) >> 4));
+            }
+          }
+          const int s = static_cast<int>(it % S);
+          if (!mbar_wait(&full[s], (it / S) & 1u, budget, abort)) {
+            fail(kErrWaitFull);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t stage = static_cast<uint64_t>(s * (Cfg::kStageBytes >> 4));
+          const uint32_t idesc = instr_desc_mx(Cfg::kTileM, Cfg::kTileN, static_cast<uint32_t>(kb & 3));
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            mma_mx<G>(d, a_desc + stage + ks * 2, b_desc + stage + ks * 2, idesc, sf, sf + 4, (kb > 0 || ks > 0) ? 1u : 0u);
+          }
+          if constexpr (G == 2) {
+            mma_commit_pair(&empty[s], 0x3);
+          } else {
+            mma_commit(&empty[s]);
+          }
+          ++it;
+          if ((kb & 3) == 3 || kb == kblocks - 1) {
+            if constexpr (G == 2) {
+              mma_commit_pair(&sf_empty[slot], 0x3);
+            } else {
+              mma_commit(&sf_empty[slot]);
+            }
+            ++sf_it;
+          }
+        }
+        if (!ok) break;
+        if constexpr (G == 2) {
+          mma_commit_pair(&acc_full[buf], 0x3);
+        } else {
+          mma_commit(&acc_full[buf]);
+        }
+        ++acc_it;
+      }
+      if (*abort) {
+        if constexpr (G == 2) {
+          mma_commit_pair(drain_bar, 0x1);
+        } else {
+          mma_commit(drain_bar);
+        }
+        if (!mbar_wait(drain_bar, 0, budget, never)) atomicOr(p.error_word, kErrWaitTeardown);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // -------------------------------------------------------------- scales
+    MxWalk walk;
+    uint32_t sf_it = 0;
+    bool ok = true;
+    // Four consecutive bytes of a scale row from K block kb on; blocks past the end are 1.
+    const bool words = p.scale_words;
+    auto word = [&](const uint8_t* row, int64_t kb) -> uint32_t {
+      if (words) return __ldg(reinterpret_cast<const uint32_t*>(row + kb));
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w |= (kb + i < p.kb ? static_cast<uint32_t>(__ldg(row + kb + i)) : 127u) << (8 * i);
+      return w;
+    };
+    for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+      int64_t mb, nb;
+      walk.blocks(t, mb, nb);
+      const int64_t m0 = mb * Cfg::kTileM + rank * 128, n0 = nb * Cfg::kTileN;
+      const uint8_t* row[4 * Cfg::kScaleAtoms];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t m = m0 + j * 32 + lane;  // rows past the segment read its last row's scales: never stored
+        row[j] = p.sa + (walk.start + (m < walk.len ? m : walk.len - 1)) * p.kb;
+      }
+#pragma unroll
+      for (int j = 4; j < 4 * Cfg::kScaleAtoms; ++j) {
+        const int64_t n = n0 + (j - 4) * 32 + lane;
+        row[j] = p.sb + (walk.e * p.nb + (n < p.n ? n : p.n - 1) / 128) * p.kb;
+      }
+      for (int64_t kb = 0; kb < kblocks; kb += 4) {
+        const int slot = static_cast<int>(sf_it & 1);
+        uint32_t w[4 * Cfg::kScaleAtoms];
+#pragma unroll
+        for (int j = 0; j < 4 * Cfg::kScaleAtoms; ++j) w[j] = word(row[j], kb);  // in flight during the wait
+        if (!mbar_wait_warp(&sf_empty[slot], ((sf_it >> 1) & 1u) ^ 1u, budget, abort)) {
+          if (lane == 0) fail(kErrWaitEmpty);
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int i = 0; i < Cfg::kScaleAtoms; ++i) {
+          *reinterpret_cast<uint4*>(scales + slot * Cfg::kScaleBytes + i * 512 + lane * 16) =
+              make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
+        fence_proxy_async_smem();  // generic writes -> visible to the copy into TMEM
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(G == 2 ? mapa_shared(smem_u32(&sf_full[slot]), 0) : smem_u32(&sf_full[slot]));
+        ++sf_it;
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue
+    const int quarter = warp & 3;
+    uint8_t* blocks = epi_stage + quarter * Cfg::kEpiBlocks * kEpiWarpBytes;
+    const uint64_t pol_out = policy_evict_normal();
+    MxWalk walk;
+    uint32_t acc_it = 0, chunk_seq = 0;
+    int built = -1;
+    for (int64_t t = first_item; walk.seek(p, t); t += items_step) {
+      int64_t mb, nb;
+      walk.blocks(t, mb, nb);
+      const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.e) * 3;
+      if (walk.e != built) {
+        if (lane == 0) tmap_acquire(&g[2]);
+        __syncwarp();
+        built = walk.e;
+      }
+      const int buf = static_cast<int>(acc_it & 1);
+      if (!mbar_wait_warp(&acc_full[buf], (acc_it >> 1) & 1u, budget, abort)) {
+        if (lane == 0) fail(kErrWaitAccFull);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * Cfg::kTileN;
+      const int32_t row0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128 + quarter * 32);
+      const int32_t c0 = static_cast<int32_t>(nb * Cfg::kTileN);
+      if (row0 < walk.len) {
+        // Chunks of 32 columns (a 224-column tile is seven); the map clips C's edges.
+        const int64_t cols = p.n - c0 < Cfg::kTileN ? p.n - c0 : Cfg::kTileN;
+#pragma unroll 1
+        for (int c = 0; c * 32 < cols; ++c) {
+          uint8_t* block = blocks + (chunk_seq & 1) * kEpiWarpBytes;
+          if (lane == 0) bulk_wait_group_read<1>();
+          __syncwarp();
+          uint32_t v[32];
+          tmem_ld32(taddr + c * 32, v);
+          tmem_ld_wait();
+          // 32 rows x 64 bytes, 64-byte swizzle: 16-byte unit j of row r at j ^ ((r / 2) % 4).
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            *reinterpret_cast<uint4*>(block + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(pack_pair<__nv_bfloat16>(v[8 * j], v[8 * j + 1]), pack_pair<__nv_bfloat16>(v[8 * j + 2], v[8 * j + 3]),
+                           pack_pair<__nv_bfloat16>(v[8 * j + 4], v[8 * j + 5]),
+                           pack_pair<__nv_bfloat16>(v[8 * j + 6], v[8 * j + 7]));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&g[2], block, c0 + c * 32, row0, pol_out);
+            bulk_commit_group();
+          }
+          ++chunk_seq;
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (G == 2) {
+          mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&acc_empty[buf]), 0));
+        } else {
+          mbar_arrive_relaxed(&acc_empty[buf]);
+        }
+      }
+      ++acc_it;
+    }
+    if (lane == 0) bulk_wait_group_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (G == 2) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (G == 2) {
+      tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    } else {
+      tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    }
+  }
+}
+
+// -------------------------------------------------------------- few tokens
+// Decoding: at most a few tokens per expert, so the weights' bytes bound the
+// product and the tensor pipe idles whatever drives it.  The 128-row tiles
+// above would run on n / 128 SMs and stream the weights through too few of
+// them; here a CTA takes 16 weight rows and its 8 warps split K (interleaved
+// 128-deep blocks), so n / 16 CTAs stream with every load independent of the
+// others: no shared-memory ring, no barrier until the warps' sums are joined
+// in shared memory in warp order (the result does not depend on timing).
+// Weights are the 16-row operand of the warp-level m16n8k32 MMA, 8 NT tokens
+// its columns.  A lane loads 16 consecutive bytes of a row and uses them as
+// the fragments of two MMAs; weights and tokens are permuted along K alike, so
+// the sum is over the same products.  Each 128-deep block starts from zero and
+// is added to the fp32 sums times its two scales.
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int kFewWarps = 8;
+
+template <int NT>
+__global__ void __launch_bounds__(kFewWarps * 32) mx_few_kernel(const __grid_constant__ MxParams p) {
+  __shared__ float sums[kFewWarps][NT * 8][17];  // [warp][token][row], padded against bank conflicts
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int64_t n_groups = ceil_div64(p.n, 16);
+  const int e = static_cast<int>(blockIdx.x / n_groups);
+  const int64_t r0 = (blockIdx.x - e * n_groups) * 16;
+  int64_t start;
+  bool bad = false;
+  const int64_t len = mx_segment(p, e, start, &bad);
+  if (bad && r0 == 0 && threadIdx.x == 0) atomicOr(p.error_word, kErrBadDims);
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  const uint8_t* wrow[2];
+  bool live[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t r = r0 + g + 8 * h;
+    live[h] = r < p.n;
+    wrow[h] = p.b + e * p.b_stride + (live[h] ? r : 0) * p.b_pitch + t * 16;
+  }
+  const uint8_t* wscale = p.sb + (e * p.nb + r0 / 128) * p.kb;  // 16 rows lie inside one 128-row block
+  for (int64_t m0 = 0; m0 < len; m0 += 8 * NT) {
+    float acc[NT][4];
+    const uint8_t* xrow[NT];
+    bool has[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+      const int64_t m = m0 + i * 8 + g;
+      has[i] = m < len;
+      xrow[i] = p.a + (start + (has[i] ? m : 0)) * p.a_pitch + t * 16;
+    }
+#pragma unroll(NT <= 1 ? 4 : 2)
+    for (int64_t kb = warp; kb < p.kb; kb += kFewWarps) {
+      // K is a multiple of 16: a 16-byte piece is inside the row or past its end.
+      uint4 w[2][2], x[NT][2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int64_t k = kb * 128 + c * 64;
+        const bool in = k + t * 16 < p.k;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          w[h][c] = in && live[h] ? __ldcs(reinterpret_cast<const uint4*>(wrow[h] + k)) : zero;
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          x[i][c] = in && has[i] ? __ldg(reinterpret_cast<const uint4*>(xrow[i] + k)) : zero;
+        }
+      }
+      const float sw = scale_value(__ldg(wscale + kb));
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          mma_e4m3(part, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, x[i][c].x, x[i][c].y);
+          mma_e4m3(part, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, x[i][c].z, x[i][c].w);
+        }
+        // Columns 2t, 2t + 1 of the accumulator are tokens m0 + 8 i + 2t (+ 1).
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int64_t m = m0 + i * 8 + 2 * t + j;
+          const float sx = m < len ? scale_value(__ldg(p.sa + (start + m) * p.kb + kb)) : 0.0f;
+          acc[i][j] += part[j] * sw * sx;
+          acc[i][2 + j] += part[2 + j] * sw * sx;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        sums[warp][i * 8 + 2 * t + j][g] = acc[i][j];
+        sums[warp][i * 8 + 2 * t + j][g + 8] = acc[i][2 + j];
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * 128; i += kFewWarps * 32) {
+      const int row = i & 15, tok = i >> 4;
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) s += sums[w][tok][row];
+      const int64_t m = m0 + tok;
+      if (m < len && r0 + row < p.n) p.c[(start + m) * p.c_pitch + r0 + row] = __float2bfloat16_rn(s);
+    }
+    __syncthreads();  // the sums are rewritten by the next tokens
+  }
+}
+
+}  // namespace mgb

@@ -26,6 +26,12 @@ from .fp8 import (
     quantize_activations,
     quantize_weight,
 )
+from .fp8_blocks import (
+    last_block_scaled_info,
+    launch_block_scaled_mm,
+    launch_quantize_blocks,
+    launch_quantize_rows,
+)
 from .gated_ffn import (
     gated_ffn_backward,
     gated_ffn_forward,
@@ -42,6 +48,10 @@ from .matmul import (
 )
 
 __all__ = [
+    "last_block_scaled_info",
+    "launch_block_scaled_mm",
+    "launch_quantize_blocks",
+    "launch_quantize_rows",
     "gated_ffn_backward",
     "gated_ffn_forward",
     "launch_grouped_mm_dgrad",

@@ -49,6 +49,10 @@ EXPORTED_SYMBOLS = (
     "moe_ep_combine",
     "grouped_gemm_fp8_launch",
     "grouped_gemm_launch_noalloc",
+    "quantize_rows_launch",
+    "quantize_blocks_launch",
+    "block_scaled_mm_scratch_bytes",
+    "block_scaled_mm_launch",
     "ffn_scratch_bytes",
     "gated_ffn_forward_launch",
     "gated_ffn_backward_launch",
@@ -108,7 +112,7 @@ class LaunchInfo(ctypes.Structure):
 
     def as_dict(self) -> dict[str, int | str]:
         return {
-            "path": {0: "tcgen05_tma", 1: "simt_generic", 2: "tcgen05_tma_pair"}.get(int(self.path), "unknown"),
+            "path": {0: "tcgen05_tma", 1: "simt_generic", 2: "tcgen05_tma_pair", 3: "warp_mma"}.get(int(self.path), "unknown"),
             "swap_ab": int(self.swap_ab),
             "tile_m": int(self.tile_m),
             "tile_n": int(self.tile_n),
@@ -278,6 +282,15 @@ def _declare(lib) -> None:
     ]
     lib.grouped_gemm_fp8_launch.restype = ctypes.c_int
     i32, i64, ptr, size = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
+    lib.quantize_rows_launch.argtypes = [ptr, i64, i64, i64, i32, ptr, i64, ptr, ptr]
+    lib.quantize_rows_launch.restype = ctypes.c_int
+    lib.quantize_blocks_launch.argtypes = [ptr, i64, i64, i64, i64, i64, i32, ptr, ptr, ptr]
+    lib.quantize_blocks_launch.restype = ctypes.c_int
+    lib.block_scaled_mm_scratch_bytes.argtypes = [i32]
+    lib.block_scaled_mm_scratch_bytes.restype = size
+    lib.block_scaled_mm_launch.argtypes = [ptr, i64, ptr, ptr, i64, i64, ptr, ptr, i64, ptr, i32, i64, i64, i64, ptr,
+                                           size, ptr, ctypes.POINTER(LaunchInfo)]
+    lib.block_scaled_mm_launch.restype = ctypes.c_int
     lib.ffn_scratch_bytes.argtypes = [i32, i32]
     lib.ffn_scratch_bytes.restype = size
     for entry in (lib.gated_ffn_forward_launch, lib.gated_ffn_backward_launch):
@@ -540,6 +553,34 @@ def grouped_wgrad(a: int, a_pitch: int, dc: int, dc_pitch: int, offs: int, exper
     _check(load().grouped_gemm_wgrad_launch(a, a_pitch, dc, dc_pitch, offs, experts, rows, n, k, db, db_pitch,
                                             db_stride, dtype, scratch, scratch_nbytes, stream),
            "grouped_gemm_wgrad_launch")
+
+
+def quantize_rows(x: int, rows: int, cols: int, pitch: int, dtype: int, q: int, q_pitch: int, scale: int,
+                  stream: int) -> None:
+    """quantize_rows_launch (`dtype` an enum value)."""
+    _check(load().quantize_rows_launch(x, rows, cols, pitch, dtype, q, q_pitch, scale, stream), "quantize_rows_launch")
+
+
+def quantize_blocks(x: int, matrices: int, rows: int, cols: int, pitch: int, stride: int, dtype: int, q: int,
+                    scale: int, stream: int) -> None:
+    """quantize_blocks_launch (`dtype` an enum value)."""
+    _check(load().quantize_blocks_launch(x, matrices, rows, cols, pitch, stride, dtype, q, scale, stream),
+           "quantize_blocks_launch")
+
+
+def block_scaled_scratch_bytes(experts: int) -> int:
+    return int(load().block_scaled_mm_scratch_bytes(int(experts)))
+
+
+def block_scaled_mm(a: int, a_pitch: int, sa: int, b: int, b_pitch: int, b_stride: int, sb: int, c: int, c_pitch: int,
+                    offs: int, experts: int, rows: int, n: int, k: int, scratch: int, scratch_nbytes: int,
+                    stream: int) -> LaunchInfo:
+    """block_scaled_mm_launch: e4m3 operands, e8m0 block scales, bf16 C."""
+    info = LaunchInfo()
+    _check(load().block_scaled_mm_launch(a, a_pitch, sa, b, b_pitch, b_stride, sb, c, c_pitch, offs, experts, rows, n,
+                                         k, scratch, scratch_nbytes, stream, ctypes.byref(info)),
+           "block_scaled_mm_launch")
+    return info
 
 
 # Size of the library's fixed scratch array (MGB_NOALLOC_SCRATCH_BYTES in the header).

@@ -1,0 +1,153 @@
+"""e4m3 products with power-of-two block scales, and the quantisation to them.
+
+``kernels.fp8`` multiplies e4m3 experts whose 128-deep K blocks carry fp32
+scales.  Checkpoints and training recipes that keep those scales as powers of
+two (e8m0, one byte: 2^(byte - 127), ``torch.float8_e8m0fnu``) leave nothing
+to do outside the tensor core, whose block-scaled MMA applies them itself:
+
+    C[rows of e] (bf16) = sum_kb 2^sa[:, kb] * (A[rows of e, kb] @ B[e][:, kb].T) * 2^sb[e][n // 128, kb]
+
+``launch_quantize_rows`` (activations: a scale per token and 128-deep block)
+and ``launch_quantize_blocks`` (weights: a scale per 128 x 128 block) produce
+the operands: s is the smallest power of two with max |x| <= 448 s over the
+block's finite values (1 for a block of zeros), q = x / s rounded to nearest
+even, infinities and NaNs become NaN.  ``launch_block_scaled_mm`` multiplies
+them, dense or over expert-sorted rows, from one token to whole prompts.
+Every call is launches only, on the current stream of the tensors' device, and
+can be captured in a CUDA graph.  The reference has no counterpart (it does not
+emulate the model's FP8 quantization, README.md:298).
+"""
+
+from __future__ import annotations
+
+try:
+    import torch
+except ImportError:  # pragma: no cover - the CPU tests import the host helpers only
+    torch = None
+
+from . import _native
+from .fp8 import FP8_BLOCK, _blocks
+from .gated_ffn import _offsets, _require_runtime
+from .matmul import dtype_name
+
+_last_info: dict | None = None
+
+
+def last_block_scaled_info() -> dict | None:
+    """Native kernel of the most recent launch_block_scaled_mm call (path, tile, grid)."""
+    return _last_info
+
+
+def _source(x) -> int:
+    if not x.is_cuda:
+        raise ValueError("the tensor to quantise must be on a CUDA device")
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        raise ValueError("the tensor to quantise needs contiguous columns")
+    return _native.DTYPE_CODES[dtype_name(x.dtype)]
+
+
+def _target(name: str, t, shape: tuple, dtype, device):
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} {shape} tensor on {device}")
+    return t
+
+
+def launch_quantize_rows(x, q=None, scale=None):
+    """(q, scale) of activations ``x [M, K]`` (fp16, bf16 or fp32; rows may be
+    padded): q float8_e4m3fn ``[M, K]``, scale float8_e8m0fnu ``[M, ceil(K / 128)]``."""
+    _require_runtime()
+    if x.ndim != 2 or x.shape[1] == 0:
+        raise ValueError(f"expected x [M, K], got {tuple(x.shape)}")
+    code = _source(x)
+    rows, cols = x.shape
+    device = x.device
+    q = _target("q", q, (rows, cols), torch.float8_e4m3fn, device)
+    scale = _target("scale", scale, (rows, _blocks(cols)), torch.float8_e8m0fnu, device)
+    pitch = x.stride(0) if rows > 1 else cols
+    if pitch < cols:
+        raise ValueError("rows of x must not overlap")
+    with torch.cuda.device(device):
+        _native.quantize_rows(x.data_ptr(), rows, cols, pitch, code, q.data_ptr(), cols, scale.data_ptr(),
+                              torch.cuda.current_stream(device).cuda_stream)
+    return q, scale
+
+
+def launch_quantize_blocks(w, q=None, scale=None):
+    """(q, scale) of weights ``w [N, K]`` or ``[E, N, K]`` (fp16, bf16 or
+    fp32): q float8_e4m3fn of w's shape, scale float8_e8m0fnu ``[(E,)
+    ceil(N / 128), ceil(K / 128)]``."""
+    _require_runtime()
+    if w.ndim not in (2, 3) or w.shape[-1] == 0 or w.shape[-2] == 0:
+        raise ValueError(f"expected w [N, K] or [E, N, K], got {tuple(w.shape)}")
+    code = _source(w)
+    *lead, n, k = w.shape
+    matrices = lead[0] if lead else 1
+    device = w.device
+    q = _target("q", q, tuple(w.shape), torch.float8_e4m3fn, device)
+    scale = _target("scale", scale, (*lead, _blocks(n), _blocks(k)), torch.float8_e8m0fnu, device)
+    pitch = w.stride(-2) if n > 1 else k
+    stride = w.stride(0) if matrices > 1 else n * pitch
+    if pitch < k or (matrices > 1 and stride < (n - 1) * pitch + k):
+        raise ValueError("rows and matrices of w must not overlap")
+    with torch.cuda.device(device):
+        _native.quantize_blocks(w.data_ptr(), matrices, n, k, pitch, stride, code, q.data_ptr(), scale.data_ptr(),
+                                torch.cuda.current_stream(device).cuda_stream)
+    return q, scale
+
+
+def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
+    """``out [T, N]`` (bf16) of tokens ``a [T, K]`` with scales ``sa [T,
+    ceil(K / 128)]`` and weights ``b [N, K]`` or ``[E, N, K]`` with scales ``sb
+    [(E,) ceil(N / 128), ceil(K / 128)]``; with experts the rows are sorted and
+    ``offs`` (int32 ``[E]``) holds their cumulative row ends.  Empty experts are
+    fine; rows past ``offs[-1]`` are neither read nor written.  K is a multiple
+    of 16, N of 8; rows of a, b and out may be padded to whole 16 bytes, scales
+    are contiguous.  With few tokens per expert (32 on average) the weights are
+    streamed by many small CTAs, else 128 x 128 or CTA-pair 256 x 224 tiles run
+    on the block-scaled tensor-core MMA."""
+    global _last_info
+    _require_runtime()
+    if a.ndim != 2 or b.ndim not in (2, 3):
+        raise ValueError("expected a [T, K] and b [N, K] or [E, N, K]")
+    if not a.is_cuda or len({a.device, sa.device, b.device, sb.device}) != 1:
+        raise ValueError("a, sa, b and sb must be on the same CUDA device")
+    if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
+        raise ValueError("a and b must be float8_e4m3fn")
+    if sa.dtype != torch.float8_e8m0fnu or sb.dtype != torch.float8_e8m0fnu:
+        raise ValueError("sa and sb must be float8_e8m0fnu")
+    rows, k = a.shape
+    *lead, n, kb = b.shape
+    experts = lead[0] if lead else 1
+    if kb != k or k == 0 or n == 0 or experts == 0 or k % 16 or n % 8:
+        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} need one K, a multiple of 16, and N a multiple of 8")
+    if tuple(sa.shape) != (rows, _blocks(k)) or tuple(sb.shape) != (*lead, _blocks(n), _blocks(k)):
+        raise ValueError(f"scale shapes {tuple(sa.shape)} / {tuple(sb.shape)} do not match a {tuple(a.shape)}, "
+                         f"b {tuple(b.shape)} in blocks of {FP8_BLOCK}")
+    if not sa.is_contiguous() or not sb.is_contiguous():
+        raise ValueError("scales must be contiguous")
+    device = a.device
+    ends = _offsets(offs, experts, a)
+    if out is None:
+        out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
+    elif tuple(out.shape) != (rows, n) or out.dtype != torch.bfloat16 or out.device != device:
+        raise ValueError(f"out must be [{rows}, {n}] bfloat16 on {device}")
+    a_pitch = a.stride(0) if rows > 1 else k
+    out_pitch = out.stride(0) if rows > 1 else n
+    b_pitch = b.stride(-2) if n > 1 else k
+    b_stride = b.stride(0) if experts > 1 else n * b_pitch
+    if a.stride(1) != 1 or b.stride(-1) != 1 or out.stride(1) != 1 or a_pitch < k or a_pitch % 16 or b_pitch < k or (
+            b_pitch % 16) or b_stride % 16 or (experts > 1 and b_stride < (n - 1) * b_pitch + k) or out_pitch < n or (
+            out_pitch % 8) or (a.data_ptr() | b.data_ptr() | out.data_ptr()) % 16:
+        raise ValueError("a, b and out need contiguous columns, 16-byte aligned bases and rows a whole number of 16 "
+                         "bytes apart that do not overlap")
+    scratch = torch.empty(_native.block_scaled_scratch_bytes(experts), dtype=torch.uint8, device=device)
+    with torch.cuda.device(device):
+        info = _native.block_scaled_mm(
+            a.data_ptr(), a_pitch, sa.data_ptr(), b.data_ptr(), b_pitch, b_stride, sb.data_ptr(), out.data_ptr(),
+            out_pitch, ends, experts, rows, n, k, scratch.data_ptr(), scratch.numel(),
+            torch.cuda.current_stream(device).cuda_stream,
+        )
+    _last_info = info.as_dict()
+    return out
