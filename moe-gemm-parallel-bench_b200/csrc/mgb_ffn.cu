@@ -88,111 +88,128 @@ int launch_epilogue(int dtype, int g, const FfnParams& p, int64_t tiles, int sms
   return g == 2 ? launch_kernel<__half, EPI, 2>(p, tiles, sms, s) : launch_kernel<__half, EPI, 1>(p, tiles, sms, s);
 }
 
-// Tile edge of a launch over `p`'s jobs: pairs' 256 x 256 tiles when they
-// cover the device's pairs once, else one CTA's 128 x 128 tiles (four times
-// as many).  Rows of ragged segments are estimated as evenly spread.
-int tile_group(const FfnParams& p, int epi, int sms) {
-  int64_t tiles = 0;
-  for (int i = 0; i < p.jobs; ++i) {
-    const FfnJob& j = p.job[i];
-    const int64_t n = cdiv(j.n, epi == kFfnSwiglu ? 128 : 256);
-    const int64_t m = j.wgrad ? p.experts * cdiv(j.m, 256)
-                              : std::max<int64_t>(cdiv(p.rows, 256), std::min<int64_t>(p.experts, p.rows));
-    tiles += m * n;
-  }
-  return tiles >= sms / 2 ? 2 : 1;
-}
-
-struct Plan {
-  FfnParams p;
-  FfnTemplates tmpl;
-};
-
 FfnTensor tensor(const void* data, int64_t pitch, int64_t expert_stride, bool token) {
   return FfnTensor{static_cast<char*>(const_cast<void*>(data)), pitch, expert_stride, token ? 1 : 0};
 }
 
-size_t job_bytes(int64_t experts, int jobs) {
-  const size_t pairs = static_cast<size_t>(experts) * jobs;
-  return pairs * kFfnMaps * kMapBytes + (pairs + 1 + 15) / 16 * 16 * sizeof(int64_t);
+// Scratch of a call: the maps of every (job, expert), then at most
+// kFfnPlanLaunches tile lists.
+size_t maps_bytes(int64_t experts, int jobs) { return static_cast<size_t>(experts) * jobs * kFfnMaps * kMapBytes; }
+size_t list_bytes(int64_t experts, int jobs) {
+  return (static_cast<size_t>(experts) * jobs + 1 + 15) / 16 * 16 * sizeof(int64_t);
 }
 
-// One launch: the plan kernel (maps and tile list) and the product kernel.
-// `at` moves past the scratch it takes, so that launches of one call that
-// may overlap (programmatic launch) never share any.
+// The launches of one call: jobs are added launch by launch, then run()
+// issues the plan kernel (every map and tile list) and the product kernels.
 struct Launcher {
+  FfnPlan plan;
+  int epilogue[kFfnPlanLaunches];
   int dtype;
-  int64_t rows;
-  int32_t experts;
-  const int32_t* offs;
-  uint8_t* at;
+  uint8_t* scratch;
   cudaStream_t stream;
   int sms;
-  uint32_t* error_word;
   long long budget;
+  bool ok = true;
 
-  void init(Plan& plan, int jobs) {
-    std::memset(static_cast<void*>(&plan), 0, sizeof(plan));
-    plan.p.jobs = jobs;
-    plan.p.experts = experts;
-    plan.p.offs = offs;
-    plan.p.rows = rows;
-    plan.p.wait_budget = budget;
-    plan.p.error_word = error_word;
+  void begin_launch(int epi) {
+    FfnPlan::Launch& l = plan.launch[plan.launches];
+    l.first_job = plan.jobs;
+    epilogue[plan.launches++] = epi;
   }
-
-  // Rows job i: C[rows, n] = A[rows, k] op(B_e).
-  bool rows_job(Plan& plan, int i, FfnTensor a, FfnTensor b, bool b_mn, int64_t n, int64_t k, int64_t b_cols) {
-    FfnJob& j = plan.p.job[i];
-    j.t[0] = a;
-    j.t[1] = b;
-    j.maps = 2;
+  FfnJob& begin_job() {
+    ++plan.launch[plan.launches - 1].jobs;
+    return plan.job[plan.jobs++];
+  }
+  // The last job's next tensor, [rows, cols] of box `box`.
+  void add(const FfnTensor& t, int64_t rows, int64_t cols, Box box) {
+    FfnJob& j = plan.job[plan.jobs - 1];
+    const int i = j.maps++;
+    j.t[i] = t;
+    ok = ok && encode(&plan.map[plan.jobs - 1][i], dtype, t, rows, cols, box, scratch) &&
+         (!t.token || encode(&plan.small[plan.jobs - 1][i], dtype, t, 1, cols, box, scratch));
+  }
+  // Rows job: C[rows, n] = A[rows, k] op(B_e); its epilogue's tensors follow.
+  void rows_job(const FfnTensor& a, const FfnTensor& b, bool b_mn, int64_t n, int64_t k, int64_t b_cols) {
+    FfnJob& j = begin_job();
     j.b_mn = b_mn;
     j.n = n;
     j.k = k;
-    return encode(&plan.tmpl.map[i][0], dtype, a, rows, k, kKMajor, at) &&
-           (b_mn ? encode(&plan.tmpl.map[i][1], dtype, b, k, b_cols, kMnMajor, at)
-                 : encode(&plan.tmpl.map[i][1], dtype, b, n, k, kKMajor, at));
+    add(a, plan.rows, k, kKMajor);
+    if (b_mn) {
+      add(b, k, b_cols, kMnMajor);
+    } else {
+      add(b, n, k, kKMajor);
+    }
   }
-  // Weight gradient job i: C_e[m, n] = A[rows, m]^T B[rows, n].
-  bool wgrad_job(Plan& plan, int i, FfnTensor a, FfnTensor b, FfnTensor c, int64_t m, int64_t n) {
-    FfnJob& j = plan.p.job[i];
-    j.t[0] = a;
-    j.t[1] = b;
-    j.maps = 2;
+  // Weight gradient job: C_e[m, n] = A[rows, m]^T B[rows, n].
+  void wgrad_job(const FfnTensor& a, const FfnTensor& b, const FfnTensor& c, int64_t m, int64_t n) {
+    FfnJob& j = begin_job();
     j.wgrad = 1;
     j.a_mn = j.b_mn = 1;
     j.m = m;
     j.n = n;
-    return encode(&plan.tmpl.map[i][0], dtype, a, rows, m, kMnMajor, at) &&
-           encode(&plan.tmpl.map[i][1], dtype, b, rows, n, kMnMajor, at) && add(plan, i, c, m, n);
-  }
-  // The next tensor of job i's epilogue.
-  bool add(Plan& plan, int i, FfnTensor t, int64_t t_rows, int64_t cols) {
-    FfnJob& j = plan.p.job[i];
-    j.t[j.maps] = t;
-    return encode(&plan.tmpl.map[i][j.maps++], dtype, t, t_rows, cols, kStage, at);
+    add(a, plan.rows, m, kMnMajor);
+    add(b, plan.rows, n, kMnMajor);
+    add(c, m, n, kStage);
   }
 
-  template <int EPI>
-  int run(Plan& plan) {
-    FfnParams& p = plan.p;
-    const int g = tile_group(p, EPI, sms);
-    p.tile_rows = 128 * g;
-    p.tile_cols = EPI == kFfnSwiglu ? 64 * g : 128 * g;
-    const size_t pairs = static_cast<size_t>(experts) * p.jobs;
-    p.maps = at;
-    p.tile_start = reinterpret_cast<int64_t*>(at + pairs * kFfnMaps * kMapBytes);
-    at += job_bytes(experts, p.jobs);
-    int64_t tiles = 0;  // at most: a segment boundary adds one row block
-    for (int i = 0; i < p.jobs; ++i) {
-      const FfnJob& j = p.job[i];
-      const int64_t m = j.wgrad ? experts * cdiv(j.m, p.tile_rows) : cdiv(rows, p.tile_rows) + experts - 1;
-      tiles += m * cdiv(j.n, p.tile_cols);
+  // Tile edge of a launch: pairs' 256 x 256 tiles when they cover the
+  // device's pairs once, else one CTA's 128 x 128 tiles (four times as many).
+  // Rows of ragged segments are estimated as evenly spread.
+  int tile_group(const FfnPlan::Launch& l, int epi) const {
+    int64_t tiles = 0;
+    for (int i = 0; i < l.jobs; ++i) {
+      const FfnJob& j = plan.job[l.first_job + i];
+      const int64_t n = cdiv(j.n, epi == kFfnSwiglu ? 128 : 256);
+      const int64_t m = j.wgrad ? plan.experts * cdiv(j.m, 256)
+                                : std::max<int64_t>(cdiv(plan.rows, 256), std::min<int64_t>(plan.experts, plan.rows));
+      tiles += m * n;
     }
-    ffn_plan_kernel<<<static_cast<unsigned>(pairs + 1), 32, 0, stream>>>(plan.tmpl, p);
+    return tiles >= sms / 2 ? 2 : 1;
+  }
+
+  int run() {
+    if (!ok) return MGB_ERR_CUDA;
+    const int64_t experts = plan.experts;
+    plan.maps = scratch;
+    uint8_t* list = scratch + maps_bytes(experts, plan.jobs);
+    int group[kFfnPlanLaunches];
+    for (int i = 0; i < plan.launches; ++i) {
+      FfnPlan::Launch& l = plan.launch[i];
+      group[i] = tile_group(l, epilogue[i]);
+      l.tile_rows = 128 * group[i];
+      l.tile_cols = (epilogue[i] == kFfnSwiglu ? 64 : 128) * group[i];
+      l.tile_start = reinterpret_cast<int64_t*>(list);
+      list += list_bytes(experts, l.jobs);
+    }
+    ffn_plan_kernel<<<static_cast<unsigned>(plan.jobs * experts + plan.launches), 32, 0, stream>>>(plan);
     if (cudaGetLastError() != cudaSuccess) return MGB_ERR_CUDA;
-    return launch_epilogue<EPI>(dtype, g, p, tiles, sms, stream);
+    for (int i = 0; i < plan.launches; ++i) {
+      const FfnPlan::Launch& l = plan.launch[i];
+      FfnParams p;
+      std::memset(static_cast<void*>(&p), 0, sizeof(p));
+      int64_t tiles = 0;  // at most: a segment boundary adds one row block
+      for (int k = 0; k < l.jobs; ++k) {
+        const FfnJob& j = p.job[k] = plan.job[l.first_job + k];
+        const int64_t m = j.wgrad ? experts * cdiv(j.m, l.tile_rows) : cdiv(plan.rows, l.tile_rows) + experts - 1;
+        tiles += m * cdiv(j.n, l.tile_cols);
+      }
+      p.jobs = l.jobs;
+      p.experts = plan.experts;
+      p.offs = plan.offs;
+      p.rows = plan.rows;
+      p.maps = scratch + maps_bytes(experts, l.first_job);
+      p.tile_start = l.tile_start;
+      p.tile_rows = l.tile_rows;
+      p.tile_cols = l.tile_cols;
+      p.wait_budget = budget;
+      p.error_word = plan.error_word;
+      const int st = epilogue[i] == kFfnPlain    ? launch_epilogue<kFfnPlain>(dtype, group[i], p, tiles, sms, stream)
+                     : epilogue[i] == kFfnSwiglu ? launch_epilogue<kFfnSwiglu>(dtype, group[i], p, tiles, sms, stream)
+                                                 : launch_epilogue<kFfnSwigluBwd>(dtype, group[i], p, tiles, sms, stream);
+      if (st) return st;
+    }
+    return MGB_OK;
   }
 };
 
@@ -223,37 +240,32 @@ int start(Launcher& l, int32_t dtype, int64_t rows, int32_t experts, const int32
       scratch_bytes < ffn_scratch_bytes(experts, jobs)) {
     return MGB_ERR_SCRATCH;
   }
-  int sms = 0;
-  uint32_t* word = current_error_word();
-  if (word == nullptr || !current_launch_limits(&sms, &l.budget)) return MGB_ERR_CUDA;
+  std::memset(static_cast<void*>(&l.plan), 0, sizeof(l.plan));
+  l.plan.error_word = current_error_word();
+  if (l.plan.error_word == nullptr || !current_launch_limits(&l.sms, &l.budget)) return MGB_ERR_CUDA;
+  l.plan.experts = experts;
+  l.plan.offs = offs;
+  l.plan.rows = rows;
   l.dtype = dtype;
-  l.rows = rows;
-  l.experts = experts;
-  l.offs = offs;
-  l.at = static_cast<uint8_t*>(scratch);
+  l.scratch = static_cast<uint8_t*>(scratch);
   l.stream = static_cast<cudaStream_t>(stream);
-  l.sms = sms;
-  l.error_word = word;
   return MGB_OK;
 }
 
-// dgate_up = swiglu backward of dc b^T, or da = dc b^T.
-int dgrad(Launcher& l, FfnTensor dc, FfnTensor b, FfnTensor out, const void* gate_up, int64_t gate_up_pitch, int64_t n,
-          int64_t k) {
-  Plan plan;
-  l.init(plan, 1);
-  bool ok = l.rows_job(plan, 0, dc, b, false, k, n, 0);
-  if (gate_up == nullptr) {
-    return ok && l.add(plan, 0, out, l.rows, k) ? l.run<kFfnPlain>(plan) : MGB_ERR_CUDA;
-  }
-  const auto half = [&](const void* base, int64_t pitch, int64_t at) {
+// A launch of dgate_up = swiglu backward of dc b^T, or da = dc b^T.
+void dgrad(Launcher& l, const FfnTensor& dc, const FfnTensor& b, const FfnTensor& out, const void* gate_up,
+           int64_t gate_up_pitch, int64_t n, int64_t k) {
+  l.begin_launch(gate_up != nullptr ? kFfnSwigluBwd : kFfnPlain);
+  l.rows_job(dc, b, false, k, n, 0);
+  const auto half = [](const void* base, int64_t pitch, int64_t at) {
     return tensor(base != nullptr ? static_cast<const char*>(base) + at * 2 : nullptr, pitch, 0, true);
   };
-  ok = ok && l.add(plan, 0, half(out.data, out.pitch, 0), l.rows, k) &&
-       l.add(plan, 0, half(out.data, out.pitch, k), l.rows, k) &&
-       l.add(plan, 0, half(gate_up, gate_up_pitch, 0), l.rows, k) &&
-       l.add(plan, 0, half(gate_up, gate_up_pitch, k), l.rows, k);
-  return ok ? l.run<kFfnSwigluBwd>(plan) : MGB_ERR_CUDA;
+  l.add(half(out.data, out.pitch, 0), l.plan.rows, k, kStage);
+  if (gate_up != nullptr) {
+    l.add(half(out.data, out.pitch, k), l.plan.rows, k, kStage);
+    l.add(half(gate_up, gate_up_pitch, 0), l.plan.rows, k, kStage);
+    l.add(half(gate_up, gate_up_pitch, k), l.plan.rows, k, kStage);
+  }
 }
 
 }  // namespace
@@ -262,10 +274,7 @@ extern "C" {
 
 size_t ffn_scratch_bytes(int32_t experts, int32_t jobs) {
   if (experts <= 0 || jobs <= 0) return 0;
-  // One plan per job at most (the jobs of a call share plans or take turns).
-  size_t bytes = 0;
-  for (int32_t i = 0; i < jobs; ++i) bytes += job_bytes(experts, 1) + 128;
-  return bytes;
+  return maps_bytes(experts, jobs) + kFfnPlanLaunches * list_bytes(experts, jobs);
 }
 
 int gated_ffn_forward_launch(const mgb_ffn_args* f) {
@@ -287,26 +296,23 @@ int gated_ffn_forward_launch(const mgb_ffn_args* f) {
     return st;
   }
   if (rows == 0) return MGB_OK;
-  Plan plan;
-  l.init(plan, 1);
   const auto half = [&](int64_t at) {
     return tensor(static_cast<const char*>(f->gate_up) + at * 2, f->gate_up_pitch, 0, true);
   };
-  plan.p.job[0].up = ffn;
   const FfnTensor h = tensor(f->h, f->h_pitch, 0, true);
-  if (!l.rows_job(plan, 0, tensor(f->x, f->x_pitch, 0, true), tensor(f->w13, f->w13_pitch, f->w13_stride, false), true,
-                  ffn, hid, 2 * ffn) ||
-      !l.add(plan, 0, h, rows, ffn) || !l.add(plan, 0, half(0), rows, ffn) || !l.add(plan, 0, half(ffn), rows, ffn)) {
-    return MGB_ERR_CUDA;
+  l.begin_launch(kFfnSwiglu);
+  l.rows_job(tensor(f->x, f->x_pitch, 0, true), tensor(f->w13, f->w13_pitch, f->w13_stride, false), true, ffn, hid,
+             2 * ffn);
+  l.plan.job[0].up = ffn;
+  l.add(h, rows, ffn, kStage);
+  l.add(half(0), rows, ffn, kStage);
+  l.add(half(ffn), rows, ffn, kStage);
+  if (down) {
+    l.begin_launch(kFfnPlain);
+    l.rows_job(h, tensor(f->w2, f->w2_pitch, f->w2_stride, false), true, hid, ffn, hid);
+    l.add(tensor(f->y, f->y_pitch, 0, true), rows, hid, kStage);
   }
-  if (int st = l.run<kFfnSwiglu>(plan)) return st;
-  if (!down) return MGB_OK;
-  l.init(plan, 1);
-  if (!l.rows_job(plan, 0, h, tensor(f->w2, f->w2_pitch, f->w2_stride, false), true, hid, ffn, hid) ||
-      !l.add(plan, 0, tensor(f->y, f->y_pitch, 0, true), rows, hid)) {
-    return MGB_ERR_CUDA;
-  }
-  return l.run<kFfnPlain>(plan);
+  return l.run();
 }
 
 int gated_ffn_backward_launch(const mgb_ffn_args* f) {
@@ -327,21 +333,15 @@ int gated_ffn_backward_launch(const mgb_ffn_args* f) {
   const FfnTensor dy = tensor(f->y, f->y_pitch, 0, true), x = tensor(f->x, f->x_pitch, 0, true);
   const FfnTensor h = tensor(f->h, f->h_pitch, 0, true), dgu = tensor(f->dgate_up, f->dgate_up_pitch, 0, true);
   if (rows > 0) {
-    if (int st = dgrad(l, dy, tensor(f->w2, f->w2_pitch, f->w2_stride, false), dgu, f->gate_up, f->gate_up_pitch, hid,
-                       ffn)) {
-      return st;
-    }
+    dgrad(l, dy, tensor(f->w2, f->w2_pitch, f->w2_stride, false), dgu, f->gate_up, f->gate_up_pitch, hid, ffn);
   }
   // dx, dW13 and dW2 depend on nothing but dgate_up: one launch.
-  Plan plan;
-  l.init(plan, 3);
-  if (!l.rows_job(plan, 0, dgu, tensor(f->w13, f->w13_pitch, f->w13_stride, false), false, hid, 2 * ffn, 0) ||
-      !l.add(plan, 0, tensor(f->dx, f->dx_pitch, 0, true), rows, hid) ||
-      !l.wgrad_job(plan, 1, x, dgu, tensor(f->dw13, f->dw13_pitch, f->dw13_stride, false), hid, 2 * ffn) ||
-      !l.wgrad_job(plan, 2, h, dy, tensor(f->dw2, f->dw2_pitch, f->dw2_stride, false), ffn, hid)) {
-    return MGB_ERR_CUDA;
-  }
-  return l.run<kFfnPlain>(plan);
+  l.begin_launch(kFfnPlain);
+  l.rows_job(dgu, tensor(f->w13, f->w13_pitch, f->w13_stride, false), false, hid, 2 * ffn, 0);
+  l.add(tensor(f->dx, f->dx_pitch, 0, true), rows, hid, kStage);
+  l.wgrad_job(x, dgu, tensor(f->dw13, f->dw13_pitch, f->dw13_stride, false), hid, 2 * ffn);
+  l.wgrad_job(h, dy, tensor(f->dw2, f->dw2_pitch, f->dw2_stride, false), ffn, hid);
+  return l.run();
 }
 
 int grouped_gemm_dgrad_launch(const void* dc, int64_t dc_pitch, const void* b, int64_t b_pitch, int64_t b_stride,
@@ -358,8 +358,9 @@ int grouped_gemm_dgrad_launch(const void* dc, int64_t dc_pitch, const void* b, i
   Launcher l;
   if (int st = start(l, dtype, rows, experts, offs, 1, scratch, scratch_bytes, stream)) return st;
   if (rows == 0) return MGB_OK;
-  return dgrad(l, tensor(dc, dc_pitch, 0, true), tensor(b, b_pitch, b_stride, false), tensor(out, out_pitch, 0, true),
-               gate_up, gate_up_pitch, n, k);
+  dgrad(l, tensor(dc, dc_pitch, 0, true), tensor(b, b_pitch, b_stride, false), tensor(out, out_pitch, 0, true), gate_up,
+        gate_up_pitch, n, k);
+  return l.run();
 }
 
 int grouped_gemm_wgrad_launch(const void* a, int64_t a_pitch, const void* dc, int64_t dc_pitch, const int32_t* offs,
@@ -372,13 +373,9 @@ int grouped_gemm_wgrad_launch(const void* a, int64_t a_pitch, const void* dc, in
   }
   Launcher l;
   if (int st = start(l, dtype, rows, experts, offs, 1, scratch, scratch_bytes, stream)) return st;
-  Plan plan;
-  l.init(plan, 1);
-  if (!l.wgrad_job(plan, 0, tensor(a, a_pitch, 0, true), tensor(dc, dc_pitch, 0, true),
-                   tensor(db, db_pitch, db_stride, false), k, n)) {
-    return MGB_ERR_CUDA;
-  }
-  return l.run<kFfnPlain>(plan);
+  l.begin_launch(kFfnPlain);
+  l.wgrad_job(tensor(a, a_pitch, 0, true), tensor(dc, dc_pitch, 0, true), tensor(db, db_pitch, db_stride, false), k, n);
+  return l.run();
 }
 
 }  // extern "C"

@@ -38,6 +38,7 @@
 namespace mgb {
 
 constexpr int kFfnMaxJobs = 3;
+constexpr int kFfnPlanJobs = 4, kFfnPlanLaunches = 2;  // one plan kernel covers a call's launches
 constexpr int kFfnMaps = 6;  // per job and expert: A, B, then the epilogue's
 enum FfnEpilogue : int { kFfnPlain = 0, kFfnSwiglu = 1, kFfnSwigluBwd = 2 };
 
@@ -74,39 +75,53 @@ struct FfnParams {
   uint32_t* error_word;
 };
 
-struct FfnTemplates {
-  CUtensorMap map[kFfnMaxJobs][kFfnMaps];
+// What the plan kernel prepares: the tensor maps of every job's experts and
+// every launch's tile list.
+struct FfnPlan {
+  FfnJob job[kFfnPlanJobs];
+  // Templates for the whole tensor and for one of less than kLargeMapBytes.
+  CUtensorMap map[kFfnPlanJobs][kFfnMaps], small[kFfnPlanJobs][kFfnMaps];
+  struct Launch {
+    int32_t first_job, jobs, tile_rows, tile_cols;
+    int64_t* tile_start;
+  } launch[kFfnPlanLaunches];
+  int32_t jobs, launches, experts;
+  const int32_t* offs;
+  int64_t rows;
+  uint8_t* maps;
+  uint32_t* error_word;
 };
 
 // Rows [start, start + len) of expert e, clamped into the tensor whatever offs holds.
-__device__ __forceinline__ int64_t ffn_segment(const FfnParams& p, int e, int64_t& start, bool* bad = nullptr) {
-  if (p.offs == nullptr) {
+__device__ __forceinline__ int64_t ffn_segment(const int32_t* offs, int64_t rows, int e, int64_t& start,
+                                               bool* bad = nullptr) {
+  if (offs == nullptr) {
     start = 0;
-    return p.rows;
+    return rows;
   }
-  const int64_t lo = e > 0 ? p.offs[e - 1] : 0, hi = p.offs[e];
-  if (bad != nullptr) *bad = lo < 0 || hi < lo || hi > p.rows;
-  start = lo < 0 ? 0 : lo > p.rows ? p.rows : lo;
-  const int64_t end = hi < start ? start : hi > p.rows ? p.rows : hi;
+  const int64_t lo = e > 0 ? offs[e - 1] : 0, hi = offs[e];
+  if (bad != nullptr) *bad = lo < 0 || hi < lo || hi > rows;
+  start = lo < 0 ? 0 : lo > rows ? rows : lo;
+  const int64_t end = hi < start ? start : hi > rows ? rows : hi;
   return end - start;
 }
 
-// Tensor maps of every (job, expert), one warp each, and the tiles' prefix
-// sums (last block).
-__global__ void __launch_bounds__(32)
-    ffn_plan_kernel(const __grid_constant__ FfnTemplates tmpl, const __grid_constant__ FfnParams p) {
+// Tensor maps of every (job, expert), one warp each, and every launch's tile
+// prefix sums (the last blocks).
+__global__ void __launch_bounds__(32) ffn_plan_kernel(const __grid_constant__ FfnPlan p) {
   __shared__ alignas(128) CUtensorMap staging[kFfnMaps];
   const int lane = threadIdx.x;
-  const int pairs = p.jobs * p.experts;
   grid_launch_dependents();
-  if (blockIdx.x == pairs) {
+  if (static_cast<int>(blockIdx.x) >= p.jobs * p.experts) {
+    const FfnPlan::Launch& l = p.launch[blockIdx.x - p.jobs * p.experts];
+    const int pairs = l.jobs * p.experts;
     const int per = (pairs + 31) / 32;
     const int lo = lane * per, hi = lo + per < pairs ? lo + per : pairs;
     auto tiles_of = [&](int i) -> int64_t {
-      const FfnJob& j = p.job[i / p.experts];
+      const FfnJob& j = p.job[l.first_job + i / p.experts];
       int64_t start;
-      const int64_t rows = j.wgrad ? j.m : ffn_segment(p, i % p.experts, start);
-      return ceil_div64(rows, p.tile_rows) * ceil_div64(j.n, p.tile_cols);
+      const int64_t rows = j.wgrad ? j.m : ffn_segment(p.offs, p.rows, i % p.experts, start);
+      return ceil_div64(rows, l.tile_rows) * ceil_div64(j.n, l.tile_cols);
     };
     int64_t sum = 0;
     for (int i = lo; i < hi; ++i) sum += tiles_of(i);
@@ -118,24 +133,25 @@ __global__ void __launch_bounds__(32)
     }
     int64_t run = incl - sum;
     for (int i = lo; i < hi; ++i) {
-      p.tile_start[i] = run;
+      l.tile_start[i] = run;
       run += tiles_of(i);
     }
-    if (lane == 31) p.tile_start[pairs] = incl;
+    if (lane == 31) l.tile_start[pairs] = incl;
     return;
   }
   const int job = blockIdx.x / p.experts, e = blockIdx.x % p.experts;
   const FfnJob& j = p.job[job];
   bool bad = false;
   int64_t start = 0;
-  const int64_t len = ffn_segment(p, e, start, &bad);
+  const int64_t len = ffn_segment(p.offs, p.rows, e, start, &bad);
   if (bad && lane == 0) atomicOr(p.error_word, kErrBadDims);
   // One lane per map: copy the template, move its base, end its rows with the segment.
   if (lane < j.maps) {
-    const uint4* src = reinterpret_cast<const uint4*>(&tmpl.map[job][lane]);
+    const FfnTensor& t = j.t[lane];
+    const bool small = t.token && len * t.pitch * 2 < kLargeMapBytes;
+    const uint4* src = reinterpret_cast<const uint4*>(small ? &p.small[job][lane] : &p.map[job][lane]);
     uint4* dst = reinterpret_cast<uint4*>(&staging[lane]);
     for (int i = 0; i < 8; ++i) dst[i] = src[i];
-    const FfnTensor& t = j.t[lane];
     if (t.token) {
       if (len > 0) {  // an empty segment's maps are never used
         tmap_replace_address(&staging[lane], t.data + start * t.pitch * 2);
@@ -179,7 +195,7 @@ struct FfnWalk {
       end = ts[lo + 1];
       job = &p.job[lo / p.experts];
       int64_t start;
-      len = ffn_segment(p, lo % p.experts, start);
+      len = ffn_segment(p.offs, p.rows, lo % p.experts, start);
       rows = job->wgrad ? job->m : len;
       m_blocks = ceil_div64(rows, p.tile_rows);
       n_blocks = ceil_div64(job->n, p.tile_cols);
