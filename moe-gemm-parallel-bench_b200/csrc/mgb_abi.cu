@@ -487,10 +487,15 @@ int launch_grouped_params(GroupedParams& p, const DeviceState& ds, const TileBou
     const uint64_t wgt_pitch = ((static_cast<uint64_t>(n) * es + 15) / 16) * 16;
     const uint64_t out_n = swiglu ? static_cast<uint64_t>(n) / 2 : static_cast<uint64_t>(n);
     const uint64_t out_pitch = ((out_n * es + 15) / 16) * 16;
+    // Maps whose rows the device sets start from one-row templates (see
+    // tmap_replace_dim).
+    const bool token_rows_set = !p.homogeneous && !p.single;
+    const bool weight_rows_set = token_rows_set && p.offs == nullptr;
+    const uint64_t token_rows = token_rows_set ? 1 : static_cast<uint64_t>(std::max<int64_t>(m, 1));
     CUtensorMap act, wgt, out;
-    if (!encode_2d(&act, dtype, scratch, k, std::max<int64_t>(m, 1), act_pitch, vi.bk, vi.box_rows, kActSwizzle) ||
-        !encode_2d(&wgt, dtype, scratch, n, k, wgt_pitch, vi.bk, vi.bk, wgt_swizzle(dtype)) ||
-        !encode_out(&out, dtype, scratch, out_n, std::max<int64_t>(m, 1), out_pitch)) {
+    if (!encode_2d(&act, dtype, scratch, k, token_rows, act_pitch, vi.bk, vi.box_rows, kActSwizzle) ||
+        !encode_2d(&wgt, dtype, scratch, n, weight_rows_set ? 1 : k, wgt_pitch, vi.bk, vi.bk, wgt_swizzle(dtype)) ||
+        !encode_out(&out, dtype, scratch, out_n, token_rows, out_pitch)) {
       return MGB_ERR_CUDA;
     }
     if (maps_launch_typed(dtype, act, wgt, out, p, s) != 0) return MGB_ERR_CUDA;
@@ -775,12 +780,15 @@ int grouped_gemm_fp8_launch(const int64_t* a_ptrs, const int64_t* b_ptrs, const 
   // addresses, and for heterogeneous groups extents and pitches, per problem).
   const uint64_t row_bytes = ((static_cast<uint64_t>(std::max<int64_t>(k, 1)) + 15) / 16) * 16;
   const uint64_t out_pitch = ((static_cast<uint64_t>(n) * 2 + 15) / 16) * 16;
+  // Maps whose rows the device sets start from one-row templates (see
+  // tmap_replace_dim).
+  const uint64_t token_rows = homogeneous ? m : 1, weight_rows = homogeneous ? n : 1;
   CUtensorMap act, wgt, out;
-  if (!encode_2d(&act, kDtypeU8, scratch, std::max<int64_t>(k, 1), m, row_bytes, 128, vi.box_rows,
+  if (!encode_2d(&act, kDtypeU8, scratch, std::max<int64_t>(k, 1), token_rows, row_bytes, 128, vi.box_rows,
                  CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !encode_2d(&wgt, kDtypeU8, scratch, std::max<int64_t>(k, 1), n, row_bytes, 128, vi.box_cols,
+      !encode_2d(&wgt, kDtypeU8, scratch, std::max<int64_t>(k, 1), weight_rows, row_bytes, 128, vi.box_cols,
                  CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !encode_out(&out, MGB_BF16, scratch, n, m, out_pitch)) {
+      !encode_out(&out, MGB_BF16, scratch, n, token_rows, out_pitch)) {
     return MGB_ERR_CUDA;
   }
   if (mgb::fp8_maps_launch(act, wgt, out, p, s) != 0) return MGB_ERR_CUDA;
