@@ -29,9 +29,9 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 enum Box { kKMajor, kMnMajor, kStage };
 
 bool encode(CUtensorMap* map, int dtype, const FfnTensor& t, int64_t rows, int64_t cols, Box box, const void* dummy) {
-  // A tensor without rows is never read; its template still needs a legal base and extent.
+  // A tensor without rows is never read; its template still needs a legal base.
   const void* base = t.data != nullptr ? t.data : dummy;
-  return encode_map_2d(map, dtype, base, static_cast<uint64_t>(cols), static_cast<uint64_t>(std::max<int64_t>(rows, 1)),
+  return encode_map_2d(map, dtype, base, static_cast<uint64_t>(cols), static_cast<uint64_t>(rows),
                        static_cast<uint64_t>(t.pitch) * 2, 64, box == kKMajor ? 128 : box == kMnMajor ? 64 : 32);
 }
 
@@ -125,8 +125,7 @@ struct Launcher {
     FfnJob& j = plan.job[plan.jobs - 1];
     const int i = j.maps++;
     j.t[i] = t;
-    ok = ok && encode(&plan.map[plan.jobs - 1][i], dtype, t, rows, cols, box, scratch) &&
-         (!t.token || encode(&plan.small[plan.jobs - 1][i], dtype, t, 1, cols, box, scratch));
+    ok = ok && encode(&plan.map[plan.jobs - 1][i], dtype, t, t.token ? 1 : rows, cols, box, scratch);
   }
   // Rows job: C[rows, n] = A[rows, k] op(B_e); its epilogue's tensors follow.
   void rows_job(const FfnTensor& a, const FfnTensor& b, bool b_mn, int64_t n, int64_t k, int64_t b_cols) {

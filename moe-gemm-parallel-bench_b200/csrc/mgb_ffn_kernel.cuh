@@ -79,8 +79,7 @@ struct FfnParams {
 // every launch's tile list.
 struct FfnPlan {
   FfnJob job[kFfnPlanJobs];
-  // Templates for the whole tensor and for one of less than kLargeMapBytes.
-  CUtensorMap map[kFfnPlanJobs][kFfnMaps], small[kFfnPlanJobs][kFfnMaps];
+  CUtensorMap map[kFfnPlanJobs][kFfnMaps];  // templates; token tensors' have one row
   struct Launch {
     int32_t first_job, jobs, tile_rows, tile_cols;
     int64_t* tile_start;
@@ -148,8 +147,7 @@ __global__ void __launch_bounds__(32) ffn_plan_kernel(const __grid_constant__ Ff
   // One lane per map: copy the template, move its base, end its rows with the segment.
   if (lane < j.maps) {
     const FfnTensor& t = j.t[lane];
-    const bool small = t.token && len * t.pitch * 2 < kLargeMapBytes;
-    const uint4* src = reinterpret_cast<const uint4*>(small ? &p.small[job][lane] : &p.map[job][lane]);
+    const uint4* src = reinterpret_cast<const uint4*>(&p.map[job][lane]);
     uint4* dst = reinterpret_cast<uint4*>(&staging[lane]);
     for (int i = 0; i < 8; ++i) dst[i] = src[i];
     if (t.token) {

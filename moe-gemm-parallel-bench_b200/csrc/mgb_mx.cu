@@ -188,11 +188,8 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   p.maps = static_cast<uint8_t*>(scratch);
   p.tile_start = reinterpret_cast<int64_t*>(p.maps + static_cast<size_t>(experts) * 3 * sizeof(CUtensorMap));
   MxTemplates tmpl;
-  const auto token_maps = [&](CUtensorMap* maps, int64_t r) {
-    return encode_map_2d(&maps[0], kMapBytes8, a, k, r, a_pitch, 128, 128) &&
-           encode_map_2d(&maps[2], MGB_BF16, c, n, r, c_pitch * 2, 32, 32, 64);
-  };
-  if (!token_maps(tmpl.map, rows) || !token_maps(tmpl.small, 1) ||
+  if (!encode_map_2d(&tmpl.map[0], kMapBytes8, a, k, 1, a_pitch, 128, 128) ||
+      !encode_map_2d(&tmpl.map[2], MGB_BF16, c, n, 1, c_pitch * 2, 32, 32, 64) ||
       !encode_map_2d(&tmpl.map[1], kMapBytes8, b, k, n, b_pitch, 128, pair ? MxCfg<2>::kColsCta : MxCfg<1>::kColsCta)) {
     return MGB_ERR_CUDA;
   }

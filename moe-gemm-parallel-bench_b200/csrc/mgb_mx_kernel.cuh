@@ -223,7 +223,7 @@ __device__ __forceinline__ int64_t mx_segment(const MxParams& p, int e, int64_t&
 }
 
 struct MxTemplates {
-  CUtensorMap map[3], small[3];  // for the whole tensor, and for one of less than kLargeMapBytes
+  CUtensorMap map[3];  // A and C of one row: the plan kernel sets every segment's
 };
 
 // Tensor maps of every expert, one warp each, and the tiles' prefix sums (last block).
@@ -262,9 +262,7 @@ __global__ void __launch_bounds__(32)
   const int64_t len = mx_segment(p, e, start, &bad);
   if (bad && lane == 0) atomicOr(p.error_word, kErrBadDims);
   if (lane < 3) {
-    const int64_t row_bytes = lane == 0 ? p.a_pitch : p.c_pitch * 2;
-    const bool small = lane != 1 && len * row_bytes < kLargeMapBytes;
-    const uint4* src = reinterpret_cast<const uint4*>(small ? &tmpl.small[lane] : &tmpl.map[lane]);
+    const uint4* src = reinterpret_cast<const uint4*>(&tmpl.map[lane]);
     uint4* dst = reinterpret_cast<uint4*>(&staging[lane]);
     for (int i = 0; i < 8; ++i) dst[i] = src[i];
     if (lane == 1) {
