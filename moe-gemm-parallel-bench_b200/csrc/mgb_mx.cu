@@ -64,20 +64,33 @@ int launch_mx(const MxParams& p, int64_t tiles, int sm_count, cudaStream_t strea
   return cudaLaunchKernelEx(&cfg, mx_kernel<G>, p) == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
 }
 
+FastDiv fast_div(int64_t d) {
+  uint32_t log = 0;
+  while ((1ll << log) < d) ++log;
+  const uint32_t s = 31 + log;
+  return FastDiv{static_cast<uint32_t>(d), static_cast<uint32_t>(((1ull << s) + d - 1) / d), s};
+}
+
 template <typename T>
 int rows_typed(const void* x, int64_t rows, int64_t cols, int64_t pitch, void* q, int64_t q_pitch, void* scale, int sms,
                cudaStream_t s) {
   const int64_t blocks = rows * cdiv(cols, 128);
-  const int grid = static_cast<int>(std::min<int64_t>(cdiv(blocks, 16), 8ll * sms));
+  if (blocks >= (1ll << 31) - (1ll << 22)) return MGB_ERR_INVALID;  // 2^38 elements: more than the GPU holds
+  // Every half warp takes kRowsUnroll blocks at once (no short last sweep);
+  // fewer where that would leave SMs without a CTA.
+  const unsigned grid = static_cast<unsigned>(
+      std::max<int64_t>(cdiv(blocks, 16 * kRowsUnroll), std::min<int64_t>(cdiv(blocks, 16), 4ll * sms)));
+  const FastDiv kb = fast_div(cdiv(cols, 128));
+  const uint32_t nb = static_cast<uint32_t>(blocks);
   const bool vec = aligned(x, 16) && pitch % (16 / static_cast<int>(sizeof(T))) == 0 && cols % 8 == 0 && aligned(q, 8) &&
                    q_pitch % 8 == 0;
   const T* in = static_cast<const T*>(x);
   uint8_t* out = static_cast<uint8_t*>(q);
   uint8_t* sc = static_cast<uint8_t*>(scale);
   if (vec) {
-    quantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(in, rows, cols, pitch, out, q_pitch, sc);
+    quantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(in, nb, kb, cols, pitch, out, q_pitch, sc);
   } else {
-    quantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(in, rows, cols, pitch, out, q_pitch, sc);
+    quantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(in, nb, kb, cols, pitch, out, q_pitch, sc);
   }
   return cudaGetLastError() == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
 }
@@ -94,9 +107,11 @@ int blocks_typed(const void* x, int64_t matrices, int64_t rows, int64_t cols, in
   uint8_t* out = static_cast<uint8_t*>(q);
   uint8_t* sc = static_cast<uint8_t*>(scale);
   if (vec) {
-    quantize_blocks_kernel<T, true><<<grid, 256, 0, s>>>(in, rows, cols, pitch, stride, out, cols, rows * cols, sc, kb, per);
+    quantize_blocks_kernel<T, true><<<grid, 256, 0, s>>>(in, rows, cols, pitch, stride, out, cols, rows * cols, sc, fast_div(kb),
+                                                         fast_div(per));
   } else {
-    quantize_blocks_kernel<T, false><<<grid, 256, 0, s>>>(in, rows, cols, pitch, stride, out, cols, rows * cols, sc, kb, per);
+    quantize_blocks_kernel<T, false><<<grid, 256, 0, s>>>(in, rows, cols, pitch, stride, out, cols, rows * cols, sc, fast_div(kb),
+                                                         fast_div(per));
   }
   return cudaGetLastError() == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
 }
@@ -109,8 +124,8 @@ constexpr int64_t kFewRows = 32;
 
 extern "C" {
 
-size_t block_scaled_mm_scratch_bytes(int32_t experts) {
-  if (experts <= 0) return 0;
+size_t block_scaled_mm_scratch_bytes(int32_t experts, int64_t rows) {
+  if (experts <= 0 || rows <= 0 || cdiv(rows, experts) <= kFewRows) return 0;
   return static_cast<size_t>(experts) * 3 * sizeof(CUtensorMap) +
          (static_cast<size_t>(experts) + 1 + 15) / 16 * 16 * sizeof(int64_t);
 }
@@ -120,7 +135,7 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
                            int32_t experts, int64_t rows, int64_t n, int64_t k, void* scratch, size_t scratch_bytes,
                            void* stream, mgb_launch_info* info) {
   if (experts <= 0 || experts > (1 << 20) || rows < 0 || rows >= (1ll << 31) || n <= 0 || n >= (1ll << 31) || k <= 0 ||
-      k >= (1ll << 31) || k % 16 != 0 || n % 8 != 0 || (offs == nullptr && experts != 1)) {
+      k >= (1ll << 30) || k % 16 != 0 || n % 8 != 0 || (offs == nullptr && experts != 1)) {
     return MGB_ERR_INVALID;
   }
   if ((rows > 0 && (a == nullptr || sa == nullptr || c == nullptr)) || b == nullptr || sb == nullptr ||
@@ -129,9 +144,8 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
       c_pitch % 8 != 0) {
     return MGB_ERR_INVALID;
   }
-  if (scratch == nullptr || !aligned(scratch, 128) || scratch_bytes < block_scaled_mm_scratch_bytes(experts)) {
-    return MGB_ERR_SCRATCH;
-  }
+  const size_t need = block_scaled_mm_scratch_bytes(experts, rows);
+  if (need > 0 && (scratch == nullptr || !aligned(scratch, 128) || scratch_bytes < need)) return MGB_ERR_SCRATCH;
   int sms = 0;
   MxParams p;
   std::memset(&p, 0, sizeof(p));
@@ -159,7 +173,8 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t each = cdiv(rows, experts);
   const int64_t groups = cdiv(n, 16) * experts;
-  if (each <= kFewRows && groups < (1ll << 31)) {
+  if (each <= kFewRows) {
+    if (groups >= (1ll << 31)) return MGB_ERR_UNSUPPORTED;
     const unsigned grid = static_cast<unsigned>(groups);
     const int nt = each <= 8 ? 1 : each <= 16 ? 2 : 4;
     if (nt == 1) {

@@ -37,59 +37,119 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
   return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
 }
 
-// |v| as bits, 0 for infinities and NaNs: the scale goes by the finite values.
-__device__ __forceinline__ uint32_t finite_abs(float v) {
-  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
-  return b >= 0x7F800000u ? 0u : b;
+// Two e4m3 values of a * inv, b * inv, round to nearest even.
+__device__ __forceinline__ uint32_t e4m3_pair(float a, float b, float inv) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
 }
 
-// Two e4m3 values, round to nearest even; infinities and NaNs become NaN.
-__device__ __forceinline__ uint32_t e4m3_pair(float a, float b, float inv) {
-  const float nan = __uint_as_float(0x7FC00000u);
-  a = isinf(a) ? nan : a * inv;
-  b = isinf(b) ? nan : b * inv;
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+// Eight consecutive elements of a row as loaded (16-bit types stay packed).
+template <typename T>
+struct Eight {
+  static constexpr int kWords = 2 * static_cast<int>(sizeof(T));
+  uint32_t w[kWords];
+};
+
+// From column `col`; columns past `cols` are 0.  VEC: the address is 16-byte
+// aligned and the eight lie inside the row or all past it.
+template <typename T, bool VEC>
+__device__ __forceinline__ Eight<T> load8(const T* row, int64_t col, int64_t cols) {
+  Eight<T> v;
+  if constexpr (VEC) {
+    uint4* to = reinterpret_cast<uint4*>(v.w);
+#pragma unroll
+    for (int i = 0; i < Eight<T>::kWords / 4; ++i) {
+      to[i] = col < cols ? __ldcs(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.w[i] = col + i < cols ? __float_as_uint(row[col + i]) : 0u;
+  } else {
+    const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = col + 2 * i < cols ? r[col + 2 * i] : 0u, hi = col + 2 * i + 1 < cols ? r[col + 2 * i + 1] : 0u;
+      v.w[i] = lo | (hi << 16);
+    }
+  }
+  return v;
 }
 
 template <typename T>
-__device__ __forceinline__ float to_float(T v) {
-  if constexpr (std::is_same<T, float>::value) {
-    return v;
-  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    return __bfloat162float(v);
-  } else {
-    return __half2float(v);
-  }
-}
-
-// Eight consecutive elements from column `col`; columns past `cols` are 0.
-// VEC: the address is 16-byte aligned and the eight lie inside the row.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int64_t col, int64_t cols, float (&v)[8]) {
-  if constexpr (VEC) {
-    alignas(16) T raw[8];
-    if (col < cols) {
+__device__ __forceinline__ void to_floats(const Eight<T>& v, float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
-        reinterpret_cast<uint4*>(raw)[i] = __ldcs(reinterpret_cast<const uint4*>(row + col) + i);
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v.w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 p;
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        p = make_float2(__uint_as_float(v.w[i] << 16), __uint_as_float(v.w[i] & 0xFFFF0000u));
+      } else {
+        p = __half22float2(*reinterpret_cast<const __half2*>(&v.w[i]));
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_float(raw[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      f[2 * i] = p.x;
+      f[2 * i + 1] = p.y;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? to_float(row[col + i]) : 0.0f;
   }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store8(uint8_t* row, int64_t col, int64_t cols, const float (&v)[8], float inv) {
+// Largest |element| as the type's bits: sign cleared, a floating value's bits
+// order as an unsigned integer, so 16-bit pairs take one packed maximum.
+// Infinities and NaNs come out on top (>= kNonFinite).
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const Eight<T>& v, uint32_t top) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, v.w[i] & 0x7FFFFFFFu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __vmaxu2(top, v.w[i] & 0x7FFF7FFFu);
+  }
+  return top;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t fold_top(uint32_t top) {
+  return sizeof(T) == 4 ? top : max(top & 0xFFFFu, top >> 16);
+}
+template <typename T>
+constexpr uint32_t non_finite() {
+  return sizeof(T) == 4 ? 0x7F800000u : std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
+}
+// The fp32 bits of a value given by the type's bits.
+template <typename T>
+__device__ __forceinline__ uint32_t float_bits(uint32_t bits) {
+  if constexpr (sizeof(T) == 4) {
+    return bits;
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return bits << 16;
+  } else {
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(bits))));
+  }
+}
+// Rare: zeroes infinities and NaNs for the maximum of a block that holds some.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_top_bits(const Eight<T>& v, uint32_t top) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t b = sizeof(T) == 4 ? v.w[i] & 0x7FFFFFFFu : (v.w[i / 2] >> (16 * (i & 1))) & 0x7FFFu;
+    if (b < non_finite<T>()) top = max(top, b);
+  }
+  return top;
+}
+
+// Eight e4m3 values; `odd`: the block holds infinities or NaNs, which become NaN.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(uint8_t* row, int64_t col, int64_t cols, const Eight<T>& v, float inv, bool odd) {
+  float f[8];
+  to_floats(v, f);
+  if (odd) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = isinf(f[i]) ? __uint_as_float(0x7FC00000u) : f[i];
+  }
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = e4m3_pair(v[2 * i], v[2 * i + 1], inv);
+  for (int i = 0; i < 4; ++i) w[i] = e4m3_pair(f[2 * i], f[2 * i + 1], inv);
   if constexpr (VEC) {
     if (col < cols) {
       *reinterpret_cast<uint2*>(row + col) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
@@ -102,47 +162,55 @@ __device__ __forceinline__ void store8(uint8_t* row, int64_t col, int64_t cols, 
   }
 }
 
+// n / d for n < 2^31 as a multiply and a shift: with 2^(s-1) < d <= 2^s and
+// m = ceil(2^(31+s) / d), n m / 2^(31+s) exceeds n / d by less than 1 / d.
+struct FastDiv {
+  uint32_t d, m, s;
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> s);
+  }
+};
+
 // Rows: 16 lanes hold one 1 x 128 block (8 elements each), so a warp's loads
-// are whole 256-byte pieces; kRowsUnroll blocks per half warp are in flight.
+// are whole 256-byte pieces; the loads of kRowsUnroll blocks per half warp are
+// in flight before the first is used.  One read and one write of every
+// element: bound by memory.
 constexpr int kRowsUnroll = 4;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
-                                                            int64_t pitch, uint8_t* __restrict__ q, int64_t q_pitch,
-                                                            uint8_t* __restrict__ scale) {
-  const int64_t kb = (cols + 127) / 128;
-  const int64_t blocks = rows * kb;
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, uint32_t blocks, FastDiv kb,
+                                                            int64_t cols, int64_t pitch, uint8_t* __restrict__ q,
+                                                            int64_t q_pitch, uint8_t* __restrict__ scale) {
   const int l = threadIdx.x & 15;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * 16;
-  for (int64_t b0 = blockIdx.x * 16ll + (threadIdx.x >> 4); b0 < blocks; b0 += stride * kRowsUnroll) {
-    float v[kRowsUnroll][8];
-    int64_t row[kRowsUnroll], col[kRowsUnroll];
+  const uint32_t half = 0xFFFFu << (threadIdx.x & 16);  // the halves of a warp may end at different blocks
+  const uint32_t stride = gridDim.x * 16u;
+  for (uint32_t b0 = blockIdx.x * 16u + (threadIdx.x >> 4); b0 < blocks; b0 += stride * kRowsUnroll) {
+    Eight<T> v[kRowsUnroll];
 #pragma unroll
     for (int u = 0; u < kRowsUnroll; ++u) {
-      const int64_t b = b0 + u * stride;
-      row[u] = b < blocks ? b / kb : -1;
-      col[u] = b < blocks ? (b - row[u] * kb) * 128 + l * 8 : 0;
-      if (row[u] >= 0) {
-        load8<T, VEC>(x + row[u] * pitch, col[u], cols, v[u]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+      const uint32_t b = b0 + u * stride;
+      if (b < blocks) {
+        const uint32_t row = kb.div(b);
+        v[u] = load8<T, VEC>(x + row * pitch, static_cast<int64_t>(b - row * kb.d) * 128 + l * 8, cols);
       }
     }
 #pragma unroll
     for (int u = 0; u < kRowsUnroll; ++u) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, finite_abs(v[u][i]));
-      // The 16 lanes of a block take every branch together; the other half
-      // warp may be past the end, so the shuffle names its own half only.
-      const uint32_t half = 0xFFFFu << (threadIdx.x & 16);
+      const uint32_t b = b0 + u * stride;
+      if (b >= blocks) break;
+      uint32_t top = fold_top<T>(top_bits<T>(v[u], 0u));
 #pragma unroll
       for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(half, top, d));
-      if (row[u] >= 0) {
-        const int byte = scale_byte(top);
-        store8<VEC>(q + row[u] * q_pitch, col[u], cols, v[u], inverse_scale(byte));
-        if (l == 0) scale[row[u] * kb + col[u] / 128] = static_cast<uint8_t>(byte);
+      const bool odd = top >= non_finite<T>();
+      if (odd) {
+        top = finite_top_bits<T>(v[u], 0u);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(half, top, d));
       }
+      const int byte = scale_byte(float_bits<T>(top));
+      const uint32_t row = kb.div(b);
+      store8<T, VEC>(q + row * q_pitch, static_cast<int64_t>(b - row * kb.d) * 128 + l * 8, cols, v[u],
+                     inverse_scale(byte), odd);
+      if (l == 0) scale[b] = static_cast<uint8_t>(byte);
     }
   }
 }
@@ -153,39 +221,44 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
                                                               int64_t pitch, int64_t matrix, uint8_t* __restrict__ q,
                                                               int64_t q_pitch, int64_t q_matrix,
-                                                              uint8_t* __restrict__ scale, int64_t kb, int64_t per) {
+                                                              uint8_t* __restrict__ scale, FastDiv kb, FastDiv per) {
   __shared__ uint32_t tops[8];
-  const int64_t e = blockIdx.x / per, in = blockIdx.x - e * per;
-  const int64_t r0 = in / kb * 128, c = (in - in / kb * kb) * 128 + (threadIdx.x & 15) * 8;
+  const uint32_t e = per.div(blockIdx.x), in = blockIdx.x - e * per.d;
+  const uint32_t rb = kb.div(in);
+  const int64_t r0 = rb * 128ll + (threadIdx.x >> 4), c = (in - rb * kb.d) * 128ll + (threadIdx.x & 15) * 8;
   const T* base = x + e * matrix;
-  float v[8][8];
+  Eight<T> v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = r0 + i * 16;
+    v[i] = load8<T, VEC>(base + r * pitch, r < rows ? c : cols, cols);
+  }
+  const auto reduce = [&](uint32_t top) {
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
+    return top;
+  };
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + i * 16 + (threadIdx.x >> 4);
-    if (r < rows) {
-      load8<T, VEC>(base + r * pitch, c, cols, v[i]);
-    } else {
+  for (int i = 0; i < 8; ++i) top = top_bits<T>(v[i], top);
+  top = reduce(fold_top<T>(top));
+  const bool odd = top >= non_finite<T>();  // the same in every thread
+  if (odd) {
+    top = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
-    }
+    for (int i = 0; i < 8; ++i) top = finite_top_bits<T>(v[i], top);
+    top = reduce(top);
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = max(top, finite_abs(v[i][k]));
-  }
-  top = __reduce_max_sync(0xFFFFFFFFu, top);
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, tops[i]);
-  const int byte = scale_byte(top);
+  const int byte = scale_byte(float_bits<T>(top));
   const float inv = inverse_scale(byte);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + i * 16 + (threadIdx.x >> 4);
-    if (r < rows) store8<VEC>(q + e * q_matrix + r * q_pitch, c, cols, v[i], inv);
+    const int64_t r = r0 + i * 16;
+    if (r < rows) store8<T, VEC>(q + e * q_matrix + r * q_pitch, c, cols, v[i], inv, odd);
   }
   if (threadIdx.x == 0) scale[blockIdx.x] = static_cast<uint8_t>(byte);
 }
@@ -767,7 +840,7 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
 constexpr int kFewWarps = 8;
 
 template <int NT>
-__global__ void __launch_bounds__(kFewWarps * 32) mx_few_kernel(const __grid_constant__ MxParams p) {
+__global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_constant__ MxParams p) {
   __shared__ float sums[kFewWarps][NT * 8][17];  // [warp][token][row], padded against bank conflicts
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -788,50 +861,57 @@ __global__ void __launch_bounds__(kFewWarps * 32) mx_few_kernel(const __grid_con
     wrow[h] = p.b + e * p.b_stride + (live[h] ? r : 0) * p.b_pitch + t * 16;
   }
   const uint8_t* wscale = p.sb + (e * p.nb + r0 / 128) * p.kb;  // 16 rows lie inside one 128-row block
+  const int depth = static_cast<int>(p.k), kblocks = static_cast<int>(p.kb);
   for (int64_t m0 = 0; m0 < len; m0 += 8 * NT) {
     float acc[NT][4];
-    const uint8_t* xrow[NT];
-    bool has[NT];
+    const uint8_t* xrow = p.a + (start + m0 + g) * p.a_pitch + t * 16;     // token m0 + g (+ 8 i)
+    const uint8_t* xscale = p.sa + (start + m0 + 2 * t) * p.kb;            // tokens m0 + 2t, 2t + 1 (+ 8 i)
+    const int left = static_cast<int>(len - m0 < 8 * NT ? len - m0 : 8 * NT);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-      const int64_t m = m0 + i * 8 + g;
-      has[i] = m < len;
-      xrow[i] = p.a + (start + (has[i] ? m : 0)) * p.a_pitch + t * 16;
-    }
-#pragma unroll(NT <= 1 ? 4 : 2)
-    for (int64_t kb = warp; kb < p.kb; kb += kFewWarps) {
+    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+    // U blocks' weights are in flight before the first is used; a block past
+    // the end loads nothing (7 blocks a warp at K = 7168: two rounds of four).
+    constexpr int U = NT == 1 ? 4 : 2;
+#pragma unroll 1
+    for (int kb0 = warp; kb0 < kblocks; kb0 += kFewWarps * U) {
       // K is a multiple of 16: a 16-byte piece is inside the row or past its end.
-      uint4 w[2][2], x[NT][2];
+      uint4 w[U][2][2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int64_t k = kb * 128 + c * 64;
-        const bool in = k + t * 16 < p.k;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          w[h][c] = in && live[h] ? __ldcs(reinterpret_cast<const uint4*>(wrow[h] + k)) : zero;
-        }
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          x[i][c] = in && has[i] ? __ldg(reinterpret_cast<const uint4*>(xrow[i] + k)) : zero;
-        }
-      }
-      const float sw = scale_value(__ldg(wscale + kb));
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          mma_e4m3(part, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, x[i][c].x, x[i][c].y);
-          mma_e4m3(part, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, x[i][c].z, x[i][c].w);
-        }
-        // Columns 2t, 2t + 1 of the accumulator are tokens m0 + 8 i + 2t (+ 1).
+          const int k = (kb0 + u * kFewWarps) * 128 + c * 64;
+          const bool in = k + t * 16 < depth;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int64_t m = m0 + i * 8 + 2 * t + j;
-          const float sx = m < len ? scale_value(__ldg(p.sa + (start + m) * p.kb + kb)) : 0.0f;
-          acc[i][j] += part[j] * sw * sx;
-          acc[i][2 + j] += part[2 + j] * sw * sx;
+          for (int h = 0; h < 2; ++h) {
+            w[u][h][c] = in && live[h] ? __ldcs(reinterpret_cast<const uint4*>(wrow[h] + k)) : zero;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int kb = kb0 + u * kFewWarps;
+        if (kb >= kblocks) break;
+        const float sw = scale_value(__ldg(wscale + kb));
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int k = kb * 128 + c * 64;
+            const uint4 x = 8 * i + g < left && k + t * 16 < depth
+                                ? __ldg(reinterpret_cast<const uint4*>(xrow + 8 * i * p.a_pitch + k))
+                                : zero;
+            mma_e4m3(part, w[u][0][c].x, w[u][1][c].x, w[u][0][c].y, w[u][1][c].y, x.x, x.y);
+            mma_e4m3(part, w[u][0][c].z, w[u][1][c].z, w[u][0][c].w, w[u][1][c].w, x.z, x.w);
+          }
+          // Columns 2t, 2t + 1 of the accumulator are tokens m0 + 8 i + 2t (+ 1).
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float sx = 8 * i + 2 * t + j < left ? scale_value(__ldg(xscale + (8 * i + j) * p.kb + kb)) : 0.0f;
+            acc[i][j] += part[j] * sw * sx;
+            acc[i][2 + j] += part[2 + j] * sw * sx;
+          }
         }
       }
     }

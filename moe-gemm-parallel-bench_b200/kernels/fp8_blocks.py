@@ -27,15 +27,15 @@ except ImportError:  # pragma: no cover - the CPU tests import the host helpers 
 
 from . import _native
 from .fp8 import FP8_BLOCK, _blocks
-from .gated_ffn import _offsets, _require_runtime
+from .gated_ffn import _call, _offsets, _require_runtime
 from .matmul import dtype_name
 
-_last_info: dict | None = None
+_last_info = None
 
 
 def last_block_scaled_info() -> dict | None:
     """Native kernel of the most recent launch_block_scaled_mm call (path, tile, grid)."""
-    return _last_info
+    return None if _last_info is None else _last_info.as_dict()
 
 
 def _source(x) -> int:
@@ -68,9 +68,7 @@ def launch_quantize_rows(x, q=None, scale=None):
     pitch = x.stride(0) if rows > 1 else cols
     if pitch < cols:
         raise ValueError("rows of x must not overlap")
-    with torch.cuda.device(device):
-        _native.quantize_rows(x.data_ptr(), rows, cols, pitch, code, q.data_ptr(), cols, scale.data_ptr(),
-                              torch.cuda.current_stream(device).cuda_stream)
+    _call(device, _native.quantize_rows, x.data_ptr(), rows, cols, pitch, code, q.data_ptr(), cols, scale.data_ptr())
     return q, scale
 
 
@@ -91,9 +89,8 @@ def launch_quantize_blocks(w, q=None, scale=None):
     stride = w.stride(0) if matrices > 1 else n * pitch
     if pitch < k or (matrices > 1 and stride < (n - 1) * pitch + k):
         raise ValueError("rows and matrices of w must not overlap")
-    with torch.cuda.device(device):
-        _native.quantize_blocks(w.data_ptr(), matrices, n, k, pitch, stride, code, q.data_ptr(), scale.data_ptr(),
-                                torch.cuda.current_stream(device).cuda_stream)
+    _call(device, _native.quantize_blocks, w.data_ptr(), matrices, n, k, pitch, stride, code, q.data_ptr(),
+          scale.data_ptr())
     return q, scale
 
 
@@ -111,7 +108,8 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
     _require_runtime()
     if a.ndim != 2 or b.ndim not in (2, 3):
         raise ValueError("expected a [T, K] and b [N, K] or [E, N, K]")
-    if not a.is_cuda or len({a.device, sa.device, b.device, sb.device}) != 1:
+    device = a.device
+    if not a.is_cuda or sa.device != device or b.device != device or sb.device != device:
         raise ValueError("a, sa, b and sb must be on the same CUDA device")
     if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
         raise ValueError("a and b must be float8_e4m3fn")
@@ -127,27 +125,23 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
                          f"b {tuple(b.shape)} in blocks of {FP8_BLOCK}")
     if not sa.is_contiguous() or not sb.is_contiguous():
         raise ValueError("scales must be contiguous")
-    device = a.device
-    ends = _offsets(offs, experts, a)
+    ends = _offsets(offs, experts, device)
     if out is None:
         out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
     elif tuple(out.shape) != (rows, n) or out.dtype != torch.bfloat16 or out.device != device:
         raise ValueError(f"out must be [{rows}, {n}] bfloat16 on {device}")
-    a_pitch = a.stride(0) if rows > 1 else k
-    out_pitch = out.stride(0) if rows > 1 else n
-    b_pitch = b.stride(-2) if n > 1 else k
-    b_stride = b.stride(0) if experts > 1 else n * b_pitch
-    if a.stride(1) != 1 or b.stride(-1) != 1 or out.stride(1) != 1 or a_pitch < k or a_pitch % 16 or b_pitch < k or (
+    a_steps, b_steps, out_steps = a.stride(), b.stride(), out.stride()
+    a_pitch = a_steps[0] if rows > 1 else k
+    out_pitch = out_steps[0] if rows > 1 else n
+    b_pitch = b_steps[-2]
+    b_stride = b_steps[0] if experts > 1 else n * b_pitch
+    if a_steps[1] != 1 or b_steps[-1] != 1 or out_steps[1] != 1 or a_pitch < k or a_pitch % 16 or b_pitch < k or (
             b_pitch % 16) or b_stride % 16 or (experts > 1 and b_stride < (n - 1) * b_pitch + k) or out_pitch < n or (
             out_pitch % 8) or (a.data_ptr() | b.data_ptr() | out.data_ptr()) % 16:
         raise ValueError("a, b and out need contiguous columns, 16-byte aligned bases and rows a whole number of 16 "
                          "bytes apart that do not overlap")
-    scratch = torch.empty(_native.block_scaled_scratch_bytes(experts), dtype=torch.uint8, device=device)
-    with torch.cuda.device(device):
-        info = _native.block_scaled_mm(
-            a.data_ptr(), a_pitch, sa.data_ptr(), b.data_ptr(), b_pitch, b_stride, sb.data_ptr(), out.data_ptr(),
-            out_pitch, ends, experts, rows, n, k, scratch.data_ptr(), scratch.numel(),
-            torch.cuda.current_stream(device).cuda_stream,
-        )
-    _last_info = info.as_dict()
+    nbytes = _native.block_scaled_scratch_bytes(experts, rows)
+    scratch = a.new_empty(nbytes).data_ptr() if nbytes else 0
+    _last_info = _call(device, _native.block_scaled_mm, a.data_ptr(), a_pitch, sa.data_ptr(), b.data_ptr(), b_pitch,
+                       b_stride, sb.data_ptr(), out.data_ptr(), out_pitch, ends, experts, rows, n, k, scratch, nbytes)
     return out

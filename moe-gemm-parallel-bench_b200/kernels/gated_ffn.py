@@ -39,36 +39,57 @@ from . import _native
 from .matmul import dtype_name
 
 
+_ready = False
+
+
 def _require_runtime() -> None:
-    if torch is None or not torch.cuda.is_available():
-        raise RuntimeError("CUDA PyTorch and the native sm_100a library are required")
-    _native.load()
+    global _ready
+    if not _ready:
+        if torch is None or not torch.cuda.is_available():
+            raise RuntimeError("CUDA PyTorch and the native sm_100a library are required")
+        _native.load()
+        _ready = True
 
 
-def _token(name: str, t, rows: int, cols: int, like) -> tuple[int, int]:
-    """(address, pitch) of a [rows, cols] tensor of `like`'s type and device."""
-    if t.ndim != 2 or t.shape[0] != rows or t.shape[1] != cols:
+def _call(device, entry, *args):
+    """entry(*args, stream) with ``device`` current and its current stream.
+    These calls can be as short as their host side (a few microseconds on the
+    device), so the guard is taken only where it changes something and the
+    stream handle is read without building a Stream object."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _token(name: str, t, rows: int, cols: int, dtype, device) -> tuple[int, int]:
+    """(address, pitch) of a [rows, cols] tensor of the call's type and device."""
+    if tuple(t.shape) != (rows, cols):
         raise ValueError(f"{name} must be [{rows}, {cols}], got {tuple(t.shape)}")
-    if t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    pitch = t.stride(0) if rows > 1 else cols
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
+    pitch, step = t.stride()
+    if rows <= 1:
+        pitch = cols
     address = t.data_ptr()
-    if t.stride(1) != 1 or pitch < cols or pitch % 8 or address % 16:
+    if step != 1 or pitch < cols or pitch % 8 or address % 16:
         raise ValueError(f"{name} needs contiguous columns, a 16-byte aligned base and a row pitch that is a multiple of 8")
     return address, pitch
 
 
-def _weight(name: str, t, experts: int, rows: int, cols: int, like) -> tuple[int, int, int]:
+def _weight(name: str, t, experts: int, rows: int, cols: int, dtype, device) -> tuple[int, int, int]:
     """(address, pitch, expert stride) of an [experts, rows, cols] weight (or [rows, cols] for one expert)."""
-    dense = t.ndim == 2 and experts == 1
-    if tuple(t.shape) != ((rows, cols) if dense else (experts, rows, cols)):
-        raise ValueError(f"{name} must be [{experts}, {rows}, {cols}], got {tuple(t.shape)}")
-    if t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    pitch = t.stride(-2)
-    stride = t.stride(0) if experts > 1 else rows * pitch
+    shape = tuple(t.shape)
+    if shape != (experts, rows, cols) and not (experts == 1 and shape == (rows, cols)):
+        raise ValueError(f"{name} must be [{experts}, {rows}, {cols}], got {shape}")
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
+    strides = t.stride()
+    pitch = strides[-2]
+    stride = strides[0] if experts > 1 else rows * pitch
     address = t.data_ptr()
-    if t.stride(-1) != 1 or pitch < cols or pitch % 8 or stride % 8 or address % 16 or (
+    if strides[-1] != 1 or pitch < cols or pitch % 8 or stride % 8 or address % 16 or (
             experts > 1 and stride < (rows - 1) * pitch + cols):
         raise ValueError(f"{name} needs contiguous columns, a 16-byte aligned base, a row pitch and an expert stride "
                          "that are multiples of 8, and experts that do not overlap")
@@ -84,15 +105,15 @@ def _operand_type(name: str, t) -> int:
     return code
 
 
-def _offsets(offs, experts: int, like) -> int:
+def _offsets(offs, experts: int, device) -> int:
     """Address of the row ends (0: one segment of every row)."""
     if offs is None:
         if experts != 1:
             raise ValueError("offs (int32 cumulative row ends) is needed with more than one expert")
         return 0
-    if offs.ndim != 1 or offs.shape[0] != experts or offs.dtype != torch.int32 or not offs.is_contiguous():
+    if tuple(offs.shape) != (experts,) or offs.dtype != torch.int32 or not offs.is_contiguous():
         raise ValueError(f"offs must be contiguous int32 [{experts}] cumulative row ends")
-    if offs.device != like.device:
+    if offs.device != device:
         raise ValueError("offs must be on the tensors' device")
     return offs.data_ptr()
 
@@ -110,10 +131,6 @@ def _block_shape(x, w13, w2) -> tuple[int, int, int, int]:
     return x.shape[0], (w13.shape[0] if w13.ndim == 3 else 1), hidden, ffn
 
 
-def _scratch(experts: int, jobs: int, device):
-    return torch.empty(_native.ffn_scratch_bytes(experts, jobs), dtype=torch.uint8, device=device)
-
-
 def gated_ffn_forward(x, w13, w2, offs=None, *, out=None, h=None, gate_up=None):
     """(y, h, gate_up) of the block: ``x [T, H]``, ``w13 [E, H, 2F]`` packed
     [gate | up], ``w2 [E, F, H]``; ``[H, 2F]`` and ``[F, H]`` for one expert.
@@ -123,24 +140,23 @@ def gated_ffn_forward(x, w13, w2, offs=None, *, out=None, h=None, gate_up=None):
     _require_runtime()
     rows, experts, hidden, ffn = _block_shape(x, w13, w2)
     code = _operand_type("x", x)
-    device = x.device
-    args = _native.FfnArgs(code, experts, rows, hidden, ffn, _offsets(offs, experts, x))
-    args.x, args.x_pitch = _token("x", x, rows, hidden, x)
-    args.w13, args.w13_pitch, args.w13_stride = _weight("w13", w13, experts, hidden, 2 * ffn, x)
-    args.w2, args.w2_pitch, args.w2_stride = _weight("w2", w2, experts, ffn, hidden, x)
+    dtype, device = x.dtype, x.device
+    args = _native.FfnArgs(code, experts, rows, hidden, ffn, _offsets(offs, experts, device))
+    args.x, args.x_pitch = _token("x", x, rows, hidden, dtype, device)
+    args.w13, args.w13_pitch, args.w13_stride = _weight("w13", w13, experts, hidden, 2 * ffn, dtype, device)
+    args.w2, args.w2_pitch, args.w2_stride = _weight("w2", w2, experts, ffn, hidden, dtype, device)
     if out is None:
-        out = torch.empty((rows, hidden), dtype=x.dtype, device=device)
+        out = x.new_empty((rows, hidden))
     if h is None:
-        h = torch.empty((rows, ffn), dtype=x.dtype, device=device)
+        h = x.new_empty((rows, ffn))
     if gate_up is None:
-        gate_up = torch.empty((rows, 2 * ffn), dtype=x.dtype, device=device)
-    args.y, args.y_pitch = _token("out", out, rows, hidden, x)
-    args.h, args.h_pitch = _token("h", h, rows, ffn, x)
-    args.gate_up, args.gate_up_pitch = _token("gate_up", gate_up, rows, 2 * ffn, x)
-    scratch = _scratch(experts, 2, device)
-    with torch.cuda.device(device):
-        _native.gated_ffn_forward(args, scratch.data_ptr(), scratch.numel(),
-                                  torch.cuda.current_stream(device).cuda_stream)
+        gate_up = x.new_empty((rows, 2 * ffn))
+    args.y, args.y_pitch = _token("out", out, rows, hidden, dtype, device)
+    args.h, args.h_pitch = _token("h", h, rows, ffn, dtype, device)
+    args.gate_up, args.gate_up_pitch = _token("gate_up", gate_up, rows, 2 * ffn, dtype, device)
+    nbytes = _native.ffn_scratch_bytes(experts, 2)
+    scratch = x.new_empty(nbytes // 2)
+    _call(device, _native.gated_ffn_forward, args, scratch.data_ptr(), nbytes)
     return out, h, gate_up
 
 
@@ -152,29 +168,31 @@ def gated_ffn_backward(dy, x, w13, w2, h, gate_up, offs=None, *, dx=None, dw13=N
     _require_runtime()
     rows, experts, hidden, ffn = _block_shape(x, w13, w2)
     code = _operand_type("x", x)
-    device = x.device
-    args = _native.FfnArgs(code, experts, rows, hidden, ffn, _offsets(offs, experts, x))
-    args.y, args.y_pitch = _token("dy", dy, rows, hidden, x)
-    args.x, args.x_pitch = _token("x", x, rows, hidden, x)
-    args.w13, args.w13_pitch, args.w13_stride = _weight("w13", w13, experts, hidden, 2 * ffn, x)
-    args.w2, args.w2_pitch, args.w2_stride = _weight("w2", w2, experts, ffn, hidden, x)
-    args.h, args.h_pitch = _token("h", h, rows, ffn, x)
-    args.gate_up, args.gate_up_pitch = _token("gate_up", gate_up, rows, 2 * ffn, x)
+    dtype, device = x.dtype, x.device
+    args = _native.FfnArgs(code, experts, rows, hidden, ffn, _offsets(offs, experts, device))
+    args.y, args.y_pitch = _token("dy", dy, rows, hidden, dtype, device)
+    args.x, args.x_pitch = _token("x", x, rows, hidden, dtype, device)
+    args.w13, args.w13_pitch, args.w13_stride = _weight("w13", w13, experts, hidden, 2 * ffn, dtype, device)
+    args.w2, args.w2_pitch, args.w2_stride = _weight("w2", w2, experts, ffn, hidden, dtype, device)
+    args.h, args.h_pitch = _token("h", h, rows, ffn, dtype, device)
+    args.gate_up, args.gate_up_pitch = _token("gate_up", gate_up, rows, 2 * ffn, dtype, device)
     if dx is None:
-        dx = torch.empty((rows, hidden), dtype=x.dtype, device=device)
+        dx = x.new_empty((rows, hidden))
     if dw13 is None:
-        dw13 = torch.empty(w13.shape, dtype=x.dtype, device=device)
+        dw13 = w13.new_empty(w13.shape)
     if dw2 is None:
-        dw2 = torch.empty(w2.shape, dtype=x.dtype, device=device)
-    dgate_up = torch.empty((rows, 2 * ffn), dtype=x.dtype, device=device)
-    args.dgate_up, args.dgate_up_pitch = dgate_up.data_ptr(), 2 * ffn
-    args.dx, args.dx_pitch = _token("dx", dx, rows, hidden, x)
-    args.dw13, args.dw13_pitch, args.dw13_stride = _weight("dw13", dw13, experts, hidden, 2 * ffn, x)
-    args.dw2, args.dw2_pitch, args.dw2_stride = _weight("dw2", dw2, experts, ffn, hidden, x)
-    scratch = _scratch(experts, 4, device)
-    with torch.cuda.device(device):
-        _native.gated_ffn_backward(args, scratch.data_ptr(), scratch.numel(),
-                                   torch.cuda.current_stream(device).cuda_stream)
+        dw2 = w2.new_empty(w2.shape)
+    args.dx, args.dx_pitch = _token("dx", dx, rows, hidden, dtype, device)
+    args.dw13, args.dw13_pitch, args.dw13_stride = _weight("dw13", dw13, experts, hidden, 2 * ffn, dtype, device)
+    args.dw2, args.dw2_pitch, args.dw2_stride = _weight("dw2", dw2, experts, ffn, hidden, dtype, device)
+    # One workspace: the gradient of gate_up between the two launches, then
+    # the scratch (128-byte aligned behind it).
+    behind = -(-rows * 2 * ffn // 64) * 64
+    nbytes = _native.ffn_scratch_bytes(experts, 4)
+    workspace = x.new_empty(behind + nbytes // 2)
+    at = workspace.data_ptr()
+    args.dgate_up, args.dgate_up_pitch = at, 2 * ffn
+    _call(device, _native.gated_ffn_backward, args, at + behind * 2, nbytes)
     return dx, dw13, dw2
 
 
@@ -194,21 +212,20 @@ def launch_grouped_mm_dgrad(dc, mat_b, offs=None, out=None, *, gate_up=None):
     _sizes(n, k)
     code = _operand_type("dc", dc)
     device = dc.device
-    ends = _offsets(offs, experts, dc)
-    dc_at, dc_pitch = _token("dc", dc, rows, n, dc)
-    b_at, b_pitch, b_stride = _weight("mat_b", mat_b, experts, k, n, dc)
+    ends = _offsets(offs, experts, device)
+    dc_at, dc_pitch = _token("dc", dc, rows, n, dc.dtype, device)
+    b_at, b_pitch, b_stride = _weight("mat_b", mat_b, experts, k, n, dc.dtype, device)
     cols = k if gate_up is None else 2 * k
-    gu_at, gu_pitch = (0, 0) if gate_up is None else _token("gate_up", gate_up, rows, cols, dc)
+    gu_at, gu_pitch = (0, 0) if gate_up is None else _token("gate_up", gate_up, rows, cols, dc.dtype, device)
     if out is None:
-        out = torch.empty((rows, cols), dtype=dc.dtype, device=device)
-    out_at, out_pitch = _token("out", out, rows, cols, dc)
+        out = dc.new_empty((rows, cols))
+    out_at, out_pitch = _token("out", out, rows, cols, dc.dtype, device)
     if rows == 0:
         return out
-    scratch = _scratch(experts, 1, device)
-    with torch.cuda.device(device):
-        _native.grouped_dgrad(dc_at, dc_pitch, b_at, b_pitch, b_stride, ends, experts, rows, n, k, gu_at, gu_pitch,
-                              out_at, out_pitch, code, scratch.data_ptr(), scratch.numel(),
-                              torch.cuda.current_stream(device).cuda_stream)
+    nbytes = _native.ffn_scratch_bytes(experts, 1)
+    scratch = dc.new_empty(nbytes // 2)
+    _call(device, _native.grouped_dgrad, dc_at, dc_pitch, b_at, b_pitch, b_stride, ends, experts, rows, n, k, gu_at,
+          gu_pitch, out_at, out_pitch, code, scratch.data_ptr(), nbytes)
     return out
 
 
@@ -228,15 +245,14 @@ def launch_grouped_mm_wgrad(mat_a, dc, offs=None, out=None):
     experts = 1 if offs is None else int(offs.numel())
     if experts == 0:
         raise ValueError("offs is empty")
-    ends = _offsets(offs, experts, mat_a)
-    a_at, a_pitch = _token("mat_a", mat_a, rows, k, mat_a)
-    dc_at, dc_pitch = _token("dc", dc, rows, n, mat_a)
+    ends = _offsets(offs, experts, device)
+    a_at, a_pitch = _token("mat_a", mat_a, rows, k, mat_a.dtype, device)
+    dc_at, dc_pitch = _token("dc", dc, rows, n, mat_a.dtype, device)
     if out is None:
-        out = torch.empty((k, n) if offs is None else (experts, k, n), dtype=mat_a.dtype, device=device)
-    out_at, out_pitch, out_stride = _weight("out", out, experts, k, n, mat_a)
-    scratch = _scratch(experts, 1, device)
-    with torch.cuda.device(device):
-        _native.grouped_wgrad(a_at, a_pitch, dc_at, dc_pitch, ends, experts, rows, n, k, out_at, out_pitch,
-                              out_stride, code, scratch.data_ptr(), scratch.numel(),
-                              torch.cuda.current_stream(device).cuda_stream)
+        out = mat_a.new_empty((k, n) if offs is None else (experts, k, n))
+    out_at, out_pitch, out_stride = _weight("out", out, experts, k, n, mat_a.dtype, device)
+    nbytes = _native.ffn_scratch_bytes(experts, 1)
+    scratch = mat_a.new_empty(nbytes // 2)
+    _call(device, _native.grouped_wgrad, a_at, a_pitch, dc_at, dc_pitch, ends, experts, rows, n, k, out_at, out_pitch,
+          out_stride, code, scratch.data_ptr(), nbytes)
     return out

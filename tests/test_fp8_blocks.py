@@ -356,8 +356,9 @@ def test_abi_refuses_bad_arguments_before_any_launch():
     for change in bad:
         assert product(**change) == _native.STATUS_INVALID, change
     for change in (dict(scratch=None), dict(scratch=at + 16), dict(scratch_bytes=64)):
+        change["rows"] = 100  # more than a few a expert: maps are needed
         assert product(**change) == _native.STATUS_SCRATCH, change
-    assert lib.block_scaled_mm_scratch_bytes(0) == 0
+    assert lib.block_scaled_mm_scratch_bytes(0, 10) == 0 and lib.block_scaled_mm_scratch_bytes(2, 10) == 0
     for change in ((None, 4, 8, 8, 1, at, 8, at, None), (at, 4, 0, 8, 1, at, 8, at, None),
                    (at, 4, 8, 7, 1, at, 8, at, None), (at, 4, 8, 8, 5, at, 8, at, None), (at + 1, 4, 8, 8, 1, at, 8, at, None)):
         assert lib.quantize_rows_launch(*change) == _native.STATUS_INVALID, change
