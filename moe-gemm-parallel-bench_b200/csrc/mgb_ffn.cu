@@ -144,7 +144,6 @@ struct Launcher {
   void wgrad_job(const FfnTensor& a, const FfnTensor& b, const FfnTensor& c, int64_t m, int64_t n) {
     FfnJob& j = begin_job();
     j.wgrad = 1;
-    j.a_mn = j.b_mn = 1;
     j.m = m;
     j.n = n;
     add(a, plan.rows, m, kMnMajor);

@@ -55,7 +55,7 @@ struct FfnJob {
   FfnTensor t[kFfnMaps];
   int32_t maps;   // tensors used
   int32_t wgrad;  // contraction over the segment's rows
-  int32_t a_mn, b_mn;
+  int32_t b_mn;   // rows: B is MN-major (wgrad: both operands are)
   int64_t m;      // wgrad: output rows
   int64_t n;      // output columns
   int64_t k;      // rows: contraction depth
@@ -307,6 +307,25 @@ struct FfnGateLoads {
   }
 };
 
+// Calls f(a_mn, b_mn) with the job's operand layouts as compile-time
+// constants, so that the loops per contraction block hold no layout branch.
+template <int EPI, class F>
+__device__ __forceinline__ void by_layout(const FfnJob& j, F&& f) {
+  using No = std::integral_constant<bool, false>;
+  using Yes = std::integral_constant<bool, true>;
+  if constexpr (EPI == kFfnSwiglu) {
+    f(No{}, Yes{});
+  } else if constexpr (EPI == kFfnSwigluBwd) {
+    f(No{}, No{});
+  } else if (j.wgrad) {
+    f(Yes{}, Yes{});
+  } else if (j.b_mn) {
+    f(No{}, Yes{});
+  } else {
+    f(No{}, No{});
+  }
+}
+
 template <typename T, int EPI, int G>
 __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constant__ FfnParams p) {
   using Cfg = FfnCfg<T, EPI, G>;
@@ -374,110 +393,104 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    const uint64_t pol_keep = policy_evict_last();
-    const uint64_t pol_shared = policy_evict_normal();
-    const uint64_t pol_stream = policy_evict_first();
-    FfnWalk walk;
-    uint32_t it = 0;
-    int built = -1;
-    bool ok = true;
-    for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
-      const FfnJob& j = *walk.job;
-      int64_t mb, nb;
-      walk.blocks(t, mb, nb);
-      const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.pair) * kFfnMaps;
-      if (walk.pair != built) {
-        if (lane == 0) {
+    // One thread; stage and phase step along instead of dividing a counter.
+    if (lane == 0) {
+      const uint64_t pol_keep = policy_evict_last();
+      const uint64_t pol_shared = policy_evict_normal();
+      const uint64_t pol_stream = policy_evict_first();
+      const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), empty0 = smem_u32(empty);
+      const uint32_t lead0 = G == 2 ? mapa_shared(full0, 0) : full0;  // the leader's barriers
+      FfnWalk walk;
+      int s = 0;
+      uint32_t phase = 0, loaded = 0;
+      int built = -1;
+      bool ok = true;
+      for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+        const FfnJob& j = *walk.job;
+        int64_t mb, nb;
+        walk.blocks(t, mb, nb);
+        const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.pair) * kFfnMaps;
+        if (walk.pair != built) {
           tmap_acquire(&g[0]);
           tmap_acquire(&g[1]);
+          built = walk.pair;
         }
-        __syncwarp();
-        built = walk.pair;
-      }
-      const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128);
-      // First B column of this CTA's two 64-column boxes (swiglu: gate and up
-      // columns of the same outputs; a pair's CTA 0 holds gate, CTA 1 up).
-      int32_t b0, b1;
-      if constexpr (EPI == kFfnSwiglu) {
-        const int32_t o = static_cast<int32_t>(nb * Cfg::kTileOut);
-        if constexpr (G == 2) {
-          b0 = o + (rank ? static_cast<int32_t>(j.up) : 0);
-          b1 = b0 + 64;
+        const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128);
+        // First B column of this CTA's two 64-column boxes (swiglu: gate and up
+        // columns of the same outputs; a pair's CTA 0 holds gate, CTA 1 up).
+        int32_t b0, b1;
+        if constexpr (EPI == kFfnSwiglu) {
+          const int32_t o = static_cast<int32_t>(nb * Cfg::kTileOut);
+          if constexpr (G == 2) {
+            b0 = o + (rank ? static_cast<int32_t>(j.up) : 0);
+            b1 = b0 + 64;
+          } else {
+            b0 = o;
+            b1 = o + static_cast<int32_t>(j.up);
+          }
         } else {
-          b0 = o;
-          b1 = o + static_cast<int32_t>(j.up);
+          b0 = static_cast<int32_t>(nb * Cfg::kAccCols + rank * 128);
+          b1 = b0 + 64;
         }
-      } else {
-        b0 = static_cast<int32_t>(nb * Cfg::kAccCols + rank * 128);
-        b1 = b0 + 64;
-      }
-      // Weights that one row block reads are streamed; shared operands keep
-      // normal priority; activations of a rows job are kept for the other
-      // column blocks.
-      const uint64_t pol_a = j.wgrad ? pol_shared : pol_keep;
-      const uint64_t pol_b = !j.wgrad && walk.m_blocks == 1 ? pol_stream : pol_shared;
-      for (int64_t kb = 0; kb < walk.kblocks; ++kb) {
-        const int s = static_cast<int>(it % S);
-        if (!mbar_wait_warp(&empty[s], ((it / S) & 1u) ^ 1u, budget, abort)) {
-          if (lane == 0) fail(kErrWaitEmpty);
-          ok = false;
-          break;
-        }
-        if (lane == 0) {
-          uint8_t* st_a = ring + s * Cfg::kStageBytes;
-          uint8_t* st_b = st_a + Cfg::kOperand;
-          const int32_t kx = static_cast<int32_t>(kb * BK);
-          auto load = [&](const CUtensorMap* map, uint8_t* dst, int32_t x, int32_t y, uint64_t pol) {
-            if constexpr (G == 2) {
-              tma_load_2d_pair(map, mapa_shared(smem_u32(&full[s]), 0), dst, x, y, pol);
-            } else {
-              tma_load_2d(map, &full[s], dst, x, y, pol);
+        // Weights that one row block reads are streamed; shared operands keep
+        // normal priority; activations of a rows job are kept for the other
+        // column blocks.
+        const uint64_t pol_a = j.wgrad ? pol_shared : pol_keep;
+        const uint64_t pol_b = !j.wgrad && walk.m_blocks == 1 ? pol_stream : pol_shared;
+        const int32_t end = static_cast<int32_t>(walk.kblocks) * BK;
+        const auto load = [&](const CUtensorMap* map, uint32_t dst, int32_t x, int32_t y, uint64_t pol) {
+          tile_load<G>(map, lead0 + s * 8, dst, x, y, pol);
+        };
+        const auto run = [&](auto a_mn, auto b_mn) {
+          for (int32_t kx = 0; kx < end; kx += BK) {
+            if (!bar_wait(empty0 + s * 8, phase ^ 1u, budget, abort)) {
+              fail(kErrWaitEmpty);
+              ok = false;
+              break;
             }
-          };
-          if (leader) mbar_arrive_expect_tx(&full[s], G * Cfg::kStageBytes);
-          if (j.a_mn) {
-            load(&g[0], st_a, m0, kx, pol_a);
-            load(&g[0], st_a + Cfg::kOperand / 2, m0 + 64, kx, pol_a);
-          } else {
-            load(&g[0], st_a, kx, m0, pol_a);
+            const uint32_t st_a = ring0 + s * Cfg::kStageBytes, st_b = st_a + Cfg::kOperand;
+            if (leader) mbar_arrive_expect_tx(&full[s], G * Cfg::kStageBytes);
+            if constexpr (a_mn.value) {
+              load(&g[0], st_a, m0, kx, pol_a);
+              load(&g[0], st_a + Cfg::kOperand / 2, m0 + 64, kx, pol_a);
+            } else {
+              load(&g[0], st_a, kx, m0, pol_a);
+            }
+            if constexpr (b_mn.value) {
+              load(&g[1], st_b, b0, kx, pol_b);
+              load(&g[1], st_b + Cfg::kOperand / 2, b1, kx, pol_b);
+            } else {
+              load(&g[1], st_b, kx, b0, pol_b);
+            }
+            ++loaded;
+            if (++s == S) {
+              s = 0;
+              phase ^= 1u;
+            }
           }
-          if (j.b_mn) {
-            load(&g[1], st_b, b0, kx, pol_b);
-            load(&g[1], st_b + Cfg::kOperand / 2, b1, kx, pol_b);
-          } else {
-            load(&g[1], st_b, kx, b0, pol_b);
+        };
+        by_layout<EPI>(j, run);
+      }
+      if (*abort && leader) {  // loads in flight land before the CTA's memory goes away
+        for (uint32_t i = loaded > static_cast<uint32_t>(S) ? loaded - S : 0u; i < loaded; ++i) {
+          if (!bar_wait(full0 + (i % S) * 8, (i / S) & 1u, budget, never)) {
+            atomicOr(p.error_word, kErrWaitTeardown);
+            break;
           }
         }
-        __syncwarp();
-        ++it;
       }
     }
-    if (*abort && leader && lane == 0) {  // loads in flight land before the CTA's memory goes away
-      for (uint32_t i = it > static_cast<uint32_t>(S) ? it - S : 0u; i < it; ++i) {
-        if (!mbar_wait(&full[i % S], (i / S) & 1u, budget, never)) {
-          atomicOr(p.error_word, kErrWaitTeardown);
-          break;
-        }
-      }
-    }
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer (leader only)
     if (lane == 0 && leader) {
+      const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty);
       FfnWalk walk;
-      uint32_t it = 0, acc_it = 0;
+      int s = 0;
+      uint32_t phase = 0, acc_it = 0;
       bool ok = true;
       for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
         if (walk.kblocks <= 0) continue;
-        const FfnJob& j = *walk.job;
-        // K-major: a k-step of 16 is 32 bytes along the swizzled row.
-        // MN-major: 16 contraction rows of 128 bytes; the second 64 columns
-        // one box (8 KB) on.
-        const uint64_t a_desc = smem_desc(smem_u32(ring), j.a_mn ? Cfg::kOperand / 2 : 16, 1024, kLayoutSw128);
-        const uint64_t b_desc =
-            smem_desc(smem_u32(ring) + Cfg::kOperand, j.b_mn ? Cfg::kOperand / 2 : 16, 1024, kLayoutSw128);
-        const uint32_t a_step = j.a_mn ? 16 * 128 / 16 : 32 / 16;
-        const uint32_t b_step = j.b_mn ? 16 * 128 / 16 : 32 / 16;
-        const uint32_t idesc = instr_desc(Cfg::kFmt, j.a_mn, j.b_mn, Cfg::kTileM, Cfg::kAccCols);
         const int buf = static_cast<int>(acc_it & 1);
         if (!mbar_wait(&acc_empty[buf], ((acc_it >> 1) & 1u) ^ 1u, budget, abort)) {
           fail(kErrWaitAccEmpty);
@@ -485,38 +498,45 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
         }
         tc_fence_after();
         const uint32_t d = tmem_base + buf * Cfg::kAccCols;
-        for (int64_t kb = 0; kb < walk.kblocks; ++kb) {
-          const int s = static_cast<int>(it % S);
-          if (!mbar_wait(&full[s], (it / S) & 1u, budget, abort)) {
-            fail(kErrWaitFull);
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t stage = static_cast<uint64_t>(s * (Cfg::kStageBytes >> 4));
+        const int32_t kblocks = static_cast<int32_t>(walk.kblocks);
+        const auto run = [&](auto a_mn, auto b_mn) {
+          // K-major: a k-step of 16 is 32 bytes along the swizzled row.
+          // MN-major: 16 contraction rows of 128 bytes; the second 64 columns
+          // one box (8 KB) on.
+          constexpr uint32_t kStepA = a_mn.value ? 16 * 128 / 16 : 32 / 16, kStepB = b_mn.value ? 16 * 128 / 16 : 32 / 16;
+          constexpr uint32_t kIdesc = instr_desc(Cfg::kFmt, a_mn.value, b_mn.value, Cfg::kTileM, Cfg::kAccCols);
+          const uint64_t a_desc = smem_desc(smem_u32(ring), a_mn.value ? Cfg::kOperand / 2 : 16, 1024, kLayoutSw128);
+          const uint64_t b_desc =
+              smem_desc(smem_u32(ring) + Cfg::kOperand, b_mn.value ? Cfg::kOperand / 2 : 16, 1024, kLayoutSw128);
+          uint32_t acc = 0;
+          for (int32_t kb = 0; kb < kblocks; ++kb) {
+            if (!bar_wait(full0 + s * 8, phase, budget, abort)) {
+              fail(kErrWaitFull);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t stage = static_cast<uint32_t>(s) * (Cfg::kStageBytes >> 4);
+            const uint64_t ad = a_desc + stage, bd = b_desc + stage;
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const uint64_t ad = a_desc + stage + ks * a_step, bd = b_desc + stage + ks * b_step;
-            const uint32_t acc = (kb > 0 || ks > 0) ? 1u : 0u;
-            if constexpr (G == 2) {
-              mma_f16_pair(d, ad, bd, idesc, acc);
-            } else {
-              mma_f16(d, ad, bd, idesc, acc);
+            for (int ks = 0; ks < 4; ++ks) {
+              if constexpr (G == 2) {
+                mma_f16_pair(d, ad + ks * kStepA, bd + ks * kStepB, kIdesc, acc);
+              } else {
+                mma_f16(d, ad + ks * kStepA, bd + ks * kStepB, kIdesc, acc);
+              }
+              acc = 1;
+            }
+            tile_commit<G>(empty0 + s * 8);
+            if (++s == S) {
+              s = 0;
+              phase ^= 1u;
             }
           }
-          if constexpr (G == 2) {
-            mma_commit_pair(&empty[s], 0x3);
-          } else {
-            mma_commit(&empty[s]);
-          }
-          ++it;
-        }
+        };
+        by_layout<EPI>(*walk.job, run);
         if (!ok) break;
-        if constexpr (G == 2) {
-          mma_commit_pair(&acc_full[buf], 0x3);
-        } else {
-          mma_commit(&acc_full[buf]);
-        }
+        tile_commit<G>(smem_u32(&acc_full[buf]));
         ++acc_it;
       }
       if (*abort) {

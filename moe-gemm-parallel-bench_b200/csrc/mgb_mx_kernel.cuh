@@ -467,8 +467,10 @@ struct MxCfg {
   static constexpr int kScaleCols = 4 * kScaleAtoms;
   static constexpr int kTmemCols = 512;
   static constexpr int kScaleTmem = 2 * kTileN;  // first scale column
-  static constexpr int kEpiBlocks = 2;
-  static constexpr int kEpiBytes = 4 * kEpiBlocks * kEpiWarpBytes;
+  // One staging block of 32 rows x 64 bytes per epilogue warp: the epilogue
+  // runs under the next tile's MMAs, and the shared memory makes a stage.
+  static constexpr int kBlockBytes = 32 * 64;
+  static constexpr int kEpiBytes = 4 * kBlockBytes;
   static constexpr int kStages = (kTcSmemBudget - kEpiBytes - 2 * kScaleBytes) / kStageBytes;
   static constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + 2 * kScaleBytes + 2048 + 1024;
   static_assert(kStageBytes % 1024 == 0 && kABytes % 1024 == 0, "swizzle atoms");
@@ -553,68 +555,70 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    const uint64_t pol_keep = policy_evict_last(), pol_shared = policy_evict_normal(), pol_stream = policy_evict_first();
-    MxWalk walk;
-    uint32_t it = 0;
-    int built = -1;
-    bool ok = true;
-    for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
-      int64_t mb, nb;
-      walk.blocks(t, mb, nb);
-      const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.e) * 3;
-      if (walk.e != built) {
-        if (lane == 0) {
+    // One thread; stage and phase step along instead of dividing a counter.
+    if (lane == 0) {
+      const uint64_t pol_keep = policy_evict_last(), pol_shared = policy_evict_normal();
+      const uint64_t pol_stream = policy_evict_first();
+      const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), empty0 = smem_u32(empty);
+      const uint32_t lead0 = G == 2 ? mapa_shared(full0, 0) : full0;  // the leader's barriers
+      MxWalk walk;
+      int s = 0;
+      uint32_t phase = 0, loaded = 0;
+      int built = -1;
+      bool ok = true;
+      const int32_t end = static_cast<int32_t>(kblocks) * Cfg::kBK;
+      for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+        int64_t mb, nb;
+        walk.blocks(t, mb, nb);
+        const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.e) * 3;
+        if (walk.e != built) {
           tmap_acquire(&g[0]);
           tmap_acquire(&g[1]);
+          built = walk.e;
         }
-        __syncwarp();
-        built = walk.e;
-      }
-      const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128);
-      const int32_t n0 = static_cast<int32_t>(nb * Cfg::kTileN + rank * Cfg::kColsCta);
-      const uint64_t pol_b = walk.m_blocks == 1 ? pol_stream : pol_shared;
-      for (int64_t kb = 0; kb < kblocks; ++kb) {
-        const int s = static_cast<int>(it % S);
-        if (!mbar_wait_warp(&empty[s], ((it / S) & 1u) ^ 1u, budget, abort)) {
-          if (lane == 0) fail(kErrWaitEmpty);
-          ok = false;
-          break;
-        }
-        if (lane == 0) {
-          uint8_t* st = ring + s * Cfg::kStageBytes;
-          const int32_t kx = static_cast<int32_t>(kb * Cfg::kBK);
+        const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128);
+        const int32_t n0 = static_cast<int32_t>(nb * Cfg::kTileN + rank * Cfg::kColsCta);
+        const uint64_t pol_b = walk.m_blocks == 1 ? pol_stream : pol_shared;
+        for (int32_t kx = 0; kx < end; kx += Cfg::kBK) {
+          if (!bar_wait(empty0 + s * 8, phase ^ 1u, budget, abort)) {
+            fail(kErrWaitEmpty);
+            ok = false;
+            break;
+          }
+          const uint32_t st = ring0 + s * Cfg::kStageBytes;
           if (leader) mbar_arrive_expect_tx(&full[s], G * Cfg::kStageBytes);
-          if constexpr (G == 2) {
-            const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
-            tma_load_2d_pair(&g[0], bar, st, kx, m0, pol_keep);
-            tma_load_2d_pair(&g[1], bar, st + Cfg::kABytes, kx, n0, pol_b);
-          } else {
-            tma_load_2d(&g[0], &full[s], st, kx, m0, pol_keep);
-            tma_load_2d(&g[1], &full[s], st + Cfg::kABytes, kx, n0, pol_b);
+          tile_load<G>(&g[0], lead0 + s * 8, st, kx, m0, pol_keep);
+          tile_load<G>(&g[1], lead0 + s * 8, st + Cfg::kABytes, kx, n0, pol_b);
+          ++loaded;
+          if (++s == S) {
+            s = 0;
+            phase ^= 1u;
           }
         }
-        __syncwarp();
-        ++it;
       }
-    }
-    if (*abort && leader && lane == 0) {
-      for (uint32_t i = it > static_cast<uint32_t>(S) ? it - S : 0u; i < it; ++i) {
-        if (!mbar_wait(&full[i % S], (i / S) & 1u, budget, never)) {
-          atomicOr(p.error_word, kErrWaitTeardown);
-          break;
+      if (*abort && leader) {
+        for (uint32_t i = loaded > static_cast<uint32_t>(S) ? loaded - S : 0u; i < loaded; ++i) {
+          if (!bar_wait(full0 + (i % S) * 8, (i / S) & 1u, budget, never)) {
+            atomicOr(p.error_word, kErrWaitTeardown);
+            break;
+          }
         }
       }
     }
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer (leader only)
     if (lane == 0 && leader) {
+      const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty);
       MxWalk walk;
-      uint32_t it = 0, acc_it = 0, sf_it = 0;
+      int s = 0;
+      uint32_t phase = 0, acc_it = 0, sf_it = 0;
       bool ok = true;
       const uint64_t a_desc = smem_desc(smem_u32(ring), 16, 1024, kLayoutSw128);
       const uint64_t b_desc = smem_desc(smem_u32(ring) + Cfg::kABytes, 16, 1024, kLayoutSw128);
       // Scale atoms: no swizzle, 8-row groups of 16-byte rows 128 bytes apart.
       const uint64_t s_desc = smem_desc(smem_u32(scales), 0, 128, 0);
+      const int32_t blocks = static_cast<int32_t>(kblocks);
       for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
         const int buf = static_cast<int>(acc_it & 1);
         if (!mbar_wait(&acc_empty[buf], ((acc_it >> 1) & 1u) ^ 1u, budget, abort)) {
@@ -623,63 +627,52 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
         }
         tc_fence_after();
         const uint32_t d = tmem_base + buf * Cfg::kTileN;
-        for (int64_t kb = 0; kb < kblocks; ++kb) {
+        uint32_t acc = 0;
+        for (int32_t kb4 = 0; ok && kb4 < blocks; kb4 += 4) {
           const int slot = static_cast<int>(sf_it & 1);
           const uint32_t sf = tmem_base + Cfg::kScaleTmem + slot * Cfg::kScaleCols;
-          if ((kb & 3) == 0) {
-            if (!mbar_wait_cluster(&sf_full[slot], (sf_it >> 1) & 1u, budget, abort)) {
-              fail(kErrWaitFull);
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-#pragma unroll
-            for (int i = 0; i < Cfg::kScaleAtoms; ++i) {
-              tmem_copy_scales<G>(sf + 4 * i, s_desc + ((slot * Cfg::kScaleBytes + i * 512) >> 4));
-            }
-          }
-          const int s = static_cast<int>(it % S);
-          if (!mbar_wait(&full[s], (it / S) & 1u, budget, abort)) {
+          if (!mbar_wait_cluster(&sf_full[slot], (sf_it >> 1) & 1u, budget, abort)) {
             fail(kErrWaitFull);
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t stage = static_cast<uint64_t>(s * (Cfg::kStageBytes >> 4));
-          const uint32_t idesc = instr_desc_mx(Cfg::kTileM, Cfg::kTileN, static_cast<uint32_t>(kb & 3));
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            mma_mx<G>(d, a_desc + stage + ks * 2, b_desc + stage + ks * 2, idesc, sf, sf + 4, (kb > 0 || ks > 0) ? 1u : 0u);
+          for (int i = 0; i < Cfg::kScaleAtoms; ++i) {
+            tmem_copy_scales<G>(sf + 4 * i, s_desc + ((slot * Cfg::kScaleBytes + i * 512) >> 4));
           }
-          if constexpr (G == 2) {
-            mma_commit_pair(&empty[s], 0x3);
-          } else {
-            mma_commit(&empty[s]);
-          }
-          ++it;
-          if ((kb & 3) == 3 || kb == kblocks - 1) {
-            if constexpr (G == 2) {
-              mma_commit_pair(&sf_empty[slot], 0x3);
-            } else {
-              mma_commit(&sf_empty[slot]);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {  // K block kb4 + b names byte b of its scale words
+            if (kb4 + b >= blocks) break;
+            if (!bar_wait(full0 + s * 8, phase, budget, abort)) {
+              fail(kErrWaitFull);
+              ok = false;
+              break;
             }
-            ++sf_it;
+            tc_fence_after();
+            const uint32_t stage = static_cast<uint32_t>(s) * (Cfg::kStageBytes >> 4);
+            const uint64_t ad = a_desc + stage, bd = b_desc + stage;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              mma_mx<G>(d, ad + ks * 2, bd + ks * 2, instr_desc_mx(Cfg::kTileM, Cfg::kTileN, b), sf, sf + 4, acc);
+              acc = 1;
+            }
+            tile_commit<G>(empty0 + s * 8);
+            if (++s == S) {
+              s = 0;
+              phase ^= 1u;
+            }
           }
+          if (!ok) break;
+          tile_commit<G>(smem_u32(&sf_empty[slot]));
+          ++sf_it;
         }
         if (!ok) break;
-        if constexpr (G == 2) {
-          mma_commit_pair(&acc_full[buf], 0x3);
-        } else {
-          mma_commit(&acc_full[buf]);
-        }
+        tile_commit<G>(smem_u32(&acc_full[buf]));
         ++acc_it;
       }
       if (*abort) {
-        if constexpr (G == 2) {
-          mma_commit_pair(drain_bar, 0x1);
-        } else {
-          mma_commit(drain_bar);
-        }
+        tile_commit<G>(smem_u32(drain_bar));
         if (!mbar_wait(drain_bar, 0, budget, never)) atomicOr(p.error_word, kErrWaitTeardown);
       }
     }
@@ -737,10 +730,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3;
-    uint8_t* blocks = epi_stage + quarter * Cfg::kEpiBlocks * kEpiWarpBytes;
+    uint8_t* block = epi_stage + quarter * Cfg::kBlockBytes;
     const uint64_t pol_out = policy_evict_normal();
     MxWalk walk;
-    uint32_t acc_it = 0, chunk_seq = 0;
+    uint32_t acc_it = 0;
     int built = -1;
     for (int64_t t = first_item; walk.seek(p, t); t += items_step) {
       int64_t mb, nb;
@@ -765,11 +758,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
         const int64_t cols = p.n - c0 < Cfg::kTileN ? p.n - c0 : Cfg::kTileN;
 #pragma unroll 1
         for (int c = 0; c * 32 < cols; ++c) {
-          uint8_t* block = blocks + (chunk_seq & 1) * kEpiWarpBytes;
-          if (lane == 0) bulk_wait_group_read<1>();
-          __syncwarp();
           uint32_t v[32];
           tmem_ld32(taddr + c * 32, v);
+          if (lane == 0) bulk_wait_group_read<0>();  // the previous chunk's store has read the block
+          __syncwarp();
           tmem_ld_wait();
           // 32 rows x 64 bytes, 64-byte swizzle: 16-byte unit j of row r at j ^ ((r / 2) % 4).
 #pragma unroll
@@ -785,7 +777,6 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
             tma_store_2d(&g[2], block, c0 + c * 32, row0, pol_out);
             bulk_commit_group();
           }
-          ++chunk_seq;
         }
       }
       tc_fence_before();

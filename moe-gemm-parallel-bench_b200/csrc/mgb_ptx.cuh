@@ -389,6 +389,64 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint16_t cta_mask
       : "memory");
 }
 
+// ------------------------------- one CTA (G = 1) or a pair (G = 2), by address
+// The inner loops of a producer and an MMA issuer, one thread each, keep
+// their barriers as shared-memory addresses.
+// Tile load to a shared-memory address, counted on the barrier at `bar` (the
+// leader CTA's for a pair).
+template <int G>
+__device__ __forceinline__ void tile_load(const void* map, uint32_t bar, uint32_t dst, int32_t x, int32_t y,
+                                         uint64_t policy) {
+  if constexpr (G == 2) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "l"(policy)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "l"(policy)
+        : "memory");
+  }
+}
+
+// Arrives on the barrier at this address (in both CTAs of a pair) when every
+// MMA issued so far is done.
+template <int G>
+__device__ __forceinline__ void tile_commit(uint32_t bar) {
+  if constexpr (G == 2) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(0x3))
+        : "memory");
+  } else {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  }
+}
+
+// Bounded wait of one thread on the barrier at a shared-memory address.
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, long long budget, volatile int* abort) {
+  if (bar_try(bar, parity)) return true;
+  const long long start = clock64();
+  while (true) {
+    if (bar_try(bar, parity)) return true;
+    if (*abort || clock64() - start > budget) return false;
+  }
+}
+
 // ------------------------------------------------------ UMMA descriptors
 // Shared-memory matrix descriptor layout types used here.
 constexpr uint32_t kLayoutSw128 = 2;        // 128-byte swizzle, 16-byte granules, 8-row atoms
