@@ -21,9 +21,9 @@ using namespace mgb;
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-template <int G>
+template <int G, int ROWS>
 int launch_mx(const MxParams& p, int64_t tiles, int sm_count, cudaStream_t stream) {
-  using Cfg = MxCfg<G>;
+  using Cfg = MxCfg<G, ROWS>;
   static bool configured[128] = {};
   static int clusters[128] = {};
   int dev = 0;
@@ -35,11 +35,11 @@ int launch_mx(const MxParams& p, int64_t tiles, int sm_count, cudaStream_t strea
   cfg.stream = stream;
   cfg.attrs = attr;
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = G;
+  attr[0].val.clusterDim.x = G * p.split;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   if (!configured[dev]) {
-    if (cudaFuncSetAttribute(mx_kernel<G>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) !=
+    if (cudaFuncSetAttribute(mx_kernel<G, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) !=
         cudaSuccess) {
       return MGB_ERR_CUDA;
     }
@@ -48,7 +48,7 @@ int launch_mx(const MxParams& p, int64_t tiles, int sm_count, cudaStream_t strea
       cfg.gridDim = dim3(static_cast<unsigned>(sm_count & ~1), 1, 1);
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, mx_kernel<G>, &cfg) == cudaSuccess && n > 0) {
+      if (cudaOccupancyMaxActiveClusters(&n, mx_kernel<G, ROWS>, &cfg) == cudaSuccess && n > 0) {
         clusters[dev] = n;
       } else {
         cudaGetLastError();
@@ -56,12 +56,13 @@ int launch_mx(const MxParams& p, int64_t tiles, int sm_count, cudaStream_t strea
     }
     configured[dev] = true;
   }
-  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(tiles, clusters[dev]));
-  cfg.gridDim = dim3(static_cast<unsigned>(grid * G), 1, 1);
+  // A split launch has one cluster per tile (never more CTAs than SMs).
+  const int64_t grid = p.split > 1 ? tiles : std::max<int64_t>(1, std::min<int64_t>(tiles, clusters[dev]));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid * G * p.split), 1, 1);
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, mx_kernel<G>, p) == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, mx_kernel<G, ROWS>, p) == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
 }
 
 FastDiv fast_div(int64_t d) {
@@ -194,32 +195,45 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
     }
     return cudaGetLastError() == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
   }
-  // Pairs' 256 x 224 tiles where experts fill 256 rows and the tiles the
-  // device; else one CTA's 128 x 128 tiles.
+  // Pairs' 256 x 224 tiles from 112 rows an expert where they cover the
+  // device's pairs once (a half-empty pair tile still reads its weights once;
+  // 32 experts, n 4096, k 7168: 273 against 283 us at 128 rows, 255 against
+  // 228 at 64); else one CTA's 128 x 128, or 64 x 128 up to 48 rows an expert
+  // (182 against 203 us at 48; 241 against 228 at 64, where uneven routing
+  // gives some experts a second tile).
   const int64_t pair_tiles = (cdiv(rows, 256) + experts - 1) * cdiv(n, MxCfg<2>::kTileN);
-  const bool pair = each > 192 && pair_tiles >= sms / 2;
-  p.tile_rows = pair ? MxCfg<2>::kTileM : MxCfg<1>::kTileM;
+  const bool pair = each >= 112 && pair_tiles >= sms / 2;
+  const bool half = !pair && each <= 48;
+  p.tile_rows = pair ? 256 : half ? 64 : 128;
   p.tile_cols = pair ? MxCfg<2>::kTileN : MxCfg<1>::kTileN;
+  const int64_t tiles = (cdiv(rows, p.tile_rows) + experts - 1) * cdiv(n, p.tile_cols);
+  // Split K: as many CTAs a tile (2, 4 or 8) as the SMs hold at once, each
+  // with at least four K blocks.  Clusters do not cross a GPC, whose SMs (16
+  // to 18) hold whole clusters only: an eighth of the SMs stays out.
+  p.split = 1;
+  while (!pair && p.split < 8 && tiles * p.split * 2 <= sms - sms / 8 && p.kb >= 8 * p.split) p.split *= 2;
+  p.split_blocks = static_cast<int32_t>(cdiv(cdiv(p.kb, p.split), 4) * 4);
   p.maps = static_cast<uint8_t*>(scratch);
   p.tile_start = reinterpret_cast<int64_t*>(p.maps + static_cast<size_t>(experts) * 3 * sizeof(CUtensorMap));
   MxTemplates tmpl;
-  if (!encode_map_2d(&tmpl.map[0], kMapBytes8, a, k, 1, a_pitch, 128, 128) ||
+  if (!encode_map_2d(&tmpl.map[0], kMapBytes8, a, k, 1, a_pitch, 128, half ? 64 : 128) ||
       !encode_map_2d(&tmpl.map[2], MGB_BF16, c, n, 1, c_pitch * 2, 32, 32, 64) ||
       !encode_map_2d(&tmpl.map[1], kMapBytes8, b, k, n, b_pitch, 128, pair ? MxCfg<2>::kColsCta : MxCfg<1>::kColsCta)) {
     return MGB_ERR_CUDA;
   }
   mx_plan_kernel<<<static_cast<unsigned>(experts) + 1, 32, 0, s>>>(tmpl, p);
   if (cudaGetLastError() != cudaSuccess) return MGB_ERR_CUDA;
-  const int64_t tiles = (cdiv(rows, p.tile_rows) + experts - 1) * cdiv(n, p.tile_cols);
   if (info != nullptr) {
     info->path = pair ? 2 : 0;
     info->tile_m = p.tile_rows;
     info->tile_n = p.tile_cols;
     info->tile_k = 128;
-    info->stages = pair ? MxCfg<2>::kStages : MxCfg<1>::kStages;
-    info->grid = static_cast<int32_t>(std::min<int64_t>(tiles, sms));
+    info->stages = pair ? MxCfg<2>::kStages : half ? MxCfg<1, 64>::kStages : MxCfg<1>::kStages;
+    info->grid = static_cast<int32_t>(std::min<int64_t>(tiles * p.split, sms));
   }
-  return pair ? launch_mx<2>(p, tiles, sms, s) : launch_mx<1>(p, tiles, sms, s);
+  return pair   ? launch_mx<2, 128>(p, tiles, sms, s)
+         : half ? launch_mx<1, 64>(p, tiles, sms, s)
+                : launch_mx<1, 128>(p, tiles, sms, s);
 }
 
 int quantize_rows_launch(const void* x, int64_t rows, int64_t cols, int64_t pitch, int32_t dtype, void* q,

@@ -279,6 +279,8 @@ struct MxParams {
   uint8_t* maps;        // [experts][3] tensor maps: A, B, C
   int64_t* tile_start;  // [experts + 1]
   int32_t tile_rows, tile_cols;
+  int32_t split;        // CTAs of a cluster that share a tile's K (one CTA tiles; 1: none)
+  int32_t split_blocks; // K blocks of each, a multiple of 4
   long long wait_budget;
   uint32_t* error_word;
 };
@@ -452,15 +454,22 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// Tile: 256 x 224 for a pair, 128 x 128 for one CTA.  Two accumulators and the
-// scale words share the 512 TMEM columns: 2 x 224 + 2 x 12 for a pair (N = 256
-// would leave none for the scales), 2 x 128 + 2 x 8 for one CTA.
-template <int G>
+// Tile: 256 x 224 for a pair; ROWS x 128 for one CTA, ROWS = 128 or 64 token
+// rows.  Two accumulators and the scale words share the 512 TMEM columns:
+// 2 x 224 + 2 x 12 for a pair (N = 256 would leave none for the scales),
+// 2 x 128 + 2 x 8 for one CTA.  A 64-row tile still runs M = 128 MMAs: the
+// operand's upper rows are whatever lies behind it in shared memory and only
+// reach accumulator rows that are never stored.  It halves the token half of a
+// stage, so eight stages (128 KB of weights per SM) are in flight instead of
+// five while the weights' bytes bound the launch.
+template <int G, int ROWS = 128>
 struct MxCfg {
+  static_assert(ROWS == 128 || (G == 1 && ROWS == 64), "token rows a CTA loads");
   static constexpr int kBK = 128;
   static constexpr int kColsCta = G == 2 ? 112 : 128;  // weight rows a CTA loads
-  static constexpr int kTileM = 128 * G, kTileN = kColsCta * G;
-  static constexpr int kABytes = 128 * 128, kBBytes = kColsCta * 128;
+  static constexpr int kTileM = ROWS * G, kTileN = kColsCta * G;
+  static constexpr int kMmaM = 128 * G;
+  static constexpr int kABytes = ROWS * 128, kBBytes = kColsCta * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kScaleAtoms = 1 + G;           // 128 rows x 4 bytes each: A, then B's 128-row groups
   static constexpr int kScaleBytes = kScaleAtoms * 512;  // one slot: four K blocks
@@ -476,6 +485,9 @@ struct MxCfg {
   static_assert(kStageBytes % 1024 == 0 && kABytes % 1024 == 0, "swizzle atoms");
   static_assert(kScaleTmem + 2 * kScaleCols <= kTmemCols, "TMEM columns");
   static_assert(kSmemBytes <= 232448 && kStages >= 4, "shared memory");
+  // Split K (one CTA): a row of partial sums, padded against bank conflicts.
+  static constexpr int kSumRow = kTileN * 4 + 16;
+  static_assert(G == 2 || kTileM * kSumRow <= kStages * kStageBytes, "partial sums fit the ring");
 };
 
 constexpr int kMxThreads = 256;
@@ -486,9 +498,14 @@ constexpr int kMxThreads = 256;
 // copies them to TMEM and names byte kb % 4 in the MMAs of K block kb.  A
 // slot (its shared memory and its TMEM columns) is free again when the MMAs
 // of its four K blocks are done.
-template <int G>
+// Split K (p.split > 1, at most one tile per cluster): the CTAs of a cluster
+// compute one tile over consecutive K ranges and leave fp32 sums in their own
+// (then idle) operand rings; CTA r adds rows [r ROWS / split, ...) of all of
+// them over distributed shared memory, in rank order, and stores them.  For
+// launches whose tiles would leave at least half of the SMs idle.
+template <int G, int ROWS>
 __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant__ MxParams p) {
-  using Cfg = MxCfg<G>;
+  using Cfg = MxCfg<G, ROWS>;
   constexpr int S = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -510,8 +527,13 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   const int lane = threadIdx.x & 31;
   const uint32_t rank = G == 2 ? cluster_ctarank() : 0u;
   const bool leader = rank == 0;
-  const int64_t first_item = blockIdx.x / G;
-  const int64_t items_step = gridDim.x / G;
+  const int split = G == 2 ? 1 : p.split;
+  const int64_t first_item = blockIdx.x / (G * split);
+  const int64_t items_step = gridDim.x / (G * split);
+  // This CTA's K blocks of every tile.
+  const int32_t share = split > 1 ? static_cast<int32_t>(cluster_ctarank()) : 0;
+  const int32_t kb_from = share * p.split_blocks;
+  const int32_t kb_to = static_cast<int32_t>(split > 1 && kb_from + p.split_blocks < p.kb ? kb_from + p.split_blocks : p.kb);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -546,7 +568,6 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   const long long budget = p.wait_budget;
   grid_dependency_wait();
   const CUtensorMap* all_maps = reinterpret_cast<const CUtensorMap*>(p.maps);
-  const int64_t kblocks = p.kb;
 
   auto fail = [&](uint32_t bits) {
     atomicOr(p.error_word, bits);
@@ -566,7 +587,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       uint32_t phase = 0, loaded = 0;
       int built = -1;
       bool ok = true;
-      const int32_t end = static_cast<int32_t>(kblocks) * Cfg::kBK;
+      const int32_t begin = kb_from * Cfg::kBK, end = kb_to * Cfg::kBK;
       for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
         int64_t mb, nb;
         walk.blocks(t, mb, nb);
@@ -576,10 +597,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
           tmap_acquire(&g[1]);
           built = walk.e;
         }
-        const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128);
+        const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * ROWS);
         const int32_t n0 = static_cast<int32_t>(nb * Cfg::kTileN + rank * Cfg::kColsCta);
         const uint64_t pol_b = walk.m_blocks == 1 ? pol_stream : pol_shared;
-        for (int32_t kx = 0; kx < end; kx += Cfg::kBK) {
+        for (int32_t kx = begin; kx < end; kx += Cfg::kBK) {
           if (!bar_wait(empty0 + s * 8, phase ^ 1u, budget, abort)) {
             fail(kErrWaitEmpty);
             ok = false;
@@ -618,7 +639,6 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       const uint64_t b_desc = smem_desc(smem_u32(ring) + Cfg::kABytes, 16, 1024, kLayoutSw128);
       // Scale atoms: no swizzle, 8-row groups of 16-byte rows 128 bytes apart.
       const uint64_t s_desc = smem_desc(smem_u32(scales), 0, 128, 0);
-      const int32_t blocks = static_cast<int32_t>(kblocks);
       for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
         const int buf = static_cast<int>(acc_it & 1);
         if (!mbar_wait(&acc_empty[buf], ((acc_it >> 1) & 1u) ^ 1u, budget, abort)) {
@@ -628,7 +648,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
         tc_fence_after();
         const uint32_t d = tmem_base + buf * Cfg::kTileN;
         uint32_t acc = 0;
-        for (int32_t kb4 = 0; ok && kb4 < blocks; kb4 += 4) {
+        for (int32_t kb4 = kb_from; ok && kb4 < kb_to; kb4 += 4) {
           const int slot = static_cast<int>(sf_it & 1);
           const uint32_t sf = tmem_base + Cfg::kScaleTmem + slot * Cfg::kScaleCols;
           if (!mbar_wait_cluster(&sf_full[slot], (sf_it >> 1) & 1u, budget, abort)) {
@@ -643,7 +663,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
           }
 #pragma unroll
           for (int b = 0; b < 4; ++b) {  // K block kb4 + b names byte b of its scale words
-            if (kb4 + b >= blocks) break;
+            if (kb4 + b >= kb_to) break;
             if (!bar_wait(full0 + s * 8, phase, budget, abort)) {
               fail(kErrWaitFull);
               ok = false;
@@ -654,7 +674,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
             const uint64_t ad = a_desc + stage, bd = b_desc + stage;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-              mma_mx<G>(d, ad + ks * 2, bd + ks * 2, instr_desc_mx(Cfg::kTileM, Cfg::kTileN, b), sf, sf + 4, acc);
+              mma_mx<G>(d, ad + ks * 2, bd + ks * 2, instr_desc_mx(Cfg::kMmaM, Cfg::kTileN, b), sf, sf + 4, acc);
               acc = 1;
             }
             tile_commit<G>(empty0 + s * 8);
@@ -694,7 +714,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
       int64_t mb, nb;
       walk.blocks(t, mb, nb);
-      const int64_t m0 = mb * Cfg::kTileM + rank * 128, n0 = nb * Cfg::kTileN;
+      const int64_t m0 = mb * Cfg::kTileM + rank * ROWS, n0 = nb * Cfg::kTileN;
       const uint8_t* row[4 * Cfg::kScaleAtoms];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -706,7 +726,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
         const int64_t n = n0 + (j - 4) * 32 + lane;
         row[j] = p.sb + (walk.e * p.nb + (n < p.n ? n : p.n - 1) / 128) * p.kb;
       }
-      for (int64_t kb = 0; kb < kblocks; kb += 4) {
+      for (int64_t kb = kb_from; kb < kb_to; kb += 4) {
         const int slot = static_cast<int>(sf_it & 1);
         uint32_t w[4 * Cfg::kScaleAtoms];
 #pragma unroll
@@ -751,9 +771,26 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       }
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * Cfg::kTileN;
-      const int32_t row0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128 + quarter * 32);
+      const int32_t row0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * ROWS + quarter * 32);
       const int32_t c0 = static_cast<int32_t>(nb * Cfg::kTileN);
-      if (row0 < walk.len) {
+      if (G == 1 && split > 1) {
+        // The last MMAs are done and nothing more is loaded: the ring holds the sums.
+        if (quarter * 32 < ROWS) {
+          float* sums = reinterpret_cast<float*>(ring + (quarter * 32 + lane) * Cfg::kSumRow);
+#pragma unroll 1
+          for (int c = 0; c < Cfg::kTileN; c += 32) {
+            uint32_t v[32];
+            tmem_ld32(taddr + c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              *reinterpret_cast<uint4*>(sums + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            }
+          }
+        }
+        break;  // one tile per cluster
+      }
+      if (quarter * 32 < ROWS && row0 < walk.len) {
         // Chunks of 32 columns (a 224-column tile is seven); the map clips C's edges.
         const int64_t cols = p.n - c0 < Cfg::kTileN ? p.n - c0 : Cfg::kTileN;
 #pragma unroll 1
@@ -796,7 +833,43 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
 
   tc_fence_before();
   __syncthreads();
-  if constexpr (G == 2) cluster_sync();
+  if (G == 2 || split > 1) cluster_sync();
+  if (G == 1 && split > 1) {
+    MxWalk walk;
+    if (walk.seek(p, first_item) && !*abort) {
+      int64_t mb, nb;
+      walk.blocks(first_item, mb, nb);
+      const int per = ROWS / split;
+      const int col = (threadIdx.x & 31) * 4;
+      const int64_t c = nb * Cfg::kTileN + col;
+      // CTAs without K blocks (a short last share) left no sums.
+      const int parts = static_cast<int>((p.kb + p.split_blocks - 1) / p.split_blocks);
+      for (int r = share * per + warp; r < (share + 1) * per; r += kMxThreads / 32) {
+        const int64_t m = mb * Cfg::kTileM + r;
+        if (m >= walk.len) break;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const uint32_t at = smem_u32(ring + r * Cfg::kSumRow + col * 4);
+        for (int i = 0; i < parts; ++i) {
+          float4 v;
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                       : "r"(mapa_shared(at, i))
+                       : "memory");
+          sum.x += v.x;
+          sum.y += v.y;
+          sum.z += v.z;
+          sum.w += v.w;
+        }
+        if (c < p.n) {  // n is a multiple of 8: four columns are inside or past the end
+          uint2 out;
+          out.x = pack_pair<__nv_bfloat16>(__float_as_uint(sum.x), __float_as_uint(sum.y));
+          out.y = pack_pair<__nv_bfloat16>(__float_as_uint(sum.z), __float_as_uint(sum.w));
+          *reinterpret_cast<uint2*>(p.c + (walk.start + m) * p.c_pitch + c) = out;
+        }
+      }
+    }
+    cluster_sync();  // the others' sums are read until here
+  }
   if (warp == 1) {
     tc_fence_after();
     if constexpr (G == 2) {

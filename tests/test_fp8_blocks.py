@@ -187,6 +187,9 @@ PRODUCTS = [
     ([32], 40, 656), ([1, 0, 7, 0, 23], 136, 528), ([0, 0, 90, 1], 200, 272), ([2] * 37, 72, 144),
     # one CTA's 128 x 128 tiles
     ([33], 128, 128), ([127], 136, 272), ([100, 0, 1, 129], 264, 656), ([300], 1032, 2000), ([64] * 5, 128, 512),
+    # 64 x 128 tiles; a tile's K shared by the CTAs of a cluster
+    ([50] * 3, 136, 1040), ([33], 264, 2064), ([100], 264, 4112), ([40, 0, 50], 136, 2064), ([128], 1024, 7168),
+    ([5, 70, 45], 520, 1104), ([0, 200, 10], 136, 16384), ([64], 8, 2320),
     # CTA pairs' 256 x 224 tiles
     ([2048], 4096, 512), ([1, 0, 1500, 255, 257], 4096, 1168), ([1999], 2248, 1040),
 ]
@@ -204,14 +207,14 @@ def test_product(shape):
 @pytest.mark.gpu
 def test_every_kernel_was_reached():
     paths = set()
-    for shape in (PRODUCTS[0], PRODUCTS[10], PRODUCTS[15]):
+    for shape in (PRODUCTS[0], PRODUCTS[10], PRODUCTS[-3]):
         Product(*shape).run()
         paths.add(kernels.last_block_scaled_info()["path"])
     assert paths == {"warp_mma", "tcgen05_tma", "tcgen05_tma_pair"}
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", [PRODUCTS[1], PRODUCTS[13], PRODUCTS[17]], ids=["few", "one", "pair"])
+@pytest.mark.parametrize("shape", [PRODUCTS[1], PRODUCTS[13], PRODUCTS[17], PRODUCTS[-1]], ids=["few", "one", "split", "pair"])
 def test_one_scale_at_a_time(shape):
     """One scale byte differs from 1: only its row and K block may change."""
     product = Product(*shape, dense=True)
