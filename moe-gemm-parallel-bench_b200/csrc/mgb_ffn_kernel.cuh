@@ -26,7 +26,8 @@
 //                    stores dg = dh u s (1 + g (1 - s)), du = dh g s, s = sigmoid(g)
 //
 // One CTA per SM, roles by warp: 0 TMA producer, 1 MMA issuer, 2-5 epilogue.
-// G = 2: CTA pairs, 256 x 256 tiles (tcgen05 cta_group::2, M = 256, N = 256);
+// G = 2: CTA pairs, 256 x 256 tiles (tcgen05 cta_group::2, M = 256, N = 256),
+// or 256 x 512 (two of those MMAs on the same rows);
 // G = 1: one CTA, 128 x 128 tiles, four times as many, for launches whose
 // 256 x 256 tiles would leave most SMs idle.  Both load 128 rows of A and
 // 128 columns of B per CTA and 64-deep contraction block (32 KB a stage).
@@ -213,16 +214,22 @@ struct FfnWalk {
   }
 };
 
-template <typename T, int EPI, int G>
+// NH = 256-column halves of a pair's tile: 2 is the 256 x 512 tile of the
+// plain epilogue.  It moves 48 KB into a CTA per 128 x 512 x 64 products
+// where the 256 x 256 tile moves 32 KB per 128 x 256 x 64, a quarter less per
+// product; its one 512-column accumulator fills TMEM and is freed by halves.
+template <typename T, int EPI, int G, int NH = 1>
 struct FfnCfg {
   static_assert(sizeof(T) == 2 && (G == 1 || G == 2), "16-bit types, one CTA or a pair");
+  static_assert(NH == 1 || (NH == 2 && G == 2 && EPI == kFfnPlain), "wide tiles: pairs, plain epilogue");
   static constexpr int kBK = 64;
   static constexpr int kOperand = 128 * 128;  // 128 rows (or columns) x 64 contraction
-  static constexpr int kStageBytes = 2 * kOperand;
+  static constexpr int kStageBytes = (1 + NH) * kOperand;
   static constexpr int kTileM = 128 * G;
-  static constexpr int kAccCols = 128 * G;
+  static constexpr int kMmaN = 128 * G;
+  static constexpr int kAccCols = NH * kMmaN;
   static constexpr int kTileOut = EPI == kFfnSwiglu ? kAccCols / 2 : kAccCols;  // output columns per tile
-  static constexpr int kTmemCols = 2 * kAccCols;                                // two accumulators
+  static constexpr int kTmemCols = NH == 2 ? 512 : 2 * kAccCols;                // two accumulators, or two halves
   // Staging blocks (32 rows x 128 bytes) per epilogue warp: plain two, in
   // turn; swiglu h, g and u of one chunk; backward two pairs (g, u), each
   // overwritten in place by (dg, du).
@@ -326,9 +333,9 @@ __device__ __forceinline__ void by_layout(const FfnJob& j, F&& f) {
   }
 }
 
-template <typename T, int EPI, int G>
+template <typename T, int EPI, int G, int NH>
 __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constant__ FfnParams p) {
-  using Cfg = FfnCfg<T, EPI, G>;
+  using Cfg = FfnCfg<T, EPI, G, NH>;
   constexpr int S = Cfg::kStages;
   constexpr int BK = Cfg::kBK;
 
@@ -456,11 +463,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
             } else {
               load(&g[0], st_a, kx, m0, pol_a);
             }
-            if constexpr (b_mn.value) {
-              load(&g[1], st_b, b0, kx, pol_b);
-              load(&g[1], st_b + Cfg::kOperand / 2, b1, kx, pol_b);
-            } else {
-              load(&g[1], st_b, kx, b0, pol_b);
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+              const uint32_t dst = st_b + h * Cfg::kOperand;
+              if constexpr (b_mn.value) {
+                load(&g[1], dst, b0 + 256 * h, kx, pol_b);
+                load(&g[1], dst + Cfg::kOperand / 2, b1 + 256 * h, kx, pol_b);
+              } else {
+                load(&g[1], dst, kx, b0 + 256 * h, pol_b);
+              }
             }
             ++loaded;
             if (++s == S) {
@@ -491,8 +502,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
       bool ok = true;
       for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
         if (walk.kblocks <= 0) continue;
-        const int buf = static_cast<int>(acc_it & 1);
-        if (!mbar_wait(&acc_empty[buf], ((acc_it >> 1) & 1u) ^ 1u, budget, abort)) {
+        // Two accumulators in turn, or (wide) the halves of one.
+        const int buf = NH == 2 ? 0 : static_cast<int>(acc_it & 1);
+        const uint32_t acc_phase = ((NH == 2 ? acc_it : acc_it >> 1) & 1u) ^ 1u;
+        if (!mbar_wait(&acc_empty[buf], acc_phase, budget, abort)) {
           fail(kErrWaitAccEmpty);
           break;
         }
@@ -504,29 +517,68 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
           // MN-major: 16 contraction rows of 128 bytes; the second 64 columns
           // one box (8 KB) on.
           constexpr uint32_t kStepA = a_mn.value ? 16 * 128 / 16 : 32 / 16, kStepB = b_mn.value ? 16 * 128 / 16 : 32 / 16;
-          constexpr uint32_t kIdesc = instr_desc(Cfg::kFmt, a_mn.value, b_mn.value, Cfg::kTileM, Cfg::kAccCols);
+          constexpr uint32_t kIdesc = instr_desc(Cfg::kFmt, a_mn.value, b_mn.value, Cfg::kTileM, Cfg::kMmaN);
           const uint64_t a_desc = smem_desc(smem_u32(ring), a_mn.value ? Cfg::kOperand / 2 : 16, 1024, kLayoutSw128);
           const uint64_t b_desc =
               smem_desc(smem_u32(ring) + Cfg::kOperand, b_mn.value ? Cfg::kOperand / 2 : 16, 1024, kLayoutSw128);
-          uint32_t acc = 0;
-          for (int32_t kb = 0; kb < kblocks; ++kb) {
+          // The four MMAs of half h on stage `at`.
+          const auto issue = [&](int at, int h, bool first) {
+            const uint32_t stage = static_cast<uint32_t>(at) * (Cfg::kStageBytes >> 4);
+            const uint64_t ad = a_desc + stage, bd = b_desc + stage + h * (Cfg::kOperand >> 4);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              const uint32_t acc = ks > 0 || !first ? 1u : 0u;
+              if constexpr (G == 2) {
+                mma_f16_pair(d + h * Cfg::kMmaN, ad + ks * kStepA, bd + ks * kStepB, kIdesc, acc);
+              } else {
+                mma_f16(d + h * Cfg::kMmaN, ad + ks * kStepA, bd + ks * kStepB, kIdesc, acc);
+              }
+            }
+          };
+          int32_t kb = 0;
+          if constexpr (NH == 2) {
+            // Half 0 is free: its MMAs of the first k-blocks (up to a ring of
+            // them, their stages kept) run while the epilogue drains half 1.
+            const int32_t held = kblocks < S ? kblocks : S;
+            int at = s;
+            uint32_t at_phase = phase;
+            for (; kb < held; ++kb) {
+              if (!bar_wait(full0 + at * 8, at_phase, budget, abort)) {
+                fail(kErrWaitFull);
+                ok = false;
+                return;
+              }
+              tc_fence_after();
+              issue(at, 0, kb == 0);
+              if (++at == S) {
+                at = 0;
+                at_phase ^= 1u;
+              }
+            }
+            if (!mbar_wait(&acc_empty[1], acc_phase, budget, abort)) {
+              fail(kErrWaitAccEmpty);
+              ok = false;
+              return;
+            }
+            tc_fence_after();
+            for (kb = 0; kb < held; ++kb) {
+              issue(s, 1, kb == 0);
+              tile_commit<G>(empty0 + s * 8);
+              if (++s == S) {
+                s = 0;
+                phase ^= 1u;
+              }
+            }
+          }
+          for (; kb < kblocks; ++kb) {
             if (!bar_wait(full0 + s * 8, phase, budget, abort)) {
               fail(kErrWaitFull);
               ok = false;
-              break;
+              return;
             }
             tc_fence_after();
-            const uint32_t stage = static_cast<uint32_t>(s) * (Cfg::kStageBytes >> 4);
-            const uint64_t ad = a_desc + stage, bd = b_desc + stage;
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-              if constexpr (G == 2) {
-                mma_f16_pair(d, ad + ks * kStepA, bd + ks * kStepB, kIdesc, acc);
-              } else {
-                mma_f16(d, ad + ks * kStepA, bd + ks * kStepB, kIdesc, acc);
-              }
-              acc = 1;
-            }
+            for (int h = 0; h < NH; ++h) issue(s, h, kb == 0);
             tile_commit<G>(empty0 + s * 8);
             if (++s == S) {
               s = 0;
@@ -593,14 +645,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
           ++gates.issued;
         }
       }
-      const int buf = static_cast<int>(acc_it & 1);
-      if (!mbar_wait_warp(&acc_full[buf], (acc_it >> 1) & 1u, budget, abort)) {
+      const int buf = NH == 2 ? 0 : static_cast<int>(acc_it & 1);
+      if (!mbar_wait_warp(&acc_full[buf], (NH == 2 ? acc_it : acc_it >> 1) & 1u, budget, abort)) {
         if (lane == 0) fail(kErrWaitAccFull);
         break;
       }
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * Cfg::kAccCols;
-      if constexpr (EPI == kFfnPlain) {
+      if constexpr (NH == 2) {
+        Problem q;
+        q.m = walk.rows;
+        q.n = j.n;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // each half is released as soon as it is drained
+          store_rows_tma<T, 256, Cfg::kEpiBlocks>(q, &g[2], taddr + h * 256, row0, n0 + h * 256, blocks, lane, chunk_seq,
+                                                  pol_out, p.error_word);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&acc_empty[h]), 0));
+        }
+        ++acc_it;
+        continue;
+      } else if constexpr (EPI == kFfnPlain) {
         Problem q;
         q.m = walk.rows;
         q.n = j.n;
