@@ -72,6 +72,25 @@ constexpr int kMapBytes8 = 100;
 bool encode_map_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch,
                    uint32_t box_inner, uint32_t box_outer, int swizzle_bytes = 128);
 
+// Launches `kernel` with programmatic stream serialization: its blocks may be
+// set up while the kernel before it on the stream still runs, so it must call
+// grid_dependency_wait before it touches global memory.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_overlapped(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem,
+                                     cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1] = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // Launches simt_grouped_kernel<T>; returns a cudaError_t value.
 template <typename T>
 int simt_launch(const GroupedParams& p, int grid, cudaStream_t stream);

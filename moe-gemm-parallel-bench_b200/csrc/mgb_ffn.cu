@@ -194,8 +194,10 @@ struct Launcher {
       l.tile_start = reinterpret_cast<int64_t*>(list);
       list += list_bytes(experts, l.jobs);
     }
-    ffn_plan_kernel<<<static_cast<unsigned>(plan.jobs * experts + plan.launches), 32, 0, stream>>>(plan);
-    if (cudaGetLastError() != cudaSuccess) return MGB_ERR_CUDA;
+    if (launch_overlapped(ffn_plan_kernel, static_cast<unsigned>(plan.jobs * experts + plan.launches), 32, 0, stream,
+                          plan) != cudaSuccess) {
+      return MGB_ERR_CUDA;
+    }
     for (int i = 0; i < plan.launches; ++i) {
       const FfnPlan::Launch& l = plan.launch[i];
       FfnParams p;

@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(32) ffn_plan_kernel(const __grid_constant__ Ff
   __shared__ alignas(128) CUtensorMap staging[kFfnMaps];
   const int lane = threadIdx.x;
   grid_launch_dependents();
+  grid_dependency_wait();  // offs and this scratch may be in use until here
   if (static_cast<int>(blockIdx.x) >= p.jobs * p.experts) {
     const FfnPlan::Launch& l = p.launch[blockIdx.x - p.jobs * p.experts];
     const int pairs = l.jobs * p.experts;

@@ -88,12 +88,10 @@ int rows_typed(const void* x, int64_t rows, int64_t cols, int64_t pitch, void* q
   const T* in = static_cast<const T*>(x);
   uint8_t* out = static_cast<uint8_t*>(q);
   uint8_t* sc = static_cast<uint8_t*>(scale);
-  if (vec) {
-    quantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(in, nb, kb, cols, pitch, out, q_pitch, sc);
-  } else {
-    quantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(in, nb, kb, cols, pitch, out, q_pitch, sc);
-  }
-  return cudaGetLastError() == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
+  const auto kernel = vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
+  return launch_overlapped(kernel, grid, 256, 0, s, in, nb, kb, cols, pitch, out, q_pitch, sc) == cudaSuccess
+             ? MGB_OK
+             : MGB_ERR_CUDA;
 }
 
 template <typename T>
@@ -107,14 +105,28 @@ int blocks_typed(const void* x, int64_t matrices, int64_t rows, int64_t cols, in
   const T* in = static_cast<const T*>(x);
   uint8_t* out = static_cast<uint8_t*>(q);
   uint8_t* sc = static_cast<uint8_t*>(scale);
-  if (vec) {
-    quantize_blocks_kernel<T, true><<<grid, 256, 0, s>>>(in, rows, cols, pitch, stride, out, cols, rows * cols, sc, fast_div(kb),
-                                                         fast_div(per));
-  } else {
-    quantize_blocks_kernel<T, false><<<grid, 256, 0, s>>>(in, rows, cols, pitch, stride, out, cols, rows * cols, sc, fast_div(kb),
-                                                         fast_div(per));
+  const auto kernel = vec ? quantize_blocks_kernel<T, true> : quantize_blocks_kernel<T, false>;
+  return launch_overlapped(kernel, grid, 256, 0, s, in, rows, cols, pitch, stride, out, cols, rows * cols, sc,
+                           fast_div(kb), fast_div(per)) == cudaSuccess
+             ? MGB_OK
+             : MGB_ERR_CUDA;
+}
+
+template <int NT>
+int launch_few(const MxParams& p, unsigned grid, cudaStream_t s) {
+  using Cfg = FewCfg<NT>;
+  static bool configured[128] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return MGB_ERR_CUDA;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(mx_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) !=
+        cudaSuccess) {
+      return MGB_ERR_CUDA;
+    }
+    configured[dev] = true;
   }
-  return cudaGetLastError() == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
+  return launch_overlapped(mx_few_kernel<NT>, grid, kFewWarps * 32, Cfg::kSmemBytes, s, p) == cudaSuccess ? MGB_OK
+                                                                                                          : MGB_ERR_CUDA;
 }
 
 // Average rows of an expert up to which the weight-streaming kernel runs
@@ -178,13 +190,6 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
     if (groups >= (1ll << 31)) return MGB_ERR_UNSUPPORTED;
     const unsigned grid = static_cast<unsigned>(groups);
     const int nt = each <= 8 ? 1 : each <= 16 ? 2 : 4;
-    if (nt == 1) {
-      mx_few_kernel<1><<<grid, kFewWarps * 32, 0, s>>>(p);
-    } else if (nt == 2) {
-      mx_few_kernel<2><<<grid, kFewWarps * 32, 0, s>>>(p);
-    } else {
-      mx_few_kernel<4><<<grid, kFewWarps * 32, 0, s>>>(p);
-    }
     if (info != nullptr) {
       info->path = 3;
       info->swap_ab = 1;
@@ -193,7 +198,7 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
       info->tile_k = 128;
       info->grid = static_cast<int32_t>(grid);
     }
-    return cudaGetLastError() == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
+    return nt == 1 ? launch_few<1>(p, grid, s) : nt == 2 ? launch_few<2>(p, grid, s) : launch_few<4>(p, grid, s);
   }
   // Pairs' 256 x 224 tiles from 112 rows an expert where they cover the
   // device's pairs once (a half-empty pair tile still reads its weights once;
@@ -221,8 +226,9 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
       !encode_map_2d(&tmpl.map[1], kMapBytes8, b, k, n, b_pitch, 128, pair ? MxCfg<2>::kColsCta : MxCfg<1>::kColsCta)) {
     return MGB_ERR_CUDA;
   }
-  mx_plan_kernel<<<static_cast<unsigned>(experts) + 1, 32, 0, s>>>(tmpl, p);
-  if (cudaGetLastError() != cudaSuccess) return MGB_ERR_CUDA;
+  if (launch_overlapped(mx_plan_kernel, static_cast<unsigned>(experts) + 1, 32, 0, s, tmpl, p) != cudaSuccess) {
+    return MGB_ERR_CUDA;
+  }
   if (info != nullptr) {
     info->path = pair ? 2 : 0;
     info->tile_m = p.tile_rows;

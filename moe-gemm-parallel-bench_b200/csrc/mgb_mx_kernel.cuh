@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
   const int l = threadIdx.x & 15;
   const uint32_t half = 0xFFFFu << (threadIdx.x & 16);  // the halves of a warp may end at different blocks
   const uint32_t stride = gridDim.x * 16u;
+  grid_dependency_wait();
   for (uint32_t b0 = blockIdx.x * 16u + (threadIdx.x >> 4); b0 < blocks; b0 += stride * kRowsUnroll) {
     Eight<T> v[kRowsUnroll];
 #pragma unroll
@@ -228,6 +229,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
   const int64_t r0 = rb * 128ll + (threadIdx.x >> 4), c = (in - rb * kb.d) * 128ll + (threadIdx.x & 15) * 8;
   const T* base = x + e * matrix;
   Eight<T> v[8];
+  grid_dependency_wait();
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t r = r0 + i * 16;
@@ -307,6 +309,7 @@ __global__ void __launch_bounds__(32)
   __shared__ alignas(128) CUtensorMap staging[3];
   const int lane = threadIdx.x;
   grid_launch_dependents();
+  grid_dependency_wait();  // offs and this scratch may be in use until here
   if (blockIdx.x == p.experts) {
     const int per = (p.experts + 31) / 32;
     const int lo = lane * per, hi = lo + per < p.experts ? lo + per : p.experts;
@@ -885,11 +888,14 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
 // product and the tensor pipe idles whatever drives it.  The 128-row tiles
 // above would run on n / 128 SMs and stream the weights through too few of
 // them; here a CTA takes 16 weight rows and its 8 warps split K (interleaved
-// 128-deep blocks), so n / 16 CTAs stream with every load independent of the
-// others: no shared-memory ring, no barrier until the warps' sums are joined
-// in shared memory in warp order (the result does not depend on timing).
+// 128-deep blocks), so n / 16 CTAs stream.  Every thread copies the weight
+// bytes that it will use itself into its own shared-memory slots (cp.async,
+// no barrier), kFewDepth K blocks ahead: two CTAs keep 192 KB of weights per
+// SM in flight without holding registers for them.  The warps' sums are
+// joined in shared memory in warp order (the result does not depend on
+// timing).
 // Weights are the 16-row operand of the warp-level m16n8k32 MMA, 8 NT tokens
-// its columns.  A lane loads 16 consecutive bytes of a row and uses them as
+// its columns.  A thread loads 16 consecutive bytes of a row and uses them as
 // the fragments of two MMAs; weights and tokens are permuted along K alike, so
 // the sum is over the same products.  Each 128-deep block starts from zero and
 // is added to the fp32 sums times its two scales.
@@ -901,31 +907,63 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// 16 bytes global -> shared, zeros unless `in` (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+
 constexpr int kFewWarps = 8;
+constexpr int kFewDepth = 6;            // K blocks of 2 KB per warp in flight
+constexpr int kFewBlock = 16 * 128;     // 16 weight rows x 128
+template <int NT>
+struct FewCfg {
+  static constexpr int kSums = kFewWarps * NT * 8 * 17 * 4;  // [warp][token][row], padded against bank conflicts
+  static constexpr int kSmemBytes = kFewWarps * kFewDepth * kFewBlock + kSums;
+  static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
+};
 
 template <int NT>
 __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_constant__ MxParams p) {
-  __shared__ float sums[kFewWarps][NT * 8][17];  // [warp][token][row], padded against bank conflicts
+  extern __shared__ uint8_t few_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
+  float(*sums)[NT * 8][17] = reinterpret_cast<float(*)[NT * 8][17]>(few_smem + kFewWarps * kFewDepth * kFewBlock);
+  const uint32_t slots = smem_u32(few_smem) + warp * kFewDepth * kFewBlock + lane * 16;
   const int64_t n_groups = ceil_div64(p.n, 16);
   const int e = static_cast<int>(blockIdx.x / n_groups);
   const int64_t r0 = (blockIdx.x - e * n_groups) * 16;
-  int64_t start;
-  bool bad = false;
-  const int64_t len = mx_segment(p, e, start, &bad);
-  if (bad && r0 == 0 && threadIdx.x == 0) atomicOr(p.error_word, kErrBadDims);
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  const uint8_t* wrow[2];
+  const int depth = static_cast<int>(p.k), kblocks = static_cast<int>(p.kb);
   bool live[2];
+  const uint8_t* wrow[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int64_t r = r0 + g + 8 * h;
     live[h] = r < p.n;
     wrow[h] = p.b + e * p.b_stride + (live[h] ? r : 0) * p.b_pitch + t * 16;
   }
+  grid_dependency_wait();  // global memory is read only from here on
+  int64_t start;
+  bool bad = false;
+  const int64_t len = mx_segment(p, e, start, &bad);
+  if (bad && r0 == 0 && threadIdx.x == 0) atomicOr(p.error_word, kErrBadDims);
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   const uint8_t* wscale = p.sb + (e * p.nb + r0 / 128) * p.kb;  // 16 rows lie inside one 128-row block
-  const int depth = static_cast<int>(p.k), kblocks = static_cast<int>(p.kb);
+  // Copies of this warp's i-th K block (warp + 8 i) into slot i % depth, as one group.
+  const auto fetch = [&](int i) {
+    const int kb = warp + i * kFewWarps;
+    if (kb < kblocks) {
+      const uint32_t slot = slots + (i % kFewDepth) * kFewBlock;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        // K is a multiple of 16: a 16-byte piece is inside the row or past its end.
+        const int k = kb * 128 + c * 64;
+        const bool in = k + t * 16 < depth;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) copy16(slot + (2 * h + c) * 512, wrow[h] + (in ? k : 0), in && live[h]);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   for (int64_t m0 = 0; m0 < len; m0 += 8 * NT) {
     float acc[NT][4];
     const uint8_t* xrow = p.a + (start + m0 + g) * p.a_pitch + t * 16;     // token m0 + g (+ 8 i)
@@ -933,52 +971,46 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_
     const int left = static_cast<int>(len - m0 < 8 * NT ? len - m0 : 8 * NT);
 #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-    // U blocks' weights are in flight before the first is used; a block past
-    // the end loads nothing (7 blocks a warp at K = 7168: two rounds of four).
-    constexpr int U = NT == 1 ? 4 : 2;
-#pragma unroll 1
-    for (int kb0 = warp; kb0 < kblocks; kb0 += kFewWarps * U) {
-      // K is a multiple of 16: a 16-byte piece is inside the row or past its end.
-      uint4 w[U][2][2];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+    for (int i = 0; i < kFewDepth; ++i) fetch(i);
+#pragma unroll 1
+    for (int b = 0; warp + b * kFewWarps < kblocks; ++b) {
+      const int kb = warp + b * kFewWarps;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kFewDepth - 1) : "memory");
+      uint4 w[2][2];
+      const uint32_t slot = slots + (b % kFewDepth) * kFewBlock;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4& v = w[i / 2][i % 2];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(slot + i * 512)
+                     : "memory");
+      }
+      const float sw = scale_value(__ldg(wscale + kb));
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int k = (kb0 + u * kFewWarps) * 128 + c * 64;
-          const bool in = k + t * 16 < depth;
+          const int k = kb * 128 + c * 64;
+          const uint4 x = 8 * i + g < left && k + t * 16 < depth
+                              ? __ldg(reinterpret_cast<const uint4*>(xrow + 8 * i * p.a_pitch + k))
+                              : zero;
+          mma_e4m3(part, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, x.x, x.y);
+          mma_e4m3(part, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, x.z, x.w);
+        }
+        // Columns 2t, 2t + 1 of the accumulator are tokens m0 + 8 i + 2t (+ 1).
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            w[u][h][c] = in && live[h] ? __ldcs(reinterpret_cast<const uint4*>(wrow[h] + k)) : zero;
-          }
+        for (int j = 0; j < 2; ++j) {
+          const float sx = 8 * i + 2 * t + j < left ? scale_value(__ldg(xscale + (8 * i + j) * p.kb + kb)) : 0.0f;
+          acc[i][j] += part[j] * sw * sx;
+          acc[i][2 + j] += part[2 + j] * sw * sx;
         }
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int kb = kb0 + u * kFewWarps;
-        if (kb >= kblocks) break;
-        const float sw = scale_value(__ldg(wscale + kb));
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int k = kb * 128 + c * 64;
-            const uint4 x = 8 * i + g < left && k + t * 16 < depth
-                                ? __ldg(reinterpret_cast<const uint4*>(xrow + 8 * i * p.a_pitch + k))
-                                : zero;
-            mma_e4m3(part, w[u][0][c].x, w[u][1][c].x, w[u][0][c].y, w[u][1][c].y, x.x, x.y);
-            mma_e4m3(part, w[u][0][c].z, w[u][1][c].z, w[u][0][c].w, w[u][1][c].w, x.z, x.w);
-          }
-          // Columns 2t, 2t + 1 of the accumulator are tokens m0 + 8 i + 2t (+ 1).
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float sx = 8 * i + 2 * t + j < left ? scale_value(__ldg(xscale + (8 * i + j) * p.kb + kb)) : 0.0f;
-            acc[i][j] += part[j] * sw * sx;
-            acc[i][2 + j] += part[2 + j] * sw * sx;
-          }
-        }
-      }
+      fetch(b + kFewDepth);  // into the slot just read
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
 #pragma unroll

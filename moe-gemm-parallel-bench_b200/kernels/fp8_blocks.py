@@ -47,8 +47,9 @@ def _source(x) -> int:
 
 
 def _target(name: str, t, shape: tuple, dtype, device):
-    if t is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+    if t is None:  # empty_strided: the shortest way to a tensor on the host side
+        steps = (shape[1], 1) if len(shape) == 2 else (shape[1] * shape[2], shape[2], 1)
+        return torch.empty_strided(shape, steps, dtype=dtype, device=device)
     if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} {shape} tensor on {device}")
     return t
@@ -127,7 +128,7 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
         raise ValueError("scales must be contiguous")
     ends = _offsets(offs, experts, device)
     if out is None:
-        out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
+        out = torch.empty_strided((rows, n), (n, 1), dtype=torch.bfloat16, device=device)
     elif tuple(out.shape) != (rows, n) or out.dtype != torch.bfloat16 or out.device != device:
         raise ValueError(f"out must be [{rows}, {n}] bfloat16 on {device}")
     a_steps, b_steps, out_steps = a.stride(), b.stride(), out.stride()

@@ -63,6 +63,11 @@ def _call(device, entry, *args):
         return entry(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def _rows_of(like, rows: int, cols: int):
+    """An empty [rows, cols] tensor of ``like``'s type and device."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=like.dtype, device=like.device)
+
+
 def _token(name: str, t, rows: int, cols: int, dtype, device) -> tuple[int, int]:
     """(address, pitch) of a [rows, cols] tensor of the call's type and device."""
     if tuple(t.shape) != (rows, cols):
@@ -146,11 +151,11 @@ def gated_ffn_forward(x, w13, w2, offs=None, *, out=None, h=None, gate_up=None):
     args.w13, args.w13_pitch, args.w13_stride = _weight("w13", w13, experts, hidden, 2 * ffn, dtype, device)
     args.w2, args.w2_pitch, args.w2_stride = _weight("w2", w2, experts, ffn, hidden, dtype, device)
     if out is None:
-        out = x.new_empty((rows, hidden))
+        out = _rows_of(x, rows, hidden)
     if h is None:
-        h = x.new_empty((rows, ffn))
+        h = _rows_of(x, rows, ffn)
     if gate_up is None:
-        gate_up = x.new_empty((rows, 2 * ffn))
+        gate_up = _rows_of(x, rows, 2 * ffn)
     args.y, args.y_pitch = _token("out", out, rows, hidden, dtype, device)
     args.h, args.h_pitch = _token("h", h, rows, ffn, dtype, device)
     args.gate_up, args.gate_up_pitch = _token("gate_up", gate_up, rows, 2 * ffn, dtype, device)
@@ -177,7 +182,7 @@ def gated_ffn_backward(dy, x, w13, w2, h, gate_up, offs=None, *, dx=None, dw13=N
     args.h, args.h_pitch = _token("h", h, rows, ffn, dtype, device)
     args.gate_up, args.gate_up_pitch = _token("gate_up", gate_up, rows, 2 * ffn, dtype, device)
     if dx is None:
-        dx = x.new_empty((rows, hidden))
+        dx = _rows_of(x, rows, hidden)
     if dw13 is None:
         dw13 = w13.new_empty(w13.shape)
     if dw2 is None:
@@ -218,7 +223,7 @@ def launch_grouped_mm_dgrad(dc, mat_b, offs=None, out=None, *, gate_up=None):
     cols = k if gate_up is None else 2 * k
     gu_at, gu_pitch = (0, 0) if gate_up is None else _token("gate_up", gate_up, rows, cols, dc.dtype, device)
     if out is None:
-        out = dc.new_empty((rows, cols))
+        out = _rows_of(dc, rows, cols)
     out_at, out_pitch = _token("out", out, rows, cols, dc.dtype, device)
     if rows == 0:
         return out
