@@ -158,6 +158,7 @@ SHAPES = [
     ([31] * 40, 72, 40),
     ([700, 1, 0, 333], 4104, 2056),  # pairs' 256 x 256 tiles
     ([0, 2, 256, 0, 255, 257], 2048, 1032),
+    ([31, 32, 33, 95, 128, 160, 223, 224, 225, 480, 481], 1048, 520),  # last row blocks of every length
 ]
 
 
