@@ -72,24 +72,30 @@ FastDiv fast_div(int64_t d) {
   return FastDiv{static_cast<uint32_t>(d), static_cast<uint32_t>(((1ull << s) + d - 1) / d), s};
 }
 
+// The widest access that the bases, pitches (elements) and row length allow.
 template <typename T>
-int rows_typed(const void* x, int64_t rows, int64_t cols, int64_t pitch, void* q, int64_t q_pitch, void* scale, int sms,
+int access_of(const void* x, int64_t pitch, int64_t stride, const void* q, int64_t q_pitch, int64_t q_stride, int64_t cols) {
+  const int size = static_cast<int>(sizeof(T));
+  const auto whole = [&](int bytes, int out) {
+    return aligned(x, bytes) && (pitch * size) % bytes == 0 && (stride * size) % bytes == 0 && cols % out == 0 &&
+           aligned(q, out) && q_pitch % out == 0 && q_stride % out == 0;
+  };
+  return whole(32, 16) ? k32Bytes : whole(16, 8) ? k16Bytes : kScalar;
+}
+
+template <typename T>
+int rows_typed(const void* x, int64_t rows, int64_t cols, int64_t pitch, void* q, int64_t q_pitch, void* scale,
                cudaStream_t s) {
   const int64_t blocks = rows * cdiv(cols, 128);
-  if (blocks >= (1ll << 31) - (1ll << 22)) return MGB_ERR_INVALID;  // 2^38 elements: more than the GPU holds
-  // Every half warp takes kRowsUnroll blocks at once (no short last sweep);
-  // fewer where that would leave SMs without a CTA.
-  const unsigned grid = static_cast<unsigned>(
-      std::max<int64_t>(cdiv(blocks, 16 * kRowsUnroll), std::min<int64_t>(cdiv(blocks, 16), 4ll * sms)));
-  const FastDiv kb = fast_div(cdiv(cols, 128));
-  const uint32_t nb = static_cast<uint32_t>(blocks);
-  const bool vec = aligned(x, 16) && pitch % (16 / static_cast<int>(sizeof(T))) == 0 && cols % 8 == 0 && aligned(q, 8) &&
-                   q_pitch % 8 == 0;
-  const T* in = static_cast<const T*>(x);
-  uint8_t* out = static_cast<uint8_t*>(q);
-  uint8_t* sc = static_cast<uint8_t*>(scale);
-  const auto kernel = vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
-  return launch_overlapped(kernel, grid, 256, 0, s, in, nb, kb, cols, pitch, out, q_pitch, sc) == cudaSuccess
+  if (blocks >= (1ll << 31)) return MGB_ERR_INVALID;  // 2^38 elements: more than the GPU holds
+  const int access = access_of<T>(x, pitch, 0, q, q_pitch, 0, cols);
+  const bool dense = pitch == cols && q_pitch == cols && cols % 128 == 0;
+  const auto kernel = access == k32Bytes   ? quantize_rows_kernel<T, k32Bytes>
+                      : access == k16Bytes ? quantize_rows_kernel<T, k16Bytes>
+                                           : quantize_rows_kernel<T, kScalar>;
+  return launch_overlapped(kernel, static_cast<unsigned>(cdiv(blocks, 32)), 256, 0, s, static_cast<const T*>(x),
+                           static_cast<uint32_t>(blocks), fast_div(cdiv(cols, 128)), cols, pitch,
+                           static_cast<uint8_t*>(q), q_pitch, static_cast<uint8_t*>(scale), dense) == cudaSuccess
              ? MGB_OK
              : MGB_ERR_CUDA;
 }
@@ -98,16 +104,14 @@ template <typename T>
 int blocks_typed(const void* x, int64_t matrices, int64_t rows, int64_t cols, int64_t pitch, int64_t stride, void* q,
                  void* scale, cudaStream_t s) {
   const int64_t kb = cdiv(cols, 128), per = cdiv(rows, 128) * kb;
-  if (matrices * per >= (1ll << 31)) return MGB_ERR_INVALID;
-  const int e = 16 / static_cast<int>(sizeof(T));
-  const bool vec = aligned(x, 16) && pitch % e == 0 && stride % e == 0 && cols % 8 == 0 && aligned(q, 8);
-  const unsigned grid = static_cast<unsigned>(matrices * per);
-  const T* in = static_cast<const T*>(x);
-  uint8_t* out = static_cast<uint8_t*>(q);
-  uint8_t* sc = static_cast<uint8_t*>(scale);
-  const auto kernel = vec ? quantize_blocks_kernel<T, true> : quantize_blocks_kernel<T, false>;
-  return launch_overlapped(kernel, grid, 256, 0, s, in, rows, cols, pitch, stride, out, cols, rows * cols, sc,
-                           fast_div(kb), fast_div(per)) == cudaSuccess
+  if (per >= (1ll << 31) || matrices * per >= (1ll << 31)) return MGB_ERR_INVALID;
+  const int access = access_of<T>(x, pitch, stride, q, cols, rows * cols, cols);
+  const auto kernel = access == k32Bytes   ? quantize_blocks_kernel<T, k32Bytes>
+                      : access == k16Bytes ? quantize_blocks_kernel<T, k16Bytes>
+                                           : quantize_blocks_kernel<T, kScalar>;
+  return launch_overlapped(kernel, static_cast<unsigned>(matrices * per), 256, 0, s, static_cast<const T*>(x), rows,
+                           cols, pitch, stride, static_cast<uint8_t*>(q), cols, rows * cols,
+                           static_cast<uint8_t*>(scale), fast_div(kb), fast_div(per)) == cudaSuccess
              ? MGB_OK
              : MGB_ERR_CUDA;
 }
@@ -249,15 +253,12 @@ int quantize_rows_launch(const void* x, int64_t rows, int64_t cols, int64_t pitc
   }
   if (dtype != MGB_FP16 && dtype != MGB_BF16 && dtype != MGB_FP32) return MGB_ERR_INVALID;
   if (!aligned(x, dtype == MGB_FP32 ? 4 : 2)) return MGB_ERR_INVALID;
-  int sms = 0;
-  long long budget = 0;
-  if (!current_launch_limits(&sms, &budget)) return MGB_ERR_CUDA;
   if (rows == 0) return MGB_OK;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case MGB_FP16: return rows_typed<__half>(x, rows, cols, pitch, q, q_pitch, scale, sms, s);
-    case MGB_BF16: return rows_typed<__nv_bfloat16>(x, rows, cols, pitch, q, q_pitch, scale, sms, s);
-    default: return rows_typed<float>(x, rows, cols, pitch, q, q_pitch, scale, sms, s);
+    case MGB_FP16: return rows_typed<__half>(x, rows, cols, pitch, q, q_pitch, scale, s);
+    case MGB_BF16: return rows_typed<__nv_bfloat16>(x, rows, cols, pitch, q, q_pitch, scale, s);
+    default: return rows_typed<float>(x, rows, cols, pitch, q, q_pitch, scale, s);
   }
 }
 

@@ -42,31 +42,54 @@ __device__ __forceinline__ uint32_t e4m3_pair(float a, float b, float inv) {
   return __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
 }
 
-// Eight consecutive elements of a row as loaded (16-bit types stay packed).
+// Sixteen consecutive elements of a row as loaded (16-bit types stay packed):
+// eight lanes hold a 1 x 128 block.
 template <typename T>
-struct Eight {
-  static constexpr int kWords = 2 * static_cast<int>(sizeof(T));
+struct Sixteen {
+  static constexpr int kWords = 4 * static_cast<int>(sizeof(T));
   uint32_t w[kWords];
 };
 
-// From column `col`; columns past `cols` are 0.  VEC: the address is 16-byte
-// aligned and the eight lie inside the row or all past it.
-template <typename T, bool VEC>
-__device__ __forceinline__ Eight<T> load8(const T* row, int64_t col, int64_t cols) {
-  Eight<T> v;
-  if constexpr (VEC) {
-    uint4* to = reinterpret_cast<uint4*>(v.w);
+// How rows may be addressed: element by element; in 16-byte pieces (rows and
+// their length in whole pieces of eight 16-bit elements); in 32-byte pieces.
+enum Access : int { kScalar = 0, k16Bytes = 1, k32Bytes = 2 };
+
+// From column `col`; columns past `cols` are 0.
+template <typename T, int ACCESS>
+__device__ __forceinline__ Sixteen<T> load16(const T* row, int64_t col, int64_t cols) {
+  Sixteen<T> v;
+  if constexpr (ACCESS == k32Bytes) {
+    const bool in = col < cols;
+    if (!in) {
 #pragma unroll
-    for (int i = 0; i < Eight<T>::kWords / 4; ++i) {
-      to[i] = col < cols ? __ldcs(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < Sixteen<T>::kWords; ++i) v.w[i] = 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < Sixteen<T>::kWords / 8; ++i) {
+        uint32_t* w = v.w + 8 * i;
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(reinterpret_cast<const uint32_t*>(row + col) + 8 * i));
+      }
+    }
+  } else if constexpr (ACCESS == k16Bytes) {
+    constexpr int kPiece = 16 / static_cast<int>(sizeof(T));  // elements per piece
+#pragma unroll
+    for (int i = 0; i < Sixteen<T>::kWords / 4; ++i) {
+      const uint4 x = col + i * kPiece < cols ? __ldcs(reinterpret_cast<const uint4*>(row + col) + i)
+                                              : make_uint4(0u, 0u, 0u, 0u);
+      v.w[4 * i] = x.x;
+      v.w[4 * i + 1] = x.y;
+      v.w[4 * i + 2] = x.z;
+      v.w[4 * i + 3] = x.w;
     }
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v.w[i] = col + i < cols ? __float_as_uint(row[col + i]) : 0u;
+    for (int i = 0; i < 16; ++i) v.w[i] = col + i < cols ? __float_as_uint(row[col + i]) : 0u;
   } else {
     const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const uint32_t lo = col + 2 * i < cols ? r[col + 2 * i] : 0u, hi = col + 2 * i + 1 < cols ? r[col + 2 * i + 1] : 0u;
       v.w[i] = lo | (hi << 16);
     }
@@ -74,37 +97,30 @@ __device__ __forceinline__ Eight<T> load8(const T* row, int64_t col, int64_t col
   return v;
 }
 
+// Elements 2 i and 2 i + 1.
 template <typename T>
-__device__ __forceinline__ void to_floats(const Eight<T>& v, float (&f)[8]) {
+__device__ __forceinline__ float2 two_floats(const Sixteen<T>& v, int i) {
   if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v.w[i]);
+    return make_float2(__uint_as_float(v.w[2 * i]), __uint_as_float(v.w[2 * i + 1]));
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return make_float2(__uint_as_float(v.w[i] << 16), __uint_as_float(v.w[i] & 0xFFFF0000u));
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 p;
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        p = make_float2(__uint_as_float(v.w[i] << 16), __uint_as_float(v.w[i] & 0xFFFF0000u));
-      } else {
-        p = __half22float2(*reinterpret_cast<const __half2*>(&v.w[i]));
-      }
-      f[2 * i] = p.x;
-      f[2 * i + 1] = p.y;
-    }
+    return __half22float2(*reinterpret_cast<const __half2*>(&v.w[i]));
   }
 }
 
 // Largest |element| as the type's bits: sign cleared, a floating value's bits
 // order as an unsigned integer, so 16-bit pairs take one packed maximum.
-// Infinities and NaNs come out on top (>= kNonFinite).
+// Infinities and NaNs come out on top (>= non_finite).
 template <typename T>
-__device__ __forceinline__ uint32_t top_bits(const Eight<T>& v, uint32_t top) {
-  if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ uint32_t top_bits(const Sixteen<T>& v, uint32_t top) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, v.w[i] & 0x7FFFFFFFu);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = __vmaxu2(top, v.w[i] & 0x7FFF7FFFu);
+  for (int i = 0; i < Sixteen<T>::kWords; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      top = max(top, v.w[i] & 0x7FFFFFFFu);
+    } else {
+      top = __vmaxu2(top, v.w[i] & 0x7FFF7FFFu);
+    }
   }
   return top;
 }
@@ -127,37 +143,40 @@ __device__ __forceinline__ uint32_t float_bits(uint32_t bits) {
     return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(bits))));
   }
 }
-// Rare: zeroes infinities and NaNs for the maximum of a block that holds some.
+// Rare: the maximum over the finite elements of a block that holds others.
 template <typename T>
-__device__ __forceinline__ uint32_t finite_top_bits(const Eight<T>& v, uint32_t top) {
+__device__ __forceinline__ uint32_t finite_top_bits(const Sixteen<T>& v, uint32_t top) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t b = sizeof(T) == 4 ? v.w[i] & 0x7FFFFFFFu : (v.w[i / 2] >> (16 * (i & 1))) & 0x7FFFu;
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t b = sizeof(T) == 4 ? v.w[i % Sixteen<T>::kWords] & 0x7FFFFFFFu : (v.w[i / 2] >> (16 * (i & 1))) & 0x7FFFu;
     if (b < non_finite<T>()) top = max(top, b);
   }
   return top;
 }
 
-// Eight e4m3 values; `odd`: the block holds infinities or NaNs, which become NaN.
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(uint8_t* row, int64_t col, int64_t cols, const Eight<T>& v, float inv, bool odd) {
-  float f[8];
-  to_floats(v, f);
-  if (odd) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = isinf(f[i]) ? __uint_as_float(0x7FC00000u) : f[i];
-  }
+// Sixteen e4m3 values; `odd`: the block holds infinities or NaNs, which become NaN.
+template <typename T, int ACCESS>
+__device__ __forceinline__ void store16(uint8_t* row, int64_t col, int64_t cols, const Sixteen<T>& v, float inv, bool odd) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = e4m3_pair(f[2 * i], f[2 * i + 1], inv);
-  if constexpr (VEC) {
-    if (col < cols) {
-      *reinterpret_cast<uint2*>(row + col) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+  for (int i = 0; i < 4; ++i) {
+    float2 a = two_floats(v, 2 * i), b = two_floats(v, 2 * i + 1);
+    if (odd) {
+      const float nan = __uint_as_float(0x7FC00000u);
+      a = make_float2(isinf(a.x) ? nan : a.x, isinf(a.y) ? nan : a.y);
+      b = make_float2(isinf(b.x) ? nan : b.x, isinf(b.y) ? nan : b.y);
     }
+    w[i] = e4m3_pair(a.x, a.y, inv) | (e4m3_pair(b.x, b.y, inv) << 16);
+  }
+  if constexpr (ACCESS == k32Bytes) {
+    if (col < cols) *reinterpret_cast<uint4*>(row + col) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else if constexpr (ACCESS == k16Bytes) {
+    if (col < cols) *reinterpret_cast<uint2*>(row + col) = make_uint2(w[0], w[1]);
+    if (col + 8 < cols) *reinterpret_cast<uint2*>(row + col + 8) = make_uint2(w[2], w[3]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (col + i < cols) row[col + i] = static_cast<uint8_t>(w[i / 2] >> (8 * (i % 2)));
+    for (int i = 0; i < 16; ++i) {
+      if (col + i < cols) row[col + i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i % 4)));
     }
   }
 }
@@ -171,54 +190,47 @@ struct FastDiv {
   }
 };
 
-// Rows: 16 lanes hold one 1 x 128 block (8 elements each), so a warp's loads
-// are whole 256-byte pieces; the loads of kRowsUnroll blocks per half warp are
-// in flight before the first is used.  One read and one write of every
-// element: bound by memory.
-constexpr int kRowsUnroll = 4;
-template <typename T, bool VEC>
+// Rows: a thread per sixteen elements, eight threads per 1 x 128 block, one
+// block of 32 blocks per CTA step: 32-byte loads, 16-byte stores, no loop.
+// One read and one write of every element, bound by memory.  `dense`: rows of
+// whole blocks without padding, whose b-th block starts at element 128 b.
+// (bf16 8191 x 7168, 176 MB: 29 us; 8 elements a thread, four blocks in flight
+// 31 us; a copy of as many bytes 26 us.)
+template <typename T, int ACCESS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, uint32_t blocks, FastDiv kb,
                                                             int64_t cols, int64_t pitch, uint8_t* __restrict__ q,
-                                                            int64_t q_pitch, uint8_t* __restrict__ scale) {
-  const int l = threadIdx.x & 15;
-  const uint32_t half = 0xFFFFu << (threadIdx.x & 16);  // the halves of a warp may end at different blocks
-  const uint32_t stride = gridDim.x * 16u;
+                                                            int64_t q_pitch, uint8_t* __restrict__ scale, bool dense) {
   grid_dependency_wait();
-  for (uint32_t b0 = blockIdx.x * 16u + (threadIdx.x >> 4); b0 < blocks; b0 += stride * kRowsUnroll) {
-    Eight<T> v[kRowsUnroll];
-#pragma unroll
-    for (int u = 0; u < kRowsUnroll; ++u) {
-      const uint32_t b = b0 + u * stride;
-      if (b < blocks) {
-        const uint32_t row = kb.div(b);
-        v[u] = load8<T, VEC>(x + row * pitch, static_cast<int64_t>(b - row * kb.d) * 128 + l * 8, cols);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kRowsUnroll; ++u) {
-      const uint32_t b = b0 + u * stride;
-      if (b >= blocks) break;
-      uint32_t top = fold_top<T>(top_bits<T>(v[u], 0u));
-#pragma unroll
-      for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(half, top, d));
-      const bool odd = top >= non_finite<T>();
-      if (odd) {
-        top = finite_top_bits<T>(v[u], 0u);
-#pragma unroll
-        for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(half, top, d));
-      }
-      const int byte = scale_byte(float_bits<T>(top));
-      const uint32_t row = kb.div(b);
-      store8<T, VEC>(q + row * q_pitch, static_cast<int64_t>(b - row * kb.d) * 128 + l * 8, cols, v[u],
-                     inverse_scale(byte), odd);
-      if (l == 0) scale[b] = static_cast<uint8_t>(byte);
-    }
+  const uint32_t b = blockIdx.x * 32u + (threadIdx.x >> 3);
+  const int l = threadIdx.x & 7;
+  const uint32_t eight = 0xFFu << (threadIdx.x & 24);  // the threads of a block
+  if (b >= blocks) return;
+  uint32_t row = 0;
+  int64_t col = b * 128ll + l * 16;
+  if (!dense) {
+    row = kb.div(b);
+    col = (b - row * kb.d) * 128ll + l * 16;
+  } else {
+    cols = static_cast<int64_t>(blocks) * 128;
   }
+  const Sixteen<T> v = load16<T, ACCESS>(x + row * pitch, col, cols);
+  uint32_t top = fold_top<T>(top_bits<T>(v, 0u));
+#pragma unroll
+  for (int d = 4; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(eight, top, d));
+  const bool odd = top >= non_finite<T>();
+  if (odd) {
+    top = finite_top_bits<T>(v, 0u);
+#pragma unroll
+    for (int d = 4; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(eight, top, d));
+  }
+  const int byte = scale_byte(float_bits<T>(top));
+  store16<T, ACCESS>(q + row * q_pitch, col, cols, v, inverse_scale(byte), odd);
+  if (l == 0) scale[b] = static_cast<uint8_t>(byte);
 }
 
-// Blocks: one CTA per 128 x 128 block, its 16384 elements in registers (16
-// threads by 8 elements across, 16 rows per step), one pass over memory.
-template <typename T, bool VEC>
+// Blocks: one CTA per 128 x 128 block, its 16384 elements in registers (8
+// threads by 16 elements across, 32 rows per step), one pass over memory.
+template <typename T, int ACCESS>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
                                                               int64_t pitch, int64_t matrix, uint8_t* __restrict__ q,
                                                               int64_t q_pitch, int64_t q_matrix,
@@ -226,14 +238,14 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
   __shared__ uint32_t tops[8];
   const uint32_t e = per.div(blockIdx.x), in = blockIdx.x - e * per.d;
   const uint32_t rb = kb.div(in);
-  const int64_t r0 = rb * 128ll + (threadIdx.x >> 4), c = (in - rb * kb.d) * 128ll + (threadIdx.x & 15) * 8;
+  const int64_t r0 = rb * 128ll + (threadIdx.x >> 3), c = (in - rb * kb.d) * 128ll + (threadIdx.x & 7) * 16;
   const T* base = x + e * matrix;
-  Eight<T> v[8];
+  Sixteen<T> v[4];
   grid_dependency_wait();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + i * 16;
-    v[i] = load8<T, VEC>(base + r * pitch, r < rows ? c : cols, cols);
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = r0 + i * 32;
+    v[i] = load16<T, ACCESS>(base + r * pitch, r < rows ? c : cols, cols);
   }
   const auto reduce = [&](uint32_t top) {
     top = __reduce_max_sync(0xFFFFFFFFu, top);
@@ -246,21 +258,21 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
   };
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = top_bits<T>(v[i], top);
+  for (int i = 0; i < 4; ++i) top = top_bits<T>(v[i], top);
   top = reduce(fold_top<T>(top));
   const bool odd = top >= non_finite<T>();  // the same in every thread
   if (odd) {
     top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = finite_top_bits<T>(v[i], top);
+    for (int i = 0; i < 4; ++i) top = finite_top_bits<T>(v[i], top);
     top = reduce(top);
   }
   const int byte = scale_byte(float_bits<T>(top));
   const float inv = inverse_scale(byte);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + i * 16;
-    if (r < rows) store8<T, VEC>(q + e * q_matrix + r * q_pitch, c, cols, v[i], inv, odd);
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = r0 + i * 32;
+    if (r < rows) store16<T, ACCESS>(q + e * q_matrix + r * q_pitch, c, cols, v[i], inv, odd);
   }
   if (threadIdx.x == 0) scale[blockIdx.x] = static_cast<uint8_t>(byte);
 }
