@@ -50,7 +50,7 @@ int launch_kernel(const FfnParams& p, int64_t tiles, int sm_count, cudaStream_t 
   cfg.stream = stream;
   cfg.attrs = attr;
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = G;
+  attr[0].val.clusterDim.x = G * p.split;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   if (!configured[dev]) {
@@ -70,8 +70,9 @@ int launch_kernel(const FfnParams& p, int64_t tiles, int sm_count, cudaStream_t 
     }
     configured[dev] = true;
   }
-  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(tiles, clusters[dev]));
-  cfg.gridDim = dim3(static_cast<unsigned>(grid * G), 1, 1);
+  // `tiles` of a split launch are its clusters (never more CTAs than SMs).
+  const int64_t grid = p.split > 1 ? tiles : std::max<int64_t>(1, std::min<int64_t>(tiles, clusters[dev]));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid * G * p.split), 1, 1);
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 2;
@@ -107,7 +108,7 @@ FfnTensor tensor(const void* data, int64_t pitch, int64_t expert_stride, bool to
 // kFfnPlanLaunches tile lists.
 size_t maps_bytes(int64_t experts, int jobs) { return static_cast<size_t>(experts) * jobs * kFfnMaps * kMapBytes; }
 size_t list_bytes(int64_t experts, int jobs) {
-  return (static_cast<size_t>(experts) * jobs + 1 + 15) / 16 * 16 * sizeof(int64_t);
+  return (static_cast<size_t>(experts) * jobs + 1 + 31) / 32 * 32 * sizeof(int32_t);
 }
 
 // The launches of one call: jobs are added launch by launch, then run()
@@ -180,6 +181,28 @@ struct Launcher {
     return Tile{tiles >= pairs ? 2 : 1, epi == kFfnPlain && tiles >= 2 * pairs};
   }
 
+  // Tiles of a job, at most (a segment boundary adds one row block).
+  int64_t tiles_of(const FfnJob& j, const FfnPlan::Launch& l) const {
+    const int64_t segments = std::min<int64_t>(plan.experts, plan.rows);
+    const int64_t m = j.wgrad ? plan.experts * cdiv(j.m, l.tile_rows)
+                              : cdiv(plan.rows, l.tile_rows) + std::max<int64_t>(segments - 1, 0);
+    return m * cdiv(j.n, l.tile_cols);
+  }
+
+  // Splits the contraction of job 0's tiles: as many CTAs a tile (2, 4 or 8)
+  // as the SMs hold at once, each with at least four blocks.  Clusters do not
+  // cross a GPC, whose SMs (16 to 18) hold whole clusters only: an eighth of
+  // the SMs stays out.  Returns the launch's clusters (its tiles, unsplit).
+  int64_t split_of(FfnParams& p, const FfnPlan::Launch& l, int64_t tiles) const {
+    if (plan.rows == 0) return tiles;
+    const int64_t own = tiles_of(p.job[0], l);
+    const int64_t blocks = cdiv(p.job[0].k, 64), cap = sms - sms / 8;
+    while (p.split < 8 && own * p.split * 2 <= cap && blocks >= 8 * p.split) p.split *= 2;
+    if (p.split == 1) return tiles;
+    // Other jobs' tiles go to every CTA one by one.
+    return std::max(own, std::min<int64_t>(cap / p.split, cdiv(tiles - own, p.split)));
+  }
+
   int run() {
     if (!ok) return MGB_ERR_CUDA;
     const int64_t experts = plan.experts;
@@ -191,22 +214,24 @@ struct Launcher {
       tile[i] = tile_of(l, epilogue[i]);
       l.tile_rows = 128 * tile[i].g;
       l.tile_cols = (epilogue[i] == kFfnSwiglu ? 64 : tile[i].wide ? 256 : 128) * tile[i].g;
-      l.tile_start = reinterpret_cast<int64_t*>(list);
+      l.tile_start = reinterpret_cast<int32_t*>(list);
       list += list_bytes(experts, l.jobs);
+      int64_t tiles = 0;
+      for (int k = 0; k < l.jobs; ++k) tiles += tiles_of(plan.job[l.first_job + k], l);
+      if (tiles >= (1ll << 31)) return MGB_ERR_INVALID;  // the list's 32-bit tile numbers
     }
-    if (launch_overlapped(ffn_plan_kernel, static_cast<unsigned>(plan.jobs * experts + plan.launches), 32, 0, stream,
-                          plan) != cudaSuccess) {
+    if (launch_overlapped(ffn_plan_kernel, static_cast<unsigned>(plan.jobs * experts + plan.launches),
+                          32 * kFfnMaps, 0, stream, plan) != cudaSuccess) {
       return MGB_ERR_CUDA;
     }
     for (int i = 0; i < plan.launches; ++i) {
       const FfnPlan::Launch& l = plan.launch[i];
       FfnParams p;
       std::memset(static_cast<void*>(&p), 0, sizeof(p));
-      int64_t tiles = 0;  // at most: a segment boundary adds one row block
+      int64_t tiles = 0;
       for (int k = 0; k < l.jobs; ++k) {
-        const FfnJob& j = p.job[k] = plan.job[l.first_job + k];
-        const int64_t m = j.wgrad ? experts * cdiv(j.m, l.tile_rows) : cdiv(plan.rows, l.tile_rows) + experts - 1;
-        tiles += m * cdiv(j.n, l.tile_cols);
+        p.job[k] = plan.job[l.first_job + k];
+        tiles += tiles_of(p.job[k], l);
       }
       p.jobs = l.jobs;
       p.experts = plan.experts;
@@ -218,6 +243,8 @@ struct Launcher {
       p.tile_cols = l.tile_cols;
       p.wait_budget = budget;
       p.error_word = plan.error_word;
+      p.split = 1;
+      if (tile[i].g == 1 && !plan.job[l.first_job].wgrad) tiles = split_of(p, l, tiles);
       const int st = epilogue[i] == kFfnPlain    ? launch_epilogue<kFfnPlain>(dtype, tile[i], p, tiles, sms, stream)
                      : epilogue[i] == kFfnSwiglu ? launch_epilogue<kFfnSwiglu>(dtype, tile[i], p, tiles, sms, stream)
                                                  : launch_epilogue<kFfnSwigluBwd>(dtype, tile[i], p, tiles, sms, stream);

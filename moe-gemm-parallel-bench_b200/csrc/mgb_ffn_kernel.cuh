@@ -31,6 +31,13 @@
 // G = 1: one CTA, 128 x 128 tiles, four times as many, for launches whose
 // 256 x 256 tiles would leave most SMs idle.  Both load 128 rows of A and
 // 128 columns of B per CTA and 64-deep contraction block (32 KB a stage).
+// Split contraction (G = 1, p.split > 1; for launches whose row tiles would
+// leave at least half of the SMs idle through a long contraction): the CTAs of
+// a cluster first take the other jobs' tiles one by one, then share one tile
+// of job 0: each sums a range of its contraction, leaves fp32 sums in its own
+// (then idle) operand ring, and CTA r adds rows [128 r / split, ...) of all of
+// them over distributed shared memory, in rank order, and applies the
+// epilogue.
 // Every wait is bounded; loads carry no multicast.
 #pragma once
 
@@ -70,8 +77,9 @@ struct FfnParams {
   const int32_t* offs;  // [experts] row ends; nullptr: one segment of `rows`
   int64_t rows;
   uint8_t* maps;        // [jobs][experts][kFfnMaps] tensor maps
-  int64_t* tile_start;  // [jobs * experts + 1] first tile of every (job, expert)
+  int32_t* tile_start;  // [jobs * experts + 1] first tile of every (job, expert)
   int32_t tile_rows, tile_cols;  // output tile (the walk's)
+  int32_t split;        // CTAs of a cluster that share the contraction of job 0's tiles (one CTA tiles; 1: none)
   long long wait_budget;
   uint32_t* error_word;
 };
@@ -83,7 +91,7 @@ struct FfnPlan {
   CUtensorMap map[kFfnPlanJobs][kFfnMaps];  // templates; token tensors' have one row
   struct Launch {
     int32_t first_job, jobs, tile_rows, tile_cols;
-    int64_t* tile_start;
+    int32_t* tile_start;
   } launch[kFfnPlanLaunches];
   int32_t jobs, launches, experts;
   const int32_t* offs;
@@ -106,18 +114,21 @@ __device__ __forceinline__ int64_t ffn_segment(const int32_t* offs, int64_t rows
   return end - start;
 }
 
-// Tensor maps of every (job, expert), one warp each, and every launch's tile
-// prefix sums (the last blocks).
-__global__ void __launch_bounds__(32) ffn_plan_kernel(const __grid_constant__ FfnPlan p) {
+// Tensor maps of every (job, expert), one block each and a warp per map, and
+// every launch's tile prefix sums (the last blocks).  A warp per map because
+// the parameters are cold: their constant-cache misses, one after another in
+// one warp, were most of this kernel's time.
+__global__ void __launch_bounds__(32 * kFfnMaps) ffn_plan_kernel(const __grid_constant__ FfnPlan p) {
   __shared__ alignas(128) CUtensorMap staging[kFfnMaps];
-  const int lane = threadIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_launch_dependents();
-  grid_dependency_wait();  // offs and this scratch may be in use until here
   if (static_cast<int>(blockIdx.x) >= p.jobs * p.experts) {
+    if (warp > 0) return;
     const FfnPlan::Launch& l = p.launch[blockIdx.x - p.jobs * p.experts];
     const int pairs = l.jobs * p.experts;
     const int per = (pairs + 31) / 32;
     const int lo = lane * per, hi = lo + per < pairs ? lo + per : pairs;
+    grid_dependency_wait();  // offs and this scratch may be in use until here
     auto tiles_of = [&](int i) -> int64_t {
       const FfnJob& j = p.job[l.first_job + i / p.experts];
       int64_t start;
@@ -134,74 +145,80 @@ __global__ void __launch_bounds__(32) ffn_plan_kernel(const __grid_constant__ Ff
     }
     int64_t run = incl - sum;
     for (int i = lo; i < hi; ++i) {
-      l.tile_start[i] = run;
+      l.tile_start[i] = static_cast<int32_t>(run);
       run += tiles_of(i);
     }
-    if (lane == 31) l.tile_start[pairs] = incl;
+    if (lane == 31) l.tile_start[pairs] = static_cast<int32_t>(incl);
     return;
   }
   const int job = blockIdx.x / p.experts, e = blockIdx.x % p.experts;
   const FfnJob& j = p.job[job];
-  bool bad = false;
-  int64_t start = 0;
-  const int64_t len = ffn_segment(p.offs, p.rows, e, start, &bad);
-  if (bad && lane == 0) atomicOr(p.error_word, kErrBadDims);
-  // One lane per map: copy the template, move its base, end its rows with the segment.
-  if (lane < j.maps) {
-    const FfnTensor& t = j.t[lane];
-    const uint4* src = reinterpret_cast<const uint4*>(&p.map[job][lane]);
-    uint4* dst = reinterpret_cast<uint4*>(&staging[lane]);
-    for (int i = 0; i < 8; ++i) dst[i] = src[i];
-    if (t.token) {
-      if (len > 0) {  // an empty segment's maps are never used
-        tmap_replace_address(&staging[lane], t.data + start * t.pitch * 2);
-        tmap_replace_dim(&staging[lane], 1, static_cast<uint32_t>(len));
-      }
-    } else {
-      tmap_replace_address(&staging[lane], t.data + e * t.expert_stride * 2);
+  if (warp >= j.maps) return;
+  const FfnTensor t = j.t[warp];
+  if (lane < 8) {
+    reinterpret_cast<uint4*>(&staging[warp])[lane] = reinterpret_cast<const uint4*>(&p.map[job][warp])[lane];
+  }
+  __syncwarp();
+  grid_dependency_wait();
+  if (lane == 0) {  // move the base, end the rows with the segment
+    bool bad = false;
+    int64_t start = 0;
+    const int64_t len = ffn_segment(p.offs, p.rows, e, start, &bad);
+    if (bad) atomicOr(p.error_word, kErrBadDims);
+    if (!t.token) {
+      tmap_replace_address(&staging[warp], t.data + e * t.expert_stride * 2);
+    } else if (len > 0) {  // an empty segment's maps are never used
+      tmap_replace_address(&staging[warp], t.data + start * t.pitch * 2);
+      tmap_replace_dim(&staging[warp], 1, static_cast<uint32_t>(len));
     }
   }
   __syncwarp();
-  CUtensorMap* g = reinterpret_cast<CUtensorMap*>(p.maps) + static_cast<int64_t>(blockIdx.x) * kFfnMaps;
-  for (int i = 0; i < j.maps; ++i) tmap_publish(&g[i], &staging[i]);
+  tmap_publish(reinterpret_cast<CUtensorMap*>(p.maps) + static_cast<int64_t>(blockIdx.x) * kFfnMaps + warp,
+               &staging[warp]);
 }
 
-// A role's position in the tile list.
+// Words of shared memory for the launch's tile list and row ends, if they fit:
+// a role then finds a tile without a chain of global loads.
+constexpr int kListWords = 400;
+
+// A role's position in the tile list (`ts` and `offs` in shared or global memory).
 struct FfnWalk {
+  const FfnParams& p;
+  const int32_t* ts;
+  const int32_t* offs;
   int pair = -1;  // job * experts + e
   int64_t first = 0, end = 0;
-  int64_t len = 0;     // rows of the expert's segment
+  int64_t start = 0, len = 0;  // rows of the expert's segment
   int64_t rows = 0;    // output rows
   int64_t m_blocks = 1, n_blocks = 1;
   int64_t kblocks = 0;
   const FfnJob* job = nullptr;
 
-  __device__ __forceinline__ bool seek(const FfnParams& p, int64_t t) {
-    const int64_t* ts = p.tile_start;
-    const int pairs = p.jobs * p.experts;
-    if (t >= end || pair < 0) {
-      if (t >= ts[pairs]) return false;
-      int lo = pair < 0 ? 0 : pair, hi = pairs - 1;
-      while (lo < hi) {  // the last pair whose first tile is <= t owns it (empty pairs share their successor's)
-        const int mid = (lo + hi + 1) >> 1;
-        if (ts[mid] <= t) {
-          lo = mid;
-        } else {
-          hi = mid - 1;
-        }
+  __device__ __forceinline__ FfnWalk(const FfnParams& params, const int32_t* list, const int32_t* ends)
+      : p(params), ts(list), offs(ends) {}
+
+  // Moves to the (job, expert) of tile t.
+  __device__ __forceinline__ void seek(int64_t t) {
+    if (pair >= 0 && t >= first && t < end) return;
+    // The last pair whose first tile is <= t owns it (empty pairs share their successor's).
+    int lo = pair >= 0 && t >= end ? pair : 0, hi = p.jobs * p.experts - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (ts[mid] <= t) {
+        lo = mid;
+      } else {
+        hi = mid - 1;
       }
-      pair = lo;
-      first = ts[lo];
-      end = ts[lo + 1];
-      job = &p.job[lo / p.experts];
-      int64_t start;
-      len = ffn_segment(p.offs, p.rows, lo % p.experts, start);
-      rows = job->wgrad ? job->m : len;
-      m_blocks = ceil_div64(rows, p.tile_rows);
-      n_blocks = ceil_div64(job->n, p.tile_cols);
-      kblocks = ceil_div64(job->wgrad ? len : job->k, 64);
     }
-    return true;
+    pair = lo;
+    first = ts[lo];
+    end = ts[lo + 1];
+    job = &p.job[lo / p.experts];
+    len = ffn_segment(offs, p.rows, lo % p.experts, start);
+    rows = job->wgrad ? job->m : len;
+    m_blocks = ceil_div64(rows, p.tile_rows);
+    n_blocks = ceil_div64(job->n, p.tile_cols);
+    kblocks = ceil_div64(job->wgrad ? len : job->k, 64);
   }
   // Bands of 8 row blocks, row block fastest inside a band (as TileWalk).
   __device__ __forceinline__ void blocks(int64_t t, int64_t& mb, int64_t& nb) const {
@@ -219,6 +236,55 @@ struct FfnWalk {
 // plain epilogue.  It moves 48 KB into a CTA per 128 x 512 x 64 products
 // where the 256 x 256 tile moves 32 KB per 128 x 256 x 64, a quarter less per
 // product; its one 512-column accumulator fills TMEM and is freed by halves.
+// The tiles a CTA (or pair) works on, in order: `first`, `first + step`, ...
+// below `end`, then with a split the cluster's tile of job 0 (`shared`, -1:
+// none), of which it takes contraction blocks [kb_from, kb_to).
+struct FfnItems {
+  int64_t next, step, end, shared;
+  int share, split;
+  bool last = false;  // the current item is the shared one
+  int32_t kb_from = 0, kb_to = 0;
+
+  __device__ __forceinline__ FfnItems(const FfnWalk& walk, int group) {
+    const FfnParams& p = walk.p;
+    split = p.split;
+    end = walk.ts[p.jobs * p.experts];
+    next = blockIdx.x / group;
+    step = gridDim.x / group;
+    shared = -1;
+    share = 0;
+    if (split > 1) {
+      const int64_t mine = walk.ts[p.experts];  // tiles of job 0
+      next += mine;
+      share = static_cast<int>(cluster_ctarank());
+      const int64_t c = blockIdx.x / split;
+      if (c < mine) shared = c;
+    }
+  }
+  __device__ __forceinline__ bool advance(FfnWalk& walk, int64_t& t) {
+    if (next < end) {
+      t = next;
+      next += step;
+      walk.seek(t);
+      kb_from = 0;
+      kb_to = static_cast<int32_t>(walk.kblocks);
+      return true;
+    }
+    if (last || shared < 0) return false;
+    last = true;
+    t = shared;
+    walk.seek(t);
+    const int32_t per = blocks_each(walk);
+    kb_from = share * per;
+    const int32_t all = static_cast<int32_t>(walk.kblocks);
+    kb_to = kb_from + per < all ? kb_from + per : all;
+    return true;
+  }
+  __device__ __forceinline__ int32_t blocks_each(const FfnWalk& walk) const {
+    return static_cast<int32_t>((walk.kblocks + split - 1) / split);
+  }
+};
+
 template <typename T, int EPI, int G, int NH = 1>
 struct FfnCfg {
   static_assert(sizeof(T) == 2 && (G == 1 || G == 2), "16-bit types, one CTA or a pair");
@@ -238,8 +304,12 @@ struct FfnCfg {
   static constexpr int kEpiBytes = 4 * kEpiBlocks * kEpiWarpBytes;
   static constexpr int kStages = (kTcSmemBudget - kEpiBytes) / kStageBytes;
   static constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + 2048 + 1024;
+  static_assert((2 * kStages + 13) * 8 + 12 + kListWords * 4 <= 2048, "barriers and the tile list");
   static constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   static_assert(kStages >= 4 && kSmemBytes <= 232448, "shared memory");
+  // Split contraction: a row of partial sums, padded against bank conflicts.
+  static constexpr int kSumRow = kAccCols * 4 + 16;
+  static_assert(G == 2 || kTileM * kSumRow <= kStages * kStageBytes, "partial sums fit the ring");
 };
 
 // Swiglu epilogue of one warp: gate columns [0, TO), up columns [TO, 2 TO) of
@@ -334,6 +404,77 @@ __device__ __forceinline__ void by_layout(const FfnJob& j, F&& f) {
   }
 }
 
+// Four consecutive 16-bit values (columns are multiples of 8: all inside a row or past it).
+template <typename T>
+__device__ __forceinline__ void store4(const FfnTensor& t, int64_t row, int64_t col, float a, float b, float c, float d) {
+  uint2 v;
+  v.x = pack_pair<T>(__float_as_uint(a), __float_as_uint(b));
+  v.y = pack_pair<T>(__float_as_uint(c), __float_as_uint(d));
+  *reinterpret_cast<uint2*>(t.data + (row * t.pitch + col) * 2) = v;
+}
+template <typename T>
+__device__ __forceinline__ float4 load4(const FfnTensor& t, int64_t row, int64_t col) {
+  const uint2 v = *reinterpret_cast<const uint2*>(t.data + (row * t.pitch + col) * 2);
+  const float2 a = unpack_pair<T>(v.x), b = unpack_pair<T>(v.y);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// This CTA's rows of a split tile: the `parts` partial sums in rank order,
+// then the epilogue; a warp per row, a lane per four accumulator columns.
+template <typename T, int EPI, class Cfg>
+__device__ __forceinline__ void ffn_join(const FfnParams& p, const FfnWalk& walk, const FfnItems& items, int parts,
+                                         uint32_t ring, int warp, int lane) {
+  const FfnJob& j = *walk.job;
+  int64_t mb, nb;
+  walk.blocks(items.shared, mb, nb);
+  const int rows = Cfg::kTileM / items.split;
+  for (int r = items.share * rows + warp; r < (items.share + 1) * rows; r += kTcThreads / 32) {
+    const int64_t m = mb * Cfg::kTileM + r;
+    if (m >= walk.rows) break;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < parts; ++i) {
+      float4 v;
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                   : "r"(mapa_shared(ring + r * Cfg::kSumRow + lane * 16, i))
+                   : "memory");
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+    const int64_t row = walk.start + m;
+    if constexpr (EPI == kFfnSwiglu) {
+      // Lanes 0-15 hold gate columns, lane l + 16 the up columns of lane l's.
+      const float4 u = make_float4(__shfl_down_sync(0xffffffffu, s.x, 16), __shfl_down_sync(0xffffffffu, s.y, 16),
+                                   __shfl_down_sync(0xffffffffu, s.z, 16), __shfl_down_sync(0xffffffffu, s.w, 16));
+      const int64_t col = nb * Cfg::kTileOut + (lane & 15) * 4;
+      if (col < j.n) {
+        store4<T>(j.t[lane < 16 ? 3 : 4], row, col, s.x, s.y, s.z, s.w);
+        if (lane < 16) {
+          store4<T>(j.t[2], row, col, silu_mul(s.x, u.x), silu_mul(s.y, u.y), silu_mul(s.z, u.z), silu_mul(s.w, u.w));
+        }
+      }
+    } else {
+      const int64_t col = nb * Cfg::kTileOut + lane * 4;
+      if (col < j.n) {
+        if constexpr (EPI == kFfnPlain) {
+          store4<T>(j.t[2], row, col, s.x, s.y, s.z, s.w);
+        } else {
+          const float4 g = load4<T>(j.t[4], row, col), u = load4<T>(j.t[5], row, col);
+          float4 dg, du;
+          swiglu_grad(s.x, g.x, u.x, dg.x, du.x);
+          swiglu_grad(s.y, g.y, u.y, dg.y, du.y);
+          swiglu_grad(s.z, g.z, u.z, dg.z, du.z);
+          swiglu_grad(s.w, g.w, u.w, dg.w, du.w);
+          store4<T>(j.t[2], row, col, dg.x, dg.y, dg.z, dg.w);
+          store4<T>(j.t[3], row, col, du.x, du.y, du.z, du.w);
+        }
+      }
+    }
+  }
+}
+
 template <typename T, int EPI, int G, int NH>
 __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constant__ FfnParams p) {
   using Cfg = FfnCfg<T, EPI, G, NH>;
@@ -353,14 +494,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gate_bars + 8);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* never = abort + 1;
+  int32_t* list = reinterpret_cast<int32_t*>(tmem_slot + 3);  // kListWords
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = G == 2 ? cluster_ctarank() : 0u;
   const bool leader = rank == 0;
-  const int64_t first_item = blockIdx.x / G;
-  const int64_t items_step = gridDim.x / G;
-
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
@@ -392,6 +531,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
   const uint32_t tmem_base = *tmem_slot;
   const long long budget = p.wait_budget;
   grid_dependency_wait();  // global memory is read only from here on
+  const int32_t* ts = p.tile_start;
+  const int32_t* offs = p.offs;
+  const int pairs = p.jobs * p.experts;
+  if (pairs + 1 + p.experts <= kListWords) {
+    for (int i = threadIdx.x; i <= pairs; i += kTcThreads) list[i] = p.tile_start[i];
+    if (p.offs != nullptr) {
+      for (int i = threadIdx.x; i < p.experts; i += kTcThreads) list[pairs + 1 + i] = p.offs[i];
+      offs = list + pairs + 1;
+    }
+    ts = list;
+    __syncthreads();
+  }
   const CUtensorMap* all_maps = reinterpret_cast<const CUtensorMap*>(p.maps);
 
   auto fail = [&](uint32_t bits) {
@@ -408,12 +559,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
       const uint64_t pol_stream = policy_evict_first();
       const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), empty0 = smem_u32(empty);
       const uint32_t lead0 = G == 2 ? mapa_shared(full0, 0) : full0;  // the leader's barriers
-      FfnWalk walk;
+      FfnWalk walk(p, ts, offs);
+      FfnItems items(walk, G);
       int s = 0;
       uint32_t phase = 0, loaded = 0;
       int built = -1;
       bool ok = true;
-      for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+      for (int64_t t; ok && items.advance(walk, t);) {
         const FfnJob& j = *walk.job;
         int64_t mb, nb;
         walk.blocks(t, mb, nb);
@@ -445,12 +597,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
         // column blocks.
         const uint64_t pol_a = j.wgrad ? pol_shared : pol_keep;
         const uint64_t pol_b = !j.wgrad && walk.m_blocks == 1 ? pol_stream : pol_shared;
-        const int32_t end = static_cast<int32_t>(walk.kblocks) * BK;
+        const int32_t begin = items.kb_from * BK, end = items.kb_to * BK;
         const auto load = [&](const CUtensorMap* map, uint32_t dst, int32_t x, int32_t y, uint64_t pol) {
           tile_load<G>(map, lead0 + s * 8, dst, x, y, pol);
         };
         const auto run = [&](auto a_mn, auto b_mn) {
-          for (int32_t kx = 0; kx < end; kx += BK) {
+          for (int32_t kx = begin; kx < end; kx += BK) {
             if (!bar_wait(empty0 + s * 8, phase ^ 1u, budget, abort)) {
               fail(kErrWaitEmpty);
               ok = false;
@@ -497,12 +649,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
     // ------------------------------------------------ MMA issuer (leader only)
     if (lane == 0 && leader) {
       const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty);
-      FfnWalk walk;
+      FfnWalk walk(p, ts, offs);
+      FfnItems items(walk, G);
       int s = 0;
       uint32_t phase = 0, acc_it = 0;
       bool ok = true;
-      for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
-        if (walk.kblocks <= 0) continue;
+      for (int64_t t; ok && items.advance(walk, t);) {
+        if (items.kb_to <= items.kb_from) continue;
         // Two accumulators in turn, or (wide) the halves of one.
         const int buf = NH == 2 ? 0 : static_cast<int>(acc_it & 1);
         const uint32_t acc_phase = ((NH == 2 ? acc_it : acc_it >> 1) & 1u) ^ 1u;
@@ -512,7 +665,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
         }
         tc_fence_after();
         const uint32_t d = tmem_base + buf * Cfg::kAccCols;
-        const int32_t kblocks = static_cast<int32_t>(walk.kblocks);
+        const int32_t kblocks = items.kb_to - items.kb_from;
         const auto run = [&](auto a_mn, auto b_mn) {
           // K-major: a k-step of 16 is 32 bytes along the swizzled row.
           // MN-major: 16 contraction rows of 128 bytes; the second 64 columns
@@ -608,10 +761,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
     uint8_t* blocks = epi_stage + quarter * Cfg::kEpiBlocks * kEpiWarpBytes;
     const uint64_t pol_out = policy_evict_normal();
     FfnGateLoads gates{blocks, gate_bars + 2 * quarter};
-    FfnWalk walk;
+    FfnWalk walk(p, ts, offs);
+    FfnItems items(walk, G);
     uint32_t acc_it = 0, chunk_seq = 0;
     int built = -1;
-    for (int64_t t = first_item; walk.seek(p, t); t += items_step) {
+    for (int64_t t; items.advance(walk, t);) {
       const FfnJob& j = *walk.job;
       int64_t mb, nb;
       walk.blocks(t, mb, nb);
@@ -625,6 +779,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
       }
       const int32_t row0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128 + quarter * 32);
       const int32_t n0 = static_cast<int32_t>(nb * Cfg::kTileOut);
+      if (items.last) {
+        if (items.kb_to <= items.kb_from) break;  // a short last share has no blocks and leaves no sums
+        if (!mbar_wait_warp(&acc_full[acc_it & 1], (acc_it >> 1) & 1u, budget, abort)) {
+          if (lane == 0) fail(kErrWaitAccFull);
+          break;
+        }
+        tc_fence_after();
+        // The last MMAs are done and nothing more is loaded: the ring holds the sums.
+        const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (acc_it & 1) * Cfg::kAccCols;
+        uint8_t* sums = ring + (quarter * 32 + lane) * Cfg::kSumRow;
+#pragma unroll 1
+        for (int c = 0; c < Cfg::kAccCols; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(from + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            reinterpret_cast<uint4*>(sums + c * 4)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        }
+        break;  // the last item
+      }
       if (walk.kblocks <= 0) {
         // An expert without rows: its weight gradient is zero.
         const FfnTensor& c = j.t[2];
@@ -748,13 +924,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
         }
       }
     }
-    if (lane == 0) bulk_wait_group_all();  // tensor stores done before the CTA's shared memory goes away
+    if (lane == 0) bulk_wait_group_read<0>();  // tensor stores have read the CTA's shared memory before it goes away
     __syncwarp();
   }
 
   tc_fence_before();
   __syncthreads();
-  if constexpr (G == 2) cluster_sync();
+  if (G == 2 || p.split > 1) cluster_sync();
+  if constexpr (G == 1) {
+    if (p.split > 1) {
+      FfnWalk walk(p, ts, offs);
+      FfnItems items(walk, 1);
+      if (items.shared >= 0 && !*abort) {
+        walk.seek(items.shared);
+        const int32_t per = items.blocks_each(walk);
+        ffn_join<T, EPI, Cfg>(p, walk, items, static_cast<int>((walk.kblocks + per - 1) / per), smem_u32(ring), warp, lane);
+      }
+      cluster_sync();  // the others' sums are read until here
+    }
+  }
   if (warp == 1) {
     tc_fence_after();
     if constexpr (G == 2) {

@@ -116,35 +116,37 @@ int blocks_typed(const void* x, int64_t matrices, int64_t rows, int64_t cols, in
              : MGB_ERR_CUDA;
 }
 
-template <int NT>
 int launch_few(const MxParams& p, unsigned grid, cudaStream_t s) {
-  using Cfg = FewCfg<NT>;
   static bool configured[128] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return MGB_ERR_CUDA;
   if (!configured[dev]) {
-    if (cudaFuncSetAttribute(mx_few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) !=
-        cudaSuccess) {
+    if (cudaFuncSetAttribute(mx_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemBytes) != cudaSuccess) {
       return MGB_ERR_CUDA;
     }
     configured[dev] = true;
   }
-  return launch_overlapped(mx_few_kernel<NT>, grid, kFewWarps * 32, Cfg::kSmemBytes, s, p) == cudaSuccess ? MGB_OK
+  return launch_overlapped(mx_few_kernel, grid, kFewWarps * 32, kFewSmemBytes, s, p) == cudaSuccess ? MGB_OK
                                                                                                           : MGB_ERR_CUDA;
 }
 
-// Average rows of an expert up to which the weight-streaming kernel runs
-// (dense: the rows), and the tokens it takes per pass over its weight rows.
-constexpr int64_t kFewRows = 32;
+// Whether the weight-streaming kernel runs: at most 8 rows an expert on
+// average (one pass over its weight rows) and weights of at most 256 MB.  It
+// starts about 8 us sooner than the tiles (1 row, n 4096, k 7168: 8.4 against
+// 15.9 us) but streams large weights at 4.3 TB/s where they reach 5.4 (32
+// experts of that size: 216 against 173 us; 8 of them about even).
+bool few_rows(int64_t rows, int64_t experts, int64_t n, int64_t k) {
+  return rows <= 8 * experts && experts * n * k <= (256ll << 20);
+}
 
 }  // namespace
 
 extern "C" {
 
-size_t block_scaled_mm_scratch_bytes(int32_t experts, int64_t rows) {
-  if (experts <= 0 || rows <= 0 || cdiv(rows, experts) <= kFewRows) return 0;
+size_t block_scaled_mm_scratch_bytes(int32_t experts, int64_t rows, int64_t n, int64_t k) {
+  if (experts <= 0 || rows <= 0 || few_rows(rows, experts, n, k)) return 0;
   return static_cast<size_t>(experts) * 3 * sizeof(CUtensorMap) +
-         (static_cast<size_t>(experts) + 1 + 15) / 16 * 16 * sizeof(int64_t);
+         (static_cast<size_t>(experts) + 1 + 31) / 32 * 32 * sizeof(int32_t);
 }
 
 int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const void* b, int64_t b_pitch,
@@ -161,7 +163,7 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
       c_pitch % 8 != 0) {
     return MGB_ERR_INVALID;
   }
-  const size_t need = block_scaled_mm_scratch_bytes(experts, rows);
+  const size_t need = block_scaled_mm_scratch_bytes(experts, rows, n, k);
   if (need > 0 && (scratch == nullptr || !aligned(scratch, 128) || scratch_bytes < need)) return MGB_ERR_SCRATCH;
   int sms = 0;
   MxParams p;
@@ -189,20 +191,17 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   p.scale_words = p.kb % 4 == 0 && aligned(sa, 4) && aligned(sb, 4);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t each = cdiv(rows, experts);
-  const int64_t groups = cdiv(n, 16) * experts;
-  if (each <= kFewRows) {
-    if (groups >= (1ll << 31)) return MGB_ERR_UNSUPPORTED;
-    const unsigned grid = static_cast<unsigned>(groups);
-    const int nt = each <= 8 ? 1 : each <= 16 ? 2 : 4;
+  if (few_rows(rows, experts, n, k)) {
+    const unsigned grid = static_cast<unsigned>(cdiv(n, 16) * experts);
     if (info != nullptr) {
       info->path = 3;
       info->swap_ab = 1;
-      info->tile_m = 8 * nt;
+      info->tile_m = 8;
       info->tile_n = 16;
       info->tile_k = 128;
       info->grid = static_cast<int32_t>(grid);
     }
-    return nt == 1 ? launch_few<1>(p, grid, s) : nt == 2 ? launch_few<2>(p, grid, s) : launch_few<4>(p, grid, s);
+    return launch_few(p, grid, s);
   }
   // Pairs' 256 x 224 tiles from 112 rows an expert where they cover the
   // device's pairs once (a half-empty pair tile still reads its weights once;
@@ -210,12 +209,14 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   // 228 at 64); else one CTA's 128 x 128, or 64 x 128 up to 48 rows an expert
   // (182 against 203 us at 48; 241 against 228 at 64, where uneven routing
   // gives some experts a second tile).
-  const int64_t pair_tiles = (cdiv(rows, 256) + experts - 1) * cdiv(n, MxCfg<2>::kTileN);
+  const int64_t segments = std::min<int64_t>(experts, rows);
+  const int64_t pair_tiles = (cdiv(rows, 256) + segments - 1) * cdiv(n, MxCfg<2>::kTileN);
   const bool pair = each >= 112 && pair_tiles >= sms / 2;
   const bool half = !pair && each <= 48;
   p.tile_rows = pair ? 256 : half ? 64 : 128;
   p.tile_cols = pair ? MxCfg<2>::kTileN : MxCfg<1>::kTileN;
-  const int64_t tiles = (cdiv(rows, p.tile_rows) + experts - 1) * cdiv(n, p.tile_cols);
+  const int64_t tiles = (cdiv(rows, p.tile_rows) + segments - 1) * cdiv(n, p.tile_cols);
+  if (tiles >= (1ll << 31)) return MGB_ERR_INVALID;  // the list's 32-bit tile numbers
   // Split K: as many CTAs a tile (2, 4 or 8) as the SMs hold at once, each
   // with at least four K blocks.  Clusters do not cross a GPC, whose SMs (16
   // to 18) hold whole clusters only: an eighth of the SMs stays out.
@@ -223,14 +224,14 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   while (!pair && p.split < 8 && tiles * p.split * 2 <= sms - sms / 8 && p.kb >= 8 * p.split) p.split *= 2;
   p.split_blocks = static_cast<int32_t>(cdiv(cdiv(p.kb, p.split), 4) * 4);
   p.maps = static_cast<uint8_t*>(scratch);
-  p.tile_start = reinterpret_cast<int64_t*>(p.maps + static_cast<size_t>(experts) * 3 * sizeof(CUtensorMap));
+  p.tile_start = reinterpret_cast<int32_t*>(p.maps + static_cast<size_t>(experts) * 3 * sizeof(CUtensorMap));
   MxTemplates tmpl;
   if (!encode_map_2d(&tmpl.map[0], kMapBytes8, a, k, 1, a_pitch, 128, half ? 64 : 128) ||
       !encode_map_2d(&tmpl.map[2], MGB_BF16, c, n, 1, c_pitch * 2, 32, 32, 64) ||
       !encode_map_2d(&tmpl.map[1], kMapBytes8, b, k, n, b_pitch, 128, pair ? MxCfg<2>::kColsCta : MxCfg<1>::kColsCta)) {
     return MGB_ERR_CUDA;
   }
-  if (launch_overlapped(mx_plan_kernel, static_cast<unsigned>(experts) + 1, 32, 0, s, tmpl, p) != cudaSuccess) {
+  if (launch_overlapped(mx_plan_kernel, static_cast<unsigned>(experts) + 1, 96, 0, s, tmpl, p) != cudaSuccess) {
     return MGB_ERR_CUDA;
   }
   if (info != nullptr) {

@@ -291,7 +291,7 @@ struct MxParams {
   int64_t kb, nb;       // scale columns and rows: ceil(k / 128), ceil(n / 128)
   int32_t scale_words;  // scale rows are whole, aligned 32-bit words
   uint8_t* maps;        // [experts][3] tensor maps: A, B, C
-  int64_t* tile_start;  // [experts + 1]
+  int32_t* tile_start;  // [experts + 1]
   int32_t tile_rows, tile_cols;
   int32_t split;        // CTAs of a cluster that share a tile's K (one CTA tiles; 1: none)
   int32_t split_blocks; // K blocks of each, a multiple of 4
@@ -299,15 +299,17 @@ struct MxParams {
   uint32_t* error_word;
 };
 
-__device__ __forceinline__ int64_t mx_segment(const MxParams& p, int e, int64_t& start, bool* bad = nullptr) {
-  if (p.offs == nullptr) {
+// Rows [start, start + len) of expert e, clamped into the tensor whatever offs holds.
+__device__ __forceinline__ int64_t mx_segment(const int32_t* offs, int64_t rows, int e, int64_t& start,
+                                              bool* bad = nullptr) {
+  if (offs == nullptr) {
     start = 0;
-    return p.rows;
+    return rows;
   }
-  const int64_t lo = e > 0 ? p.offs[e - 1] : 0, hi = p.offs[e];
-  if (bad != nullptr) *bad = lo < 0 || hi < lo || hi > p.rows;
-  start = lo < 0 ? 0 : lo > p.rows ? p.rows : lo;
-  const int64_t end = hi < start ? start : hi > p.rows ? p.rows : hi;
+  const int64_t lo = e > 0 ? offs[e - 1] : 0, hi = offs[e];
+  if (bad != nullptr) *bad = lo < 0 || hi < lo || hi > rows;
+  start = lo < 0 ? 0 : lo > rows ? rows : lo;
+  const int64_t end = hi < start ? start : hi > rows ? rows : hi;
   return end - start;
 }
 
@@ -315,20 +317,23 @@ struct MxTemplates {
   CUtensorMap map[3];  // A and C of one row: the plan kernel sets every segment's
 };
 
-// Tensor maps of every expert, one warp each, and the tiles' prefix sums (last block).
-__global__ void __launch_bounds__(32)
+// Tensor maps of every expert, one block each and a warp per map (the
+// parameters' constant-cache misses then overlap), and the tiles' prefix sums
+// (last block).
+__global__ void __launch_bounds__(96)
     mx_plan_kernel(const __grid_constant__ MxTemplates tmpl, const __grid_constant__ MxParams p) {
   __shared__ alignas(128) CUtensorMap staging[3];
-  const int lane = threadIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_launch_dependents();
-  grid_dependency_wait();  // offs and this scratch may be in use until here
   if (blockIdx.x == p.experts) {
+    if (warp > 0) return;
     const int per = (p.experts + 31) / 32;
     const int lo = lane * per, hi = lo + per < p.experts ? lo + per : p.experts;
     const int64_t n_blocks = ceil_div64(p.n, p.tile_cols);
+    grid_dependency_wait();  // offs and this scratch may be in use until here
     auto tiles_of = [&](int e) -> int64_t {
       int64_t start;
-      return ceil_div64(mx_segment(p, e, start), p.tile_rows) * n_blocks;
+      return ceil_div64(mx_segment(p.offs, p.rows, e, start), p.tile_rows) * n_blocks;
     };
     int64_t sum = 0;
     for (int e = lo; e < hi; ++e) sum += tiles_of(e);
@@ -340,40 +345,50 @@ __global__ void __launch_bounds__(32)
     }
     int64_t run = incl - sum;
     for (int e = lo; e < hi; ++e) {
-      p.tile_start[e] = run;
+      p.tile_start[e] = static_cast<int32_t>(run);
       run += tiles_of(e);
     }
-    if (lane == 31) p.tile_start[p.experts] = incl;
+    if (lane == 31) p.tile_start[p.experts] = static_cast<int32_t>(incl);
     return;
   }
   const int e = blockIdx.x;
-  bool bad = false;
-  int64_t start = 0;
-  const int64_t len = mx_segment(p, e, start, &bad);
-  if (bad && lane == 0) atomicOr(p.error_word, kErrBadDims);
-  if (lane < 3) {
-    const uint4* src = reinterpret_cast<const uint4*>(&tmpl.map[lane]);
-    uint4* dst = reinterpret_cast<uint4*>(&staging[lane]);
-    for (int i = 0; i < 8; ++i) dst[i] = src[i];
-    if (lane == 1) {
+  if (lane < 8) {
+    reinterpret_cast<uint4*>(&staging[warp])[lane] = reinterpret_cast<const uint4*>(&tmpl.map[warp])[lane];
+  }
+  __syncwarp();
+  grid_dependency_wait();
+  if (lane == 0) {
+    bool bad = false;
+    int64_t start = 0;
+    const int64_t len = mx_segment(p.offs, p.rows, e, start, &bad);
+    if (bad) atomicOr(p.error_word, kErrBadDims);
+    if (warp == 1) {
       tmap_replace_address(&staging[1], p.b + e * p.b_stride);
     } else if (len > 0) {  // an empty segment's maps are never used
-      tmap_replace_address(&staging[lane], lane == 0 ? static_cast<const void*>(p.a + start * p.a_pitch)
+      tmap_replace_address(&staging[warp], warp == 0 ? static_cast<const void*>(p.a + start * p.a_pitch)
                                                      : static_cast<const void*>(p.c + start * p.c_pitch));
-      tmap_replace_dim(&staging[lane], 1, static_cast<uint32_t>(len));
+      tmap_replace_dim(&staging[warp], 1, static_cast<uint32_t>(len));
     }
   }
   __syncwarp();
-  CUtensorMap* g = reinterpret_cast<CUtensorMap*>(p.maps) + static_cast<int64_t>(e) * 3;
-  for (int i = 0; i < 3; ++i) tmap_publish(&g[i], &staging[i]);
+  tmap_publish(reinterpret_cast<CUtensorMap*>(p.maps) + static_cast<int64_t>(e) * 3 + warp, &staging[warp]);
 }
 
+// Words of shared memory for the tile list and row ends, if they fit.
+constexpr int kMxListWords = 400;
+
+// A role's position in the tile list (`ts` and `offs` in shared or global memory).
 struct MxWalk {
+  const MxParams& p;
+  const int32_t* ts;
+  const int32_t* offs;
   int e = -1;
   int64_t first = 0, end = 0, len = 0, start = 0, m_blocks = 1;
 
-  __device__ __forceinline__ bool seek(const MxParams& p, int64_t t) {
-    const int64_t* ts = p.tile_start;
+  __device__ __forceinline__ MxWalk(const MxParams& params, const int32_t* list, const int32_t* ends)
+      : p(params), ts(list), offs(ends) {}
+
+  __device__ __forceinline__ bool seek(int64_t t) {
     if (t >= end || e < 0) {
       if (t >= ts[p.experts]) return false;
       int lo = e < 0 ? 0 : e, hi = p.experts - 1;
@@ -388,7 +403,7 @@ struct MxWalk {
       e = lo;
       first = ts[lo];
       end = ts[lo + 1];
-      len = mx_segment(p, lo, start);
+      len = mx_segment(offs, p.rows, lo, start);
       m_blocks = ceil_div64(len, p.tile_rows);
     }
     return true;
@@ -500,6 +515,7 @@ struct MxCfg {
   static_assert(kStageBytes % 1024 == 0 && kABytes % 1024 == 0, "swizzle atoms");
   static_assert(kScaleTmem + 2 * kScaleCols <= kTmemCols, "TMEM columns");
   static_assert(kSmemBytes <= 232448 && kStages >= 4, "shared memory");
+  static_assert((2 * kStages + 9) * 8 + 12 + 400 * 4 <= 2048, "barriers and the tile list");
   // Split K (one CTA): a row of partial sums, padded against bank conflicts.
   static constexpr int kSumRow = kTileN * 4 + 16;
   static_assert(G == 2 || kTileM * kSumRow <= kStages * kStageBytes, "partial sums fit the ring");
@@ -537,6 +553,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* never = abort + 1;
+  int32_t* list = reinterpret_cast<int32_t*>(tmem_slot + 3);  // kMxListWords
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -544,7 +561,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   const bool leader = rank == 0;
   const int split = G == 2 ? 1 : p.split;
   const int64_t first_item = blockIdx.x / (G * split);
-  const int64_t items_step = gridDim.x / (G * split);
+  const int64_t items_step = split > 1 ? 1ll << 60 : gridDim.x / G;  // one tile where K is split
   // This CTA's K blocks of every tile.
   const int32_t share = split > 1 ? static_cast<int32_t>(cluster_ctarank()) : 0;
   const int32_t kb_from = share * p.split_blocks;
@@ -581,7 +598,18 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const long long budget = p.wait_budget;
-  grid_dependency_wait();
+  grid_dependency_wait();  // global memory is read only from here on
+  const int32_t* ts = p.tile_start;
+  const int32_t* offs = p.offs;
+  if (2 * p.experts + 1 <= kMxListWords) {
+    for (int i = threadIdx.x; i <= p.experts; i += kMxThreads) list[i] = p.tile_start[i];
+    if (p.offs != nullptr) {
+      for (int i = threadIdx.x; i < p.experts; i += kMxThreads) list[p.experts + 1 + i] = p.offs[i];
+      offs = list + p.experts + 1;
+    }
+    ts = list;
+    __syncthreads();
+  }
   const CUtensorMap* all_maps = reinterpret_cast<const CUtensorMap*>(p.maps);
 
   auto fail = [&](uint32_t bits) {
@@ -597,13 +625,13 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       const uint64_t pol_stream = policy_evict_first();
       const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), empty0 = smem_u32(empty);
       const uint32_t lead0 = G == 2 ? mapa_shared(full0, 0) : full0;  // the leader's barriers
-      MxWalk walk;
+      MxWalk walk(p, ts, offs);
       int s = 0;
       uint32_t phase = 0, loaded = 0;
       int built = -1;
       bool ok = true;
       const int32_t begin = kb_from * Cfg::kBK, end = kb_to * Cfg::kBK;
-      for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+      for (int64_t t = first_item; ok && walk.seek(t); t += items_step) {
         int64_t mb, nb;
         walk.blocks(t, mb, nb);
         const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.e) * 3;
@@ -646,7 +674,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     // ------------------------------------------------ MMA issuer (leader only)
     if (lane == 0 && leader) {
       const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty);
-      MxWalk walk;
+      MxWalk walk(p, ts, offs);
       int s = 0;
       uint32_t phase = 0, acc_it = 0, sf_it = 0;
       bool ok = true;
@@ -654,7 +682,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       const uint64_t b_desc = smem_desc(smem_u32(ring) + Cfg::kABytes, 16, 1024, kLayoutSw128);
       // Scale atoms: no swizzle, 8-row groups of 16-byte rows 128 bytes apart.
       const uint64_t s_desc = smem_desc(smem_u32(scales), 0, 128, 0);
-      for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+      for (int64_t t = first_item; ok && walk.seek(t); t += items_step) {
         const int buf = static_cast<int>(acc_it & 1);
         if (!mbar_wait(&acc_empty[buf], ((acc_it >> 1) & 1u) ^ 1u, budget, abort)) {
           fail(kErrWaitAccEmpty);
@@ -714,7 +742,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     __syncwarp();
   } else if (warp == 2) {
     // -------------------------------------------------------------- scales
-    MxWalk walk;
+    MxWalk walk(p, ts, offs);
     uint32_t sf_it = 0;
     bool ok = true;
     // Four consecutive bytes of a scale row from K block kb on; blocks past the end are 1.
@@ -726,7 +754,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       for (int i = 0; i < 4; ++i) w |= (kb + i < p.kb ? static_cast<uint32_t>(__ldg(row + kb + i)) : 127u) << (8 * i);
       return w;
     };
-    for (int64_t t = first_item; ok && walk.seek(p, t); t += items_step) {
+    for (int64_t t = first_item; ok && walk.seek(t); t += items_step) {
       int64_t mb, nb;
       walk.blocks(t, mb, nb);
       const int64_t m0 = mb * Cfg::kTileM + rank * ROWS, n0 = nb * Cfg::kTileN;
@@ -767,10 +795,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     const int quarter = warp & 3;
     uint8_t* block = epi_stage + quarter * Cfg::kBlockBytes;
     const uint64_t pol_out = policy_evict_normal();
-    MxWalk walk;
+    MxWalk walk(p, ts, offs);
     uint32_t acc_it = 0;
     int built = -1;
-    for (int64_t t = first_item; walk.seek(p, t); t += items_step) {
+    for (int64_t t = first_item; walk.seek(t); t += items_step) {
       int64_t mb, nb;
       walk.blocks(t, mb, nb);
       const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.e) * 3;
@@ -842,7 +870,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       }
       ++acc_it;
     }
-    if (lane == 0) bulk_wait_group_all();
+    if (lane == 0) bulk_wait_group_read<0>();  // tensor stores have read the CTA's shared memory before it goes away
     __syncwarp();
   }
 
@@ -850,8 +878,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   __syncthreads();
   if (G == 2 || split > 1) cluster_sync();
   if (G == 1 && split > 1) {
-    MxWalk walk;
-    if (walk.seek(p, first_item) && !*abort) {
+    MxWalk walk(p, ts, offs);
+    if (walk.seek(first_item) && !*abort) {
       int64_t mb, nb;
       walk.blocks(first_item, mb, nb);
       const int per = ROWS / split;
@@ -906,8 +934,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
 // SM in flight without holding registers for them.  The warps' sums are
 // joined in shared memory in warp order (the result does not depend on
 // timing).
-// Weights are the 16-row operand of the warp-level m16n8k32 MMA, 8 NT tokens
-// its columns.  A thread loads 16 consecutive bytes of a row and uses them as
+// Weights are the 16-row operand of the warp-level m16n8k32 MMA, 8 tokens its
+// columns (more tokens take further passes).  A thread loads 16 consecutive bytes of a row and uses them as
 // the fragments of two MMAs; weights and tokens are permuted along K alike, so
 // the sum is over the same products.  Each 128-deep block starts from zero and
 // is added to the fp32 sums times its two scales.
@@ -927,19 +955,15 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
 constexpr int kFewWarps = 8;
 constexpr int kFewDepth = 6;            // K blocks of 2 KB per warp in flight
 constexpr int kFewBlock = 16 * 128;     // 16 weight rows x 128
-template <int NT>
-struct FewCfg {
-  static constexpr int kSums = kFewWarps * NT * 8 * 17 * 4;  // [warp][token][row], padded against bank conflicts
-  static constexpr int kSmemBytes = kFewWarps * kFewDepth * kFewBlock + kSums;
-  static_assert(2 * (kSmemBytes + 1024) <= 233472, "two CTAs per SM");
-};
+constexpr int kFewSums = kFewWarps * 8 * 17 * 4;  // [warp][token][row], padded against bank conflicts
+constexpr int kFewSmemBytes = kFewWarps * kFewDepth * kFewBlock + kFewSums;
+static_assert(2 * (kFewSmemBytes + 1024) <= 233472, "two CTAs per SM");
 
-template <int NT>
 __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_constant__ MxParams p) {
   extern __shared__ uint8_t few_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  float(*sums)[NT * 8][17] = reinterpret_cast<float(*)[NT * 8][17]>(few_smem + kFewWarps * kFewDepth * kFewBlock);
+  float(*sums)[8][17] = reinterpret_cast<float(*)[8][17]>(few_smem + kFewWarps * kFewDepth * kFewBlock);
   const uint32_t slots = smem_u32(few_smem) + warp * kFewDepth * kFewBlock + lane * 16;
   const int64_t n_groups = ceil_div64(p.n, 16);
   const int e = static_cast<int>(blockIdx.x / n_groups);
@@ -956,7 +980,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_
   grid_dependency_wait();  // global memory is read only from here on
   int64_t start;
   bool bad = false;
-  const int64_t len = mx_segment(p, e, start, &bad);
+  const int64_t len = mx_segment(p.offs, p.rows, e, start, &bad);
   if (bad && r0 == 0 && threadIdx.x == 0) atomicOr(p.error_word, kErrBadDims);
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   const uint8_t* wscale = p.sb + (e * p.nb + r0 / 128) * p.kb;  // 16 rows lie inside one 128-row block
@@ -976,13 +1000,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  for (int64_t m0 = 0; m0 < len; m0 += 8 * NT) {
-    float acc[NT][4];
-    const uint8_t* xrow = p.a + (start + m0 + g) * p.a_pitch + t * 16;     // token m0 + g (+ 8 i)
-    const uint8_t* xscale = p.sa + (start + m0 + 2 * t) * p.kb;            // tokens m0 + 2t, 2t + 1 (+ 8 i)
-    const int left = static_cast<int>(len - m0 < 8 * NT ? len - m0 : 8 * NT);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+  for (int64_t m0 = 0; m0 < len; m0 += 8) {
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint8_t* xrow = p.a + (start + m0 + g) * p.a_pitch + t * 16;  // token m0 + g
+    const uint8_t* xscale = p.sa + (start + m0 + 2 * t) * p.kb;         // tokens m0 + 2t, 2t + 1
+    const int left = static_cast<int>(len - m0 < 8 ? len - m0 : 8);
 #pragma unroll
     for (int i = 0; i < kFewDepth; ++i) fetch(i);
 #pragma unroll 1
@@ -1000,40 +1022,32 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_
                      : "memory");
       }
       const float sw = scale_value(__ldg(wscale + kb));
+      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int c = 0; c < 2; ++c) {
+        const int k = kb * 128 + c * 64;
+        const uint4 x = g < left && k + t * 16 < depth ? __ldg(reinterpret_cast<const uint4*>(xrow + k)) : zero;
+        mma_e4m3(part, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, x.x, x.y);
+        mma_e4m3(part, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, x.z, x.w);
+      }
+      // Columns 2t, 2t + 1 of the accumulator are tokens m0 + 2t, m0 + 2t + 1.
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int k = kb * 128 + c * 64;
-          const uint4 x = 8 * i + g < left && k + t * 16 < depth
-                              ? __ldg(reinterpret_cast<const uint4*>(xrow + 8 * i * p.a_pitch + k))
-                              : zero;
-          mma_e4m3(part, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, x.x, x.y);
-          mma_e4m3(part, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, x.z, x.w);
-        }
-        // Columns 2t, 2t + 1 of the accumulator are tokens m0 + 8 i + 2t (+ 1).
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float sx = 8 * i + 2 * t + j < left ? scale_value(__ldg(xscale + (8 * i + j) * p.kb + kb)) : 0.0f;
-          acc[i][j] += part[j] * sw * sx;
-          acc[i][2 + j] += part[2 + j] * sw * sx;
-        }
+      for (int j = 0; j < 2; ++j) {
+        const float sx = 2 * t + j < left ? scale_value(__ldg(xscale + j * p.kb + kb)) : 0.0f;
+        acc[j] += part[j] * sw * sx;
+        acc[2 + j] += part[2 + j] * sw * sx;
       }
       fetch(b + kFewDepth);  // into the slot just read
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        sums[warp][i * 8 + 2 * t + j][g] = acc[i][j];
-        sums[warp][i * 8 + 2 * t + j][g + 8] = acc[i][2 + j];
-      }
+    for (int j = 0; j < 2; ++j) {
+      sums[warp][2 * t + j][g] = acc[j];
+      sums[warp][2 * t + j][g + 8] = acc[2 + j];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < NT * 128; i += kFewWarps * 32) {
-      const int row = i & 15, tok = i >> 4;
+    if (threadIdx.x < 128) {
+      const int row = threadIdx.x & 15, tok = threadIdx.x >> 4;
       float s = 0.0f;
 #pragma unroll
       for (int w = 0; w < kFewWarps; ++w) s += sums[w][tok][row];

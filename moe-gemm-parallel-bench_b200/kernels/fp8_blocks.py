@@ -102,9 +102,9 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
     ``offs`` (int32 ``[E]``) holds their cumulative row ends.  Empty experts are
     fine; rows past ``offs[-1]`` are neither read nor written.  K is a multiple
     of 16, N of 8; rows of a, b and out may be padded to whole 16 bytes, scales
-    are contiguous.  With few tokens per expert (32 on average) the weights are
-    streamed by many small CTAs, else 128 x 128 or CTA-pair 256 x 224 tiles run
-    on the block-scaled tensor-core MMA."""
+    are contiguous.  With few tokens per expert (8 on average, weights up to 256
+    MB) the weights are streamed by many small CTAs, else 64 x 128, 128 x 128 or
+    CTA-pair 256 x 224 tiles run on the block-scaled tensor-core MMA."""
     global _last_info
     _require_runtime()
     if a.ndim != 2 or b.ndim not in (2, 3):
@@ -141,7 +141,7 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
             out_pitch % 8) or (a.data_ptr() | b.data_ptr() | out.data_ptr()) % 16:
         raise ValueError("a, b and out need contiguous columns, 16-byte aligned bases and rows a whole number of 16 "
                          "bytes apart that do not overlap")
-    nbytes = _native.block_scaled_scratch_bytes(experts, rows)
+    nbytes = _native.block_scaled_scratch_bytes(experts, rows, n, k)
     scratch = a.new_empty(nbytes).data_ptr() if nbytes else 0
     _last_info = _call(device, _native.block_scaled_mm, a.data_ptr(), a_pitch, sa.data_ptr(), b.data_ptr(), b_pitch,
                        b_stride, sb.data_ptr(), out.data_ptr(), out_pitch, ends, experts, rows, n, k, scratch, nbytes)

@@ -184,7 +184,7 @@ class Product:
 PRODUCTS = [
     # few tokens per expert
     ([1], 8, 16), ([1], 4096, 7168), ([3], 136, 2064), ([8], 264, 128), ([9], 24, 400), ([16], 128, 1024),
-    ([32], 40, 656), ([1, 0, 7, 0, 23], 136, 528), ([0, 0, 90, 1], 200, 272), ([2] * 37, 72, 144),
+    ([32], 40, 656), ([1, 0, 7, 0, 23], 136, 528), ([0, 0, 20, 1], 200, 272), ([2] * 37, 72, 144),
     # one CTA's 128 x 128 tiles
     ([33], 128, 128), ([127], 136, 272), ([100, 0, 1, 129], 264, 656), ([300], 1032, 2000), ([64] * 5, 128, 512),
     # 64 x 128 tiles; a tile's K shared by the CTAs of a cluster
@@ -361,7 +361,8 @@ def test_abi_refuses_bad_arguments_before_any_launch():
     for change in (dict(scratch=None), dict(scratch=at + 16), dict(scratch_bytes=64)):
         change["rows"] = 100  # more than a few a expert: maps are needed
         assert product(**change) == _native.STATUS_SCRATCH, change
-    assert lib.block_scaled_mm_scratch_bytes(0, 10) == 0 and lib.block_scaled_mm_scratch_bytes(2, 10) == 0
+    assert lib.block_scaled_mm_scratch_bytes(0, 10, 64, 64) == 0
+    assert lib.block_scaled_mm_scratch_bytes(2, 16, 64, 64) == 0 < lib.block_scaled_mm_scratch_bytes(2, 17, 64, 64)
     for change in ((None, 4, 8, 8, 1, at, 8, at, None), (at, 4, 0, 8, 1, at, 8, at, None),
                    (at, 4, 8, 7, 1, at, 8, at, None), (at, 4, 8, 8, 5, at, 8, at, None), (at + 1, 4, 8, 8, 1, at, 8, at, None)):
         assert lib.quantize_rows_launch(*change) == _native.STATUS_INVALID, change
