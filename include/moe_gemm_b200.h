@@ -301,8 +301,9 @@ int grouped_gemm_offsets_scatter_launch(const void* a, const void* b, const int3
  * 1).  Rows past the last end are neither read nor written.  An end below its
  * predecessor or past `rows` is clamped and reported (error bit 6).
  * dtype MGB_FP16 or MGB_BF16; bases 16-byte aligned; columns contiguous; row
- * pitches and expert strides in elements, multiples of 8; hidden and ffn
- * multiples of 8; otherwise MGB_ERR_INVALID.  fp32 accumulation, one rounding
+ * pitches and expert strides in elements, pitches multiples of 8, strides
+ * whole multiples of the pitch; hidden and ffn multiples of 8; otherwise
+ * MGB_ERR_INVALID.  fp32 accumulation, one rounding
  * per stored value.  Inputs and outputs must not overlap.
  * scratch: ffn_scratch_bytes(experts, jobs) bytes, 128-byte aligned, not
  * shared by launches that overlap. */

@@ -559,6 +559,18 @@ bool current_launch_limits(int* sm_count, long long* wait_budget) {
   return true;
 }
 
+bool encode_map_3d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t outer,
+                   uint64_t pitch, uint64_t stride, uint32_t box_inner, uint32_t box_rows) {
+  if (g_encode == nullptr) return false;
+  cuuint64_t dims[3] = {inner, rows, outer};
+  cuuint64_t strides[2] = {pitch, stride};
+  cuuint32_t box[3] = {box_inner, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return g_encode(map, map_type(dtype), 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool encode_map_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch,
                    uint32_t box_inner, uint32_t box_outer, int swizzle_bytes) {
   return g_encode != nullptr &&

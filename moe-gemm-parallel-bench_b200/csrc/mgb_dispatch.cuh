@@ -72,6 +72,11 @@ constexpr int kMapBytes8 = 100;
 bool encode_map_2d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch,
                    uint32_t box_inner, uint32_t box_outer, int swizzle_bytes = 128);
 
+// 3-D map of `outer` such matrices `stride` bytes apart (a whole number of
+// pitches), one of them per box, with the 128-byte swizzle.
+bool encode_map_3d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t outer,
+                   uint64_t pitch, uint64_t stride, uint32_t box_inner, uint32_t box_rows);
+
 // Launches `kernel` with programmatic stream serialization: its blocks may be
 // set up while the kernel before it on the stream still runs, so it must call
 // grid_dependency_wait before it touches global memory.

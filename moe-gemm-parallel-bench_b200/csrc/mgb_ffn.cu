@@ -7,6 +7,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 
@@ -25,15 +26,8 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// The box of an operand or staged block.
-enum Box { kKMajor, kMnMajor, kStage };
-
-bool encode(CUtensorMap* map, int dtype, const FfnTensor& t, int64_t rows, int64_t cols, Box box, const void* dummy) {
-  // A tensor without rows is never read; its template still needs a legal base.
-  const void* base = t.data != nullptr ? t.data : dummy;
-  return encode_map_2d(map, dtype, base, static_cast<uint64_t>(cols), static_cast<uint64_t>(rows),
-                       static_cast<uint64_t>(t.pitch) * 2, 64, box == kKMajor ? 128 : box == kMnMajor ? 64 : 32);
-}
+// The box of an operand or staged block, in rows of 64 columns.
+enum Box : uint32_t { kKMajor = 128, kMnMajor = 64, kStage = 32 };
 
 template <typename T, int EPI, int G, int NH>
 int launch_kernel(const FfnParams& p, int64_t tiles, int sm_count, cudaStream_t stream) {
@@ -104,98 +98,153 @@ FfnTensor tensor(const void* data, int64_t pitch, int64_t expert_stride, bool to
   return FfnTensor{static_cast<char*>(const_cast<void*>(data)), pitch, expert_stride, token ? 1 : 0};
 }
 
-// Scratch of a call: the maps of every (job, expert), then at most
-// kFfnPlanLaunches tile lists.
-size_t maps_bytes(int64_t experts, int jobs) { return static_cast<size_t>(experts) * jobs * kFfnMaps * kMapBytes; }
+// Scratch of a call: the operand maps of weight gradients, and a tile list per
+// launch (used where it does not fit shared memory).
+size_t maps_bytes(int64_t experts, int wgrads) { return static_cast<size_t>(experts) * wgrads * 2 * kMapBytes; }
 size_t list_bytes(int64_t experts, int jobs) {
   return (static_cast<size_t>(experts) * jobs + 1 + 31) / 32 * 32 * sizeof(int32_t);
 }
 
 // The launches of one call: jobs are added launch by launch, then run()
-// issues the plan kernel (every map and tile list) and the product kernels.
+// issues the plan kernel where one is needed and the product kernels.
 struct Launcher {
   FfnPlan plan;
-  int epilogue[kFfnPlanLaunches];
+  FfnParams params[kFfnLaunches];
+  Tile tile[kFfnLaunches];
+  int epilogue[kFfnLaunches];
+  int launches = 0;
   int dtype;
+  int64_t rows, experts;
   uint8_t* scratch;
   cudaStream_t stream;
   int sms;
   long long budget;
   bool ok = true;
 
+  FfnParams& now() { return params[launches - 1]; }
   void begin_launch(int epi) {
-    FfnPlan::Launch& l = plan.launch[plan.launches];
-    l.first_job = plan.jobs;
-    epilogue[plan.launches++] = epi;
+    FfnParams& p = params[launches];
+    std::memset(static_cast<void*>(&p), 0, sizeof(p));
+    p.experts = static_cast<int32_t>(experts);
+    p.offs = plan.offs;
+    p.rows = rows;
+    p.wait_budget = budget;
+    p.error_word = plan.error_word;
+    p.split = 1;
+    epilogue[launches++] = epi;
   }
-  FfnJob& begin_job() {
-    ++plan.launch[plan.launches - 1].jobs;
-    return plan.job[plan.jobs++];
-  }
-  // The last job's next tensor, [rows, cols] of box `box`.
-  void add(const FfnTensor& t, int64_t rows, int64_t cols, Box box) {
-    FfnJob& j = plan.job[plan.jobs - 1];
-    const int i = j.maps++;
-    j.t[i] = t;
-    ok = ok && encode(&plan.map[plan.jobs - 1][i], dtype, t, t.token ? 1 : rows, cols, box, scratch);
+  FfnJob& job() { return now().job[now().jobs - 1]; }
+  // The last job's tensor i, [t_rows, cols] in boxes of `box`.
+  void set(int i, const FfnTensor& t, int64_t t_rows, int64_t cols, Box box) {
+    job().t[i] = t;
+    CUtensorMap* map = &now().map[now().jobs - 1][i];
+    const uint64_t pitch = static_cast<uint64_t>(t.pitch) * 2;
+    if (t.token) {
+      ok = ok && encode_map_2d(map, dtype, t.data, cols, t_rows, pitch, 64, box);
+    } else {
+      const uint64_t stride = experts > 1 ? static_cast<uint64_t>(t.expert_stride) * 2 : pitch * t_rows;
+      ok = ok && encode_map_3d(map, dtype, t.data, cols, t_rows, experts, pitch, stride, 64, box);
+    }
   }
   // Rows job: C[rows, n] = A[rows, k] op(B_e); its epilogue's tensors follow.
   void rows_job(const FfnTensor& a, const FfnTensor& b, bool b_mn, int64_t n, int64_t k, int64_t b_cols) {
-    FfnJob& j = begin_job();
+    ++now().jobs;
+    FfnJob& j = job();
     j.b_mn = b_mn;
     j.n = n;
     j.k = k;
-    add(a, plan.rows, k, kKMajor);
+    if (rows > 0) set(0, a, rows, k, kKMajor);
     if (b_mn) {
-      add(b, k, b_cols, kMnMajor);
+      set(1, b, k, b_cols, kMnMajor);
     } else {
-      add(b, n, k, kKMajor);
+      set(1, b, n, k, kKMajor);
+    }
+  }
+  void output(int i, const FfnTensor& t, int64_t cols) {
+    if (rows > 0) {
+      set(i, t, rows, cols, kStage);
+    } else {
+      job().t[i] = t;
     }
   }
   // Weight gradient job: C_e[m, n] = A[rows, m]^T B[rows, n].
   void wgrad_job(const FfnTensor& a, const FfnTensor& b, const FfnTensor& c, int64_t m, int64_t n) {
-    FfnJob& j = begin_job();
+    ++now().jobs;
+    FfnJob& j = job();
     j.wgrad = 1;
+    j.b_mn = 1;
     j.m = m;
     j.n = n;
-    add(a, plan.rows, m, kMnMajor);
-    add(b, plan.rows, n, kMnMajor);
-    add(c, m, n, kStage);
+    set(2, c, m, n, kStage);
+    const int w = plan.wgrads++;
+    const FfnTensor operand[2] = {a, b};
+    const int64_t cols[2] = {m, n};
+    for (int i = 0; i < 2; ++i) {
+      plan.t[w][i] = operand[i];
+      // Without rows the maps are never used; the template still needs a legal base.
+      const void* base = operand[i].data != nullptr ? operand[i].data : static_cast<const void*>(scratch);
+      ok = ok && encode_map_2d(&plan.map[w][i], dtype, base, cols[i], 1, static_cast<uint64_t>(operand[i].pitch) * 2, 64,
+                               kMnMajor);
+    }
   }
 
-  // Output tile of a launch: pairs' 256 x 256 tiles when they cover the
-  // device's pairs once, else one CTA's 128 x 128 tiles (four times as many);
-  // plain launches that cover them twice take 256 x 512 ones (bf16 4096^3
-  // 98 against 104 us, 8192^3 690 against 760).  Rows of ragged segments are
-  // estimated as evenly spread.
-  Tile tile_of(const FfnPlan::Launch& l, int epi) const {
-    int64_t tiles = 0;
-    for (int i = 0; i < l.jobs; ++i) {
-      const FfnJob& j = plan.job[l.first_job + i];
-      const int64_t n = cdiv(j.n, epi == kFfnSwiglu ? 128 : 256);
-      const int64_t m = j.wgrad ? plan.experts * cdiv(j.m, 256)
-                                : std::max<int64_t>(cdiv(plan.rows, 256), std::min<int64_t>(plan.experts, plan.rows));
-      tiles += m * n;
+  // Output tile of a launch: the least estimated time among one CTA's
+  // 128 x 128 tiles (whose long contractions may be split), pairs' 256 x 256
+  // and, for the plain epilogue, 256 x 512 ones.  The unit is a 64-deep block
+  // of a CTA or pair (0.3 us; a 512-column one 1.9 of them); a tile adds its
+  // start and epilogue (4, 5 and 9 units by size, measured on contractions of
+  // a few blocks).  bf16 4096^3: 512 columns 98 us, 256 104; 8192^3: 690
+  // against 760.  Rows of ragged segments are estimated as evenly spread.
+  Tile tile_of(const FfnParams& p, int epi) const {
+    const Tile tiles[3] = {{2, true}, {2, false}, {1, false}};
+    const double block[3] = {1.9, 1.0, 1.0}, fixed[3] = {9.0, 5.0, 4.0};
+    Tile best = tiles[1];
+    double least = 1e300;
+    for (int c = epi == kFfnPlain ? 0 : 1; c < 3; ++c) {
+      const Tile t = tiles[c];
+      const int64_t segments = std::max<int64_t>(1, std::min(experts, rows));
+      const double each = static_cast<double>(std::max<int64_t>(rows, 1)) / segments;
+      FfnParams q;
+      q.split = 1;
+      if (t.g == 1) {
+        q.job[0] = p.job[0];
+        split_of(q, t, epi, 0);
+      }
+      double work = 0, longest = 0;
+      for (int i = 0; i < p.jobs; ++i) {
+        const FfnJob& j = p.job[i];
+        const double m = j.wgrad ? experts * cdiv(j.m, tile_rows(t)) : segments * std::ceil(each / tile_rows(t));
+        const double depth = j.wgrad ? std::ceil(each / 64) : cdiv(j.k, 64);
+        const int split = i == 0 ? q.split : 1;
+        const double one = depth / split * block[c] + fixed[c];
+        work += m * cdiv(j.n, tile_cols(t, epi)) * one * split;
+        longest = std::max(longest, one);
+      }
+      const double time = std::max(work / (sms / t.g), longest);
+      if (time < least * 0.999) {
+        least = time;
+        best = t;
+      }
     }
-    const int pairs = sms / 2;
-    return Tile{tiles >= pairs ? 2 : 1, epi == kFfnPlain && tiles >= 2 * pairs};
+    return best;
   }
+  static int tile_rows(Tile t) { return 128 * t.g; }
+  static int tile_cols(Tile t, int epi) { return (epi == kFfnSwiglu ? 64 : t.wide ? 256 : 128) * t.g; }
 
   // Tiles of a job, at most (a segment boundary adds one row block).
-  int64_t tiles_of(const FfnJob& j, const FfnPlan::Launch& l) const {
-    const int64_t segments = std::min<int64_t>(plan.experts, plan.rows);
-    const int64_t m = j.wgrad ? plan.experts * cdiv(j.m, l.tile_rows)
-                              : cdiv(plan.rows, l.tile_rows) + std::max<int64_t>(segments - 1, 0);
-    return m * cdiv(j.n, l.tile_cols);
+  int64_t tiles_of(const FfnJob& j, Tile t, int epi) const {
+    const int64_t m = j.wgrad ? experts * cdiv(j.m, tile_rows(t))
+                              : cdiv(rows, tile_rows(t)) + std::max<int64_t>(std::min(experts, rows) - 1, 0);
+    return m * cdiv(j.n, tile_cols(t, epi));
   }
 
   // Splits the contraction of job 0's tiles: as many CTAs a tile (2, 4 or 8)
   // as the SMs hold at once, each with at least four blocks.  Clusters do not
   // cross a GPC, whose SMs (16 to 18) hold whole clusters only: an eighth of
   // the SMs stays out.  Returns the launch's clusters (its tiles, unsplit).
-  int64_t split_of(FfnParams& p, const FfnPlan::Launch& l, int64_t tiles) const {
-    if (plan.rows == 0) return tiles;
-    const int64_t own = tiles_of(p.job[0], l);
+  int64_t split_of(FfnParams& p, Tile t, int epi, int64_t tiles) const {
+    if (rows == 0 || t.g != 1 || p.job[0].wgrad) return tiles;
+    const int64_t own = tiles_of(p.job[0], t, epi);
     const int64_t blocks = cdiv(p.job[0].k, 64), cap = sms - sms / 8;
     while (p.split < 8 && own * p.split * 2 <= cap && blocks >= 8 * p.split) p.split *= 2;
     if (p.split == 1) return tiles;
@@ -205,49 +254,49 @@ struct Launcher {
 
   int run() {
     if (!ok) return MGB_ERR_CUDA;
-    const int64_t experts = plan.experts;
-    plan.maps = scratch;
-    uint8_t* list = scratch + maps_bytes(experts, plan.jobs);
-    Tile tile[kFfnPlanLaunches];
-    for (int i = 0; i < plan.launches; ++i) {
-      FfnPlan::Launch& l = plan.launch[i];
-      tile[i] = tile_of(l, epilogue[i]);
-      l.tile_rows = 128 * tile[i].g;
-      l.tile_cols = (epilogue[i] == kFfnSwiglu ? 64 : tile[i].wide ? 256 : 128) * tile[i].g;
-      l.tile_start = reinterpret_cast<int32_t*>(list);
-      list += list_bytes(experts, l.jobs);
-      int64_t tiles = 0;
-      for (int k = 0; k < l.jobs; ++k) tiles += tiles_of(plan.job[l.first_job + k], l);
-      if (tiles >= (1ll << 31)) return MGB_ERR_INVALID;  // the list's 32-bit tile numbers
+    CUtensorMap* maps = reinterpret_cast<CUtensorMap*>(scratch);
+    uint8_t* list = scratch + maps_bytes(experts, plan.wgrads);
+    int64_t tiles[kFfnLaunches];
+    int wgrad = 0;
+    for (int i = 0; i < launches; ++i) {
+      FfnParams& p = params[i];
+      tile[i] = tile_of(p, epilogue[i]);
+      tiles[i] = 0;
+      for (int k = 0; k < p.jobs; ++k) {
+        tiles[i] += tiles_of(p.job[k], tile[i], epilogue[i]);
+        if (p.job[k].wgrad) {
+          plan.operands[wgrad] = maps;
+          p.job[k].operands = maps;
+          maps += 2 * experts;
+          ++wgrad;
+        }
+      }
+      if (tiles[i] >= (1ll << 31)) return MGB_ERR_INVALID;  // the list's 32-bit tile numbers
+      if ((p.jobs + 1) * experts + 1 > kListWords) {
+        FfnPlan::List& l = plan.list[plan.lists++];
+        l.jobs = p.jobs;
+        l.tile_rows = tile_rows(tile[i]);
+        l.tile_cols = tile_cols(tile[i], epilogue[i]);
+        for (int k = 0; k < p.jobs; ++k) {
+          l.wgrad[k] = p.job[k].wgrad;
+          l.m[k] = p.job[k].m;
+          l.n[k] = p.job[k].n;
+        }
+        l.tile_start = reinterpret_cast<int32_t*>(list);
+        p.tile_start = l.tile_start;
+        list += list_bytes(experts, p.jobs);
+      }
     }
-    if (launch_overlapped(ffn_plan_kernel, static_cast<unsigned>(plan.jobs * experts + plan.launches),
-                          32 * kFfnMaps, 0, stream, plan) != cudaSuccess) {
+    const int64_t blocks = plan.wgrads * experts + plan.lists;
+    if (blocks > 0 && launch_overlapped(ffn_plan_kernel, static_cast<unsigned>(blocks), 64, 0, stream, plan) != cudaSuccess) {
       return MGB_ERR_CUDA;
     }
-    for (int i = 0; i < plan.launches; ++i) {
-      const FfnPlan::Launch& l = plan.launch[i];
-      FfnParams p;
-      std::memset(static_cast<void*>(&p), 0, sizeof(p));
-      int64_t tiles = 0;
-      for (int k = 0; k < l.jobs; ++k) {
-        p.job[k] = plan.job[l.first_job + k];
-        tiles += tiles_of(p.job[k], l);
-      }
-      p.jobs = l.jobs;
-      p.experts = plan.experts;
-      p.offs = plan.offs;
-      p.rows = plan.rows;
-      p.maps = scratch + maps_bytes(experts, l.first_job);
-      p.tile_start = l.tile_start;
-      p.tile_rows = l.tile_rows;
-      p.tile_cols = l.tile_cols;
-      p.wait_budget = budget;
-      p.error_word = plan.error_word;
-      p.split = 1;
-      if (tile[i].g == 1 && !plan.job[l.first_job].wgrad) tiles = split_of(p, l, tiles);
-      const int st = epilogue[i] == kFfnPlain    ? launch_epilogue<kFfnPlain>(dtype, tile[i], p, tiles, sms, stream)
-                     : epilogue[i] == kFfnSwiglu ? launch_epilogue<kFfnSwiglu>(dtype, tile[i], p, tiles, sms, stream)
-                                                 : launch_epilogue<kFfnSwigluBwd>(dtype, tile[i], p, tiles, sms, stream);
+    for (int i = 0; i < launches; ++i) {
+      FfnParams& p = params[i];
+      const int64_t grid = split_of(p, tile[i], epilogue[i], tiles[i]);
+      const int st = epilogue[i] == kFfnPlain    ? launch_epilogue<kFfnPlain>(dtype, tile[i], p, grid, sms, stream)
+                     : epilogue[i] == kFfnSwiglu ? launch_epilogue<kFfnSwiglu>(dtype, tile[i], p, grid, sms, stream)
+                                                 : launch_epilogue<kFfnSwigluBwd>(dtype, tile[i], p, grid, sms, stream);
       if (st) return st;
     }
     return MGB_OK;
@@ -271,8 +320,9 @@ bool token_ok(const void* data, int64_t pitch, int64_t rows, int64_t cols) {
 }
 
 bool weight_ok(const void* data, int64_t pitch, int64_t stride, int64_t experts, int64_t rows, int64_t cols) {
-  return data != nullptr && aligned16(data) && pitch >= cols && pitch % 8 == 0 && stride % 8 == 0 &&
-         (experts == 1 || stride >= (rows - 1) * pitch + cols);
+  // A 3-D tensor map's strides are whole multiples of one another.
+  return data != nullptr && aligned16(data) && pitch >= cols && pitch % 8 == 0 &&
+         (experts == 1 || (stride % pitch == 0 && stride >= rows * pitch));
 }
 
 int start(Launcher& l, int32_t dtype, int64_t rows, int32_t experts, const int32_t* offs, int jobs, void* scratch,
@@ -287,6 +337,8 @@ int start(Launcher& l, int32_t dtype, int64_t rows, int32_t experts, const int32
   l.plan.experts = experts;
   l.plan.offs = offs;
   l.plan.rows = rows;
+  l.rows = rows;
+  l.experts = experts;
   l.dtype = dtype;
   l.scratch = static_cast<uint8_t*>(scratch);
   l.stream = static_cast<cudaStream_t>(stream);
@@ -301,11 +353,11 @@ void dgrad(Launcher& l, const FfnTensor& dc, const FfnTensor& b, const FfnTensor
   const auto half = [](const void* base, int64_t pitch, int64_t at) {
     return tensor(base != nullptr ? static_cast<const char*>(base) + at * 2 : nullptr, pitch, 0, true);
   };
-  l.add(half(out.data, out.pitch, 0), l.plan.rows, k, kStage);
+  l.output(2, half(out.data, out.pitch, 0), k);
   if (gate_up != nullptr) {
-    l.add(half(out.data, out.pitch, k), l.plan.rows, k, kStage);
-    l.add(half(gate_up, gate_up_pitch, 0), l.plan.rows, k, kStage);
-    l.add(half(gate_up, gate_up_pitch, k), l.plan.rows, k, kStage);
+    l.output(3, half(out.data, out.pitch, k), k);
+    l.output(4, half(gate_up, gate_up_pitch, 0), k);
+    l.output(5, half(gate_up, gate_up_pitch, k), k);
   }
 }
 
@@ -315,7 +367,7 @@ extern "C" {
 
 size_t ffn_scratch_bytes(int32_t experts, int32_t jobs) {
   if (experts <= 0 || jobs <= 0) return 0;
-  return maps_bytes(experts, jobs) + kFfnPlanLaunches * list_bytes(experts, jobs);
+  return maps_bytes(experts, jobs) + kFfnLaunches * list_bytes(experts, jobs);
 }
 
 int gated_ffn_forward_launch(const mgb_ffn_args* f) {
@@ -344,14 +396,14 @@ int gated_ffn_forward_launch(const mgb_ffn_args* f) {
   l.begin_launch(kFfnSwiglu);
   l.rows_job(tensor(f->x, f->x_pitch, 0, true), tensor(f->w13, f->w13_pitch, f->w13_stride, false), true, ffn, hid,
              2 * ffn);
-  l.plan.job[0].up = ffn;
-  l.add(h, rows, ffn, kStage);
-  l.add(half(0), rows, ffn, kStage);
-  l.add(half(ffn), rows, ffn, kStage);
+  l.job().up = ffn;
+  l.output(2, h, ffn);
+  l.output(3, half(0), ffn);
+  l.output(4, half(ffn), ffn);
   if (down) {
     l.begin_launch(kFfnPlain);
     l.rows_job(h, tensor(f->w2, f->w2_pitch, f->w2_stride, false), true, hid, ffn, hid);
-    l.add(tensor(f->y, f->y_pitch, 0, true), rows, hid, kStage);
+    l.output(2, tensor(f->y, f->y_pitch, 0, true), hid);
   }
   return l.run();
 }
@@ -379,7 +431,7 @@ int gated_ffn_backward_launch(const mgb_ffn_args* f) {
   // dx, dW13 and dW2 depend on nothing but dgate_up: one launch.
   l.begin_launch(kFfnPlain);
   l.rows_job(dgu, tensor(f->w13, f->w13_pitch, f->w13_stride, false), false, hid, 2 * ffn, 0);
-  l.add(tensor(f->dx, f->dx_pitch, 0, true), rows, hid, kStage);
+  l.output(2, tensor(f->dx, f->dx_pitch, 0, true), hid);
   l.wgrad_job(x, dgu, tensor(f->dw13, f->dw13_pitch, f->dw13_stride, false), hid, 2 * ffn);
   l.wgrad_job(h, dy, tensor(f->dw2, f->dw2_pitch, f->dw2_stride, false), ffn, hid);
   return l.run();

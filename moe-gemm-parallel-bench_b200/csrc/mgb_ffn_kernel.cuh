@@ -13,10 +13,14 @@
 //   x W13, h W2          A K-major,  B MN-major
 //   dy W2^T, dgu W13^T   A K-major,  B K-major
 //   x^T dgu, h^T dy      A MN-major, B MN-major
-// Every expert has its own tensor maps, whose row extent ends with the
-// segment: the tail of a segment's last contraction block reads zeros, never
-// the next expert's rows (a zero times their NaN would be NaN), and stores
-// past a segment are clipped.
+// The last contraction block of a weight gradient's segment must not see the
+// next expert's rows (a zero times their NaN would be NaN): its operands have a
+// tensor map per expert whose rows end with the segment, so the tail reads
+// zeros; ffn_plan_kernel builds those from the row ends on the device.  A rows
+// job may load rows past its segment (they only reach accumulator rows that
+// are not stored), so one map of the whole tensor serves, addressed by
+// absolute rows, and one 3-D map of all experts' weights; groups of 32 rows
+// that cross a segment's end are written by ordinary stores.
 //
 // Epilogues (fp32 accumulators, one rounding per stored value):
 //   plain            C
@@ -46,7 +50,8 @@
 namespace mgb {
 
 constexpr int kFfnMaxJobs = 3;
-constexpr int kFfnPlanJobs = 4, kFfnPlanLaunches = 2;  // one plan kernel covers a call's launches
+constexpr int kFfnLaunches = 2;  // of one call
+constexpr int kFfnWgrads = 2;    // weight gradient jobs of one call
 constexpr int kFfnMaps = 6;  // per job and expert: A, B, then the epilogue's
 enum FfnEpilogue : int { kFfnPlain = 0, kFfnSwiglu = 1, kFfnSwigluBwd = 2 };
 
@@ -61,13 +66,13 @@ struct FfnTensor {
 
 struct FfnJob {
   FfnTensor t[kFfnMaps];
-  int32_t maps;   // tensors used
   int32_t wgrad;  // contraction over the segment's rows
   int32_t b_mn;   // rows: B is MN-major (wgrad: both operands are)
   int64_t m;      // wgrad: output rows
   int64_t n;      // output columns
   int64_t k;      // rows: contraction depth
   int64_t up;     // swiglu: column of B where the up half starts
+  const CUtensorMap* operands;  // wgrad: [experts][2] maps of A and B, built by ffn_plan_kernel
 };
 
 struct FfnParams {
@@ -76,27 +81,31 @@ struct FfnParams {
   int32_t experts;
   const int32_t* offs;  // [experts] row ends; nullptr: one segment of `rows`
   int64_t rows;
-  uint8_t* maps;        // [jobs][experts][kFfnMaps] tensor maps
-  int32_t* tile_start;  // [jobs * experts + 1] first tile of every (job, expert)
-  int32_t tile_rows, tile_cols;  // output tile (the walk's)
+  const int32_t* tile_start;  // [jobs * experts + 1] first tile of every (job, expert); nullptr: built in shared memory
   int32_t split;        // CTAs of a cluster that share the contraction of job 0's tiles (one CTA tiles; 1: none)
   long long wait_budget;
   uint32_t* error_word;
+  // 2-D of a token tensor, 3-D of weights; not of a wgrad job's operands.
+  // Behind the scalars, which then share few lines of the constant cache.
+  CUtensorMap map[kFfnMaxJobs][kFfnMaps];
 };
 
-// What the plan kernel prepares: the tensor maps of every job's experts and
-// every launch's tile list.
+// What the plan kernel prepares from the row ends: the operand maps of weight
+// gradients, and the tile lists of launches with too many experts for shared
+// memory.
 struct FfnPlan {
-  FfnJob job[kFfnPlanJobs];
-  CUtensorMap map[kFfnPlanJobs][kFfnMaps];  // templates; token tensors' have one row
-  struct Launch {
-    int32_t first_job, jobs, tile_rows, tile_cols;
+  CUtensorMap map[kFfnWgrads][2];  // templates of one row
+  FfnTensor t[kFfnWgrads][2];
+  CUtensorMap* operands[kFfnWgrads];
+  struct List {
+    int32_t jobs, tile_rows, tile_cols;
+    int32_t wgrad[kFfnMaxJobs];
+    int64_t m[kFfnMaxJobs], n[kFfnMaxJobs];
     int32_t* tile_start;
-  } launch[kFfnPlanLaunches];
-  int32_t jobs, launches, experts;
+  } list[kFfnLaunches];
+  int32_t wgrads, lists, experts;
   const int32_t* offs;
   int64_t rows;
-  uint8_t* maps;
   uint32_t* error_word;
 };
 
@@ -114,35 +123,40 @@ __device__ __forceinline__ int64_t ffn_segment(const int32_t* offs, int64_t rows
   return end - start;
 }
 
-// Tensor maps of every (job, expert), one block each and a warp per map, and
-// every launch's tile prefix sums (the last blocks).  A warp per map because
-// the parameters are cold: their constant-cache misses, one after another in
-// one warp, were most of this kernel's time.
-__global__ void __launch_bounds__(32 * kFfnMaps) ffn_plan_kernel(const __grid_constant__ FfnPlan p) {
-  __shared__ alignas(128) CUtensorMap staging[kFfnMaps];
+// Inclusive scan over the lanes of a warp.
+__device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+
+// A block per weight gradient and expert, a warp per operand (the parameters'
+// constant-cache misses then overlap), then a block per tile list.
+__global__ void __launch_bounds__(64) ffn_plan_kernel(const __grid_constant__ FfnPlan p) {
+  __shared__ alignas(128) CUtensorMap staging[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_launch_dependents();
-  if (static_cast<int>(blockIdx.x) >= p.jobs * p.experts) {
+  if (static_cast<int>(blockIdx.x) >= p.wgrads * p.experts) {
     if (warp > 0) return;
-    const FfnPlan::Launch& l = p.launch[blockIdx.x - p.jobs * p.experts];
+    const FfnPlan::List& l = p.list[blockIdx.x - p.wgrads * p.experts];
     const int pairs = l.jobs * p.experts;
     const int per = (pairs + 31) / 32;
     const int lo = lane * per, hi = lo + per < pairs ? lo + per : pairs;
     grid_dependency_wait();  // offs and this scratch may be in use until here
     auto tiles_of = [&](int i) -> int64_t {
-      const FfnJob& j = p.job[l.first_job + i / p.experts];
+      const int job = i / p.experts;
       int64_t start;
-      const int64_t rows = j.wgrad ? j.m : ffn_segment(p.offs, p.rows, i % p.experts, start);
-      return ceil_div64(rows, l.tile_rows) * ceil_div64(j.n, l.tile_cols);
+      bool bad = false;
+      const int64_t len = ffn_segment(p.offs, p.rows, i % p.experts, start, &bad);
+      if (bad) atomicOr(p.error_word, kErrBadDims);
+      return ceil_div64(l.wgrad[job] ? l.m[job] : len, l.tile_rows) * ceil_div64(l.n[job], l.tile_cols);
     };
     int64_t sum = 0;
     for (int i = lo; i < hi; ++i) sum += tiles_of(i);
-    int64_t incl = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += v;
-    }
+    const int64_t incl = warp_scan(sum, lane);
     int64_t run = incl - sum;
     for (int i = lo; i < hi; ++i) {
       l.tile_start[i] = static_cast<int32_t>(run);
@@ -152,53 +166,50 @@ __global__ void __launch_bounds__(32 * kFfnMaps) ffn_plan_kernel(const __grid_co
     return;
   }
   const int job = blockIdx.x / p.experts, e = blockIdx.x % p.experts;
-  const FfnJob& j = p.job[job];
-  if (warp >= j.maps) return;
-  const FfnTensor t = j.t[warp];
+  const FfnTensor t = p.t[job][warp];
   if (lane < 8) {
     reinterpret_cast<uint4*>(&staging[warp])[lane] = reinterpret_cast<const uint4*>(&p.map[job][warp])[lane];
   }
   __syncwarp();
   grid_dependency_wait();
   if (lane == 0) {  // move the base, end the rows with the segment
-    bool bad = false;
     int64_t start = 0;
-    const int64_t len = ffn_segment(p.offs, p.rows, e, start, &bad);
-    if (bad) atomicOr(p.error_word, kErrBadDims);
-    if (!t.token) {
-      tmap_replace_address(&staging[warp], t.data + e * t.expert_stride * 2);
-    } else if (len > 0) {  // an empty segment's maps are never used
+    const int64_t len = ffn_segment(p.offs, p.rows, e, start);
+    if (len > 0) {  // an empty segment's maps are never used
       tmap_replace_address(&staging[warp], t.data + start * t.pitch * 2);
       tmap_replace_dim(&staging[warp], 1, static_cast<uint32_t>(len));
     }
   }
   __syncwarp();
-  tmap_publish(reinterpret_cast<CUtensorMap*>(p.maps) + static_cast<int64_t>(blockIdx.x) * kFfnMaps + warp,
-               &staging[warp]);
+  tmap_publish(p.operands[job] + 2 * e + warp, &staging[warp]);
 }
 
 // Words of shared memory for the launch's tile list and row ends, if they fit:
 // a role then finds a tile without a chain of global loads.
 constexpr int kListWords = 400;
 
-// A role's position in the tile list (`ts` and `offs` in shared or global memory).
+// A role's position in the tile list (`ts` and `offs` in shared or global
+// memory) of ROWS x COLS output tiles.
+template <int ROWS, int COLS>
 struct FfnWalk {
   const FfnParams& p;
   const int32_t* ts;
   const int32_t* offs;
   int pair = -1;  // job * experts + e
-  int64_t first = 0, end = 0;
+  int32_t first = 0, end = 0;
   int64_t start = 0, len = 0;  // rows of the expert's segment
   int64_t rows = 0;    // output rows
-  int64_t m_blocks = 1, n_blocks = 1;
+  int32_t m_blocks = 1, n_blocks = 1;
   int64_t kblocks = 0;
   const FfnJob* job = nullptr;
+  const CUtensorMap* maps = nullptr;  // the job's
+  int expert = 0;
 
   __device__ __forceinline__ FfnWalk(const FfnParams& params, const int32_t* list, const int32_t* ends)
       : p(params), ts(list), offs(ends) {}
 
   // Moves to the (job, expert) of tile t.
-  __device__ __forceinline__ void seek(int64_t t) {
+  __device__ __forceinline__ void seek(int32_t t) {
     if (pair >= 0 && t >= first && t < end) return;
     // The last pair whose first tile is <= t owns it (empty pairs share their successor's).
     int lo = pair >= 0 && t >= end ? pair : 0, hi = p.jobs * p.experts - 1;
@@ -214,38 +225,38 @@ struct FfnWalk {
     first = ts[lo];
     end = ts[lo + 1];
     job = &p.job[lo / p.experts];
-    len = ffn_segment(offs, p.rows, lo % p.experts, start);
+    maps = p.map[lo / p.experts];
+    expert = lo % p.experts;
+    len = ffn_segment(offs, p.rows, expert, start);
     rows = job->wgrad ? job->m : len;
-    m_blocks = ceil_div64(rows, p.tile_rows);
-    n_blocks = ceil_div64(job->n, p.tile_cols);
+    m_blocks = static_cast<int32_t>(ceil_div64(rows, ROWS));
+    n_blocks = static_cast<int32_t>(ceil_div64(job->n, COLS));
     kblocks = ceil_div64(job->wgrad ? len : job->k, 64);
   }
   // Bands of 8 row blocks, row block fastest inside a band (as TileWalk).
-  __device__ __forceinline__ void blocks(int64_t t, int64_t& mb, int64_t& nb) const {
-    const int64_t local = t - first;
-    const int64_t band_tiles = 8 * n_blocks;
-    const int64_t band = local / band_tiles;
-    const int64_t in = local - band * band_tiles;
-    const int64_t rows_in = m_blocks - band * 8 < 8 ? m_blocks - band * 8 : 8;
-    mb = band * 8 + in % rows_in;
-    nb = in / rows_in;
+  __device__ __forceinline__ void blocks(int32_t t, int64_t& mb, int64_t& nb) const {
+    const uint32_t local = t - first;
+    const uint32_t band_tiles = 8u * n_blocks;
+    const uint32_t band = local / band_tiles;
+    const uint32_t in = local - band * band_tiles;
+    const uint32_t rows_in = m_blocks - band * 8 < 8 ? m_blocks - band * 8 : 8;
+    const uint32_t column = in / rows_in;
+    mb = band * 8 + (in - column * rows_in);
+    nb = column;
   }
 };
 
-// NH = 256-column halves of a pair's tile: 2 is the 256 x 512 tile of the
-// plain epilogue.  It moves 48 KB into a CTA per 128 x 512 x 64 products
-// where the 256 x 256 tile moves 32 KB per 128 x 256 x 64, a quarter less per
-// product; its one 512-column accumulator fills TMEM and is freed by halves.
 // The tiles a CTA (or pair) works on, in order: `first`, `first + step`, ...
 // below `end`, then with a split the cluster's tile of job 0 (`shared`, -1:
 // none), of which it takes contraction blocks [kb_from, kb_to).
 struct FfnItems {
-  int64_t next, step, end, shared;
+  int32_t next, step, end, shared;
   int share, split;
   bool last = false;  // the current item is the shared one
   int32_t kb_from = 0, kb_to = 0;
 
-  __device__ __forceinline__ FfnItems(const FfnWalk& walk, int group) {
+  template <class Walk>
+  __device__ __forceinline__ FfnItems(const Walk& walk, int group) {
     const FfnParams& p = walk.p;
     split = p.split;
     end = walk.ts[p.jobs * p.experts];
@@ -254,14 +265,15 @@ struct FfnItems {
     shared = -1;
     share = 0;
     if (split > 1) {
-      const int64_t mine = walk.ts[p.experts];  // tiles of job 0
+      const int32_t mine = walk.ts[p.experts];  // tiles of job 0
       next += mine;
       share = static_cast<int>(cluster_ctarank());
-      const int64_t c = blockIdx.x / split;
+      const int32_t c = blockIdx.x / split;
       if (c < mine) shared = c;
     }
   }
-  __device__ __forceinline__ bool advance(FfnWalk& walk, int64_t& t) {
+  template <class Walk>
+  __device__ __forceinline__ bool advance(Walk& walk, int32_t& t) {
     if (next < end) {
       t = next;
       next += step;
@@ -280,11 +292,16 @@ struct FfnItems {
     kb_to = kb_from + per < all ? kb_from + per : all;
     return true;
   }
-  __device__ __forceinline__ int32_t blocks_each(const FfnWalk& walk) const {
+  template <class Walk>
+  __device__ __forceinline__ int32_t blocks_each(const Walk& walk) const {
     return static_cast<int32_t>((walk.kblocks + split - 1) / split);
   }
 };
 
+// NH = 256-column halves of a pair's tile: 2 is the 256 x 512 tile of the
+// plain epilogue.  It moves 48 KB into a CTA per 128 x 512 x 64 products
+// where the 256 x 256 tile moves 32 KB per 128 x 256 x 64, a quarter less per
+// product; its one 512-column accumulator fills TMEM and is freed by halves.
 template <typename T, int EPI, int G, int NH = 1>
 struct FfnCfg {
   static_assert(sizeof(T) == 2 && (G == 1 || G == 2), "16-bit types, one CTA or a pair");
@@ -310,41 +327,147 @@ struct FfnCfg {
   // Split contraction: a row of partial sums, padded against bank conflicts.
   static constexpr int kSumRow = kAccCols * 4 + 16;
   static_assert(G == 2 || kTileM * kSumRow <= kStages * kStageBytes, "partial sums fit the ring");
+  using Walk = FfnWalk<kTileM, kTileOut>;
 };
+
+// 32 rows of a tile as one warp stores them: staged in shared memory and by
+// tensor stores at absolute coordinates; or, where the segment ends inside
+// (`ragged`), each lane its own row straight from registers (no staging: the
+// fence between the staging writes and the tensor store also waits for
+// ordinary stores in flight, a microsecond a chunk).
+struct RowGroup {
+  const CUtensorMap* maps;
+  int64_t start, len;  // the segment
+  int32_t row0;        // first row, inside the segment
+  int32_t z;           // weights: expert
+  bool ragged, weights;
+
+  template <class Walk>
+  __device__ __forceinline__ RowGroup(const Walk& walk, int32_t row) {
+    maps = walk.maps;
+    weights = walk.job->wgrad != 0;
+    start = weights ? 0 : walk.start;
+    len = walk.rows;
+    row0 = row;
+    z = walk.expert;
+    ragged = !weights && row + 32 > len;
+  }
+  __device__ __forceinline__ bool empty() const { return row0 >= len; }
+  // Lane 0: the staged block of columns from x to tensor i.
+  __device__ __forceinline__ void put(int i, const uint8_t* block, int32_t x, uint64_t policy) const {
+    if (weights) {
+      tma_store_3d(&maps[i], block, x, row0, z, policy);
+    } else {
+      tma_store_2d(&maps[i], block, x, static_cast<int32_t>(start + row0), policy);
+    }
+  }
+  // Every lane: 32 columns from x of its row of tensor t (ragged groups).
+  template <typename T>
+  __device__ __forceinline__ void put_row(const FfnTensor& t, const uint32_t (&v)[32], int64_t x, int64_t cols,
+                                          int lane) const {
+    if (row0 + lane >= len) return;
+    uint4* to = reinterpret_cast<uint4*>(t.data + ((start + row0 + lane) * t.pitch + x) * 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (x + 8 * i < cols) {  // columns are multiples of 8
+        to[i] = make_uint4(pack_pair<T>(v[8 * i], v[8 * i + 1]), pack_pair<T>(v[8 * i + 2], v[8 * i + 3]),
+                           pack_pair<T>(v[8 * i + 4], v[8 * i + 5]), pack_pair<T>(v[8 * i + 6], v[8 * i + 7]));
+      }
+    }
+  }
+};
+
+// Plain epilogue of one warp: TN columns from TMEM in 32-column units, the
+// next unit's load in flight while one is converted and staged; 64-column
+// chunks leave through two staging blocks in turn.
+template <typename T, int TN>
+__device__ __forceinline__ void ffn_store_plain(const FfnJob& j, const RowGroup& rows, uint32_t taddr, int32_t n0,
+                                                uint8_t* blocks, int lane, uint32_t& seq, uint64_t policy) {
+  // No TMEM load may be issued for nothing: only the loop below waits for one.
+  if (rows.empty() || n0 >= j.n) return;
+  const int64_t left = j.n - n0;
+  const int units = 2 * (left >= TN ? TN / 64 : static_cast<int>((left + 63) / 64));
+  if (rows.ragged) {
+#pragma unroll 1
+    for (int g = 0; g < units; ++g) {
+      uint32_t v[32];
+      tmem_ld32(taddr + g * 32, v);
+      tmem_ld_wait();
+      rows.put_row<T>(j.t[2], v, n0 + g * 32, j.n, lane);
+    }
+    return;
+  }
+  uint32_t v[2][32];
+  tmem_ld32(taddr, v[0]);
+#pragma unroll
+  for (int g = 0; g < TN / 32; ++g) {
+    if (g >= units) break;
+    uint8_t* block = blocks + (seq & 1) * kEpiWarpBytes;
+    if (g % 2 == 0) {
+      if (lane == 0) bulk_wait_group_read<1>();  // the store last issued from this block has read it
+      __syncwarp();
+    }
+    tmem_ld_wait();
+    if (g + 1 < units) tmem_ld32(taddr + (g + 1) * 32, v[(g + 1) & 1]);
+    write_unit_smem<T>(v[g & 1], block, lane, g % 2);
+    if (g % 2 == 1) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        rows.put(2, block, n0 + (g / 2) * 64, policy);
+        bulk_commit_group();
+      }
+      ++seq;
+    }
+  }
+}
 
 // Swiglu epilogue of one warp: gate columns [0, TO), up columns [TO, 2 TO) of
 // the accumulator; h from the fp32 values, g and u rounded once as stored.
 template <typename T, int TO>
-__device__ __forceinline__ void ffn_store_swiglu(const CUtensorMap* maps, uint32_t taddr, int64_t rows, int64_t cols,
-                                                 int32_t row0, int32_t o0, uint8_t* blocks, int lane) {
-  if (row0 >= rows || o0 >= cols) return;
-  const int64_t left = cols - o0;
+__device__ __forceinline__ void ffn_store_swiglu(const FfnJob& j, const RowGroup& rows, uint32_t taddr, int32_t o0,
+                                                 uint8_t* blocks, int lane, uint64_t policy) {
+  if (rows.empty() || o0 >= j.n) return;
+  const int64_t left = j.n - o0;
   const int chunks = left >= TO ? TO / 64 : static_cast<int>((left + 63) / 64);
 #pragma unroll 1
   for (int c = 0; c < chunks; ++c) {
-    if (lane == 0) bulk_wait_group_read<0>();  // the previous chunk's stores have read the blocks
-    __syncwarp();
+    if (!rows.ragged) {
+      if (lane == 0) bulk_wait_group_read<0>();  // the previous chunk's stores have read the blocks
+      __syncwarp();
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       uint32_t gate[32], up[32];
       tmem_ld32(taddr + c * 64 + u * 32, gate);
       tmem_ld32(taddr + TO + c * 64 + u * 32, up);
       tmem_ld_wait();
-      write_unit_smem<T>(gate, blocks + kEpiWarpBytes, lane, u);
-      write_unit_smem<T>(up, blocks + 2 * kEpiWarpBytes, lane, u);
+      const int64_t x = o0 + c * 64 + u * 32;
+      if (rows.ragged) {
+        rows.put_row<T>(j.t[3], gate, x, j.n, lane);
+        rows.put_row<T>(j.t[4], up, x, j.n, lane);
+      } else {
+        write_unit_smem<T>(gate, blocks + kEpiWarpBytes, lane, u);
+        write_unit_smem<T>(up, blocks + 2 * kEpiWarpBytes, lane, u);
+      }
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         gate[i] = __float_as_uint(silu_mul(__uint_as_float(gate[i]), __uint_as_float(up[i])));
       }
-      write_unit_smem<T>(gate, blocks, lane, u);
+      if (rows.ragged) {
+        rows.put_row<T>(j.t[2], gate, x, j.n, lane);
+      } else {
+        write_unit_smem<T>(gate, blocks, lane, u);
+      }
     }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      const uint64_t pol = policy_evict_normal();
+    if (!rows.ragged) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
 #pragma unroll
-      for (int i = 0; i < 3; ++i) tma_store_2d(&maps[2 + i], blocks + i * kEpiWarpBytes, o0 + c * 64, row0, pol);
-      bulk_commit_group();
+        for (int i = 0; i < 3; ++i) rows.put(2 + i, blocks + i * kEpiWarpBytes, o0 + c * 64, policy);
+        bulk_commit_group();
+      }
     }
   }
 }
@@ -422,7 +545,7 @@ __device__ __forceinline__ float4 load4(const FfnTensor& t, int64_t row, int64_t
 // This CTA's rows of a split tile: the `parts` partial sums in rank order,
 // then the epilogue; a warp per row, a lane per four accumulator columns.
 template <typename T, int EPI, class Cfg>
-__device__ __forceinline__ void ffn_join(const FfnParams& p, const FfnWalk& walk, const FfnItems& items, int parts,
+__device__ __forceinline__ void ffn_join(const FfnParams& p, const typename Cfg::Walk& walk, const FfnItems& items, int parts,
                                          uint32_t ring, int warp, int lane) {
   const FfnJob& j = *walk.job;
   int64_t mb, nb;
@@ -431,18 +554,7 @@ __device__ __forceinline__ void ffn_join(const FfnParams& p, const FfnWalk& walk
   for (int r = items.share * rows + warp; r < (items.share + 1) * rows; r += kTcThreads / 32) {
     const int64_t m = mb * Cfg::kTileM + r;
     if (m >= walk.rows) break;
-    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i = 0; i < parts; ++i) {
-      float4 v;
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                   : "r"(mapa_shared(ring + r * Cfg::kSumRow + lane * 16, i))
-                   : "memory");
-      s.x += v.x;
-      s.y += v.y;
-      s.z += v.z;
-      s.w += v.w;
-    }
+    const float4 s = join_parts(ring + r * Cfg::kSumRow + lane * 16, parts);
     const int64_t row = walk.start + m;
     if constexpr (EPI == kFfnSwiglu) {
       // Lanes 0-15 hold gate columns, lane l + 16 the up columns of lane l's.
@@ -500,6 +612,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
   const int lane = threadIdx.x & 31;
   const uint32_t rank = G == 2 ? cluster_ctarank() : 0u;
   const bool leader = rank == 0;
+  // The next kernel may set up as SMs come free; it waits for this one's end.
+  grid_launch_dependents();
+  if (warp == 2) {  // the parameters' maps, while the kernel before may still run
+    const int job = lane / kFfnMaps, i = lane % kFfnMaps;
+    if (job < p.jobs && (i >= 2 || !p.job[job].wgrad) && p.job[job].t[i].data != nullptr) prefetch_tmap(&p.map[job][i]);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
@@ -533,17 +651,37 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
   grid_dependency_wait();  // global memory is read only from here on
   const int32_t* ts = p.tile_start;
   const int32_t* offs = p.offs;
-  const int pairs = p.jobs * p.experts;
-  if (pairs + 1 + p.experts <= kListWords) {
-    for (int i = threadIdx.x; i <= pairs; i += kTcThreads) list[i] = p.tile_start[i];
-    if (p.offs != nullptr) {
-      for (int i = threadIdx.x; i < p.experts; i += kTcThreads) list[pairs + 1 + i] = p.offs[i];
-      offs = list + pairs + 1;
+  if (ts == nullptr) {
+    // The tile list: first tiles of every (job, expert), then the row ends.
+    const int pairs = p.jobs * p.experts;
+    int32_t* ends = list + pairs + 1;
+    for (int i = threadIdx.x; i < p.experts; i += kTcThreads) {
+      ends[i] = p.offs != nullptr ? p.offs[i] : static_cast<int32_t>(p.rows);
     }
-    ts = list;
     __syncthreads();
+    if (warp == 0) {
+      int64_t before = 0;
+      for (int base = 0; base < pairs; base += 32) {
+        const int i = base + lane;
+        int64_t tiles = 0;
+        if (i < pairs) {
+          const FfnJob& j = p.job[i / p.experts];
+          int64_t start;
+          bool bad = false;
+          const int64_t len = ffn_segment(ends, p.rows, i % p.experts, start, &bad);
+          if (bad && blockIdx.x == 0) atomicOr(p.error_word, kErrBadDims);
+          tiles = ceil_div64(j.wgrad ? j.m : len, Cfg::kTileM) * ceil_div64(j.n, Cfg::kTileOut);
+        }
+        const int64_t incl = warp_scan(tiles, lane);
+        if (i < pairs) list[i] = static_cast<int32_t>(before + incl - tiles);
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      if (lane == 0) list[pairs] = static_cast<int32_t>(before);
+    }
+    __syncthreads();
+    ts = list;
+    offs = ends;
   }
-  const CUtensorMap* all_maps = reinterpret_cast<const CUtensorMap*>(p.maps);
 
   auto fail = [&](uint32_t bits) {
     atomicOr(p.error_word, bits);
@@ -559,23 +697,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
       const uint64_t pol_stream = policy_evict_first();
       const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), empty0 = smem_u32(empty);
       const uint32_t lead0 = G == 2 ? mapa_shared(full0, 0) : full0;  // the leader's barriers
-      FfnWalk walk(p, ts, offs);
+      typename Cfg::Walk walk(p, ts, offs);
       FfnItems items(walk, G);
       int s = 0;
       uint32_t phase = 0, loaded = 0;
       int built = -1;
       bool ok = true;
-      for (int64_t t; ok && items.advance(walk, t);) {
+      for (int32_t t; ok && items.advance(walk, t);) {
         const FfnJob& j = *walk.job;
         int64_t mb, nb;
         walk.blocks(t, mb, nb);
-        const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.pair) * kFfnMaps;
-        if (walk.pair != built) {
-          tmap_acquire(&g[0]);
-          tmap_acquire(&g[1]);
-          built = walk.pair;
+        const CUtensorMap* own = nullptr;  // wgrad: the expert's operand maps
+        if (EPI == kFfnPlain && j.wgrad) {
+          own = j.operands + 2 * walk.expert;
+          if (walk.pair != built && walk.kblocks > 0) {
+            tmap_acquire(&own[0]);
+            tmap_acquire(&own[1]);
+            built = walk.pair;
+          }
         }
         const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128);
+        const int32_t y0 = static_cast<int32_t>(walk.start) + m0;  // rows job: absolute row
         // First B column of this CTA's two 64-column boxes (swiglu: gate and up
         // columns of the same outputs; a pair's CTA 0 holds gate, CTA 1 up).
         int32_t b0, b1;
@@ -601,6 +743,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
         const auto load = [&](const CUtensorMap* map, uint32_t dst, int32_t x, int32_t y, uint64_t pol) {
           tile_load<G>(map, lead0 + s * 8, dst, x, y, pol);
         };
+        const auto load_weight = [&](uint32_t dst, int32_t x, int32_t y) {
+          tile_load_3d<G>(&walk.maps[1], lead0 + s * 8, dst, x, y, walk.expert, pol_b);
+        };
         const auto run = [&](auto a_mn, auto b_mn) {
           for (int32_t kx = begin; kx < end; kx += BK) {
             if (!bar_wait(empty0 + s * 8, phase ^ 1u, budget, abort)) {
@@ -611,19 +756,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
             const uint32_t st_a = ring0 + s * Cfg::kStageBytes, st_b = st_a + Cfg::kOperand;
             if (leader) mbar_arrive_expect_tx(&full[s], G * Cfg::kStageBytes);
             if constexpr (a_mn.value) {
-              load(&g[0], st_a, m0, kx, pol_a);
-              load(&g[0], st_a + Cfg::kOperand / 2, m0 + 64, kx, pol_a);
+              load(&own[0], st_a, m0, kx, pol_a);
+              load(&own[0], st_a + Cfg::kOperand / 2, m0 + 64, kx, pol_a);
             } else {
-              load(&g[0], st_a, kx, m0, pol_a);
+              load(&walk.maps[0], st_a, kx, y0, pol_a);
             }
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
               const uint32_t dst = st_b + h * Cfg::kOperand;
-              if constexpr (b_mn.value) {
-                load(&g[1], dst, b0 + 256 * h, kx, pol_b);
-                load(&g[1], dst + Cfg::kOperand / 2, b1 + 256 * h, kx, pol_b);
+              if constexpr (a_mn.value) {
+                load(&own[1], dst, b0 + 256 * h, kx, pol_b);
+                load(&own[1], dst + Cfg::kOperand / 2, b1 + 256 * h, kx, pol_b);
+              } else if constexpr (b_mn.value) {
+                load_weight(dst, b0 + 256 * h, kx);
+                load_weight(dst + Cfg::kOperand / 2, b1 + 256 * h, kx);
               } else {
-                load(&g[1], dst, kx, b0 + 256 * h, pol_b);
+                load_weight(dst, kx, b0 + 256 * h);
               }
             }
             ++loaded;
@@ -649,12 +797,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
     // ------------------------------------------------ MMA issuer (leader only)
     if (lane == 0 && leader) {
       const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty);
-      FfnWalk walk(p, ts, offs);
+      typename Cfg::Walk walk(p, ts, offs);
       FfnItems items(walk, G);
       int s = 0;
       uint32_t phase = 0, acc_it = 0;
       bool ok = true;
-      for (int64_t t; ok && items.advance(walk, t);) {
+      for (int32_t t; ok && items.advance(walk, t);) {
         if (items.kb_to <= items.kb_from) continue;
         // Two accumulators in turn, or (wide) the halves of one.
         const int buf = NH == 2 ? 0 : static_cast<int>(acc_it & 1);
@@ -761,22 +909,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
     uint8_t* blocks = epi_stage + quarter * Cfg::kEpiBlocks * kEpiWarpBytes;
     const uint64_t pol_out = policy_evict_normal();
     FfnGateLoads gates{blocks, gate_bars + 2 * quarter};
-    FfnWalk walk(p, ts, offs);
+    typename Cfg::Walk walk(p, ts, offs);
     FfnItems items(walk, G);
     uint32_t acc_it = 0, chunk_seq = 0;
-    int built = -1;
-    for (int64_t t; items.advance(walk, t);) {
+    for (int32_t t; items.advance(walk, t);) {
       const FfnJob& j = *walk.job;
       int64_t mb, nb;
       walk.blocks(t, mb, nb);
-      const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.pair) * kFfnMaps;
-      if (walk.pair != built) {
-        if (lane == 0) {
-          for (int i = 2; i < j.maps; ++i) tmap_acquire(&g[i]);
-        }
-        __syncwarp();
-        built = walk.pair;
-      }
       const int32_t row0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128 + quarter * 32);
       const int32_t n0 = static_cast<int32_t>(nb * Cfg::kTileOut);
       if (items.last) {
@@ -804,7 +943,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
       if (walk.kblocks <= 0) {
         // An expert without rows: its weight gradient is zero.
         const FfnTensor& c = j.t[2];
-        T* out = reinterpret_cast<T*>(c.data) + (walk.pair % p.experts) * c.expert_stride;
+        T* out = reinterpret_cast<T*>(c.data) + walk.expert * c.expert_stride;
         for (int r = 0; r < 32 && row0 + r < walk.rows; ++r) {
           for (int64_t col = n0 + lane * 8; col < j.n && col < n0 + Cfg::kTileOut; col += 256) {
             T* dst = out + (row0 + r) * c.pitch + col;  // n is a multiple of 8: whole 16-byte pieces
@@ -813,12 +952,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
         }
         continue;
       }
+      const RowGroup rows(walk, row0);
+      const int32_t y0 = static_cast<int32_t>(rows.start) + row0;
       int chunks = 0;
       if constexpr (EPI == kFfnSwigluBwd) {
-        if (row0 < walk.rows) {
+        if (!rows.empty()) {
           const int64_t left = j.n - n0;
           chunks = left >= Cfg::kTileOut ? Cfg::kTileOut / 64 : static_cast<int>((left + 63) / 64);
-          if (lane == 0) gates.issue(g, n0, row0);  // the first chunk arrives while the MMAs run
+          if (lane == 0) gates.issue(walk.maps, n0, y0);  // the first chunk arrives while the MMAs run
           ++gates.issued;
         }
       }
@@ -830,13 +971,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * Cfg::kAccCols;
       if constexpr (NH == 2) {
-        Problem q;
-        q.m = walk.rows;
-        q.n = j.n;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // each half is released as soon as it is drained
-          store_rows_tma<T, 256, Cfg::kEpiBlocks>(q, &g[2], taddr + h * 256, row0, n0 + h * 256, blocks, lane, chunk_seq,
-                                                  pol_out, p.error_word);
+          ffn_store_plain<T, 256>(j, rows, taddr + h * 256, n0 + h * 256, blocks, lane, chunk_seq, pol_out);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&acc_empty[h]), 0));
@@ -844,20 +981,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
         ++acc_it;
         continue;
       } else if constexpr (EPI == kFfnPlain) {
-        Problem q;
-        q.m = walk.rows;
-        q.n = j.n;
-        store_rows_tma<T, Cfg::kTileOut, Cfg::kEpiBlocks>(q, &g[2], taddr, row0, n0, blocks, lane, chunk_seq, pol_out,
-                                                          p.error_word);
+        ffn_store_plain<T, Cfg::kTileOut>(j, rows, taddr, n0, blocks, lane, chunk_seq, pol_out);
       } else if constexpr (EPI == kFfnSwiglu) {
-        ffn_store_swiglu<T, Cfg::kTileOut>(g, taddr, walk.rows, j.n, row0, n0, blocks, lane);
+        ffn_store_swiglu<T, Cfg::kTileOut>(j, rows, taddr, n0, blocks, lane, pol_out);
       } else {
         bool lost = false;
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
           const int set = gates.used & 1;
           if (c + 1 < chunks) {
-            if (lane == 0) gates.issue(g, n0 + (c + 1) * 64, row0);
+            if (lane == 0) gates.issue(walk.maps, n0 + (c + 1) * 64, y0);
             ++gates.issued;
           }
           if (!mbar_wait_warp(&gates.bars[set], (gates.used >> 1) & 1u, budget, abort)) {
@@ -887,17 +1020,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
                 gw[w] = pack_pair<T>(__float_as_uint(dg0), __float_as_uint(dg1));
                 uw[w] = pack_pair<T>(__float_as_uint(du0), __float_as_uint(du1));
               }
-              *reinterpret_cast<uint4*>(gb + at) = gv;
-              *reinterpret_cast<uint4*>(ub + at) = uv;
+              if (!rows.ragged) {
+                *reinterpret_cast<uint4*>(gb + at) = gv;
+                *reinterpret_cast<uint4*>(ub + at) = uv;
+              } else if (row0 + lane < rows.len) {
+                const int64_t x = n0 + c * 64 + u * 32 + i * 8;
+                if (x < j.n) {
+                  const int64_t row = rows.start + row0 + lane;
+                  *reinterpret_cast<uint4*>(j.t[2].data + (row * j.t[2].pitch + x) * 2) = gv;
+                  *reinterpret_cast<uint4*>(j.t[3].data + (row * j.t[3].pitch + x) * 2) = uv;
+                }
+              }
             }
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            uint8_t* from = blocks + set * 2 * kEpiWarpBytes;
-            tma_store_2d(&g[2], from, n0 + c * 64, row0, pol_out);
-            tma_store_2d(&g[3], from + kEpiWarpBytes, n0 + c * 64, row0, pol_out);
-            bulk_commit_group();
+          if (!rows.ragged) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              const uint8_t* from = blocks + set * 2 * kEpiWarpBytes;
+              rows.put(2, from, n0 + c * 64, pol_out);
+              rows.put(3, from + kEpiWarpBytes, n0 + c * 64, pol_out);
+              bulk_commit_group();
+            }
+          } else {
+            __syncwarp();  // read by every lane before the next loads land there
           }
         }
         if (lost) {
@@ -933,7 +1079,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
   if (G == 2 || p.split > 1) cluster_sync();
   if constexpr (G == 1) {
     if (p.split > 1) {
-      FfnWalk walk(p, ts, offs);
+      typename Cfg::Walk walk(p, ts, offs);
       FfnItems items(walk, 1);
       if (items.shared >= 0 && !*abort) {
         walk.seek(items.shared);

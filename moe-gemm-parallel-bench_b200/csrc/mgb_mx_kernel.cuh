@@ -200,6 +200,7 @@ template <typename T, int ACCESS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, uint32_t blocks, FastDiv kb,
                                                             int64_t cols, int64_t pitch, uint8_t* __restrict__ q,
                                                             int64_t q_pitch, uint8_t* __restrict__ scale, bool dense) {
+  grid_launch_dependents();
   grid_dependency_wait();
   const uint32_t b = blockIdx.x * 32u + (threadIdx.x >> 3);
   const int l = threadIdx.x & 7;
@@ -241,6 +242,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
   const int64_t r0 = rb * 128ll + (threadIdx.x >> 3), c = (in - rb * kb.d) * 128ll + (threadIdx.x & 7) * 16;
   const T* base = x + e * matrix;
   Sixteen<T> v[4];
+  grid_launch_dependents();
   grid_dependency_wait();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -562,6 +564,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   const int split = G == 2 ? 1 : p.split;
   const int64_t first_item = blockIdx.x / (G * split);
   const int64_t items_step = split > 1 ? 1ll << 60 : gridDim.x / G;  // one tile where K is split
+  // The next kernel may set up as SMs come free; it waits for this one's end.
+  grid_launch_dependents();
   // This CTA's K blocks of every tile.
   const int32_t share = split > 1 ? static_cast<int32_t>(cluster_ctarank()) : 0;
   const int32_t kb_from = share * p.split_blocks;
@@ -890,19 +894,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       for (int r = share * per + warp; r < (share + 1) * per; r += kMxThreads / 32) {
         const int64_t m = mb * Cfg::kTileM + r;
         if (m >= walk.len) break;
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const uint32_t at = smem_u32(ring + r * Cfg::kSumRow + col * 4);
-        for (int i = 0; i < parts; ++i) {
-          float4 v;
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                       : "r"(mapa_shared(at, i))
-                       : "memory");
-          sum.x += v.x;
-          sum.y += v.y;
-          sum.z += v.z;
-          sum.w += v.w;
-        }
+        const float4 sum = join_parts(smem_u32(ring + r * Cfg::kSumRow + col * 4), parts);
         if (c < p.n) {  // n is a multiple of 8: four columns are inside or past the end
           uint2 out;
           out.x = pack_pair<__nv_bfloat16>(__float_as_uint(sum.x), __float_as_uint(sum.y));
@@ -977,6 +969,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_
     live[h] = r < p.n;
     wrow[h] = p.b + e * p.b_stride + (live[h] ? r : 0) * p.b_pitch + t * 16;
   }
+  grid_launch_dependents();
   grid_dependency_wait();  // global memory is read only from here on
   int64_t start;
   bool bad = false;

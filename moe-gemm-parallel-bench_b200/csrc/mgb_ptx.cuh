@@ -116,6 +116,16 @@ __device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, 
       : "memory");
 }
 
+// The same into a 3-D tensor (x, y, z).
+__device__ __forceinline__ void tma_store_3d(const void* tmap, const void* src, int32_t x, int32_t y, int32_t z,
+                                             uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group.L2::cache_hint [%0, {%2, %3, %4}], [%1], %5;" ::"l"(
+          tmap),
+      "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "l"(policy)
+      : "memory");
+}
+
 __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // Waits until at most N of this thread's bulk groups still read shared memory.
@@ -426,6 +436,25 @@ __device__ __forceinline__ void tile_commit(uint32_t bar) {
   }
 }
 
+// The same from a 3-D tensor (x, y, z).
+template <int G>
+__device__ __forceinline__ void tile_load_3d(const void* map, uint32_t bar, uint32_t dst, int32_t x, int32_t y, int32_t z,
+                                             uint64_t policy) {
+  if constexpr (G == 2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy)
+        : "memory");
+  }
+}
+
 // Bounded wait of one thread on the barrier at a shared-memory address.
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
@@ -445,6 +474,30 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, long lon
     if (bar_try(bar, parity)) return true;
     if (*abort || clock64() - start > budget) return false;
   }
+}
+
+// The sum in rank order of the values at this shared-memory address of the
+// cluster's first `parts` CTAs; every load is issued before the first is used.
+__device__ __forceinline__ float4 join_parts(uint32_t at, int parts) {
+  float4 v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (i < parts) {
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[i].x), "=f"(v[i].y), "=f"(v[i].z), "=f"(v[i].w)
+                   : "r"(mapa_shared(at, i)));
+    }
+  }
+  float4 s = v[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {  // absent parts are zeros
+    s.x += v[i].x;
+    s.y += v[i].y;
+    s.z += v[i].z;
+    s.w += v[i].w;
+  }
+  return s;
 }
 
 // ------------------------------------------------------ UMMA descriptors

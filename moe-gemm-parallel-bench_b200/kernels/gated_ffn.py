@@ -94,10 +94,9 @@ def _weight(name: str, t, experts: int, rows: int, cols: int, dtype, device) -> 
     pitch = strides[-2]
     stride = strides[0] if experts > 1 else rows * pitch
     address = t.data_ptr()
-    if strides[-1] != 1 or pitch < cols or pitch % 8 or stride % 8 or address % 16 or (
-            experts > 1 and stride < (rows - 1) * pitch + cols):
-        raise ValueError(f"{name} needs contiguous columns, a 16-byte aligned base, a row pitch and an expert stride "
-                         "that are multiples of 8, and experts that do not overlap")
+    if strides[-1] != 1 or pitch < cols or pitch % 8 or address % 16 or stride % pitch or stride < rows * pitch:
+        raise ValueError(f"{name} needs contiguous columns, a 16-byte aligned base, a row pitch that is a multiple of 8 "
+                         "and experts a whole number of rows apart")
     return address, pitch, stride
 
 
