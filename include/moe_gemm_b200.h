@@ -384,8 +384,8 @@ int quantize_rows_launch(const void* x, int64_t rows, int64_t cols, int64_t pitc
 int quantize_blocks_launch(const void* x, int64_t matrices, int64_t rows, int64_t cols, int64_t pitch, int64_t stride,
                            int32_t dtype, void* q, void* scale, void* stream);
 
-/* Scratch of block_scaled_mm_launch: 0 where the kernel for few tokens runs. */
-size_t block_scaled_mm_scratch_bytes(int32_t experts, int64_t rows, int64_t n, int64_t k);
+/* Scratch of block_scaled_mm_launch: 0 below 200 experts. */
+size_t block_scaled_mm_scratch_bytes(int32_t experts);
 
 /* c[rows of e, :] = sum over 128-deep K blocks kb of
  *   2^(sa[row, kb] - 127) 2^(sb[e, col / 128, kb] - 127) a[row, kb] b[e, col, kb]
@@ -394,9 +394,9 @@ size_t block_scaled_mm_scratch_bytes(int32_t experts, int64_t rows, int64_t n, i
  * ceil(k / 128)], c bf16 [rows, n]; fp32 accumulation.  Segments as in
  * gated_ffn_forward_launch (offs null: one segment of every row, experts 1).
  * k a multiple of 16, n of 8; a, b and c 16-byte aligned with row pitches of
- * whole 16 bytes; scales contiguous.  info->path 2: CTA pairs, 0: one CTA,
+ * whole 16 bytes, b's experts whole pitches apart; scales contiguous.  info->path 2: CTA pairs, 0: one CTA,
  * 3: the kernel for few tokens per expert.  Scratch
- * block_scaled_mm_scratch_bytes of these sizes, 128-byte aligned, not shared by
+ * of block_scaled_mm_scratch_bytes(experts), 128-byte aligned, not shared by
  * launches that overlap. */
 int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const void* b, int64_t b_pitch,
                            int64_t b_stride, const void* sb, void* c, int64_t c_pitch, const int32_t* offs,

@@ -149,6 +149,16 @@ __device__ __forceinline__ Problem load_problem(const GroupedParams& p, int e) {
 
 __device__ __forceinline__ int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Inclusive scan over the lanes of a warp.
+__device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+
 // Walks the flattened tile space problem by problem.  Each CTA visits its
 // tiles in increasing order, so the walk only ever moves forward: the whole
 // launch costs one pass over the problem table per CTA (the reference scans it

@@ -123,16 +123,6 @@ __device__ __forceinline__ int64_t ffn_segment(const int32_t* offs, int64_t rows
   return end - start;
 }
 
-// Inclusive scan over the lanes of a warp.
-__device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, v, d);
-    if (lane >= d) v += u;
-  }
-  return v;
-}
-
 // A block per weight gradient and expert, a warp per operand (the parameters'
 // constant-cache misses then overlap), then a block per tile list.
 __global__ void __launch_bounds__(64) ffn_plan_kernel(const __grid_constant__ FfnPlan p) {
@@ -717,7 +707,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
           }
         }
         const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * 128);
-        const int32_t y0 = static_cast<int32_t>(walk.start) + m0;  // rows job: absolute row
+        // Rows job: absolute row.  A pair's upper half that lies past the segment
+        // reads zeros from past the tensor (no traffic, and quieter MMAs).
+        const int32_t y0 = static_cast<int32_t>(m0 < walk.rows ? walk.start + m0 : p.rows);
         // First B column of this CTA's two 64-column boxes (swiglu: gate and up
         // columns of the same outputs; a pair's CTA 0 holds gate, CTA 1 up).
         int32_t b0, b1;

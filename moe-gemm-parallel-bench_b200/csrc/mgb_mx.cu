@@ -143,10 +143,11 @@ bool few_rows(int64_t rows, int64_t experts, int64_t n, int64_t k) {
 
 extern "C" {
 
-size_t block_scaled_mm_scratch_bytes(int32_t experts, int64_t rows, int64_t n, int64_t k) {
-  if (experts <= 0 || rows <= 0 || few_rows(rows, experts, n, k)) return 0;
-  return static_cast<size_t>(experts) * 3 * sizeof(CUtensorMap) +
-         (static_cast<size_t>(experts) + 1 + 31) / 32 * 32 * sizeof(int32_t);
+size_t block_scaled_mm_scratch_bytes(int32_t experts) {
+  // The tile list, where it does not fit shared memory.
+  return experts > 0 && 2 * static_cast<int64_t>(experts) + 1 > kMxListWords
+             ? (static_cast<size_t>(experts) + 1 + 31) / 32 * 32 * sizeof(int32_t)
+             : 0;
 }
 
 int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const void* b, int64_t b_pitch,
@@ -159,11 +160,11 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   }
   if ((rows > 0 && (a == nullptr || sa == nullptr || c == nullptr)) || b == nullptr || sb == nullptr ||
       !aligned(a, 16) || !aligned(b, 16) || !aligned(c, 16) || a_pitch < k || a_pitch % 16 != 0 || b_pitch < k ||
-      b_pitch % 16 != 0 || b_stride % 16 != 0 || (experts > 1 && b_stride < (n - 1) * b_pitch + k) || c_pitch < n ||
+      b_pitch % 16 != 0 || (experts > 1 && (b_stride % b_pitch != 0 || b_stride < n * b_pitch)) || c_pitch < n ||
       c_pitch % 8 != 0) {
     return MGB_ERR_INVALID;
   }
-  const size_t need = block_scaled_mm_scratch_bytes(experts, rows, n, k);
+  const size_t need = block_scaled_mm_scratch_bytes(experts);
   if (need > 0 && (scratch == nullptr || !aligned(scratch, 128) || scratch_bytes < need)) return MGB_ERR_SCRATCH;
   int sms = 0;
   MxParams p;
@@ -213,9 +214,9 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   const int64_t pair_tiles = (cdiv(rows, 256) + segments - 1) * cdiv(n, MxCfg<2>::kTileN);
   const bool pair = each >= 112 && pair_tiles >= sms / 2;
   const bool half = !pair && each <= 48;
-  p.tile_rows = pair ? 256 : half ? 64 : 128;
-  p.tile_cols = pair ? MxCfg<2>::kTileN : MxCfg<1>::kTileN;
-  const int64_t tiles = (cdiv(rows, p.tile_rows) + segments - 1) * cdiv(n, p.tile_cols);
+  const int tile_rows = pair ? 256 : half ? 64 : 128;
+  const int tile_cols = pair ? MxCfg<2>::kTileN : MxCfg<1>::kTileN;
+  const int64_t tiles = (cdiv(rows, tile_rows) + segments - 1) * cdiv(n, tile_cols);
   if (tiles >= (1ll << 31)) return MGB_ERR_INVALID;  // the list's 32-bit tile numbers
   // Split K: as many CTAs a tile (2, 4 or 8) as the SMs hold at once, each
   // with at least four K blocks.  Clusters do not cross a GPC, whose SMs (16
@@ -223,21 +224,22 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   p.split = 1;
   while (!pair && p.split < 8 && tiles * p.split * 2 <= sms - sms / 8 && p.kb >= 8 * p.split) p.split *= 2;
   p.split_blocks = static_cast<int32_t>(cdiv(cdiv(p.kb, p.split), 4) * 4);
-  p.maps = static_cast<uint8_t*>(scratch);
-  p.tile_start = reinterpret_cast<int32_t*>(p.maps + static_cast<size_t>(experts) * 3 * sizeof(CUtensorMap));
-  MxTemplates tmpl;
-  if (!encode_map_2d(&tmpl.map[0], kMapBytes8, a, k, 1, a_pitch, 128, half ? 64 : 128) ||
-      !encode_map_2d(&tmpl.map[2], MGB_BF16, c, n, 1, c_pitch * 2, 32, 32, 64) ||
-      !encode_map_2d(&tmpl.map[1], kMapBytes8, b, k, n, b_pitch, 128, pair ? MxCfg<2>::kColsCta : MxCfg<1>::kColsCta)) {
+  const uint64_t stride = static_cast<uint64_t>(experts > 1 ? b_stride : b_pitch * n);
+  if (!encode_map_2d(&p.map[0], kMapBytes8, a, k, rows, a_pitch, 128, half ? 64 : 128) ||
+      !encode_map_3d(&p.map[1], kMapBytes8, b, k, n, experts, b_pitch, stride, 128,
+                     pair ? MxCfg<2>::kColsCta : MxCfg<1>::kColsCta) ||
+      !encode_map_2d(&p.map[2], MGB_BF16, c, n, rows, c_pitch * 2, 32, 32, 64)) {
     return MGB_ERR_CUDA;
   }
-  if (launch_overlapped(mx_plan_kernel, static_cast<unsigned>(experts) + 1, 96, 0, s, tmpl, p) != cudaSuccess) {
-    return MGB_ERR_CUDA;
+  if (need > 0) {
+    int32_t* list = static_cast<int32_t*>(scratch);
+    if (launch_overlapped(mx_list_kernel, 1, 32, 0, s, p, list, tile_rows, tile_cols) != cudaSuccess) return MGB_ERR_CUDA;
+    p.tile_start = list;
   }
   if (info != nullptr) {
     info->path = pair ? 2 : 0;
-    info->tile_m = p.tile_rows;
-    info->tile_n = p.tile_cols;
+    info->tile_m = tile_rows;
+    info->tile_n = tile_cols;
     info->tile_k = 128;
     info->stages = pair ? MxCfg<2>::kStages : half ? MxCfg<1, 64>::kStages : MxCfg<1>::kStages;
     info->grid = static_cast<int32_t>(std::min<int64_t>(tiles * p.split, sms));

@@ -292,13 +292,14 @@ struct MxParams {
   int64_t rows, n, k;
   int64_t kb, nb;       // scale columns and rows: ceil(k / 128), ceil(n / 128)
   int32_t scale_words;  // scale rows are whole, aligned 32-bit words
-  uint8_t* maps;        // [experts][3] tensor maps: A, B, C
-  int32_t* tile_start;  // [experts + 1]
-  int32_t tile_rows, tile_cols;
+  const int32_t* tile_start;  // [experts + 1] first tile of every expert; nullptr: built in shared memory
   int32_t split;        // CTAs of a cluster that share a tile's K (one CTA tiles; 1: none)
   int32_t split_blocks; // K blocks of each, a multiple of 4
   long long wait_budget;
   uint32_t* error_word;
+  // A and C whole (a segment's rows are addressed absolutely; rows loaded past
+  // its end only reach accumulator rows that are not stored), B 3-D by expert.
+  CUtensorMap map[3];
 };
 
 // Rows [start, start + len) of expert e, clamped into the tensor whatever offs holds.
@@ -315,84 +316,56 @@ __device__ __forceinline__ int64_t mx_segment(const int32_t* offs, int64_t rows,
   return end - start;
 }
 
-struct MxTemplates {
-  CUtensorMap map[3];  // A and C of one row: the plan kernel sets every segment's
-};
+// Tiles of an expert's segment.
+__device__ __forceinline__ int64_t mx_tiles(const int32_t* offs, const MxParams& p, int e, int tile_rows, int tile_cols,
+                                            bool* bad) {
+  int64_t start;
+  return ceil_div64(mx_segment(offs, p.rows, e, start, bad), tile_rows) * ceil_div64(p.n, tile_cols);
+}
 
-// Tensor maps of every expert, one block each and a warp per map (the
-// parameters' constant-cache misses then overlap), and the tiles' prefix sums
-// (last block).
-__global__ void __launch_bounds__(96)
-    mx_plan_kernel(const __grid_constant__ MxTemplates tmpl, const __grid_constant__ MxParams p) {
-  __shared__ alignas(128) CUtensorMap staging[3];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// The tile list of a launch with too many experts for shared memory (one warp).
+__global__ void __launch_bounds__(32)
+    mx_list_kernel(const __grid_constant__ MxParams p, int32_t* list, int tile_rows, int tile_cols) {
+  const int lane = threadIdx.x;
+  const int per = (p.experts + 31) / 32;
+  const int lo = lane * per, hi = lo + per < p.experts ? lo + per : p.experts;
   grid_launch_dependents();
-  if (blockIdx.x == p.experts) {
-    if (warp > 0) return;
-    const int per = (p.experts + 31) / 32;
-    const int lo = lane * per, hi = lo + per < p.experts ? lo + per : p.experts;
-    const int64_t n_blocks = ceil_div64(p.n, p.tile_cols);
-    grid_dependency_wait();  // offs and this scratch may be in use until here
-    auto tiles_of = [&](int e) -> int64_t {
-      int64_t start;
-      return ceil_div64(mx_segment(p.offs, p.rows, e, start), p.tile_rows) * n_blocks;
-    };
-    int64_t sum = 0;
-    for (int e = lo; e < hi; ++e) sum += tiles_of(e);
-    int64_t incl = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += v;
-    }
-    int64_t run = incl - sum;
-    for (int e = lo; e < hi; ++e) {
-      p.tile_start[e] = static_cast<int32_t>(run);
-      run += tiles_of(e);
-    }
-    if (lane == 31) p.tile_start[p.experts] = static_cast<int32_t>(incl);
-    return;
-  }
-  const int e = blockIdx.x;
-  if (lane < 8) {
-    reinterpret_cast<uint4*>(&staging[warp])[lane] = reinterpret_cast<const uint4*>(&tmpl.map[warp])[lane];
-  }
-  __syncwarp();
-  grid_dependency_wait();
-  if (lane == 0) {
-    bool bad = false;
-    int64_t start = 0;
-    const int64_t len = mx_segment(p.offs, p.rows, e, start, &bad);
+  grid_dependency_wait();  // offs and this scratch may be in use until here
+  int64_t sum = 0;
+  bool bad = false;
+  for (int e = lo; e < hi; ++e) {
+    sum += mx_tiles(p.offs, p, e, tile_rows, tile_cols, &bad);
     if (bad) atomicOr(p.error_word, kErrBadDims);
-    if (warp == 1) {
-      tmap_replace_address(&staging[1], p.b + e * p.b_stride);
-    } else if (len > 0) {  // an empty segment's maps are never used
-      tmap_replace_address(&staging[warp], warp == 0 ? static_cast<const void*>(p.a + start * p.a_pitch)
-                                                     : static_cast<const void*>(p.c + start * p.c_pitch));
-      tmap_replace_dim(&staging[warp], 1, static_cast<uint32_t>(len));
-    }
   }
-  __syncwarp();
-  tmap_publish(reinterpret_cast<CUtensorMap*>(p.maps) + static_cast<int64_t>(e) * 3 + warp, &staging[warp]);
+  const int64_t incl = warp_scan(sum, lane);
+  int64_t run = incl - sum;
+  for (int e = lo; e < hi; ++e) {
+    list[e] = static_cast<int32_t>(run);
+    run += mx_tiles(p.offs, p, e, tile_rows, tile_cols, &bad);
+  }
+  if (lane == 31) list[p.experts] = static_cast<int32_t>(incl);
 }
 
 // Words of shared memory for the tile list and row ends, if they fit.
 constexpr int kMxListWords = 400;
 
 // A role's position in the tile list (`ts` and `offs` in shared or global memory).
+template <int ROWS>
 struct MxWalk {
   const MxParams& p;
   const int32_t* ts;
   const int32_t* offs;
   int e = -1;
-  int64_t first = 0, end = 0, len = 0, start = 0, m_blocks = 1;
+  int32_t first = 0, end = 0, m_blocks = 1;
+  int64_t len = 0, start = 0;
 
   __device__ __forceinline__ MxWalk(const MxParams& params, const int32_t* list, const int32_t* ends)
       : p(params), ts(list), offs(ends) {}
 
-  __device__ __forceinline__ bool seek(int64_t t) {
+  __device__ __forceinline__ bool seek(int64_t tile) {
+    if (tile >= ts[p.experts]) return false;
+    const int32_t t = static_cast<int32_t>(tile);
     if (t >= end || e < 0) {
-      if (t >= ts[p.experts]) return false;
       int lo = e < 0 ? 0 : e, hi = p.experts - 1;
       while (lo < hi) {  // empty experts share their successor's first tile
         const int mid = (lo + hi + 1) >> 1;
@@ -406,18 +379,20 @@ struct MxWalk {
       first = ts[lo];
       end = ts[lo + 1];
       len = mx_segment(offs, p.rows, lo, start);
-      m_blocks = ceil_div64(len, p.tile_rows);
+      m_blocks = static_cast<int32_t>(ceil_div64(len, ROWS));
     }
     return true;
   }
-  __device__ __forceinline__ void blocks(int64_t t, int64_t& mb, int64_t& nb) const {
-    const int64_t local = t - first;
-    const int64_t band_tiles = 8 * ((end - first) / m_blocks);
-    const int64_t band = local / band_tiles;
-    const int64_t in = local - band * band_tiles;
-    const int64_t rows_in = m_blocks - band * 8 < 8 ? m_blocks - band * 8 : 8;
-    mb = band * 8 + in % rows_in;
-    nb = in / rows_in;
+  // Bands of 8 row blocks, row block fastest inside a band.
+  __device__ __forceinline__ void blocks(int64_t tile, int64_t& mb, int64_t& nb) const {
+    const uint32_t local = static_cast<uint32_t>(tile) - first;
+    const uint32_t band_tiles = 8u * (static_cast<uint32_t>(end - first) / m_blocks);
+    const uint32_t band = local / band_tiles;
+    const uint32_t in = local - band * band_tiles;
+    const uint32_t rows_in = m_blocks - band * 8 < 8 ? m_blocks - band * 8 : 8;
+    const uint32_t column = in / rows_in;
+    mb = band * 8 + (in - column * rows_in);
+    nb = column;
   }
 };
 
@@ -566,6 +541,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   const int64_t items_step = split > 1 ? 1ll << 60 : gridDim.x / G;  // one tile where K is split
   // The next kernel may set up as SMs come free; it waits for this one's end.
   grid_launch_dependents();
+  if (threadIdx.x < 3) prefetch_tmap(&p.map[threadIdx.x]);
   // This CTA's K blocks of every tile.
   const int32_t share = split > 1 ? static_cast<int32_t>(cluster_ctarank()) : 0;
   const int32_t kb_from = share * p.split_blocks;
@@ -605,16 +581,30 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   grid_dependency_wait();  // global memory is read only from here on
   const int32_t* ts = p.tile_start;
   const int32_t* offs = p.offs;
-  if (2 * p.experts + 1 <= kMxListWords) {
-    for (int i = threadIdx.x; i <= p.experts; i += kMxThreads) list[i] = p.tile_start[i];
-    if (p.offs != nullptr) {
-      for (int i = threadIdx.x; i < p.experts; i += kMxThreads) list[p.experts + 1 + i] = p.offs[i];
-      offs = list + p.experts + 1;
+  if (ts == nullptr) {
+    // The tile list: first tiles of every expert, then the row ends.
+    int32_t* ends = list + p.experts + 1;
+    for (int i = threadIdx.x; i < p.experts; i += kMxThreads) {
+      ends[i] = p.offs != nullptr ? p.offs[i] : static_cast<int32_t>(p.rows);
     }
-    ts = list;
     __syncthreads();
+    if (warp == 0) {
+      int64_t before = 0;
+      for (int base = 0; base < p.experts; base += 32) {
+        const int e = base + lane;
+        bool bad = false;
+        const int64_t tiles = e < p.experts ? mx_tiles(ends, p, e, Cfg::kTileM, Cfg::kTileN, &bad) : 0;
+        if (bad && blockIdx.x == 0) atomicOr(p.error_word, kErrBadDims);
+        const int64_t incl = warp_scan(tiles, lane);
+        if (e < p.experts) list[e] = static_cast<int32_t>(before + incl - tiles);
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      if (lane == 0) list[p.experts] = static_cast<int32_t>(before);
+    }
+    __syncthreads();
+    ts = list;
+    offs = ends;
   }
-  const CUtensorMap* all_maps = reinterpret_cast<const CUtensorMap*>(p.maps);
 
   auto fail = [&](uint32_t bits) {
     atomicOr(p.error_word, bits);
@@ -629,22 +619,18 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       const uint64_t pol_stream = policy_evict_first();
       const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), empty0 = smem_u32(empty);
       const uint32_t lead0 = G == 2 ? mapa_shared(full0, 0) : full0;  // the leader's barriers
-      MxWalk walk(p, ts, offs);
+      MxWalk<Cfg::kTileM> walk(p, ts, offs);
       int s = 0;
       uint32_t phase = 0, loaded = 0;
-      int built = -1;
       bool ok = true;
       const int32_t begin = kb_from * Cfg::kBK, end = kb_to * Cfg::kBK;
       for (int64_t t = first_item; ok && walk.seek(t); t += items_step) {
         int64_t mb, nb;
         walk.blocks(t, mb, nb);
-        const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.e) * 3;
-        if (walk.e != built) {
-          tmap_acquire(&g[0]);
-          tmap_acquire(&g[1]);
-          built = walk.e;
-        }
-        const int32_t m0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * ROWS);
+        // Absolute row; a pair's upper half that lies past the segment reads
+        // zeros from past the tensor (no traffic, and quieter MMAs).
+        const int64_t m = mb * Cfg::kTileM + rank * ROWS;
+        const int32_t m0 = static_cast<int32_t>(m < walk.len ? walk.start + m : p.rows);
         const int32_t n0 = static_cast<int32_t>(nb * Cfg::kTileN + rank * Cfg::kColsCta);
         const uint64_t pol_b = walk.m_blocks == 1 ? pol_stream : pol_shared;
         for (int32_t kx = begin; kx < end; kx += Cfg::kBK) {
@@ -655,8 +641,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
           }
           const uint32_t st = ring0 + s * Cfg::kStageBytes;
           if (leader) mbar_arrive_expect_tx(&full[s], G * Cfg::kStageBytes);
-          tile_load<G>(&g[0], lead0 + s * 8, st, kx, m0, pol_keep);
-          tile_load<G>(&g[1], lead0 + s * 8, st + Cfg::kABytes, kx, n0, pol_b);
+          tile_load<G>(&p.map[0], lead0 + s * 8, st, kx, m0, pol_keep);
+          tile_load_3d<G>(&p.map[1], lead0 + s * 8, st + Cfg::kABytes, kx, n0, walk.e, pol_b);
           ++loaded;
           if (++s == S) {
             s = 0;
@@ -678,7 +664,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     // ------------------------------------------------ MMA issuer (leader only)
     if (lane == 0 && leader) {
       const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty);
-      MxWalk walk(p, ts, offs);
+      MxWalk<Cfg::kTileM> walk(p, ts, offs);
       int s = 0;
       uint32_t phase = 0, acc_it = 0, sf_it = 0;
       bool ok = true;
@@ -746,7 +732,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     __syncwarp();
   } else if (warp == 2) {
     // -------------------------------------------------------------- scales
-    MxWalk walk(p, ts, offs);
+    MxWalk<Cfg::kTileM> walk(p, ts, offs);
     uint32_t sf_it = 0;
     bool ok = true;
     // Four consecutive bytes of a scale row from K block kb on; blocks past the end are 1.
@@ -799,18 +785,11 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     const int quarter = warp & 3;
     uint8_t* block = epi_stage + quarter * Cfg::kBlockBytes;
     const uint64_t pol_out = policy_evict_normal();
-    MxWalk walk(p, ts, offs);
+    MxWalk<Cfg::kTileM> walk(p, ts, offs);
     uint32_t acc_it = 0;
-    int built = -1;
     for (int64_t t = first_item; walk.seek(t); t += items_step) {
       int64_t mb, nb;
       walk.blocks(t, mb, nb);
-      const CUtensorMap* g = all_maps + static_cast<int64_t>(walk.e) * 3;
-      if (walk.e != built) {
-        if (lane == 0) tmap_acquire(&g[2]);
-        __syncwarp();
-        built = walk.e;
-      }
       const int buf = static_cast<int>(acc_it & 1);
       if (!mbar_wait_warp(&acc_full[buf], (acc_it >> 1) & 1u, budget, abort)) {
         if (lane == 0) fail(kErrWaitAccFull);
@@ -840,10 +819,29 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       if (quarter * 32 < ROWS && row0 < walk.len) {
         // Chunks of 32 columns (a 224-column tile is seven); the map clips C's edges.
         const int64_t cols = p.n - c0 < Cfg::kTileN ? p.n - c0 : Cfg::kTileN;
+        // Where the segment ends inside these 32 rows, each lane stores its
+        // own row straight from registers.
+        const bool ragged = row0 + 32 > walk.len;
 #pragma unroll 1
         for (int c = 0; c * 32 < cols; ++c) {
           uint32_t v[32];
           tmem_ld32(taddr + c * 32, v);
+          if (ragged) {
+            tmem_ld_wait();
+            if (row0 + lane < walk.len) {
+              uint4* to = reinterpret_cast<uint4*>(p.c + (walk.start + row0 + lane) * p.c_pitch + c0 + c * 32);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (c * 32 + 8 * j < cols) {  // n is a multiple of 8
+                  to[j] = make_uint4(
+                      pack_pair<__nv_bfloat16>(v[8 * j], v[8 * j + 1]), pack_pair<__nv_bfloat16>(v[8 * j + 2], v[8 * j + 3]),
+                      pack_pair<__nv_bfloat16>(v[8 * j + 4], v[8 * j + 5]),
+                      pack_pair<__nv_bfloat16>(v[8 * j + 6], v[8 * j + 7]));
+                }
+              }
+            }
+            continue;
+          }
           if (lane == 0) bulk_wait_group_read<0>();  // the previous chunk's store has read the block
           __syncwarp();
           tmem_ld_wait();
@@ -858,7 +856,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&g[2], block, c0 + c * 32, row0, pol_out);
+            tma_store_2d(&p.map[2], block, c0 + c * 32, static_cast<int32_t>(walk.start) + row0, pol_out);
             bulk_commit_group();
           }
         }
@@ -882,7 +880,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   __syncthreads();
   if (G == 2 || split > 1) cluster_sync();
   if (G == 1 && split > 1) {
-    MxWalk walk(p, ts, offs);
+    MxWalk<Cfg::kTileM> walk(p, ts, offs);
     if (walk.seek(first_item) && !*abort) {
       int64_t mb, nb;
       walk.blocks(first_item, mb, nb);

@@ -286,7 +286,7 @@ def _declare(lib) -> None:
     lib.quantize_rows_launch.restype = ctypes.c_int
     lib.quantize_blocks_launch.argtypes = [ptr, i64, i64, i64, i64, i64, i32, ptr, ptr, ptr]
     lib.quantize_blocks_launch.restype = ctypes.c_int
-    lib.block_scaled_mm_scratch_bytes.argtypes = [i32, i64, i64, i64]
+    lib.block_scaled_mm_scratch_bytes.argtypes = [i32]
     lib.block_scaled_mm_scratch_bytes.restype = size
     lib.block_scaled_mm_launch.argtypes = [ptr, i64, ptr, ptr, i64, i64, ptr, ptr, i64, ptr, i32, i64, i64, i64, ptr,
                                            size, ptr, ctypes.POINTER(LaunchInfo)]
@@ -568,8 +568,8 @@ def quantize_blocks(x: int, matrices: int, rows: int, cols: int, pitch: int, str
            "quantize_blocks_launch")
 
 
-def block_scaled_scratch_bytes(experts: int, rows: int, n: int, k: int) -> int:
-    return load().block_scaled_mm_scratch_bytes(experts, rows, n, k)
+def block_scaled_scratch_bytes(experts: int) -> int:
+    return load().block_scaled_mm_scratch_bytes(experts)
 
 
 def block_scaled_mm(a: int, a_pitch: int, sa: int, b: int, b_pitch: int, b_stride: int, sb: int, c: int, c_pitch: int,

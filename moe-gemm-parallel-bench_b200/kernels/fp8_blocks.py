@@ -137,11 +137,11 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
     b_pitch = b_steps[-2]
     b_stride = b_steps[0] if experts > 1 else n * b_pitch
     if a_steps[1] != 1 or b_steps[-1] != 1 or out_steps[1] != 1 or a_pitch < k or a_pitch % 16 or b_pitch < k or (
-            b_pitch % 16) or b_stride % 16 or (experts > 1 and b_stride < (n - 1) * b_pitch + k) or out_pitch < n or (
-            out_pitch % 8) or (a.data_ptr() | b.data_ptr() | out.data_ptr()) % 16:
-        raise ValueError("a, b and out need contiguous columns, 16-byte aligned bases and rows a whole number of 16 "
-                         "bytes apart that do not overlap")
-    nbytes = _native.block_scaled_scratch_bytes(experts, rows, n, k)
+            b_pitch % 16) or b_stride % b_pitch or b_stride < n * b_pitch or out_pitch < n or out_pitch % 8 or (
+            (a.data_ptr() | b.data_ptr() | out.data_ptr()) % 16):
+        raise ValueError("a, b and out need contiguous columns, 16-byte aligned bases, rows a whole number of 16 bytes "
+                         "apart that do not overlap, and experts a whole number of rows apart")
+    nbytes = _native.block_scaled_scratch_bytes(experts)
     scratch = a.new_empty(nbytes).data_ptr() if nbytes else 0
     _last_info = _call(device, _native.block_scaled_mm, a.data_ptr(), a_pitch, sa.data_ptr(), b.data_ptr(), b_pitch,
                        b_stride, sb.data_ptr(), out.data_ptr(), out_pitch, ends, experts, rows, n, k, scratch, nbytes)

@@ -190,6 +190,7 @@ PRODUCTS = [
     # 64 x 128 tiles; a tile's K shared by the CTAs of a cluster
     ([50] * 3, 136, 1040), ([33], 264, 2064), ([100], 264, 4112), ([40, 0, 50], 136, 2064), ([128], 1024, 7168),
     ([5, 70, 45], 520, 1104), ([0, 200, 10], 136, 16384), ([64], 8, 2320),
+    ([40, 0, 1, 63] * 60, 72, 144), ([0, 300, 0, 9] * 50, 1032, 272),  # tile lists in global memory
     # CTA pairs' 256 x 224 tiles
     ([2048], 4096, 512), ([1, 0, 1500, 255, 257], 4096, 1168), ([1999], 2248, 1040),
 ]
@@ -359,10 +360,9 @@ def test_abi_refuses_bad_arguments_before_any_launch():
     for change in bad:
         assert product(**change) == _native.STATUS_INVALID, change
     for change in (dict(scratch=None), dict(scratch=at + 16), dict(scratch_bytes=64)):
-        change["rows"] = 100  # more than a few a expert: maps are needed
+        change["experts"] = 200  # their tile list is kept in scratch
         assert product(**change) == _native.STATUS_SCRATCH, change
-    assert lib.block_scaled_mm_scratch_bytes(0, 10, 64, 64) == 0
-    assert lib.block_scaled_mm_scratch_bytes(2, 16, 64, 64) == 0 < lib.block_scaled_mm_scratch_bytes(2, 17, 64, 64)
+    assert [lib.block_scaled_mm_scratch_bytes(e) for e in (0, 1, 199, 200)] == [0, 0, 0, 896]
     for change in ((None, 4, 8, 8, 1, at, 8, at, None), (at, 4, 0, 8, 1, at, 8, at, None),
                    (at, 4, 8, 7, 1, at, 8, at, None), (at, 4, 8, 8, 5, at, 8, at, None), (at + 1, 4, 8, 8, 1, at, 8, at, None)):
         assert lib.quantize_rows_launch(*change) == _native.STATUS_INVALID, change

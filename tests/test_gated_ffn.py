@@ -159,6 +159,7 @@ SHAPES = [
     ([17], 1160, 2048),  # long contractions of few tiles, shared by a cluster's CTAs
     ([300, 0, 44], 4784, 184),
     ([5, 0, 9], 824, 1600),
+    ([3, 0, 70, 1] * 55, 136, 72),  # tile lists in global memory
     ([700, 1, 0, 333], 4104, 2056),  # pairs' 256 x 256 tiles
     ([0, 2, 256, 0, 255, 257], 2048, 1032),
     ([31, 32, 33, 95, 128, 160, 223, 224, 225, 480, 481], 1048, 520),  # last row blocks of every length
@@ -191,7 +192,7 @@ def test_backward(shape, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", [SHAPES[3], SHAPES[5], SHAPES[8], SHAPES[11]], ids=["small", "ragged", "split", "wide"])
+@pytest.mark.parametrize("shape", [SHAPES[3], SHAPES[5], SHAPES[8], SHAPES[12]], ids=["small", "ragged", "split", "wide"])
 def test_single_product_gradients(shape):
     block = Block(*shape, torch.bfloat16, seed=2)
     h, gate_up = saved_of(block)
