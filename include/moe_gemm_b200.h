@@ -298,14 +298,14 @@ int grouped_gemm_offsets_scatter_launch(const void* a, const void* b, const int3
  *
  * Rows of segment e are [offs[e-1], offs[e]) (int32 cumulative row ends on the
  * device, one per expert; offs = null is one segment of every row, experts =
- * 1).  Rows past the last end are neither read nor written.  An end below its
- * predecessor or past `rows` is clamped and reported (error bit 6).
+ * 1).  Rows past the last end have no effect and are not written.  An end below
+ * its predecessor or past `rows` is clamped and reported (error bit 6).
  * dtype MGB_FP16 or MGB_BF16; bases 16-byte aligned; columns contiguous; row
  * pitches and expert strides in elements, pitches multiples of 8, strides
- * whole multiples of the pitch; hidden and ffn multiples of 8; otherwise
- * MGB_ERR_INVALID.  fp32 accumulation, one rounding
- * per stored value.  Inputs and outputs must not overlap.
- * scratch: ffn_scratch_bytes(experts, jobs) bytes, 128-byte aligned, not
+ * whole multiples of the pitch; hidden and ffn multiples of 8; rows at most
+ * 2^31 - 1024; otherwise MGB_ERR_INVALID.  fp32 accumulation, one rounding per
+ * stored value.  Inputs and outputs must not overlap.
+ * scratch: ffn_scratch_bytes(experts, call) bytes, 128-byte aligned, not
  * shared by launches that overlap. */
 typedef struct mgb_ffn_args {
   int32_t dtype;
@@ -339,9 +339,11 @@ typedef struct mgb_ffn_args {
   void* stream;
 } mgb_ffn_args;
 
-/* Scratch of a call with `jobs` products: forward 2 (1 without w2), backward
- * 4, the gradients below 1. */
-size_t ffn_scratch_bytes(int32_t experts, int32_t jobs);
+enum { MGB_FFN_FORWARD = 0, MGB_FFN_BACKWARD = 1, MGB_FFN_DGRAD = 2, MGB_FFN_WGRAD = 3 };
+
+/* Scratch of a call of that kind: 0 for MGB_FFN_FORWARD and MGB_FFN_DGRAD
+ * below 200 experts. */
+size_t ffn_scratch_bytes(int32_t experts, int32_t call);
 
 /* gate_up = x W13, h = silu(gate) * up (both from one kernel) and, unless w2
  * is null, y = h W2. */
@@ -394,10 +396,10 @@ size_t block_scaled_mm_scratch_bytes(int32_t experts);
  * ceil(k / 128)], c bf16 [rows, n]; fp32 accumulation.  Segments as in
  * gated_ffn_forward_launch (offs null: one segment of every row, experts 1).
  * k a multiple of 16, n of 8; a, b and c 16-byte aligned with row pitches of
- * whole 16 bytes, b's experts whole pitches apart; scales contiguous.  info->path 2: CTA pairs, 0: one CTA,
- * 3: the kernel for few tokens per expert.  Scratch
- * of block_scaled_mm_scratch_bytes(experts), 128-byte aligned, not shared by
- * launches that overlap. */
+ * whole 16 bytes, b's experts whole pitches apart; scales contiguous.
+ * info->path 2: CTA pairs, 0: one CTA, 3: the kernel for few tokens per expert.
+ * Scratch of block_scaled_mm_scratch_bytes(experts), 128-byte aligned, not
+ * shared by launches that overlap. */
 int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const void* b, int64_t b_pitch,
                            int64_t b_stride, const void* sb, void* c, int64_t c_pitch, const int32_t* offs,
                            int32_t experts, int64_t rows, int64_t n, int64_t k, void* scratch, size_t scratch_bytes,

@@ -149,6 +149,13 @@ __device__ __forceinline__ Problem load_problem(const GroupedParams& p, int e) {
 
 __device__ __forceinline__ int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Tiles of a launch as its list ends.  Valid row ends stay below 2^31 (checked
+// on the host); overlapping segments of malformed ones may not: no tile is run
+// then (the segments are reported).
+__device__ __forceinline__ int32_t list_end(int64_t tiles) {
+  return tiles <= 0x7FFFFFFF ? static_cast<int32_t>(tiles) : 0;
+}
+
 // Inclusive scan over the lanes of a warp.
 __device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
 #pragma unroll

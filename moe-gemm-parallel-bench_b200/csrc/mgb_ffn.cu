@@ -20,6 +20,7 @@ namespace {
 using namespace mgb;
 
 constexpr int64_t kMaxExtent = 1ll << 31;
+constexpr int64_t kMaxRows = kMaxExtent - 1024;  // a row block past the last row still has a 32-bit coordinate
 constexpr size_t kMapBytes = sizeof(CUtensorMap);
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -98,11 +99,12 @@ FfnTensor tensor(const void* data, int64_t pitch, int64_t expert_stride, bool to
   return FfnTensor{static_cast<char*>(const_cast<void*>(data)), pitch, expert_stride, token ? 1 : 0};
 }
 
-// Scratch of a call: the operand maps of weight gradients, and a tile list per
-// launch (used where it does not fit shared memory).
+// Scratch of a call: the operand maps of weight gradients, and a tile list for
+// each launch whose list does not fit shared memory.
 size_t maps_bytes(int64_t experts, int wgrads) { return static_cast<size_t>(experts) * wgrads * 2 * kMapBytes; }
+bool global_list(int64_t experts, int jobs) { return (jobs + 1) * experts + 1 > kListWords; }
 size_t list_bytes(int64_t experts, int jobs) {
-  return (static_cast<size_t>(experts) * jobs + 1 + 31) / 32 * 32 * sizeof(int32_t);
+  return global_list(experts, jobs) ? (static_cast<size_t>(experts) * jobs + 1 + 31) / 32 * 32 * sizeof(int32_t) : 0;
 }
 
 // The launches of one call: jobs are added launch by launch, then run()
@@ -272,7 +274,7 @@ struct Launcher {
         }
       }
       if (tiles[i] >= (1ll << 31)) return MGB_ERR_INVALID;  // the list's 32-bit tile numbers
-      if ((p.jobs + 1) * experts + 1 > kListWords) {
+      if (global_list(experts, p.jobs)) {
         FfnPlan::List& l = plan.list[plan.lists++];
         l.jobs = p.jobs;
         l.tile_rows = tile_rows(tile[i]);
@@ -310,7 +312,7 @@ int check_shape(int32_t dtype, int32_t experts, int64_t rows, int64_t a, int64_t
   if (experts <= 0 || experts > (1 << 20) || rows < 0 || a <= 0 || b <= 0 || a % 8 != 0 || b % 8 != 0) {
     return MGB_ERR_INVALID;
   }
-  if (rows >= kMaxExtent || a >= kMaxExtent / 2 || b >= kMaxExtent / 2) return MGB_ERR_INVALID;
+  if (rows > kMaxRows || a >= kMaxExtent / 2 || b >= kMaxExtent / 2) return MGB_ERR_INVALID;
   if (offs == nullptr && experts != 1) return MGB_ERR_INVALID;
   return MGB_OK;
 }
@@ -325,10 +327,10 @@ bool weight_ok(const void* data, int64_t pitch, int64_t stride, int64_t experts,
          (experts == 1 || (stride % pitch == 0 && stride >= rows * pitch));
 }
 
-int start(Launcher& l, int32_t dtype, int64_t rows, int32_t experts, const int32_t* offs, int jobs, void* scratch,
+int start(Launcher& l, int32_t dtype, int64_t rows, int32_t experts, const int32_t* offs, int call, void* scratch,
           size_t scratch_bytes, void* stream) {
-  if (scratch == nullptr || reinterpret_cast<uintptr_t>(scratch) % 128 != 0 ||
-      scratch_bytes < ffn_scratch_bytes(experts, jobs)) {
+  const size_t need = ffn_scratch_bytes(experts, call);
+  if (need > 0 && (scratch == nullptr || reinterpret_cast<uintptr_t>(scratch) % 128 != 0 || scratch_bytes < need)) {
     return MGB_ERR_SCRATCH;
   }
   std::memset(static_cast<void*>(&l.plan), 0, sizeof(l.plan));
@@ -365,9 +367,15 @@ void dgrad(Launcher& l, const FfnTensor& dc, const FfnTensor& b, const FfnTensor
 
 extern "C" {
 
-size_t ffn_scratch_bytes(int32_t experts, int32_t jobs) {
-  if (experts <= 0 || jobs <= 0) return 0;
-  return maps_bytes(experts, jobs) + kFfnLaunches * list_bytes(experts, jobs);
+size_t ffn_scratch_bytes(int32_t experts, int32_t call) {
+  if (experts <= 0) return 0;
+  switch (call) {
+    case MGB_FFN_FORWARD: return 2 * list_bytes(experts, 1);
+    case MGB_FFN_BACKWARD: return maps_bytes(experts, 2) + list_bytes(experts, 1) + list_bytes(experts, 3);
+    case MGB_FFN_DGRAD: return list_bytes(experts, 1);
+    case MGB_FFN_WGRAD: return maps_bytes(experts, 1) + list_bytes(experts, 1);
+    default: return 0;
+  }
 }
 
 int gated_ffn_forward_launch(const mgb_ffn_args* f) {
@@ -385,7 +393,7 @@ int gated_ffn_forward_launch(const mgb_ffn_args* f) {
     return MGB_ERR_INVALID;
   }
   Launcher l;
-  if (int st = start(l, f->dtype, rows, f->experts, f->offs, down ? 2 : 1, f->scratch, f->scratch_bytes, f->stream)) {
+  if (int st = start(l, f->dtype, rows, f->experts, f->offs, MGB_FFN_FORWARD, f->scratch, f->scratch_bytes, f->stream)) {
     return st;
   }
   if (rows == 0) return MGB_OK;
@@ -422,7 +430,7 @@ int gated_ffn_backward_launch(const mgb_ffn_args* f) {
     return MGB_ERR_INVALID;
   }
   Launcher l;
-  if (int st = start(l, f->dtype, rows, f->experts, f->offs, 4, f->scratch, f->scratch_bytes, f->stream)) return st;
+  if (int st = start(l, f->dtype, rows, f->experts, f->offs, MGB_FFN_BACKWARD, f->scratch, f->scratch_bytes, f->stream)) return st;
   const FfnTensor dy = tensor(f->y, f->y_pitch, 0, true), x = tensor(f->x, f->x_pitch, 0, true);
   const FfnTensor h = tensor(f->h, f->h_pitch, 0, true), dgu = tensor(f->dgate_up, f->dgate_up_pitch, 0, true);
   if (rows > 0) {
@@ -449,7 +457,7 @@ int grouped_gemm_dgrad_launch(const void* dc, int64_t dc_pitch, const void* b, i
     return MGB_ERR_INVALID;
   }
   Launcher l;
-  if (int st = start(l, dtype, rows, experts, offs, 1, scratch, scratch_bytes, stream)) return st;
+  if (int st = start(l, dtype, rows, experts, offs, MGB_FFN_DGRAD, scratch, scratch_bytes, stream)) return st;
   if (rows == 0) return MGB_OK;
   dgrad(l, tensor(dc, dc_pitch, 0, true), tensor(b, b_pitch, b_stride, false), tensor(out, out_pitch, 0, true), gate_up,
         gate_up_pitch, n, k);
@@ -465,7 +473,7 @@ int grouped_gemm_wgrad_launch(const void* a, int64_t a_pitch, const void* dc, in
     return MGB_ERR_INVALID;
   }
   Launcher l;
-  if (int st = start(l, dtype, rows, experts, offs, 1, scratch, scratch_bytes, stream)) return st;
+  if (int st = start(l, dtype, rows, experts, offs, MGB_FFN_WGRAD, scratch, scratch_bytes, stream)) return st;
   l.begin_launch(kFfnPlain);
   l.wgrad_job(tensor(a, a_pitch, 0, true), tensor(dc, dc_pitch, 0, true), tensor(db, db_pitch, db_stride, false), k, n);
   return l.run();

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(64) ffn_plan_kernel(const __grid_constant__ Ff
       l.tile_start[i] = static_cast<int32_t>(run);
       run += tiles_of(i);
     }
-    if (lane == 31) l.tile_start[pairs] = static_cast<int32_t>(incl);
+    if (lane == 31) l.tile_start[pairs] = list_end(incl);
     return;
   }
   const int job = blockIdx.x / p.experts, e = blockIdx.x % p.experts;
@@ -259,7 +259,7 @@ struct FfnItems {
       next += mine;
       share = static_cast<int>(cluster_ctarank());
       const int32_t c = blockIdx.x / split;
-      if (c < mine) shared = c;
+      if (c < mine && end > 0) shared = c;
     }
   }
   template <class Walk>
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
         if (i < pairs) list[i] = static_cast<int32_t>(before + incl - tiles);
         before += __shfl_sync(0xffffffffu, incl, 31);
       }
-      if (lane == 0) list[pairs] = static_cast<int32_t>(before);
+      if (lane == 0) list[pairs] = list_end(before);
     }
     __syncthreads();
     ts = list;

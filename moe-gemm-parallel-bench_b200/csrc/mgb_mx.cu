@@ -154,7 +154,7 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
                            int64_t b_stride, const void* sb, void* c, int64_t c_pitch, const int32_t* offs,
                            int32_t experts, int64_t rows, int64_t n, int64_t k, void* scratch, size_t scratch_bytes,
                            void* stream, mgb_launch_info* info) {
-  if (experts <= 0 || experts > (1 << 20) || rows < 0 || rows >= (1ll << 31) || n <= 0 || n >= (1ll << 31) || k <= 0 ||
+  if (experts <= 0 || experts > (1 << 20) || rows < 0 || rows > (1ll << 31) - 1024 || n <= 0 || n >= (1ll << 31) || k <= 0 ||
       k >= (1ll << 30) || k % 16 != 0 || n % 8 != 0 || (offs == nullptr && experts != 1)) {
     return MGB_ERR_INVALID;
   }

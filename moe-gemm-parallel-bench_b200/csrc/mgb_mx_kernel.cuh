@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(32)
     list[e] = static_cast<int32_t>(run);
     run += mx_tiles(p.offs, p, e, tile_rows, tile_cols, &bad);
   }
-  if (lane == 31) list[p.experts] = static_cast<int32_t>(incl);
+  if (lane == 31) list[p.experts] = list_end(incl);
 }
 
 // Words of shared memory for the tile list and row ends, if they fit.
@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
         if (e < p.experts) list[e] = static_cast<int32_t>(before + incl - tiles);
         before += __shfl_sync(0xffffffffu, incl, 31);
       }
-      if (lane == 0) list[p.experts] = static_cast<int32_t>(before);
+      if (lane == 0) list[p.experts] = list_end(before);
     }
     __syncthreads();
     ts = list;

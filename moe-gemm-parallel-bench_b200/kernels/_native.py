@@ -523,8 +523,11 @@ def fp8_launch(
     return info
 
 
-def ffn_scratch_bytes(experts: int, jobs: int) -> int:
-    return load().ffn_scratch_bytes(experts, jobs)
+FFN_FORWARD, FFN_BACKWARD, FFN_DGRAD, FFN_WGRAD = range(4)
+
+
+def ffn_scratch_bytes(experts: int, call: int) -> int:
+    return load().ffn_scratch_bytes(experts, call)
 
 
 def gated_ffn_forward(args: FfnArgs, scratch: int, scratch_nbytes: int, stream: int) -> None:

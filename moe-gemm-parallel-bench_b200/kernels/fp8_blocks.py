@@ -100,7 +100,7 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
     ceil(K / 128)]`` and weights ``b [N, K]`` or ``[E, N, K]`` with scales ``sb
     [(E,) ceil(N / 128), ceil(K / 128)]``; with experts the rows are sorted and
     ``offs`` (int32 ``[E]``) holds their cumulative row ends.  Empty experts are
-    fine; rows past ``offs[-1]`` are neither read nor written.  K is a multiple
+    fine; rows past ``offs[-1]`` have no effect and are not written.  K is a multiple
     of 16, N of 8; rows of a, b and out may be padded to whole 16 bytes, scales
     are contiguous.  With few tokens per expert (8 on average, weights up to 256
     MB) the weights are streamed by many small CTAs, else 64 x 128, 128 x 128 or

@@ -13,12 +13,13 @@ writes h), and the backward pass returns the gradients of x, W13 and W2:
 Rows are sorted by expert, ``offs`` (int32 ``[E]``, on the device) holding the
 cumulative row ends, as in ``launch_grouped_mm``; ``offs=None`` is the dense
 block (one expert, every row).  Empty experts are fine (their weight gradients
-are zeros); rows past ``offs[-1]`` are neither read nor written.  The single
+are zeros); rows past ``offs[-1]`` have no effect and are not written.  The single
 products' gradients are there as well: ``launch_grouped_mm_dgrad`` and
 ``launch_grouped_mm_wgrad``.
 
 fp16 or bf16; hidden and ffn sizes are multiples of 8, bases 16-byte aligned,
-columns contiguous, rows may be padded to a pitch that is a multiple of 8.
+columns contiguous; rows may be padded to a pitch that is a multiple of 8,
+experts to a whole number of rows.
 Accumulation is fp32; ``gate_up``, ``h`` and the gradient of ``gate_up`` are
 rounded once to the operands' type between products.  Inputs and outputs must
 not overlap.  Every call is launches only (no synchronisation), on the current
@@ -66,6 +67,11 @@ def _call(device, entry, *args):
 def _rows_of(like, rows: int, cols: int):
     """An empty [rows, cols] tensor of ``like``'s type and device."""
     return torch.empty_strided((rows, cols), (cols, 1), dtype=like.dtype, device=like.device)
+
+
+def _scratch(like, nbytes: int):
+    """(scratch, bytes) of a call on ``like``'s device; None where it needs none."""
+    return (like.new_empty(nbytes // 2) if nbytes else None), nbytes
 
 
 def _token(name: str, t, rows: int, cols: int, dtype, device) -> tuple[int, int]:
@@ -158,9 +164,8 @@ def gated_ffn_forward(x, w13, w2, offs=None, *, out=None, h=None, gate_up=None):
     args.y, args.y_pitch = _token("out", out, rows, hidden, dtype, device)
     args.h, args.h_pitch = _token("h", h, rows, ffn, dtype, device)
     args.gate_up, args.gate_up_pitch = _token("gate_up", gate_up, rows, 2 * ffn, dtype, device)
-    nbytes = _native.ffn_scratch_bytes(experts, 2)
-    scratch = x.new_empty(nbytes // 2)
-    _call(device, _native.gated_ffn_forward, args, scratch.data_ptr(), nbytes)
+    scratch, nbytes = _scratch(x, _native.ffn_scratch_bytes(experts, _native.FFN_FORWARD))
+    _call(device, _native.gated_ffn_forward, args, scratch.data_ptr() if nbytes else 0, nbytes)
     return out, h, gate_up
 
 
@@ -192,7 +197,7 @@ def gated_ffn_backward(dy, x, w13, w2, h, gate_up, offs=None, *, dx=None, dw13=N
     # One workspace: the gradient of gate_up between the two launches, then
     # the scratch (128-byte aligned behind it).
     behind = -(-rows * 2 * ffn // 64) * 64
-    nbytes = _native.ffn_scratch_bytes(experts, 4)
+    nbytes = _native.ffn_scratch_bytes(experts, _native.FFN_BACKWARD)
     workspace = x.new_empty(behind + nbytes // 2)
     at = workspace.data_ptr()
     args.dgate_up, args.dgate_up_pitch = at, 2 * ffn
@@ -226,10 +231,9 @@ def launch_grouped_mm_dgrad(dc, mat_b, offs=None, out=None, *, gate_up=None):
     out_at, out_pitch = _token("out", out, rows, cols, dc.dtype, device)
     if rows == 0:
         return out
-    nbytes = _native.ffn_scratch_bytes(experts, 1)
-    scratch = dc.new_empty(nbytes // 2)
+    scratch, nbytes = _scratch(dc, _native.ffn_scratch_bytes(experts, _native.FFN_DGRAD))
     _call(device, _native.grouped_dgrad, dc_at, dc_pitch, b_at, b_pitch, b_stride, ends, experts, rows, n, k, gu_at,
-          gu_pitch, out_at, out_pitch, code, scratch.data_ptr(), nbytes)
+          gu_pitch, out_at, out_pitch, code, scratch.data_ptr() if nbytes else 0, nbytes)
     return out
 
 
@@ -255,8 +259,7 @@ def launch_grouped_mm_wgrad(mat_a, dc, offs=None, out=None):
     if out is None:
         out = mat_a.new_empty((k, n) if offs is None else (experts, k, n))
     out_at, out_pitch, out_stride = _weight("out", out, experts, k, n, mat_a.dtype, device)
-    nbytes = _native.ffn_scratch_bytes(experts, 1)
-    scratch = mat_a.new_empty(nbytes // 2)
+    scratch, nbytes = _scratch(mat_a, _native.ffn_scratch_bytes(experts, _native.FFN_WGRAD))
     _call(device, _native.grouped_wgrad, a_at, a_pitch, dc_at, dc_pitch, ends, experts, rows, n, k, out_at, out_pitch,
           out_stride, code, scratch.data_ptr(), nbytes)
     return out

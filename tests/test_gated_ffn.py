@@ -418,13 +418,18 @@ def test_abi_refuses_bad_arguments_before_any_launch():
         return f
 
     bad = [dict(dtype=2), dict(experts=0), dict(rows=-1), dict(hidden=60), dict(ffn=0), dict(offs=None), dict(x=at + 2),
-           dict(x=None), dict(x_pitch=60), dict(x_pitch=68), dict(w13=None), dict(w13_stride=64 * 80 - 8),
+           dict(x=None), dict(x_pitch=60), dict(x_pitch=68), dict(w13=None), dict(w13_stride=64 * 80 - 8), dict(w13_stride=64 * 80 + 8), dict(rows=(1 << 31) - 1023),
            dict(w2_pitch=56), dict(rows=1 << 31), dict(h=None), dict(gate_up_pitch=40)]
     for change in bad:
         for entry in (lib.gated_ffn_forward_launch, lib.gated_ffn_backward_launch):
             assert entry(ctypes.byref(args(**change))) == _native.STATUS_INVALID, change
     for entry in (lib.gated_ffn_forward_launch, lib.gated_ffn_backward_launch):
         assert entry(None) == _native.STATUS_INVALID
-        assert entry(ctypes.byref(args())) == _native.STATUS_SCRATCH
-    assert _native.ffn_scratch_bytes(0, 1) == 0
-    assert _native.ffn_scratch_bytes(4, 2) >= 2 * 4 * 2 * 128  # two operand maps per gradient and expert
+        assert entry(ctypes.byref(args(experts=200))) == _native.STATUS_SCRATCH  # its tile lists are kept there
+        assert entry(ctypes.byref(args(experts=200, scratch=at, scratch_bytes=1664))) == _native.STATUS_SCRATCH
+    # Two operand maps per gradient and expert; tile lists from 200 (three jobs: 100) experts.
+    calls = _native.FFN_FORWARD, _native.FFN_BACKWARD, _native.FFN_DGRAD, _native.FFN_WGRAD
+    assert [_native.ffn_scratch_bytes(0, c) for c in calls] == [0] * 4
+    assert [_native.ffn_scratch_bytes(4, c) for c in calls] == [0, 4 * 4 * 128, 0, 4 * 2 * 128]
+    assert [_native.ffn_scratch_bytes(100, c) for c in calls] == [0, 100 * 4 * 128 + 1280, 0, 100 * 2 * 128]
+    assert [_native.ffn_scratch_bytes(200, c) for c in calls] == [1792, 200 * 4 * 128 + 896 + 2432, 896, 200 * 2 * 128 + 896]
