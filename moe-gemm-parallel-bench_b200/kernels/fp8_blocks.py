@@ -142,7 +142,8 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
         raise ValueError("a, b and out need contiguous columns, 16-byte aligned bases, rows a whole number of 16 bytes "
                          "apart that do not overlap, and experts a whole number of rows apart")
     nbytes = _native.block_scaled_scratch_bytes(experts)
-    scratch = a.new_empty(nbytes).data_ptr() if nbytes else 0
+    scratch = a.new_empty(nbytes) if nbytes else None
     _last_info = _call(device, _native.block_scaled_mm, a.data_ptr(), a_pitch, sa.data_ptr(), b.data_ptr(), b_pitch,
-                       b_stride, sb.data_ptr(), out.data_ptr(), out_pitch, ends, experts, rows, n, k, scratch, nbytes)
+                       b_stride, sb.data_ptr(), out.data_ptr(), out_pitch, ends, experts, rows, n, k,
+                       scratch.data_ptr() if nbytes else 0, nbytes)
     return out
