@@ -204,18 +204,18 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
     }
     return launch_few(p, grid, s);
   }
-  // Pairs' 256 x 224 tiles from 112 rows an expert where they cover the
-  // device's pairs once (a half-empty pair tile still reads its weights once;
-  // 32 experts, n 4096, k 7168: 273 against 283 us at 128 rows, 255 against
-  // 228 at 64); else one CTA's 128 x 128, or 64 x 128 up to 48 rows an expert
-  // (182 against 203 us at 48; 241 against 228 at 64, where uneven routing
-  // gives some experts a second tile).
+  // Pairs' tiles of up to 224 rows x 256 outputs from 112 rows an expert where
+  // they cover the device's pairs once (32 experts, n 4096, k 7168: 214 against
+  // 289 us at 128 rows, 208 against 205 at 112, 204 against 187 at 104); else
+  // one CTA's 128 x 128, or 64 x 128 up to 20 rows an expert (171 against
+  // 175 us at 16; at 32 172 against 178, but 191 against 177 under uneven
+  // routing, which gives some experts a second tile).
   const int64_t segments = std::min<int64_t>(experts, rows);
-  const int64_t pair_tiles = (cdiv(rows, 256) + segments - 1) * cdiv(n, MxCfg<2>::kTileN);
+  const int64_t pair_tiles = (cdiv(rows, MxCfg<2>::kTokens) + segments - 1) * cdiv(n, MxCfg<2>::kOut);
   const bool pair = each >= 112 && pair_tiles >= sms / 2;
-  const bool half = !pair && each <= 48;
-  const int tile_rows = pair ? 256 : half ? 64 : 128;
-  const int tile_cols = pair ? MxCfg<2>::kTileN : MxCfg<1>::kTileN;
+  const bool half = !pair && each <= 20;
+  const int tile_rows = pair ? MxCfg<2>::kTokens : half ? 64 : 128;
+  const int tile_cols = pair ? MxCfg<2>::kOut : MxCfg<1>::kOut;
   const int64_t tiles = (cdiv(rows, tile_rows) + segments - 1) * cdiv(n, tile_cols);
   if (tiles >= (1ll << 31)) return MGB_ERR_INVALID;  // the list's 32-bit tile numbers
   // Split K: as many CTAs a tile (2, 4 or 8) as the SMs hold at once, each
@@ -225,10 +225,9 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   while (!pair && p.split < 8 && tiles * p.split * 2 <= sms - sms / 8 && p.kb >= 8 * p.split) p.split *= 2;
   p.split_blocks = static_cast<int32_t>(cdiv(cdiv(p.kb, p.split), 4) * 4);
   const uint64_t stride = static_cast<uint64_t>(experts > 1 ? b_stride : b_pitch * n);
-  if (!encode_map_2d(&p.map[0], kMapBytes8, a, k, rows, a_pitch, 128, half ? 64 : 128) ||
-      !encode_map_3d(&p.map[1], kMapBytes8, b, k, n, experts, b_pitch, stride, 128,
-                     pair ? MxCfg<2>::kColsCta : MxCfg<1>::kColsCta) ||
-      !encode_map_2d(&p.map[2], MGB_BF16, c, n, rows, c_pitch * 2, 32, 32, 64)) {
+  if (!encode_map_2d(&p.map[0], kMapBytes8, a, k, rows, a_pitch, 128, pair ? MxCfg<2>::kRowsB : half ? 64 : 128) ||
+      !encode_map_3d(&p.map[1], kMapBytes8, b, k, n, experts, b_pitch, stride, 128, 128) ||
+      (!pair && !encode_map_2d(&p.map[2], MGB_BF16, c, n, rows, c_pitch * 2, 32, 32, 64))) {
     return MGB_ERR_CUDA;
   }
   if (need > 0) {

@@ -299,6 +299,7 @@ struct MxParams {
   uint32_t* error_word;
   // A and C whole (a segment's rows are addressed absolutely; rows loaded past
   // its end only reach accumulator rows that are not stored), B 3-D by expert.
+  // A pair needs no map of C.
   CUtensorMap map[3];
 };
 
@@ -350,13 +351,15 @@ __global__ void __launch_bounds__(32)
 constexpr int kMxListWords = 400;
 
 // A role's position in the tile list (`ts` and `offs` in shared or global memory).
-template <int ROWS>
+// Blocks of ROWS token rows; EVEN: of equal numbers of token rows instead,
+// ROWS or a multiple of 64 below it.
+template <int ROWS, bool EVEN>
 struct MxWalk {
   const MxParams& p;
   const int32_t* ts;
   const int32_t* offs;
   int e = -1;
-  int32_t first = 0, end = 0, m_blocks = 1;
+  int32_t first = 0, end = 0, m_blocks = 1, each = ROWS;
   int64_t len = 0, start = 0;
 
   __device__ __forceinline__ MxWalk(const MxParams& params, const int32_t* list, const int32_t* ends)
@@ -380,6 +383,7 @@ struct MxWalk {
       end = ts[lo + 1];
       len = mx_segment(offs, p.rows, lo, start);
       m_blocks = static_cast<int32_t>(ceil_div64(len, ROWS));
+      if (EVEN) each = whole(static_cast<int32_t>(ceil_div64(len, m_blocks)));
     }
     return true;
   }
@@ -393,6 +397,15 @@ struct MxWalk {
     const uint32_t column = in / rows_in;
     mb = band * 8 + (in - column * rows_in);
     nb = column;
+  }
+  static __device__ __forceinline__ int32_t whole(int32_t rows) {
+    rows = (rows + 63) / 64 * 64;
+    return rows < ROWS ? rows : ROWS;
+  }
+  // Token rows of row block mb.
+  __device__ __forceinline__ int32_t count(int64_t mb) const {
+    const int64_t left = len - mb * each;
+    return static_cast<int32_t>(left < each ? left : each);
   }
 };
 
@@ -461,29 +474,38 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// Tile: 256 x 224 for a pair; ROWS x 128 for one CTA, ROWS = 128 or 64 token
-// rows.  Two accumulators and the scale words share the 512 TMEM columns:
-// 2 x 224 + 2 x 12 for a pair (N = 256 would leave none for the scales),
-// 2 x 128 + 2 x 8 for one CTA.  A 64-row tile still runs M = 128 MMAs: the
-// operand's upper rows are whatever lies behind it in shared memory and only
-// reach accumulator rows that are never stored.  It halves the token half of a
-// stage, so eight stages (128 KB of weights per SM) are in flight instead of
-// five while the weights' bytes bound the launch.
+// Tiles.  One CTA: ROWS token rows (M = 128) x 128 outputs, ROWS = 128 or 64.
+// A 64-row tile still runs M = 128 MMAs: the operand's upper rows are whatever
+// lies behind it in shared memory and only reach accumulator rows that are
+// never stored.  It halves the token half of a stage, so eight stages (128 KB
+// of weights per SM) are in flight instead of five while the weights' bytes
+// bound the launch.
+// A pair: 256 weight rows (M) x up to 224 token rows (N: 64, 128, 192 or 224,
+// named by the instruction): an expert's rows are cut into equal blocks, so
+// MMAs are spent on its rows rounded up to such a block instead of whole
+// 256-row tiles.  (N = 16 modulo 32 is not a shape of a pair's MMA.)
+// The accumulator is transposed: lanes are outputs, columns token rows.
+// Two accumulators and the scale words share the 512 TMEM columns: 2 x 224 +
+// 2 x 12 for a pair (N = 256 would leave none for the scales), 2 x 128 + 2 x 8
+// for one CTA.
 template <int G, int ROWS = 128>
 struct MxCfg {
   static_assert(ROWS == 128 || (G == 1 && ROWS == 64), "token rows a CTA loads");
   static constexpr int kBK = 128;
-  static constexpr int kColsCta = G == 2 ? 112 : 128;  // weight rows a CTA loads
-  static constexpr int kTileM = ROWS * G, kTileN = kColsCta * G;
+  static constexpr int kRowsB = G == 2 ? 112 : 128;  // rows of the N-side operand a CTA loads
   static constexpr int kMmaM = 128 * G;
-  static constexpr int kABytes = ROWS * 128, kBBytes = kColsCta * 128;
+  static constexpr int kTileN = kRowsB * G;                    // accumulator columns
+  static constexpr int kTokens = G == 2 ? kTileN : ROWS;       // token rows of a tile, at most
+  static constexpr int kOut = G == 2 ? kMmaM : kTileN;         // output columns of a tile
+  using Walk = MxWalk<kTokens, G == 2>;
+  static constexpr int kABytes = ROWS * 128, kBBytes = kRowsB * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kScaleAtoms = 1 + G;           // 128 rows x 4 bytes each: A, then B's 128-row groups
   static constexpr int kScaleBytes = kScaleAtoms * 512;  // one slot: four K blocks
   static constexpr int kScaleCols = 4 * kScaleAtoms;
   static constexpr int kTmemCols = 512;
   static constexpr int kScaleTmem = 2 * kTileN;  // first scale column
-  // One staging block of 32 rows x 64 bytes per epilogue warp: the epilogue
+  // One CTA: a staging block of 32 rows x 64 bytes per epilogue warp: the epilogue
   // runs under the next tile's MMAs, and the shared memory makes a stage.
   static constexpr int kBlockBytes = 32 * 64;
   static constexpr int kEpiBytes = 4 * kBlockBytes;
@@ -495,7 +517,7 @@ struct MxCfg {
   static_assert((2 * kStages + 9) * 8 + 12 + 400 * 4 <= 2048, "barriers and the tile list");
   // Split K (one CTA): a row of partial sums, padded against bank conflicts.
   static constexpr int kSumRow = kTileN * 4 + 16;
-  static_assert(G == 2 || kTileM * kSumRow <= kStages * kStageBytes, "partial sums fit the ring");
+  static_assert(G == 2 || ROWS * kSumRow <= kStages * kStageBytes, "partial sums fit the ring");
 };
 
 constexpr int kMxThreads = 256;
@@ -541,7 +563,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   const int64_t items_step = split > 1 ? 1ll << 60 : gridDim.x / G;  // one tile where K is split
   // The next kernel may set up as SMs come free; it waits for this one's end.
   grid_launch_dependents();
-  if (threadIdx.x < 3) prefetch_tmap(&p.map[threadIdx.x]);
+  if (threadIdx.x < (G == 2 ? 2 : 3)) prefetch_tmap(&p.map[threadIdx.x]);
   // This CTA's K blocks of every tile.
   const int32_t share = split > 1 ? static_cast<int32_t>(cluster_ctarank()) : 0;
   const int32_t kb_from = share * p.split_blocks;
@@ -593,7 +615,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       for (int base = 0; base < p.experts; base += 32) {
         const int e = base + lane;
         bool bad = false;
-        const int64_t tiles = e < p.experts ? mx_tiles(ends, p, e, Cfg::kTileM, Cfg::kTileN, &bad) : 0;
+        const int64_t tiles = e < p.experts ? mx_tiles(ends, p, e, Cfg::kTokens, Cfg::kOut, &bad) : 0;
         if (bad && blockIdx.x == 0) atomicOr(p.error_word, kErrBadDims);
         const int64_t incl = warp_scan(tiles, lane);
         if (e < p.experts) list[e] = static_cast<int32_t>(before + incl - tiles);
@@ -619,7 +641,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       const uint64_t pol_stream = policy_evict_first();
       const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(full), empty0 = smem_u32(empty);
       const uint32_t lead0 = G == 2 ? mapa_shared(full0, 0) : full0;  // the leader's barriers
-      MxWalk<Cfg::kTileM> walk(p, ts, offs);
+      typename Cfg::Walk walk(p, ts, offs);
       int s = 0;
       uint32_t phase = 0, loaded = 0;
       bool ok = true;
@@ -627,11 +649,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       for (int64_t t = first_item; ok && walk.seek(t); t += items_step) {
         int64_t mb, nb;
         walk.blocks(t, mb, nb);
-        // Absolute row; a pair's upper half that lies past the segment reads
-        // zeros from past the tensor (no traffic, and quieter MMAs).
-        const int64_t m = mb * Cfg::kTileM + rank * ROWS;
-        const int32_t m0 = static_cast<int32_t>(m < walk.len ? walk.start + m : p.rows);
-        const int32_t n0 = static_cast<int32_t>(nb * Cfg::kTileN + rank * Cfg::kColsCta);
+        // Absolute token row: a pair's CTAs hold half of the N rows each.
+        const int32_t half = G == 2 ? static_cast<int32_t>(rank) * (Cfg::Walk::whole(walk.count(mb)) / 2) : 0;
+        const int32_t m0 = static_cast<int32_t>(walk.start + mb * walk.each) + half;
+        const int32_t n0 = static_cast<int32_t>(nb * Cfg::kOut + rank * 128);
         const uint64_t pol_b = walk.m_blocks == 1 ? pol_stream : pol_shared;
         for (int32_t kx = begin; kx < end; kx += Cfg::kBK) {
           if (!bar_wait(empty0 + s * 8, phase ^ 1u, budget, abort)) {
@@ -641,8 +662,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
           }
           const uint32_t st = ring0 + s * Cfg::kStageBytes;
           if (leader) mbar_arrive_expect_tx(&full[s], G * Cfg::kStageBytes);
-          tile_load<G>(&p.map[0], lead0 + s * 8, st, kx, m0, pol_keep);
-          tile_load_3d<G>(&p.map[1], lead0 + s * 8, st + Cfg::kABytes, kx, n0, walk.e, pol_b);
+          tile_load<G>(&p.map[0], lead0 + s * 8, st + (G == 2 ? Cfg::kABytes : 0), kx, m0, pol_keep);
+          tile_load_3d<G>(&p.map[1], lead0 + s * 8, st + (G == 2 ? 0 : Cfg::kABytes), kx, n0, walk.e, pol_b);
           ++loaded;
           if (++s == S) {
             s = 0;
@@ -664,7 +685,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     // ------------------------------------------------ MMA issuer (leader only)
     if (lane == 0 && leader) {
       const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty);
-      MxWalk<Cfg::kTileM> walk(p, ts, offs);
+      typename Cfg::Walk walk(p, ts, offs);
       int s = 0;
       uint32_t phase = 0, acc_it = 0, sf_it = 0;
       bool ok = true;
@@ -680,6 +701,12 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
         }
         tc_fence_after();
         const uint32_t d = tmem_base + buf * Cfg::kTileN;
+        uint32_t cols = Cfg::kTileN;
+        if constexpr (G == 2) {
+          int64_t mb, nb;
+          walk.blocks(t, mb, nb);
+          cols = Cfg::Walk::whole(walk.count(mb));
+        }
         uint32_t acc = 0;
         for (int32_t kb4 = kb_from; ok && kb4 < kb_to; kb4 += 4) {
           const int slot = static_cast<int>(sf_it & 1);
@@ -707,7 +734,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
             const uint64_t ad = a_desc + stage, bd = b_desc + stage;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-              mma_mx<G>(d, ad + ks * 2, bd + ks * 2, instr_desc_mx(Cfg::kMmaM, Cfg::kTileN, b), sf, sf + 4, acc);
+              mma_mx<G>(d, ad + ks * 2, bd + ks * 2, instr_desc_mx(Cfg::kMmaM, G == 2 ? cols : Cfg::kTileN, b), sf, sf + 4, acc);
               acc = 1;
             }
             tile_commit<G>(empty0 + s * 8);
@@ -732,7 +759,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     __syncwarp();
   } else if (warp == 2) {
     // -------------------------------------------------------------- scales
-    MxWalk<Cfg::kTileM> walk(p, ts, offs);
+    typename Cfg::Walk walk(p, ts, offs);
     uint32_t sf_it = 0;
     bool ok = true;
     // Four consecutive bytes of a scale row from K block kb on; blocks past the end are 1.
@@ -747,17 +774,21 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     for (int64_t t = first_item; ok && walk.seek(t); t += items_step) {
       int64_t mb, nb;
       walk.blocks(t, mb, nb);
-      const int64_t m0 = mb * Cfg::kTileM + rank * ROWS, n0 = nb * Cfg::kTileN;
+      // Rows past the segment read its last row's scales: never stored.
+      const auto token = [&](int i) {
+        const int64_t m = mb * walk.each + i;
+        return p.sa + (walk.start + (m < walk.len ? m : walk.len - 1)) * p.kb;
+      };
+      const auto weight = [&](int64_t n) { return p.sb + (walk.e * p.nb + (n < p.n ? n : p.n - 1) / 128) * p.kb; };
+      const int64_t n0 = nb * Cfg::kOut + rank * 128;
       const uint8_t* row[4 * Cfg::kScaleAtoms];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t m = m0 + j * 32 + lane;  // rows past the segment read its last row's scales: never stored
-        row[j] = p.sa + (walk.start + (m < walk.len ? m : walk.len - 1)) * p.kb;
-      }
-#pragma unroll
-      for (int j = 4; j < 4 * Cfg::kScaleAtoms; ++j) {
-        const int64_t n = n0 + (j - 4) * 32 + lane;
-        row[j] = p.sb + (walk.e * p.nb + (n < p.n ? n : p.n - 1) / 128) * p.kb;
+      for (int j = 0; j < 4 * Cfg::kScaleAtoms; ++j) {
+        if constexpr (G == 2) {
+          row[j] = j < 4 ? weight(n0) : token((j - 4) * 32 + lane);
+        } else {
+          row[j] = j < 4 ? token(j * 32 + lane) : weight(n0);
+        }
       }
       for (int64_t kb = kb_from; kb < kb_to; kb += 4) {
         const int slot = static_cast<int>(sf_it & 1);
@@ -785,7 +816,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     const int quarter = warp & 3;
     uint8_t* block = epi_stage + quarter * Cfg::kBlockBytes;
     const uint64_t pol_out = policy_evict_normal();
-    MxWalk<Cfg::kTileM> walk(p, ts, offs);
+    typename Cfg::Walk walk(p, ts, offs);
     uint32_t acc_it = 0;
     for (int64_t t = first_item; walk.seek(t); t += items_step) {
       int64_t mb, nb;
@@ -797,9 +828,36 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       }
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * Cfg::kTileN;
-      const int32_t row0 = static_cast<int32_t>(mb * Cfg::kTileM + rank * ROWS + quarter * 32);
+      if constexpr (G == 2) {
+        // Lane pairs trade values: the even lane has two outputs of an even
+        // token row, the odd lane of the next; 16 lanes store 64 bytes of a row.
+        const int64_t n = nb * Cfg::kOut + rank * 128 + quarter * 32 + (lane & ~1);
+        const int odd = lane & 1, count = walk.count(mb);
+        __nv_bfloat16* to = p.c + (walk.start + mb * walk.each + odd) * p.c_pitch + n;
+        if (n - (lane & ~1) < p.n) {
+#pragma unroll 1
+          for (int c = 0; c < count; c += 32, to += 32 * p.c_pitch) {
+            uint32_t v[32];
+            __syncwarp();
+            tmem_ld32(taddr + c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+              const uint32_t two = odd ? pack_pair<__nv_bfloat16>(other, v[j + 1]) : pack_pair<__nv_bfloat16>(v[j], other);
+              if (c + j + odd < count && n < p.n) *reinterpret_cast<uint32_t*>(to + j * p.c_pitch) = two;
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&acc_empty[buf]), 0));
+        ++acc_it;
+        continue;
+      }
+      const int32_t row0 = static_cast<int32_t>(mb * ROWS + quarter * 32);
       const int32_t c0 = static_cast<int32_t>(nb * Cfg::kTileN);
-      if (G == 1 && split > 1) {
+      if (split > 1) {
         // The last MMAs are done and nothing more is loaded: the ring holds the sums.
         if (quarter * 32 < ROWS) {
           float* sums = reinterpret_cast<float*>(ring + (quarter * 32 + lane) * Cfg::kSumRow);
@@ -817,7 +875,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
         break;  // one tile per cluster
       }
       if (quarter * 32 < ROWS && row0 < walk.len) {
-        // Chunks of 32 columns (a 224-column tile is seven); the map clips C's edges.
+        // Chunks of 32 columns; the map clips C's edges.
         const int64_t cols = p.n - c0 < Cfg::kTileN ? p.n - c0 : Cfg::kTileN;
         // Where the segment ends inside these 32 rows, each lane stores its
         // own row straight from registers.
@@ -863,13 +921,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if constexpr (G == 2) {
-          mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&acc_empty[buf]), 0));
-        } else {
-          mbar_arrive_relaxed(&acc_empty[buf]);
-        }
-      }
+      if (lane == 0) mbar_arrive_relaxed(&acc_empty[buf]);
       ++acc_it;
     }
     if (lane == 0) bulk_wait_group_read<0>();  // tensor stores have read the CTA's shared memory before it goes away
@@ -880,7 +932,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
   __syncthreads();
   if (G == 2 || split > 1) cluster_sync();
   if (G == 1 && split > 1) {
-    MxWalk<Cfg::kTileM> walk(p, ts, offs);
+    typename Cfg::Walk walk(p, ts, offs);
     if (walk.seek(first_item) && !*abort) {
       int64_t mb, nb;
       walk.blocks(first_item, mb, nb);
@@ -890,7 +942,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
       // CTAs without K blocks (a short last share) left no sums.
       const int parts = static_cast<int>((p.kb + p.split_blocks - 1) / p.split_blocks);
       for (int r = share * per + warp; r < (share + 1) * per; r += kMxThreads / 32) {
-        const int64_t m = mb * Cfg::kTileM + r;
+        const int64_t m = mb * ROWS + r;
         if (m >= walk.len) break;
         const float4 sum = join_parts(smem_u32(ring + r * Cfg::kSumRow + col * 4), parts);
         if (c < p.n) {  // n is a multiple of 8: four columns are inside or past the end

@@ -189,10 +189,11 @@ PRODUCTS = [
     ([33], 128, 128), ([127], 136, 272), ([100, 0, 1, 129], 264, 656), ([300], 1032, 2000), ([64] * 5, 128, 512),
     # 64 x 128 tiles; a tile's K shared by the CTAs of a cluster
     ([50] * 3, 136, 1040), ([33], 264, 2064), ([100], 264, 4112), ([40, 0, 50], 136, 2064), ([128], 1024, 7168),
-    ([5, 70, 45], 520, 1104), ([0, 200, 10], 136, 16384), ([64], 8, 2320),
+    ([17, 3, 40], 136, 4112), ([20], 264, 2064), ([65, 0, 2, 0, 9], 1032, 1168), ([5, 70, 45], 520, 1104), ([0, 200, 10], 136, 16384), ([64], 8, 2320),
     ([40, 0, 1, 63] * 60, 72, 144), ([0, 300, 0, 9] * 50, 1032, 272),  # tile lists in global memory
-    # CTA pairs' 256 x 224 tiles
+    # CTA pairs' tiles of up to 224 rows x 256
     ([2048], 4096, 512), ([1, 0, 1500, 255, 257], 4096, 1168), ([1999], 2248, 1040),
+    ([63, 64, 65, 128, 129, 192, 193, 224, 225, 447], 4096, 144),
 ]
 
 
