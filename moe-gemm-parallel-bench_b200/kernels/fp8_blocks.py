@@ -38,10 +38,10 @@ def last_block_scaled_info() -> dict | None:
     return None if _last_info is None else _last_info.as_dict()
 
 
-def _source(x) -> int:
+def _source(x, cols: int, steps: tuple) -> int:
     if not x.is_cuda:
         raise ValueError("the tensor to quantise must be on a CUDA device")
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    if steps[-1] != 1 and cols > 1:
         raise ValueError("the tensor to quantise needs contiguous columns")
     return _native.DTYPE_CODES[dtype_name(x.dtype)]
 
@@ -50,7 +50,7 @@ def _target(name: str, t, shape: tuple, dtype, device):
     if t is None:  # empty_strided: the shortest way to a tensor on the host side
         steps = (shape[1], 1) if len(shape) == 2 else (shape[1] * shape[2], shape[2], 1)
         return torch.empty_strided(shape, steps, dtype=dtype, device=device)
-    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} {shape} tensor on {device}")
     return t
 
@@ -59,14 +59,16 @@ def launch_quantize_rows(x, q=None, scale=None):
     """(q, scale) of activations ``x [M, K]`` (fp16, bf16 or fp32; rows may be
     padded): q float8_e4m3fn ``[M, K]``, scale float8_e8m0fnu ``[M, ceil(K / 128)]``."""
     _require_runtime()
-    if x.ndim != 2 or x.shape[1] == 0:
-        raise ValueError(f"expected x [M, K], got {tuple(x.shape)}")
-    code = _source(x)
-    rows, cols = x.shape
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"expected x [M, K], got {tuple(shape)}")
+    rows, cols = shape
+    steps = x.stride()
+    code = _source(x, cols, steps)
     device = x.device
     q = _target("q", q, (rows, cols), torch.float8_e4m3fn, device)
     scale = _target("scale", scale, (rows, _blocks(cols)), torch.float8_e8m0fnu, device)
-    pitch = x.stride(0) if rows > 1 else cols
+    pitch = steps[0] if rows > 1 else cols
     if pitch < cols:
         raise ValueError("rows of x must not overlap")
     _call(device, _native.quantize_rows, x.data_ptr(), rows, cols, pitch, code, q.data_ptr(), cols, scale.data_ptr())
@@ -80,14 +82,15 @@ def launch_quantize_blocks(w, q=None, scale=None):
     _require_runtime()
     if w.ndim not in (2, 3) or w.shape[-1] == 0 or w.shape[-2] == 0:
         raise ValueError(f"expected w [N, K] or [E, N, K], got {tuple(w.shape)}")
-    code = _source(w)
+    steps = w.stride()
     *lead, n, k = w.shape
+    code = _source(w, k, steps)
     matrices = lead[0] if lead else 1
     device = w.device
     q = _target("q", q, tuple(w.shape), torch.float8_e4m3fn, device)
     scale = _target("scale", scale, (*lead, _blocks(n), _blocks(k)), torch.float8_e8m0fnu, device)
-    pitch = w.stride(-2) if n > 1 else k
-    stride = w.stride(0) if matrices > 1 else n * pitch
+    pitch = steps[-2] if n > 1 else k
+    stride = steps[0] if matrices > 1 else n * pitch
     if pitch < k or (matrices > 1 and stride < (n - 1) * pitch + k):
         raise ValueError("rows and matrices of w must not overlap")
     _call(device, _native.quantize_blocks, w.data_ptr(), matrices, n, k, pitch, stride, code, q.data_ptr(),
@@ -107,7 +110,8 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
     CTA-pair tiles (224 x 256) run on the block-scaled tensor-core MMA."""
     global _last_info
     _require_runtime()
-    if a.ndim != 2 or b.ndim not in (2, 3):
+    a_shape, b_shape = a.shape, b.shape
+    if len(a_shape) != 2 or len(b_shape) not in (2, 3):
         raise ValueError("expected a [T, K] and b [N, K] or [E, N, K]")
     device = a.device
     if not a.is_cuda or sa.device != device or b.device != device or sb.device != device:
@@ -116,34 +120,36 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
         raise ValueError("a and b must be float8_e4m3fn")
     if sa.dtype != torch.float8_e8m0fnu or sb.dtype != torch.float8_e8m0fnu:
         raise ValueError("sa and sb must be float8_e8m0fnu")
-    rows, k = a.shape
-    *lead, n, kb = b.shape
+    rows, k = a_shape
+    *lead, n, kb = b_shape
     experts = lead[0] if lead else 1
     if kb != k or k == 0 or n == 0 or experts == 0 or k % 16 or n % 8:
-        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} need one K, a multiple of 16, and N a multiple of 8")
-    if tuple(sa.shape) != (rows, _blocks(k)) or tuple(sb.shape) != (*lead, _blocks(n), _blocks(k)):
-        raise ValueError(f"scale shapes {tuple(sa.shape)} / {tuple(sb.shape)} do not match a {tuple(a.shape)}, "
-                         f"b {tuple(b.shape)} in blocks of {FP8_BLOCK}")
+        raise ValueError(f"a {tuple(a_shape)} and b {tuple(b_shape)} need one K, a multiple of 16, and N a multiple of 8")
+    blocks = _blocks(k)
+    if sa.shape != (rows, blocks) or sb.shape != (*lead, _blocks(n), blocks):
+        raise ValueError(f"scale shapes {tuple(sa.shape)} / {tuple(sb.shape)} do not match a {tuple(a_shape)}, "
+                         f"b {tuple(b_shape)} in blocks of {FP8_BLOCK}")
     if not sa.is_contiguous() or not sb.is_contiguous():
         raise ValueError("scales must be contiguous")
     ends = _offsets(offs, experts, device)
     if out is None:
         out = torch.empty_strided((rows, n), (n, 1), dtype=torch.bfloat16, device=device)
-    elif tuple(out.shape) != (rows, n) or out.dtype != torch.bfloat16 or out.device != device:
+    elif out.shape != (rows, n) or out.dtype != torch.bfloat16 or out.device != device:
         raise ValueError(f"out must be [{rows}, {n}] bfloat16 on {device}")
     a_steps, b_steps, out_steps = a.stride(), b.stride(), out.stride()
     a_pitch = a_steps[0] if rows > 1 else k
     out_pitch = out_steps[0] if rows > 1 else n
     b_pitch = b_steps[-2]
     b_stride = b_steps[0] if experts > 1 else n * b_pitch
+    a_at, b_at, out_at = a.data_ptr(), b.data_ptr(), out.data_ptr()
     if a_steps[1] != 1 or b_steps[-1] != 1 or out_steps[1] != 1 or a_pitch < k or a_pitch % 16 or b_pitch < k or (
             b_pitch % 16) or b_stride % b_pitch or b_stride < n * b_pitch or out_pitch < n or out_pitch % 8 or (
-            (a.data_ptr() | b.data_ptr() | out.data_ptr()) % 16):
+            (a_at | b_at | out_at) % 16):
         raise ValueError("a, b and out need contiguous columns, 16-byte aligned bases, rows a whole number of 16 bytes "
                          "apart that do not overlap, and experts a whole number of rows apart")
-    nbytes = _native.block_scaled_scratch_bytes(experts)
+    nbytes = _native.block_scaled_scratch_bytes(experts) if experts > 1 else 0
     scratch = a.new_empty(nbytes) if nbytes else None
-    _last_info = _call(device, _native.block_scaled_mm, a.data_ptr(), a_pitch, sa.data_ptr(), b.data_ptr(), b_pitch,
-                       b_stride, sb.data_ptr(), out.data_ptr(), out_pitch, ends, experts, rows, n, k,
+    _last_info = _call(device, _native.block_scaled_mm, a_at, a_pitch, sa.data_ptr(), b_at, b_pitch,
+                       b_stride, sb.data_ptr(), out_at, out_pitch, ends, experts, rows, n, k,
                        scratch.data_ptr() if nbytes else 0, nbytes)
     return out

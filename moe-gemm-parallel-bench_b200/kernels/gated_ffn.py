@@ -58,7 +58,7 @@ def _call(device, entry, *args):
     device), so the guard is taken only where it changes something and the
     stream handle is read without building a Stream object."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:  # the tensors' device exists: CUDA is initialised
         return entry(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):
         return entry(*args, torch._C._cuda_getCurrentRawStream(index))
@@ -76,7 +76,7 @@ def _scratch(like, nbytes: int):
 
 def _token(name: str, t, rows: int, cols: int, dtype, device) -> tuple[int, int]:
     """(address, pitch) of a [rows, cols] tensor of the call's type and device."""
-    if tuple(t.shape) != (rows, cols):
+    if t.shape != (rows, cols):
         raise ValueError(f"{name} must be [{rows}, {cols}], got {tuple(t.shape)}")
     if t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
@@ -91,9 +91,9 @@ def _token(name: str, t, rows: int, cols: int, dtype, device) -> tuple[int, int]
 
 def _weight(name: str, t, experts: int, rows: int, cols: int, dtype, device) -> tuple[int, int, int]:
     """(address, pitch, expert stride) of an [experts, rows, cols] weight (or [rows, cols] for one expert)."""
-    shape = tuple(t.shape)
+    shape = t.shape
     if shape != (experts, rows, cols) and not (experts == 1 and shape == (rows, cols)):
-        raise ValueError(f"{name} must be [{experts}, {rows}, {cols}], got {shape}")
+        raise ValueError(f"{name} must be [{experts}, {rows}, {cols}], got {tuple(shape)}")
     if t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
     strides = t.stride()
@@ -121,7 +121,7 @@ def _offsets(offs, experts: int, device) -> int:
         if experts != 1:
             raise ValueError("offs (int32 cumulative row ends) is needed with more than one expert")
         return 0
-    if tuple(offs.shape) != (experts,) or offs.dtype != torch.int32 or not offs.is_contiguous():
+    if offs.shape != (experts,) or offs.dtype != torch.int32 or not offs.is_contiguous():
         raise ValueError(f"offs must be contiguous int32 [{experts}] cumulative row ends")
     if offs.device != device:
         raise ValueError("offs must be on the tensors' device")
