@@ -1083,7 +1083,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_
                      : "r"(slot + i * 512)
                      : "memory");
       }
-      const float sw = scale_value(__ldg(wscale + kb));
+      const int sw = __ldg(wscale + kb);
       float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -1095,9 +1095,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_
       // Columns 2t, 2t + 1 of the accumulator are tokens m0 + 2t, m0 + 2t + 1.
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float sx = 2 * t + j < left ? scale_value(__ldg(xscale + j * p.kb + kb)) : 0.0f;
-        acc[j] += part[j] * sw * sx;
-        acc[2 + j] += part[2 + j] * sw * sx;
+        // The scales' product in two equal steps: one alone may leave fp32's range.
+        const int sx = 2 * t + j < left ? __ldg(xscale + j * p.kb + kb) : 127;
+        const int half = (sw + sx) >> 1;  // 2^(sw - 127) 2^(sx - 127) = 2^(half - 127) 2^(sw + sx - half - 127)
+        const float s1 = scale_value(sw == 255 || sx == 255 ? 255 : half), s2 = scale_value(sw + sx - half);
+        acc[j] += part[j] * s1 * s2;
+        acc[2 + j] += part[2 + j] * s1 * s2;
       }
       fetch(b + kFewDepth);  // into the slot just read
     }

@@ -244,6 +244,28 @@ def test_product_rows_behind_and_padding_stay(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths,n", [([5, 2, 9], 136), ([100, 130, 20], 136), ([1500, 900, 48], 4096)],
+                         ids=["few", "one", "pair"])
+def test_malformed_row_ends_stay_inside_and_are_reported(lengths, n):
+    product = Product(lengths, n, 272, tail=3)
+    wide = torch.full((product.rows + 300, n), 3.25, device="cuda", dtype=torch.bfloat16)
+    out, good, rows = wide[:product.rows], product.offs.clone(), product.rows
+    for ends in ([-7, rows // 2, rows], [rows, 3, rows - 1], [0, rows + 100, 2**31 - 1], [-2**31, 2**31 - 1, -1]):
+        product.offs.copy_(torch.tensor(ends, dtype=torch.int32))
+        product.run(out=out)
+        with pytest.raises(RuntimeError, match="invalid dimensions"):
+            kernels.check_device_errors()
+        assert bool((wide[rows:] == 3.25).all())
+    wide.fill_(3.25)
+    product.offs.zero_()  # every row behind the last segment
+    product.run(out=out)
+    assert bool((wide == 3.25).all())
+    product.offs.copy_(good)
+    product.check(product.run(out=out))
+    kernels.check_device_errors()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [([5], 136, 528), ([100], 136, 528), ([2048], 4096, 528)], ids=["few", "one", "pair"])
 def test_extreme_scales_and_nan(shape):
     product = Product(*shape, dense=True)
@@ -256,6 +278,17 @@ def test_extreme_scales_and_nan(shape):
     kernels.check_device_errors()
     assert bool(torch.isnan(out[1]).all())
     assert bool(torch.isfinite(out[0]).all()) and bool(torch.isfinite(out[2:]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("token,weight", [(0, 254), (254, 0), (1, 250), (253, 3), (200, 50), (10, 130)])
+@pytest.mark.parametrize("shape", [([5], 136, 528), ([100], 136, 528), ([2048], 4096, 528)], ids=["few", "one", "pair"])
+def test_scales_whose_product_alone_is_in_range(shape, token, weight):
+    product = Product(*shape, dense=True)
+    product.sa.view(torch.uint8).fill_(token)
+    product.sb.view(torch.uint8).fill_(weight)
+    product.check(product.run())
+    kernels.check_device_errors()
 
 
 @pytest.mark.gpu

@@ -324,6 +324,40 @@ def test_row_ends_out_of_range_are_clamped_and_reported():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths,hidden,ffn", [([5, 2, 9], 136, 72), ([700, 333, 48], 1160, 1032)], ids=["small", "pairs"])
+def test_malformed_row_ends_stay_inside_and_are_reported(lengths, hidden, ffn):
+    block = Block(lengths, hidden, ffn, torch.bfloat16, seed=13, tail=3)
+    rows, mark = block.rows, 3.25
+
+    def out(cols):
+        return torch.full((rows + 300, cols), mark, device="cuda", dtype=torch.bfloat16)
+
+    outs = y, h, gu, dx = out(hidden), out(ffn), out(2 * ffn), out(hidden)
+
+    def run():
+        kernels.gated_ffn_forward(block.x, block.w13, block.w2, block.offs, out=y[:rows], h=h[:rows], gate_up=gu[:rows])
+        return kernels.gated_ffn_backward(block.dy, block.x, block.w13, block.w2, h[:rows], gu[:rows], block.offs,
+                                          dx=dx[:rows])
+
+    good = block.offs.clone()
+    for ends in ([-7, rows // 2, rows], [rows, 3, rows - 1], [0, rows + 100, 2**31 - 1], [-2**31, 2**31 - 1, -1]):
+        block.offs.copy_(torch.tensor(ends, dtype=torch.int32))
+        run()
+        with pytest.raises(RuntimeError, match="invalid dimensions"):
+            kernels.check_device_errors()
+        assert all(bool((t[rows:] == mark).all()) for t in outs)
+    for t in outs:
+        t.fill_(mark)
+    block.offs.zero_()  # every row behind the last segment
+    _, dw13, dw2 = run()
+    assert all(bool((t == mark).all()) for t in outs) and not dw13.any() and not dw2.any()
+    block.offs.copy_(good)
+    run()
+    kernels.check_device_errors()
+    within(y[:block.used], block.forward()["y"], "y")
+
+
+@pytest.mark.gpu
 def test_repeats_bit_for_bit_and_on_another_stream():
     block = Block([200, 0, 313], 512, 264, torch.bfloat16, seed=11)
     y, h, gu = kernels.gated_ffn_forward(block.x, block.w13, block.w2, block.offs)
