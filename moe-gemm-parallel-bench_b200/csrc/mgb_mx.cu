@@ -131,12 +131,13 @@ int launch_few(const MxParams& p, unsigned grid, cudaStream_t s) {
 }
 
 // Whether the weight-streaming kernel runs: at most 8 rows an expert on
-// average (one pass over its weight rows) and weights of at most 256 MB.  It
-// starts about 8 us sooner than the tiles (1 row, n 4096, k 7168: 8.4 against
-// 15.9 us) but streams large weights at 4.3 TB/s where they reach 5.4 (32
-// experts of that size: 216 against 173 us; 8 of them about even).
-bool few_rows(int64_t rows, int64_t experts, int64_t n, int64_t k) {
-  return rows <= 8 * experts && experts * n * k <= (256ll << 20);
+// average (one pass over its weight rows) and two waves of its CTAs (two per
+// SM), each of which starts anew.  4 rows, against the tiles: n 1024, k 1024
+// 3.0 and 7.5 us; n 4096, k 7168 9.2 and 13.3; two such experts 16.1 and 18.7;
+// 8 of 1024 x 2048 7.5 and 10.8; 16 of them 12.5 and 11.6; 32 of 1024 x 1024
+// 16.9 and 12.1; 8 of 4096 x 7168 67 and 50.
+bool few_rows(int64_t rows, int64_t experts, int64_t n, int sms) {
+  return rows <= 8 * experts && experts * cdiv(n, 16) <= 4 * static_cast<int64_t>(sms);
 }
 
 }  // namespace
@@ -192,7 +193,7 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   p.scale_words = p.kb % 4 == 0 && aligned(sa, 4) && aligned(sb, 4);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t each = cdiv(rows, experts);
-  if (few_rows(rows, experts, n, k)) {
+  if (few_rows(rows, experts, n, sms)) {
     const unsigned grid = static_cast<unsigned>(cdiv(n, 16) * experts);
     if (info != nullptr) {
       info->path = 3;

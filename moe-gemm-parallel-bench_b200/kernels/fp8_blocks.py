@@ -105,8 +105,8 @@ def launch_block_scaled_mm(a, sa, b, sb, offs=None, out=None):
     ``offs`` (int32 ``[E]``) holds their cumulative row ends.  Empty experts are
     fine; rows past ``offs[-1]`` have no effect and are not written.  K is a multiple
     of 16, N of 8; rows of a, b and out may be padded to whole 16 bytes, scales
-    are contiguous.  With few tokens per expert (8 on average, weights up to 256
-    MB) the weights are streamed by many small CTAs, else 64 x 128, 128 x 128 or
+    are contiguous.  With few tokens per expert (8 on average) and few weight
+    rows the weights are streamed by many small CTAs, else 64 x 128, 128 x 128 or
     CTA-pair tiles (224 x 256) run on the block-scaled tensor-core MMA."""
     global _last_info
     _require_runtime()
