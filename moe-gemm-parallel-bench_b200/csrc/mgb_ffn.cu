@@ -289,9 +289,20 @@ struct Launcher {
         list += list_bytes(experts, p.jobs);
       }
     }
-    const int64_t blocks = plan.wgrads * experts + plan.lists;
-    if (blocks > 0 && launch_overlapped(ffn_plan_kernel, static_cast<unsigned>(blocks), 64, 0, stream, plan) != cudaSuccess) {
-      return MGB_ERR_CUDA;
+    if (plan.lists == 0 && launches == 2 && epilogue[0] == kFfnSwigluBwd) {
+      // The first launch cuts the second one's maps.
+      FfnParams& p = params[0];
+      p.cuts = plan.wgrads;
+      for (int w = 0; w < plan.wgrads; ++w) {
+        p.job[1 + w].operands = plan.operands[w];
+        for (int i = 0; i < 2; ++i) {
+          p.map[1 + w][i] = plan.map[w][i];
+          p.job[1 + w].t[i] = plan.t[w][i];
+        }
+      }
+    } else if (const int64_t blocks = plan.wgrads * experts + plan.lists; blocks > 0) {
+      const unsigned grid = static_cast<unsigned>(blocks);
+      if (launch_overlapped(ffn_plan_kernel, grid, 64, 0, stream, plan) != cudaSuccess) return MGB_ERR_CUDA;
     }
     for (int i = 0; i < launches; ++i) {
       FfnParams& p = params[i];
