@@ -33,8 +33,8 @@
 // One CTA per SM, roles by warp: 0 TMA producer, 1 MMA issuer, 2-5 epilogue.
 // G = 2: CTA pairs, 256 x 256 tiles (tcgen05 cta_group::2, M = 256, N = 256),
 // or 256 x 512 (two of those MMAs on the same rows);
-// G = 1: one CTA, 128 x 128 tiles, four times as many, for launches whose
-// 256 x 256 tiles would leave most SMs idle.  Both load 128 rows of A and
+// G = 1: one CTA, 128 x 128 tiles, four times as many, where 256 x 256 tiles
+// would leave too many SMs idle (the host estimates both).  Both load 128 rows of A and
 // 128 columns of B per CTA and 64-deep contraction block (32 KB a stage).
 // Split contraction (G = 1, p.split > 1; for launches whose row tiles would
 // leave at least half of the SMs idle through a long contraction): the CTAs of
