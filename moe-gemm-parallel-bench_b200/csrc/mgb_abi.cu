@@ -559,6 +559,31 @@ bool current_launch_limits(int* sm_count, long long* wait_budget) {
   return true;
 }
 
+int resident_clusters(const void* kernel, int threads, int smem_bytes, int size) {
+  static int known[128][9] = {};
+  int dev = 0;
+  if (size < 2 || size > 8 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return 0;
+  if (known[dev][size] > 0) return known[dev][size];
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = size;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem_bytes;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return known[dev][size] = n;
+}
+
 bool encode_map_3d(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t rows, uint64_t outer,
                    uint64_t pitch, uint64_t stride, uint32_t box_inner, uint32_t box_rows) {
   if (g_encode == nullptr) return false;

@@ -64,6 +64,11 @@ uint32_t* current_error_word();
 // (mgb_set_debug); false when the CUDA runtime cannot resolve them.
 bool current_launch_limits(int* sm_count, long long* wait_budget);
 
+// Clusters of `size` (2, 4 or 8) CTAs that the current device holds at once,
+// for kernels of one CTA per SM like `kernel` (clusters do not cross a GPC,
+// whose SMs hold whole clusters only).
+int resident_clusters(const void* kernel, int threads, int smem_bytes, int size);
+
 // 2-D row-major tensor map with the 128- or 64-byte swizzle: `inner` contiguous
 // elements per row, `outer` rows, `pitch` bytes between rows, boxes of
 // box_inner x box_outer.  `dtype` is an mgb_dtype, or kMapBytes8 for bytes.

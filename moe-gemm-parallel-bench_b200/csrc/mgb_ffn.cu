@@ -241,17 +241,21 @@ struct Launcher {
   }
 
   // Splits the contraction of job 0's tiles: as many CTAs a tile (2, 4 or 8)
-  // as the SMs hold at once, each with at least four blocks.  Clusters do not
-  // cross a GPC, whose SMs (16 to 18) hold whole clusters only: an eighth of
-  // the SMs stays out.  Returns the launch's clusters (its tiles, unsplit).
+  // as the SMs hold at once, each with at least four blocks.  Returns the
+  // launch's clusters (its tiles, unsplit).
   int64_t split_of(FfnParams& p, Tile t, int epi, int64_t tiles) const {
     if (rows == 0 || t.g != 1 || p.job[0].wgrad) return tiles;
     const int64_t own = tiles_of(p.job[0], t, epi);
-    const int64_t blocks = cdiv(p.job[0].k, 64), cap = sms - sms / 8;
-    while (p.split < 8 && own * p.split * 2 <= cap && blocks >= 8 * p.split) p.split *= 2;
+    const int64_t blocks = cdiv(p.job[0].k, 64);
+    while (p.split < 8 && own * p.split * 2 <= sms && blocks >= 8 * p.split && own <= clusters(p.split * 2)) p.split *= 2;
     if (p.split == 1) return tiles;
     // Other jobs' tiles go to every CTA one by one.
-    return std::max(own, std::min<int64_t>(cap / p.split, cdiv(tiles - own, p.split)));
+    return std::max(own, std::min<int64_t>(clusters(p.split), cdiv(tiles - own, p.split)));
+  }
+  static int clusters(int size) {
+    using Cfg = FfnCfg<__nv_bfloat16, kFfnPlain, 1>;
+    return resident_clusters(reinterpret_cast<const void*>(ffn_kernel<__nv_bfloat16, kFfnPlain, 1, 1>), kTcThreads,
+                             Cfg::kSmemBytes, size);
   }
 
   int run() {

@@ -227,10 +227,12 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
   const int64_t tiles = (cdiv(rows, tile_rows) + segments - 1) * cdiv(n, tile_cols);
   if (tiles >= (1ll << 31)) return MGB_ERR_INVALID;  // the list's 32-bit tile numbers
   // Split K: as many CTAs a tile (2, 4 or 8) as the SMs hold at once, each
-  // with at least four K blocks.  Clusters do not cross a GPC, whose SMs (16
-  // to 18) hold whole clusters only: an eighth of the SMs stays out.
+  // with at least four K blocks.
   p.split = 1;
-  while (!pair && p.split < 8 && tiles * p.split * 2 <= sms - sms / 8 && p.kb >= 8 * p.split) p.split *= 2;
+  const auto fits = [&](int size) {
+    return tiles <= resident_clusters(reinterpret_cast<const void*>(mx_kernel<1, 128>), kMxThreads, MxCfg<1>::kSmemBytes, size);
+  };
+  while (!pair && p.split < 8 && tiles * p.split * 2 <= sms && p.kb >= 8 * p.split && fits(p.split * 2)) p.split *= 2;
   p.split_blocks = static_cast<int32_t>(cdiv(cdiv(p.kb, p.split), 4) * 4);
   const uint64_t stride = static_cast<uint64_t>(experts > 1 ? b_stride : b_pitch * n);
   if (!encode_map_2d(&p.map[0], kMapBytes8, a, k, rows, a_pitch, 128, pair ? MxCfg<2>::kRowsB : half ? 64 : 128) ||
