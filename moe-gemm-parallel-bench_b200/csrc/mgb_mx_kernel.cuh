@@ -8,6 +8,11 @@
 // four MMAs that name the same byte and the accumulator stays in TMEM for all
 // of K: no partial is read back and scaled in registers, which is what bounds
 // the fp32-scaled path (mgb_fp8_kernel.cuh).
+//
+// Kernels here may be resident while the kernel before them still writes what
+// they read (grid_dependency_wait orders the two), so none of that memory is
+// read-only for a kernel's whole life: it is read by ordinary loads, not by
+// non-coherent ones, and no pointer is declared unaliased.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -197,9 +202,9 @@ struct FastDiv {
 // (bf16 8191 x 7168, 176 MB: 29 us; 8 elements a thread, four blocks in flight
 // 31 us; a copy of as many bytes 26 us.)
 template <typename T, int ACCESS>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, uint32_t blocks, FastDiv kb,
-                                                            int64_t cols, int64_t pitch, uint8_t* __restrict__ q,
-                                                            int64_t q_pitch, uint8_t* __restrict__ scale, bool dense) {
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, uint32_t blocks, FastDiv kb, int64_t cols,
+                                                            int64_t pitch, uint8_t* q, int64_t q_pitch, uint8_t* scale,
+                                                            bool dense) {
   grid_launch_dependents();
   grid_dependency_wait();
   const uint32_t b = blockIdx.x * 32u + (threadIdx.x >> 3);
@@ -232,10 +237,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 // Blocks: one CTA per 128 x 128 block, its 16384 elements in registers (8
 // threads by 16 elements across, 32 rows per step), one pass over memory.
 template <typename T, int ACCESS>
-__global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
-                                                              int64_t pitch, int64_t matrix, uint8_t* __restrict__ q,
-                                                              int64_t q_pitch, int64_t q_matrix,
-                                                              uint8_t* __restrict__ scale, FastDiv kb, FastDiv per) {
+__global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* x, int64_t rows, int64_t cols, int64_t pitch,
+                                                              int64_t matrix, uint8_t* q, int64_t q_pitch,
+                                                              int64_t q_matrix, uint8_t* scale, FastDiv kb,
+                                                              FastDiv per) {
   __shared__ uint32_t tops[8];
   const uint32_t e = per.div(blockIdx.x), in = blockIdx.x - e * per.d;
   const uint32_t rb = kb.div(in);
@@ -789,10 +794,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
     // Four consecutive bytes of a scale row from K block kb on; blocks past the end are 1.
     const bool words = p.scale_words;
     auto word = [&](const uint8_t* row, int64_t kb) -> uint32_t {
-      if (words) return __ldg(reinterpret_cast<const uint32_t*>(row + kb));
+      if (words) return *reinterpret_cast<const uint32_t*>(row + kb);
       uint32_t w = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w |= (kb + i < p.kb ? static_cast<uint32_t>(__ldg(row + kb + i)) : 127u) << (8 * i);
+      for (int i = 0; i < 4; ++i) w |= (kb + i < p.kb ? static_cast<uint32_t>(row[kb + i]) : 127u) << (8 * i);
       return w;
     };
     for (int64_t t = first_item; ok && walk.seek(t); t += items_step) {
@@ -1078,6 +1083,17 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_
 #pragma unroll 1
     for (int b = 0; warp + b * kFewWarps < kblocks; ++b) {
       const int kb = warp + b * kFewWarps;
+      // Tokens and scales first: they arrive while the weights are waited for.
+      uint4 x[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int k = kb * 128 + c * 64;
+        x[c] = g < left && k + t * 16 < depth ? *reinterpret_cast<const uint4*>(xrow + k) : zero;
+      }
+      const int sw = wscale[kb];
+      int sx[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) sx[j] = 2 * t + j < left ? xscale[j * p.kb + kb] : 127;
       asm volatile("cp.async.wait_group %0;" ::"n"(kFewDepth - 1) : "memory");
       uint4 w[2][2];
       const uint32_t slot = slots + (b % kFewDepth) * kFewBlock;
@@ -1089,22 +1105,18 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) mx_few_kernel(const __grid_
                      : "r"(slot + i * 512)
                      : "memory");
       }
-      const int sw = __ldg(wscale + kb);
       float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int k = kb * 128 + c * 64;
-        const uint4 x = g < left && k + t * 16 < depth ? __ldg(reinterpret_cast<const uint4*>(xrow + k)) : zero;
-        mma_e4m3(part, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, x.x, x.y);
-        mma_e4m3(part, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, x.z, x.w);
+        mma_e4m3(part, w[0][c].x, w[1][c].x, w[0][c].y, w[1][c].y, x[c].x, x[c].y);
+        mma_e4m3(part, w[0][c].z, w[1][c].z, w[0][c].w, w[1][c].w, x[c].z, x[c].w);
       }
       // Columns 2t, 2t + 1 of the accumulator are tokens m0 + 2t, m0 + 2t + 1.
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         // The scales' product in two equal steps: one alone may leave fp32's range.
-        const int sx = 2 * t + j < left ? __ldg(xscale + j * p.kb + kb) : 127;
-        const int half = (sw + sx) >> 1;  // 2^(sw - 127) 2^(sx - 127) = 2^(half - 127) 2^(sw + sx - half - 127)
-        const float s1 = scale_value(sw == 255 || sx == 255 ? 255 : half), s2 = scale_value(sw + sx - half);
+        const int half = (sw + sx[j]) >> 1;  // 2^(sw - 127) 2^(sx - 127) = 2^(half - 127) 2^(sw + sx - half - 127)
+        const float s1 = scale_value(sw == 255 || sx[j] == 255 ? 255 : half), s2 = scale_value(sw + sx[j] - half);
         acc[j] += part[j] * s1 * s2;
         acc[2 + j] += part[2 + j] * s1 * s2;
       }
