@@ -22,7 +22,7 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 template <int G, int ROWS>
-int launch_mx(const MxParams& p, int64_t tiles, int sm_count, cudaStream_t stream) {
+int launch_mx(const MxParams& p, int64_t tiles, int sm_count, cudaStream_t stream, mgb_launch_info* info) {
   using Cfg = MxCfg<G, ROWS>;
   static bool configured[128] = {};
   static int clusters[128] = {};
@@ -62,6 +62,7 @@ int launch_mx(const MxParams& p, int64_t tiles, int sm_count, cudaStream_t strea
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 2;
+  if (info != nullptr) info->grid = static_cast<int32_t>(cfg.gridDim.x);
   return cudaLaunchKernelEx(&cfg, mx_kernel<G, ROWS>, p) == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
 }
 
@@ -251,11 +252,10 @@ int block_scaled_mm_launch(const void* a, int64_t a_pitch, const void* sa, const
     info->tile_n = tile_cols;
     info->tile_k = 128;
     info->stages = pair ? MxCfg<2>::kStages : half ? MxCfg<1, 64>::kStages : MxCfg<1>::kStages;
-    info->grid = static_cast<int32_t>(std::min<int64_t>(tiles * p.split, sms));
   }
-  return pair   ? launch_mx<2, 128>(p, tiles, sms, s)
-         : half ? launch_mx<1, 64>(p, tiles, sms, s)
-                : launch_mx<1, 128>(p, tiles, sms, s);
+  return pair   ? launch_mx<2, 128>(p, tiles, sms, s, info)
+         : half ? launch_mx<1, 64>(p, tiles, sms, s, info)
+                : launch_mx<1, 128>(p, tiles, sms, s, info);
 }
 
 int quantize_rows_launch(const void* x, int64_t rows, int64_t cols, int64_t pitch, int32_t dtype, void* q,
