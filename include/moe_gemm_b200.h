@@ -367,6 +367,20 @@ int grouped_gemm_wgrad_launch(const void* a, int64_t a_pitch, const void* dc, in
                               int32_t experts, int64_t rows, int64_t n, int64_t k, void* db, int64_t db_pitch,
                               int64_t db_stride, int32_t dtype, void* scratch, size_t scratch_bytes, void* stream);
 
+/* What one product launch of a feed-forward or gradient call ran. */
+typedef struct mgb_ffn_launch_info {
+  int32_t epilogue;       /* 0 the product, 1 gate, up and activation, 2 the activation's gradient */
+  int32_t pair;           /* 1: CTA pairs (cta_group::2) */
+  int32_t tile_m, tile_n; /* output tile of a CTA or pair */
+  int32_t split;          /* CTAs of a cluster that share a row product's contraction (1: none) */
+  int32_t grid;           /* CTAs */
+} mgb_ffn_launch_info;
+
+/* The product launches of the calling thread's most recent of the four calls
+ * above that passed its argument checks, in order: at most `capacity` are
+ * written to `info` (null with capacity 0).  Returns how many there were: 0 to 2. */
+int32_t ffn_last_launches(mgb_ffn_launch_info* info, int32_t capacity);
+
 /* e4m3 with power-of-two (e8m0) scales: block-scaled products whose scales the
  * tensor core applies, and the quantisation to them.  No counterpart in the
  * reference, which does not emulate the model's FP8 quantization

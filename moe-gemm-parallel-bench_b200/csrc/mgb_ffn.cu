@@ -27,6 +27,10 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// What the thread's last call launched (ffn_last_launches).
+thread_local mgb_ffn_launch_info last_launch[kFfnLaunches];
+thread_local int last_launches = 0;
+
 // The box of an operand or staged block, in rows of 64 columns.
 enum Box : uint32_t { kKMajor = 128, kMnMajor = 64, kStage = 32 };
 
@@ -72,7 +76,10 @@ int launch_kernel(const FfnParams& p, int64_t tiles, int sm_count, cudaStream_t 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
-  return e == cudaSuccess ? MGB_OK : MGB_ERR_CUDA;
+  if (e != cudaSuccess) return MGB_ERR_CUDA;
+  last_launch[last_launches++] = {EPI, G == 2 ? 1 : 0, Cfg::kTileM, Cfg::kTileOut, p.split,
+                                  static_cast<int32_t>(cfg.gridDim.x)};
+  return MGB_OK;
 }
 
 // Output tile of a launch.
@@ -348,6 +355,7 @@ int start(Launcher& l, int32_t dtype, int64_t rows, int32_t experts, const int32
   if (need > 0 && (scratch == nullptr || reinterpret_cast<uintptr_t>(scratch) % 128 != 0 || scratch_bytes < need)) {
     return MGB_ERR_SCRATCH;
   }
+  last_launches = 0;
   std::memset(static_cast<void*>(&l.plan), 0, sizeof(l.plan));
   l.plan.error_word = current_error_word();
   if (l.plan.error_word == nullptr || !current_launch_limits(&l.sms, &l.budget)) return MGB_ERR_CUDA;
@@ -492,6 +500,11 @@ int grouped_gemm_wgrad_launch(const void* a, int64_t a_pitch, const void* dc, in
   l.begin_launch(kFfnPlain);
   l.wgrad_job(tensor(a, a_pitch, 0, true), tensor(dc, dc_pitch, 0, true), tensor(db, db_pitch, db_stride, false), k, n);
   return l.run();
+}
+
+int32_t ffn_last_launches(mgb_ffn_launch_info* info, int32_t capacity) {
+  for (int i = 0; info != nullptr && i < last_launches && i < capacity; ++i) info[i] = last_launch[i];
+  return last_launches;
 }
 
 }  // extern "C"

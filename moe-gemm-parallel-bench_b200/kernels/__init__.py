@@ -35,6 +35,7 @@ from .fp8_blocks import (
 from .gated_ffn import (
     gated_ffn_backward,
     gated_ffn_forward,
+    last_gated_ffn_info,
     launch_grouped_mm_dgrad,
     launch_grouped_mm_wgrad,
 )
@@ -54,6 +55,7 @@ __all__ = [
     "launch_quantize_rows",
     "gated_ffn_backward",
     "gated_ffn_forward",
+    "last_gated_ffn_info",
     "launch_grouped_mm_dgrad",
     "launch_grouped_mm_wgrad",
     "Fp8GroupedWorkspace",

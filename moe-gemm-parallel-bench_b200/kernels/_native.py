@@ -58,6 +58,7 @@ EXPORTED_SYMBOLS = (
     "gated_ffn_backward_launch",
     "grouped_gemm_dgrad_launch",
     "grouped_gemm_wgrad_launch",
+    "ffn_last_launches",
     "matmul_launch",
     "matrix_repack",
     "matrix_split_tf32x3",
@@ -192,6 +193,22 @@ class FfnArgs(ctypes.Structure):
     ]
 
 
+class FfnLaunchInfo(ctypes.Structure):
+    """mgb_ffn_launch_info: one product launch of a feed-forward or gradient call."""
+
+    _fields_ = [(name, ctypes.c_int32) for name in ("epilogue", "pair", "tile_m", "tile_n", "split", "grid")]
+
+    def as_dict(self) -> dict[str, int | str | bool]:
+        return {
+            "epilogue": ("plain", "swiglu", "swiglu_backward")[self.epilogue],
+            "pair": bool(self.pair),
+            "tile_m": int(self.tile_m),
+            "tile_n": int(self.tile_n),
+            "split": int(self.split),
+            "grid": int(self.grid),
+        }
+
+
 class NativeLaunchError(RuntimeError):
     """A native launch returned a non-OK status."""
 
@@ -302,6 +319,8 @@ def _declare(lib) -> None:
     lib.grouped_gemm_wgrad_launch.argtypes = [ptr, i64, ptr, i64, ptr, i32, i64, i64, i64, ptr, i64, i64, i32, ptr,
                                               size, ptr]
     lib.grouped_gemm_wgrad_launch.restype = ctypes.c_int
+    lib.ffn_last_launches.argtypes = [ctypes.POINTER(FfnLaunchInfo), i32]
+    lib.ffn_last_launches.restype = i32
     lib.matmul_launch.argtypes = [
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
@@ -556,6 +575,12 @@ def grouped_wgrad(a: int, a_pitch: int, dc: int, dc_pitch: int, offs: int, exper
     _check(load().grouped_gemm_wgrad_launch(a, a_pitch, dc, dc_pitch, offs, experts, rows, n, k, db, db_pitch,
                                             db_stride, dtype, scratch, scratch_nbytes, stream),
            "grouped_gemm_wgrad_launch")
+
+
+def ffn_last_launches() -> list[FfnLaunchInfo]:
+    """The product launches of this thread's most recent feed-forward or gradient call."""
+    infos = (FfnLaunchInfo * 2)()
+    return infos[:load().ffn_last_launches(infos, 2)]
 
 
 def quantize_rows(x: int, rows: int, cols: int, pitch: int, dtype: int, q: int, q_pitch: int, scale: int,

@@ -141,6 +141,12 @@ def _block_shape(x, w13, w2) -> tuple[int, int, int, int]:
     return x.shape[0], (w13.shape[0] if w13.ndim == 3 else 1), hidden, ffn
 
 
+def last_gated_ffn_info() -> list[dict]:
+    """The product launches of the calling thread's most recent call of this
+    module, in order: epilogue, pair, output tile, split of the contraction, grid."""
+    return [info.as_dict() for info in _native.ffn_last_launches()]
+
+
 def gated_ffn_forward(x, w13, w2, offs=None, *, out=None, h=None, gate_up=None):
     """(y, h, gate_up) of the block: ``x [T, H]``, ``w13 [E, H, 2F]`` packed
     [gate | up], ``w2 [E, F, H]``; ``[H, 2F]`` and ``[F, H]`` for one expert.
