@@ -403,7 +403,7 @@ struct MxWalk {
     mb = band * 8 + (in - column * rows_in);
     nb = column;
   }
-  static __device__ __forceinline__ int32_t whole(int32_t rows) {
+  static __host__ __device__ constexpr int32_t whole(int32_t rows) {
     rows = (rows + 63) / 64 * 64;
     return rows < ROWS ? rows : ROWS;
   }
@@ -479,6 +479,17 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// Whether every block of 1 to ROWS token rows gives a pair's MMA an N that is a
+// multiple of 32 and covers the block.
+template <int ROWS>
+constexpr bool pair_sizes_hold() {
+  for (int rows = 1; rows <= ROWS; ++rows) {
+    const int n = MxWalk<ROWS, true>::whole(rows);
+    if (n % 32 != 0 || n < rows || n > ROWS) return false;
+  }
+  return true;
+}
+
 // Tiles.  One CTA: ROWS token rows (M = 128) x 128 outputs, ROWS = 128 or 64.
 // A 64-row tile still runs M = 128 MMAs: the operand's upper rows are whatever
 // lies behind it in shared memory and only reach accumulator rows that are
@@ -488,8 +499,9 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 // A pair: 256 weight rows (M) x up to 224 token rows (N: 64, 128, 192 or 224,
 // named by the instruction): an expert's rows are cut into equal blocks, so
 // MMAs are spent on its rows rounded up to such a block instead of whole
-// 256-row tiles.  (Blocks rounded to 16 rows, N = 16 modulo 32, hung launches
-// and are not used.)
+// 256-row tiles.  N stays a multiple of 32 (pair_sizes_hold): a build whose
+// blocks were rounded to 16 rows, N = 16 modulo 32, stopped twice in
+// back-to-back launches.  The cause is not known; the form is not used.
 // The accumulator is transposed: lanes are outputs, columns token rows.
 // Two accumulators and the scale words share the 512 TMEM columns: 2 x 224 +
 // 2 x 12 for a pair (N = 256 would leave none for the scales), 2 x 128 + 2 x 8
@@ -524,7 +536,8 @@ struct MxCfg {
   static_assert(kStageBytes % 1024 == 0 && kABytes % 1024 == 0, "swizzle atoms");
   static_assert(kScaleTmem + 2 * kScaleCols <= kTmemCols, "TMEM columns");
   static_assert(kSmemBytes <= 232448 && kStages >= 4, "shared memory");
-  static_assert((2 * kStages + 9) * 8 + 12 + 400 * 4 <= 2048, "barriers and the tile list");
+  static_assert((2 * kStages + 9) * 8 + 12 + kMxListWords * 4 <= 2048, "barriers and the tile list");
+  static_assert(G == 1 || pair_sizes_hold<kTokens>(), "N of a pair's MMA");
   // Split K (one CTA): a row of partial sums, padded against bank conflicts.
   static constexpr int kSumRow = kTileN * 4 + 16;
   static_assert(G == 2 || ROWS * kSumRow <= kStages * kStageBytes, "partial sums fit the ring");
