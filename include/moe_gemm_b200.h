@@ -390,13 +390,14 @@ int32_t ffn_last_launches(mgb_ffn_launch_info* info, int32_t capacity);
  * of two s with max |x| <= 448 s over the block's finite values (1 for a block
  * of zeros), q = x / s rounded to nearest even (infinities and NaNs become
  * NaN).  x [rows, cols] fp16 / bf16 / fp32 with contiguous columns, q e4m3
- * [rows, cols], scale e8m0 [rows, ceil(cols / 128)] contiguous. */
+ * [rows, cols], scale e8m0 [rows, ceil(cols / 128)] contiguous: fewer than 2^31
+ * scales, otherwise MGB_ERR_INVALID. */
 int quantize_rows_launch(const void* x, int64_t rows, int64_t cols, int64_t pitch, int32_t dtype, void* q,
                          int64_t q_pitch, void* scale, void* stream);
 
 /* The same with one scale per 128 x 128 block of each of `matrices` matrices,
  * `stride` elements apart: q [matrices, rows, cols] and scale [matrices,
- * ceil(rows / 128), ceil(cols / 128)], both contiguous. */
+ * ceil(rows / 128), ceil(cols / 128)], both contiguous; fewer than 2^31 scales. */
 int quantize_blocks_launch(const void* x, int64_t matrices, int64_t rows, int64_t cols, int64_t pitch, int64_t stride,
                            int32_t dtype, void* q, void* scale, void* stream);
 

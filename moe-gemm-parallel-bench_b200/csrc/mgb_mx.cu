@@ -18,7 +18,14 @@ namespace {
 
 using namespace mgb;
 
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t cdiv(int64_t a, int64_t b) { return a / b + (a % b != 0 ? 1 : 0); }
+
+// a * b, or -1 from 2^31 on: the quantisation kernels count blocks in 32 bits
+// (FastDiv) and a thread block each.
+int64_t block_count(int64_t a, int64_t b) {
+  constexpr int64_t limit = 1ll << 31;
+  return a < limit && b < limit && a * b < limit ? a * b : -1;
+}
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 template <int G, int ROWS>
@@ -87,8 +94,8 @@ int access_of(const void* x, int64_t pitch, int64_t stride, const void* q, int64
 template <typename T>
 int rows_typed(const void* x, int64_t rows, int64_t cols, int64_t pitch, void* q, int64_t q_pitch, void* scale,
                cudaStream_t s) {
-  const int64_t blocks = rows * cdiv(cols, 128);
-  if (blocks >= (1ll << 31)) return MGB_ERR_INVALID;  // 2^38 elements: more than the GPU holds
+  const int64_t blocks = block_count(rows, cdiv(cols, 128));
+  if (blocks < 0) return MGB_ERR_INVALID;
   const int access = access_of<T>(x, pitch, 0, q, q_pitch, 0, cols);
   const bool dense = pitch == cols && q_pitch == cols && cols % 128 == 0;
   const auto kernel = access == k32Bytes   ? quantize_rows_kernel<T, k32Bytes>
@@ -104,8 +111,8 @@ int rows_typed(const void* x, int64_t rows, int64_t cols, int64_t pitch, void* q
 template <typename T>
 int blocks_typed(const void* x, int64_t matrices, int64_t rows, int64_t cols, int64_t pitch, int64_t stride, void* q,
                  void* scale, cudaStream_t s) {
-  const int64_t kb = cdiv(cols, 128), per = cdiv(rows, 128) * kb;
-  if (per >= (1ll << 31) || matrices * per >= (1ll << 31)) return MGB_ERR_INVALID;
+  const int64_t kb = cdiv(cols, 128), per = block_count(cdiv(rows, 128), kb);
+  if (per < 0 || block_count(matrices, per) < 0) return MGB_ERR_INVALID;
   const int access = access_of<T>(x, pitch, stride, q, cols, rows * cols, cols);
   const auto kernel = access == k32Bytes   ? quantize_blocks_kernel<T, k32Bytes>
                       : access == k16Bytes ? quantize_blocks_kernel<T, k16Bytes>

@@ -11,7 +11,8 @@ to do outside the tensor core, whose block-scaled MMA applies them itself:
 and ``launch_quantize_blocks`` (weights: a scale per 128 x 128 block) produce
 the operands: s is the smallest power of two with max |x| <= 448 s over the
 block's finite values (1 for a block of zeros), q = x / s rounded to nearest
-even, infinities and NaNs become NaN.  ``launch_block_scaled_mm`` multiplies
+even, infinities and NaNs become NaN; a call makes fewer than 2^31 scales.
+``launch_block_scaled_mm`` multiplies
 them, dense or over expert-sorted rows, from one token to whole prompts.
 Every call is launches only, on the current stream of the tensors' device, and
 can be captured in a CUDA graph.  The reference has no counterpart (it does not
