@@ -169,12 +169,10 @@ struct Launcher {
       set(1, b, n, k, kKMajor);
     }
   }
+  // Without rows the tensor stays unset: the kernel prefetches the map of every
+  // tensor that is there, and there is none to encode.
   void output(int i, const FfnTensor& t, int64_t cols) {
-    if (rows > 0) {
-      set(i, t, rows, cols, kStage);
-    } else {
-      job().t[i] = t;
-    }
+    if (rows > 0) set(i, t, rows, cols, kStage);
   }
   // Weight gradient job: C_e[m, n] = A[rows, m]^T B[rows, n].
   void wgrad_job(const FfnTensor& a, const FfnTensor& b, const FfnTensor& c, int64_t m, int64_t n) {

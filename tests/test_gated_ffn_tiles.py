@@ -126,3 +126,34 @@ def test_report_without_a_launch():
     lib.ffn_last_launches(info, 0)
     assert info[0].grid == info[1].grid == -1  # nothing written past the capacity
     assert lib.gated_ffn_forward_launch(ctypes.byref(_native.FfnArgs(2))) == _native.STATUS_INVALID
+
+
+@pytest.mark.gpu
+def test_no_rows_with_tensors_given():
+    """A C caller may pass its buffers with zero rows: weight gradients become zeros, nothing else is touched."""
+    hidden, ffn, experts = 64, 40, 3
+    code = _native.DTYPE_CODES["bf16"]
+    token = torch.full((16, 2 * ffn), 5.0, device="cuda", dtype=torch.bfloat16)
+    w13 = torch.full((experts, hidden, 2 * ffn), 5.0, device="cuda", dtype=torch.bfloat16)
+    w2 = torch.full((experts, ffn, hidden), 5.0, device="cuda", dtype=torch.bfloat16)
+    dw13, dw2 = w13.clone(), w2.clone()
+    offs = torch.zeros(experts, dtype=torch.int32, device="cuda")
+    args = _native.FfnArgs(code, experts, 0, hidden, ffn, offs.data_ptr())
+    for field, cols in (("x", hidden), ("y", hidden), ("dx", hidden), ("h", ffn), ("gate_up", 2 * ffn),
+                        ("dgate_up", 2 * ffn)):
+        setattr(args, field, token.data_ptr())
+        setattr(args, field + "_pitch", cols)
+    for field, t in (("w13", w13), ("w2", w2), ("dw13", dw13), ("dw2", dw2)):
+        setattr(args, field, t.data_ptr())
+        setattr(args, field + "_pitch", t.stride(1))
+        setattr(args, field + "_stride", t.stride(0))
+    nbytes = _native.ffn_scratch_bytes(experts, _native.FFN_BACKWARD)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    _native.gated_ffn_forward(args, 0, 0, stream)
+    _native.gated_ffn_backward(args, scratch.data_ptr(), nbytes, stream)
+    torch.cuda.synchronize()
+    kernels.check_device_errors()
+    assert launches() == [(*ONE, 1)]
+    assert not dw13.any() and not dw2.any()
+    assert bool((token == 5.0).all()) and bool((w13 == 5.0).all()) and bool((w2 == 5.0).all())
