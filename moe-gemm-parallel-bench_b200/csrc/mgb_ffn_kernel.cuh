@@ -196,6 +196,10 @@ __global__ void __launch_bounds__(64) ffn_plan_kernel(const __grid_constant__ Ff
 // a role then finds a tile without a chain of global loads.
 constexpr int kListWords = 400;
 
+// Clock cycles that a 64-deep contraction block adds to the bounded wait for
+// its accumulator (it takes about 600).
+constexpr long long kBlockCycles = 4096;
+
 // A role's position in the tile list (`ts` and `offs` in shared or global
 // memory) of ROWS x COLS output tiles.
 template <int ROWS, int COLS>
@@ -940,6 +944,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
     typename Cfg::Walk walk(p, ts, offs);
     FfnItems items(walk, G);
     uint32_t acc_it = 0, chunk_seq = 0;
+    // An accumulator is waited for through its whole contraction, every block of
+    // which the other roles may wait for: 2^31 rows are seconds.
+    const auto whole_budget = [&] { return budget + (items.kb_to - items.kb_from) * kBlockCycles; };
     for (int32_t t; items.advance(walk, t);) {
       const FfnJob& j = *walk.job;
       int64_t mb, nb;
@@ -948,7 +955,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
       const int32_t n0 = static_cast<int32_t>(nb * Cfg::kTileOut);
       if (items.last) {
         if (items.kb_to <= items.kb_from) break;  // a short last share has no blocks and leaves no sums
-        if (!mbar_wait_warp(&acc_full[acc_it & 1], (acc_it >> 1) & 1u, budget, abort)) {
+        if (!mbar_wait_warp(&acc_full[acc_it & 1], (acc_it >> 1) & 1u, whole_budget(), abort)) {
           if (lane == 0) fail(kErrWaitAccFull);
           break;
         }
@@ -992,7 +999,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_kernel(const __grid_constan
         }
       }
       const int buf = NH == 2 ? 0 : static_cast<int>(acc_it & 1);
-      if (!mbar_wait_warp(&acc_full[buf], (NH == 2 ? acc_it : acc_it >> 1) & 1u, budget, abort)) {
+      if (!mbar_wait_warp(&acc_full[buf], (NH == 2 ? acc_it : acc_it >> 1) & 1u, whole_budget(), abort)) {
         if (lane == 0) fail(kErrWaitAccFull);
         break;
       }

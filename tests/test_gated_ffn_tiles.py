@@ -157,3 +157,24 @@ def test_no_rows_with_tensors_given():
     assert launches() == [(*ONE, 1)]
     assert not dw13.any() and not dw2.any()
     assert bool((token == 5.0).all()) and bool((w13 == 5.0).all()) and bool((w2 == 5.0).all())
+
+
+@pytest.mark.gpu
+def test_a_long_contraction_is_not_a_lost_one():
+    """A weight gradient's contraction is as long as its rows: here 15 thousand
+    blocks of 64, milliseconds, under waits of a tenth of one for each block."""
+    rows = 1_000_003
+    gen = torch.Generator(device="cuda").manual_seed(25)
+    a = torch.randint(-2, 3, (rows, 8), device="cuda", generator=gen).to(torch.bfloat16)
+    dc = torch.randint(-1, 2, (rows, 16), device="cuda", generator=gen).to(torch.bfloat16)
+    value = a.double().t() @ dc.double()  # whole numbers below 2^21: exact in fp32 sums
+    kernels.launch_grouped_mm_wgrad(a, dc)  # loads the kernel under the usual waits
+    torch.cuda.synchronize()
+    try:
+        _native.set_debug(200_000)
+        out = kernels.launch_grouped_mm_wgrad(a, dc)
+        torch.cuda.synchronize()
+        kernels.check_device_errors()
+    finally:
+        _native.set_debug(0)
+    assert torch.equal(out, value.to(torch.float32).to(torch.bfloat16))
