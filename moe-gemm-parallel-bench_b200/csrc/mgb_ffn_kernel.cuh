@@ -434,6 +434,28 @@ __device__ __forceinline__ void ffn_store_plain(const FfnJob& j, const RowGroup&
   }
 }
 
+// sigmoid(g) and 1 - sigmoid(g) from e = exp(-|g|), which never overflows: with
+// exp(-g) the divisor passes 2^126 from g = -87.3 on, where the fast divide
+// returns 0, although sigmoid(g) times a large u or dh is still a number.  Fast
+// exponential and divide: a few ulp in fp32, far below the 16-bit rounding of
+// what is stored.
+__device__ __forceinline__ float2 sigmoids(float g) {
+  const float e = __expf(-fabsf(g));
+  const float near = __fdividef(1.0f, 1.0f + e), far = e * near;
+  return g < 0.0f ? make_float2(far, near) : make_float2(near, far);
+}
+
+__device__ __forceinline__ float swiglu(float g, float u) { return g * sigmoids(g).x * u; }
+
+// Gradients of h = silu(g) u.  dh comes last: the other factors' product is of
+// the size of u or g times a sigmoid, where dh g alone may overflow at a gate
+// of the type's lowest value (and infinity times its sigmoid 0 is NaN).
+__device__ __forceinline__ void swiglu_grad(float dh, float g, float u, float& dg, float& du) {
+  const float2 s = sigmoids(g);
+  du = dh * (g * s.x);
+  dg = dh * (u * (s.x * (1.0f + g * s.y)));
+}
+
 // Swiglu epilogue of one warp: gate columns [0, TO), up columns [TO, 2 TO) of
 // the accumulator; h from the fp32 values, g and u rounded once as stored.
 template <typename T, int TO>
@@ -464,7 +486,7 @@ __device__ __forceinline__ void ffn_store_swiglu(const FfnJob& j, const RowGroup
       }
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        gate[i] = __float_as_uint(silu_mul(__uint_as_float(gate[i]), __uint_as_float(up[i])));
+        gate[i] = __float_as_uint(swiglu(__uint_as_float(gate[i]), __uint_as_float(up[i])));
       }
       if (rows.ragged) {
         rows.put_row<T>(j.t[2], gate, x, j.n, lane);
@@ -491,14 +513,6 @@ __device__ __forceinline__ float2 unpack_pair(uint32_t v) {
   } else {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
   }
-}
-
-// Gradients of h = silu(g) u: s = sigmoid(g) with the fast exponential and
-// divide (a few ulp in fp32, far below the 16-bit rounding of what is stored).
-__device__ __forceinline__ void swiglu_grad(float dh, float g, float u, float& dg, float& du) {
-  const float s = __fdividef(1.0f, 1.0f + __expf(-g));
-  du = dh * g * s;
-  dg = dh * u * s * (1.0f + g * (1.0f - s));
 }
 
 // One warp's state of the swiglu backward epilogue: two pairs of blocks, each
@@ -576,7 +590,7 @@ __device__ __forceinline__ void ffn_join(const FfnParams& p, const typename Cfg:
       if (col < j.n) {
         store4<T>(j.t[lane < 16 ? 3 : 4], row, col, s.x, s.y, s.z, s.w);
         if (lane < 16) {
-          store4<T>(j.t[2], row, col, silu_mul(s.x, u.x), silu_mul(s.y, u.y), silu_mul(s.z, u.z), silu_mul(s.w, u.w));
+          store4<T>(j.t[2], row, col, swiglu(s.x, u.x), swiglu(s.y, u.y), swiglu(s.z, u.z), swiglu(s.w, u.w));
         }
       }
     } else {
