@@ -24,6 +24,9 @@
 // that cross a segment's end are written by ordinary stores.
 //
 // Epilogues (fp32 accumulators, one rounding per stored value):
+// h and the gradient of gate_up are operands of the next product, so 16-bit:
+// y, dx and dW13 carry that rounding beside their own (bf16: 2.3e-3 from the
+// formula in the Frobenius norm where one rounding alone is 1.7e-3).
 //   plain            C
 //   swiglu           gate | up tiles side by side in one accumulator; stores
 //                    h = silu(g) u, g and u (the backward pass reads g, u)
@@ -43,11 +46,13 @@
 // (then idle) operand ring, and CTA r adds rows [128 r / split, ...) of all of
 // them over distributed shared memory, in rank order, and applies the
 // epilogue.
-// Large launches are bound by the tensor pipe under the power limit: bf16
-// 8192^3 runs at 1590 (wgrad) and 1600 TFLOP/s (dgrad) where the measured
-// library product has 1618; 32 experts of 512 uneven rows, hidden 7168, ffn
-// 2048: forward 1.46 ms (990 TFLOP/s at 1.2 GHz), backward 2.95 ms.  Few rows are
-// bound by the weights' bytes and by about 7 us per launch (setup 0.6, tile
+// Large launches: bf16 8192^3 runs at 1590 (wgrad) and 1600 TFLOP/s (dgrad)
+// where the measured library product has 1618; 32 experts of 512 uneven rows,
+// hidden 7168, ffn 2048: forward 1.42 to 1.53 ms, backward 2.95 to 3.09 ms, at
+// 1.2 to 1.3 GHz under the 1 kW limit.  In launches alone (16 experts of 512
+// rows, 4096 x 1536, 1.6 GHz) no unit is full: tensor pipe 50 to 66% busy, DRAM 37
+// to 44%, and operands leave L2 at 11 to 13.5 TB/s, the gate and up launch's
+// 256 x 256 tiles most.  Few rows are bound by the weights' bytes and by about 7 us per launch (setup 0.6, tile
 // list 0.8, first operands 1.4, the join, the gap to the next): 16 rows, hidden
 // 1024, ffn 704: 16.9 us for both products.
 // Every wait is bounded; loads carry no multicast.

@@ -199,8 +199,8 @@ struct FastDiv {
 // block of 32 blocks per CTA step: 32-byte loads, 16-byte stores, no loop.
 // One read and one write of every element, bound by memory.  `dense`: rows of
 // whole blocks without padding, whose b-th block starts at element 128 b.
-// (bf16 8191 x 7168, 176 MB: 29 us; 8 elements a thread, four blocks in flight
-// 31 us; a copy of as many bytes 26 us.)
+// (bf16 8191 x 7168, 176 MB: 30.0 to 32.1 us; 8 elements a thread, four blocks in
+// flight 2 us more; a copy of as many bytes 27 us.)
 template <typename T, int ACCESS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, uint32_t blocks, FastDiv kb, int64_t cols,
                                                             int64_t pitch, uint8_t* q, int64_t q_pitch, uint8_t* scale,
@@ -494,8 +494,8 @@ constexpr bool pair_sizes_hold() {
 // A 64-row tile still runs M = 128 MMAs: the operand's upper rows are whatever
 // lies behind it in shared memory and only reach accumulator rows that are
 // never stored.  It halves the token half of a stage, so eight stages (128 KB
-// of weights per SM) are in flight instead of five while the weights' bytes
-// bound the launch.
+// of weights per SM) are in flight instead of six (96 KB) while the weights'
+// bytes bound the launch.
 // A pair: 256 weight rows (M) x up to 224 token rows (N: 64, 128, 192 or 224,
 // named by the instruction): an expert's rows are cut into equal blocks, so
 // MMAs are spent on its rows rounded up to such a block instead of whole
@@ -543,6 +543,8 @@ struct MxCfg {
   static_assert(G == 2 || ROWS * kSumRow <= kStages * kStageBytes, "partial sums fit the ring");
 };
 
+static_assert(MxCfg<1, 64>::kStages == 8 && MxCfg<1, 128>::kStages == 6, "as the text above has it");
+
 constexpr int kMxThreads = 256;
 
 // Warps: 0 TMA producer, 1 MMA issuer, 2 scales, 3 idle, 4-7 epilogue.
@@ -556,10 +558,12 @@ constexpr int kMxThreads = 256;
 // (then idle) operand rings; CTA r adds rows [r ROWS / split, ...) of all of
 // them over distributed shared memory, in rank order, and stores them.  For
 // launches whose tiles would leave at least half of the SMs idle.
-// Bound by the weights' bytes up to about 200 rows an expert, then by the
-// tensor pipe under the power limit.  32 experts, n 4096, k 7168 (940 MB, 144 us
-// to read): 171 us at 16 rows each, 187 at 104, 214 at 128; 8191 x 4096 x 7168
-// 204 us alone (2.35 PFLOP/s), 239 in a row at 1.5 GHz.
+// 32 experts, n 4096, k 7168 (940 MB, 144 us to read), launches in a row: 189 us
+// at 16 rows each, 213 at 128.  8191 x 4096 x 7168: 210 to 230 us in a row (2.1 to
+// 2.3 PFLOP/s) at 1.5 GHz under the power limit, where the tensor pipe could do
+// 3.6.  In a launch alone the pipe is 65% busy, DRAM 11%, and operands leave L2 at
+// 13.5 TB/s (2.6 GB; a 224 x 256 tile loads 60 KB a K block): the operand traffic
+// is the likeliest bound.
 template <int G, int ROWS>
 __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant__ MxParams p) {
   using Cfg = MxCfg<G, ROWS>;
@@ -1017,13 +1021,13 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_kernel(const __grid_constant
 // no barrier), kFewDepth K blocks ahead: two CTAs keep 192 KB of weights per
 // SM in flight without holding registers for them.  The warps' sums are
 // joined in shared memory in warp order (the result does not depend on
-// timing).  1 x 4096 x 7168 (29 MB, 4.5 us to read): 8.8 us.
+// timing).
 // Weights are the 16-row operand of the warp-level m16n8k32 MMA, 8 tokens its
 // columns (more tokens take further passes).  A thread loads 16 consecutive
 // bytes of a row and uses them as the fragments of two MMAs; weights and tokens are permuted along K alike, so
 // the sum is over the same products.  Each 128-deep block starts from zero and
 // is added to the fp32 sums times its two scales.  1 x 4096 x 7168 (29 MB,
-// 4.5 us to read): 8.8 us, of which about 2.5 are the launch and the join.
+// 4.5 us to read), launches in a row on weights that L2 does not hold: 10.3 us.
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(

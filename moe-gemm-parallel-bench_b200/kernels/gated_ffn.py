@@ -21,11 +21,13 @@ fp16 or bf16; hidden and ffn sizes are multiples of 8, bases 16-byte aligned,
 columns contiguous; rows may be padded to a pitch that is a multiple of 8,
 experts to a whole number of rows.
 Accumulation is fp32; ``gate_up``, ``h`` and the gradient of ``gate_up`` are
-rounded once to the operands' type between products.  Inputs and outputs must
+rounded once to the operands' type between products, weight gradients are
+overwritten and of the weights' type.  Inputs and outputs must
 not overlap.  Every call is launches only (no synchronisation), on the current
 stream of the tensors' device, with its scratch allocated on that stream, so it
 can be captured in a CUDA graph.  The calls are explicit: autograd does not see
-them.  The reference has no counterpart (SiLU(gate) * up and all gradients stay
+them, and their outputs carry no history even where an input requires a
+gradient.  The reference has no counterpart (SiLU(gate) * up and all gradients stay
 outside its timed path, README.md:55-60).
 """
 
@@ -212,7 +214,9 @@ def gated_ffn_backward(dy, x, w13, w2, h, gate_up, offs=None, *, dx=None, dw13=N
 
 
 def launch_grouped_mm_dgrad(dc, mat_b, offs=None, out=None, *, gate_up=None):
-    """Gradient of ``launch_grouped_mm(a, mat_b, offs)`` with respect to ``a``:
+    """Gradient of ``launch_grouped_mm(a, mat_b, offs)`` with respect to ``a``,
+    for fp16 and bf16, sizes that are multiples of 8 and one segment per expert
+    (not for offsets of several segments per expert):
     ``out[rows of e] = dc[rows of e] @ mat_b[e].T`` with ``dc [T, N]``,
     ``mat_b [E, K, N]`` (or ``[K, N]``), ``out [T, K]``.  With ``gate_up
     [T, 2K]`` the product is the gradient of ``h = silu(gate) * up`` and the
@@ -244,7 +248,9 @@ def launch_grouped_mm_dgrad(dc, mat_b, offs=None, out=None, *, gate_up=None):
 
 
 def launch_grouped_mm_wgrad(mat_a, dc, offs=None, out=None):
-    """Gradient of ``launch_grouped_mm(mat_a, b, offs)`` with respect to ``b``:
+    """Gradient of ``launch_grouped_mm(mat_a, b, offs)`` with respect to ``b``,
+    in the types and sizes of ``launch_grouped_mm_dgrad``, one matrix per segment
+    (the sum over an expert's segments, where it has several, is the caller's):
     ``out[e] = mat_a[rows of e].T @ dc[rows of e]`` with ``mat_a [T, K]``,
     ``dc [T, N]``, ``out [E, K, N]`` (``[K, N]`` without ``offs``); zeros for an
     expert without rows.  Returns ``out``."""
