@@ -47,6 +47,14 @@ struct DeviceState {
 int device_state(DeviceState* out) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return MGB_ERR_CUDA;
+  // The driver call that encodes tensor maps needs a current context, which a
+  // thread whose first CUDA call this is does not have: cudaGetDevice binds
+  // none, cudaSetDevice does (and may be called during a capture).
+  thread_local bool bound[kMaxDevices] = {};
+  if (!bound[dev]) {
+    if (cudaSetDevice(dev) != cudaSuccess) return MGB_ERR_CUDA;
+    bound[dev] = true;
+  }
   std::lock_guard<std::mutex> lock(g_mutex);
   if (g_error_ptr[dev] == nullptr) {
     void* ptr = nullptr;
