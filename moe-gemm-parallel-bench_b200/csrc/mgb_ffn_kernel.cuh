@@ -452,13 +452,14 @@ __device__ __forceinline__ float2 sigmoids(float g) {
 
 __device__ __forceinline__ float swiglu(float g, float u) { return g * sigmoids(g).x * u; }
 
-// Gradients of h = silu(g) u.  dh comes last: the other factors' product is of
-// the size of u or g times a sigmoid, where dh g alone may overflow at a gate
-// of the type's lowest value (and infinity times its sigmoid 0 is NaN).
+// Gradients of h = silu(g) u.  u and g meet the sigmoid first and dh then, so
+// that no step leaves fp32's range where the result does not: dh g alone may at a
+// gate of the type's lowest value (and infinity times its sigmoid 0 is NaN), u
+// times silu'(g), which reaches 1.1, at the largest u.
 __device__ __forceinline__ void swiglu_grad(float dh, float g, float u, float& dg, float& du) {
   const float2 s = sigmoids(g);
   du = dh * (g * s.x);
-  dg = dh * (u * (s.x * (1.0f + g * s.y)));
+  dg = dh * (u * s.x) * (1.0f + g * s.y);
 }
 
 // Swiglu epilogue of one warp: gate columns [0, TO), up columns [TO, 2 TO) of

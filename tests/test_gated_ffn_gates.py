@@ -74,3 +74,21 @@ def test_forward_where_sigmoid_is_tiny(rows, hidden):
     bound = (half_step(torch.bfloat16) + FAST * (1 + g.abs().clamp_max(1e3))) * value.abs() + 2.0**-149 * (g * u).abs().clamp_max(1e38)
     within(h, (value, 1.01 * bound), "h")
     assert not y.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,hidden", [(40, 512), (700, 448)], ids=["split", "tiles"])
+@pytest.mark.parametrize("gate", [2.5, -1.25, 0.0, 88.0])
+def test_gradients_of_the_largest_up_values(gate, rows, hidden):
+    """silu'(2.5) is 1.1: up times it passes fp32's range, times a small dh it does not."""
+    f, scale = 64, 1e-38
+    block = Block([rows], hidden, f, torch.bfloat16, seed=33, dense=True)
+    block.dy = (block.dy.double() * scale * 2.0**20).to(torch.bfloat16)
+    block.w2 = (block.w2.double() * 2.0**-10).to(torch.bfloat16)
+    gu = torch.empty((rows, 2 * f), device="cuda", dtype=torch.bfloat16)
+    gu[:, :f], gu[:, f:] = gate, torch.finfo(torch.bfloat16).max
+    gu[::2, f:] *= -1
+    h = torch.zeros((rows, f), device="cuda", dtype=torch.bfloat16)
+    out = kernels.launch_grouped_mm_dgrad(block.dy, block.w2, gate_up=gu)
+    kernels.check_device_errors()
+    within(out, block.backward(h, gu)["dgate_up"], "dgate_up")
