@@ -52,9 +52,9 @@
 // 1.2 to 1.3 GHz under the 1 kW limit.  In launches alone (16 experts of 512
 // rows, 4096 x 1536, 1.6 GHz) no unit is full: tensor pipe 50 to 66% busy, DRAM 37
 // to 44%, and operands leave L2 at 11 to 13.5 TB/s, the gate and up launch's
-// 256 x 256 tiles most.  Few rows are bound by the weights' bytes and by about 7 us per launch (setup 0.6, tile
-// list 0.8, first operands 1.4, the join, the gap to the next): 16 rows, hidden
-// 1024, ffn 704: 16.9 us for both products.
+// 256 x 256 tiles most.  Few rows are bound by the weights' bytes and by about
+// 7 us per launch (setup 0.6, tile list 0.8, first operands 1.4, the join, the gap
+// to the next): 16 rows, hidden 1024, ffn 704: 17.1 us for both products.
 // Every wait is bounded; loads carry no multicast.
 #pragma once
 

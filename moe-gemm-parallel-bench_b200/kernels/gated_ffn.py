@@ -239,8 +239,6 @@ def launch_grouped_mm_dgrad(dc, mat_b, offs=None, out=None, *, gate_up=None):
     if out is None:
         out = _rows_of(dc, rows, cols)
     out_at, out_pitch = _token("out", out, rows, cols, dc.dtype, device)
-    if rows == 0:
-        return out
     scratch, nbytes = _scratch(dc, _native.ffn_scratch_bytes(experts, _native.FFN_DGRAD))
     _call(device, _native.grouped_dgrad, dc_at, dc_pitch, b_at, b_pitch, b_stride, ends, experts, rows, n, k, gu_at,
           gu_pitch, out_at, out_pitch, code, scratch.data_ptr() if nbytes else 0, nbytes)

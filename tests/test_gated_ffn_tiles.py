@@ -178,3 +178,18 @@ def test_a_long_contraction_is_not_a_lost_one():
     finally:
         _native.set_debug(0)
     assert torch.equal(out, value.to(torch.float32).to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_report_of_a_call_without_rows():
+    """A call that launches nothing reports nothing, not the call before it."""
+    block = Block([20, 30], 64, 40, torch.bfloat16, seed=26)
+    kernels.launch_grouped_mm_dgrad(block.dy, block.w2, block.offs)
+    assert len(launches()) == 1
+    offs = torch.zeros(2, dtype=torch.int32, device="cuda")
+    assert kernels.launch_grouped_mm_dgrad(block.dy[:0], block.w2, offs).shape == (0, 40)
+    assert launches() == []
+    many = Block([1] * 220, 64, 40, torch.bfloat16, seed=27)
+    assert kernels.launch_grouped_mm_dgrad(many.dy[:0], many.w2, torch.zeros_like(many.offs)).shape == (0, 40)
+    assert launches() == []
+    kernels.check_device_errors()
